@@ -185,6 +185,84 @@ typedef struct sfa_indexer_args {
   int32_t flags;                                  /* reserved, must be 0                       */
 } sfa_indexer_args;
 
+/* ---- rotary positions and per-head norms of q and k -----------------------
+ * A row is one head of one token, x[D].  With n normed dims (the first n, 0:
+ * none) and R rotated dims from rope_offset, frequencies inv_freq[R / 2]:
+ *   u_d = x_d w_d / sqrt(mean_{d < n} x_d^2 + eps)  (d < n), else x_d
+ *   y1 = s (u1 cos a - u2 sin a), y2 = s (u2 cos a + u1 sin a),
+ *   a = position * inv_freq[i], s = rope_scale,
+ * over the pairs (i, i + R/2) of the rotated dims, or (2i, 2i+1) when
+ * interleaved.  float32 between load and store, angles reduced in float64.
+ * The reference has neither step (its q and kv come ready made, SFA.py:86-94). */
+typedef struct sfa_rope_args {
+  int32_t dtype;                 /* SFA_DTYPE_F32 or SFA_DTYPE_BF16                   */
+  int32_t B, S, D, Hq, Hkv, Dv;  /* Hkv = 0: no k; Dv: the appended v rows (0: none)  */
+  int32_t rotary_dim, rope_offset, interleaved;
+  int32_t q_norm, k_norm;        /* normed dims (0: no norm)                          */
+  int32_t w_dtype;               /* of the weights and their gradients: float32 or dtype */
+  int32_t pos_i64, slots_i64;    /* positions / slots are int64 (else int32)          */
+  float eps, rope_scale;
+  const void* positions; int64_t p_sb, p_ss;       /* [B, S]                          */
+  const double* inv_freq;                          /* [rotary_dim / 2]                */
+  const void* q;  int64_t q_sb, q_ss, q_sh;        /* [B, S, Hq, D]                   */
+  const void* k;  int64_t k_sb, k_ss, k_sh;        /* [B, S, Hkv, D]                  */
+  const void* q_weight;  const void* k_weight;     /* [q_norm], [k_norm]              */
+  /* forward: written (each may be its input); backward: the gradients of the
+   * results, read.  append: k_out is the page pool [num_pages, page_size, Hkv, D]
+   * with page, row and head strides                                                 */
+  void* q_out;    int64_t qo_sb, qo_ss, qo_sh;
+  void* k_out;    int64_t ko_sb, ko_ss, ko_sh;
+  const void* v;  int64_t v_sb, v_ss, v_sh;        /* append: [B, S, Hkv, Dv] or NULL */
+  void* v_out;    int64_t vo_sb, vo_ss, vo_sh;     /* append: the pool of the v rows  */
+  const void* slots; int64_t s_sb, s_ss;           /* append: [B, S] logical cache rows;
+                                                      one outside the table or on an
+                                                      unmapped page is not written    */
+  void* dq;       int64_t dq_sb, dq_ss, dq_sh;     /* backward                        */
+  void* dk;       int64_t dk_sb, dk_ss, dk_sh;
+  void* dq_weight; void* dk_weight;                /* backward: [q_norm], [k_norm]    */
+  int32_t flags;                                   /* reserved, must be 0             */
+} sfa_rope_args;
+
+/* ---- attention of a tree of drafted tokens over a paged cache --------------
+ * Token t of sequence b sees the cache's rows [0, ctx_lens[b]) and the drafted
+ * rows ctx_lens[b] + j, j < tree_lens[b], with bit j of tree_mask[b, t] set.  Rows of
+ * unmapped pages are not seen.  A token t >= tree_lens[b] gives out = 0 and
+ * lse = -inf, as does one that sees nothing (with a sink its lse is the sink). */
+typedef struct sfa_tree_args {
+  int32_t dtype;
+  int32_t B, T, Hq, Hkv, Dqk, Dv;                  /* T <= 64, head dims <= 1024      */
+  float scale;                                     /* > 0                             */
+  const void* q;  int64_t q_sb, q_ss, q_sh;        /* [B, T, Hq, Dqk]                 */
+  const void* k;  int64_t k_sb, k_ss, k_sh;        /* pools: page, row, head strides  */
+  const void* v;  int64_t v_sb, v_ss, v_sh;        /* (v may be the first Dv dims of k) */
+  const int32_t* ctx_lens;                         /* [B]                             */
+  const int64_t* tree_mask; int64_t tm_sb, tm_ss;  /* [B, T]                          */
+  const int32_t* tree_lens;                        /* [B] or NULL: T                  */
+  const float* sink;                               /* [Hq] or NULL                    */
+  void* out;      int64_t o_sb, o_ss, o_sh;        /* [B, T, Hq, Dv]                  */
+  float* lse;     int64_t l_sb, l_ss, l_sh;        /* [B, T, Hq]                      */
+  int32_t flags;                                   /* reserved, must be 0             */
+} sfa_tree_args;
+
+/* ---- pages of a cache -------------------------------------------------------
+ * block_table [B, max_pages] as in sfa_kv_pages (-1: none), ref_counts
+ * [num_pages] the number of entries that map a page: a page is free iff its
+ * count is 0, and the pages a call takes are the lowest free ones.  A pool is
+ * [num_pages, page_size, ...] with each page contiguous.                      */
+typedef struct sfa_cache_pool {
+  void* base;
+  int64_t page_stride, page_bytes;  /* bytes */
+} sfa_cache_pool;
+typedef struct sfa_cache {
+  const sfa_cache_pool* pools;      /* host array                                     */
+  int32_t npools;
+  int32_t B, max_pages, page_size, num_pages;
+  int32_t flags;                    /* reserved, must be 0                            */
+  int32_t* block_table; int64_t bt_sb;
+  int32_t* ref_counts;
+  int32_t* kv_lens;                 /* [B]                                            */
+} sfa_cache;
+
 /* Library ABI version (SFA_ABI_VERSION of the build). */
 SFA_API int sfa_abi_version(void);
 
@@ -277,6 +355,61 @@ SFA_API size_t sfa_bwd_workspace_size(const sfa_bwd_args* a);
  * second stream joins the capture and is joined back.  Such calls on one
  * device enqueue one at a time (a mutex). */
 SFA_API int sfa_bwd(const sfa_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotation and norms: q_out and k_out from q and k.  With pages (append) the k
+ * rows, and the v rows unchanged, go to the cache rows that `slots` names;
+ * pages NULL: k_out is a tensor like k.  Two tokens of a call with the same
+ * cache row leave one of them there, which is not specified. */
+SFA_API int sfa_rope_fwd(const sfa_rope_args* a, const sfa_kv_pages* pages, void* stream);
+
+/* dq, dk and the weights' gradients (summed in a fixed order) from the results'
+ * gradients in q_out / k_out.  Workspace: 8 KiB per workgroup, up to 8 MiB, with
+ * a norm; 0 without. */
+SFA_API size_t sfa_rope_bwd_workspace_size(const sfa_rope_args* a);
+SFA_API int sfa_rope_bwd(const sfa_rope_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of a drafted tree.  Workspace: float32 partials where the keys are
+ * cut into ranges (few query rows on long tables). */
+SFA_API size_t sfa_tree_fwd_workspace_size(const sfa_tree_args* a, const sfa_kv_pages* pages);
+SFA_API int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Workspace of the sfa_cache_* calls on n pairs (or sequences). */
+SFA_API size_t sfa_cache_workspace_size(const sfa_cache* c, int32_t n);
+
+/* Page src[i] to page dst[i] in every pool.  A pair is left out if a page is
+ * outside the pool, if a later pair has its destination, or if its
+ * destination is the source of another pair. */
+SFA_API int sfa_cache_copy(const sfa_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Row children[i] of the table becomes a fork of row parents[i]: its whole
+ * pages are shared (counts raised), the rows of its last page, filled in part,
+ * are copied to a free page in every pool; kv_lens[child] = kv_lens[parent].
+ * ok[i] = 0 and nothing is written for a pair with a row outside the table,
+ * whose child an earlier pair has or any pair has as parent, or that finds no
+ * free page.  The child's own pages are not freed (sfa_cache_free first). */
+SFA_API int sfa_cache_fork(const sfa_cache* c, const int32_t* parents, const int32_t* children, int32_t n, int32_t* ok,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* The entries of rows[i] past the pages of its first keep_lens[i] rows (NULL:
+ * all) become -1 and their pages lose a reference. */
+SFA_API int sfa_cache_free(const sfa_cache* c, const int32_t* rows, const int32_t* keep_lens, int32_t n, void* stream);
+
+/* Free pages for rows kv_lens[b] .. new_lens[b] - 1 of every sequence where none
+ * is mapped: all of a sequence's or none (ok[b] = 0), in order of b while they
+ * last.  kv_lens is not changed. */
+SFA_API int sfa_cache_extend(const sfa_cache* c, const int32_t* new_lens, int32_t* ok, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* The pages in use moved to the low end of every pool, the table and counts
+ * with them; used[0]: how many there are. */
+SFA_API int sfa_cache_compact(const sfa_cache* c, int32_t* used, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row ctx_lens[b] + i becomes what row ctx_lens[b] + path[b, i] was, i < plen <= 64;
+ * negative entries leave theirs. */
+SFA_API int sfa_cache_keep_path(const sfa_cache* c, const int32_t* ctx_lens, const int32_t* path, int64_t path_sb,
+                                int32_t plen, void* stream);
 
 #ifdef __cplusplus
 }

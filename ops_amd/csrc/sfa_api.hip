@@ -14,7 +14,7 @@
 #include <initializer_list>
 #include <mutex>
 
-#include "sfa_common.h"
+#include "sfa_ops.h"
 
 namespace {
 
@@ -302,6 +302,11 @@ int run_fwd(const sfa_fwd_args* a, const sfa_kv_pages* pg, void* workspace, size
 }
 
 }  // namespace
+
+namespace sfa {
+int api_fail(int code, const char* msg) { return fail(code, "%s", msg); }
+void api_clear() { g_err[0] = 0; }
+}  // namespace sfa
 
 extern "C" {
 
