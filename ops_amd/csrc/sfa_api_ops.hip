@@ -147,6 +147,8 @@ int check_tree(const sfa_tree_args* a, const sfa_kv_pages* pg) {
   if (!(a->scale > 0.f) || isinf(a->scale)) return fail(SFA_E_INVALID, "scale must be finite and > 0");
   const int rc = check_pages(pg, a->B);
   if (rc != SFA_OK) return rc;
+  if ((int64_t)pg->max_pages * pg->page_size > (int64_t)1 << 30)
+    return fail(SFA_E_UNSUPPORTED, "a table of more than 2^30 rows a sequence");
   if ((int64_t)a->B * a->T * a->Hq > (int64_t)INT_MAX / 4) return fail(SFA_E_UNSUPPORTED, "more than 2^29 query rows");
   return SFA_OK;
 }
