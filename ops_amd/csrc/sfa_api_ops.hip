@@ -147,8 +147,8 @@ int check_tree(const sfa_tree_args* a, const sfa_kv_pages* pg) {
   if (!(a->scale > 0.f) || isinf(a->scale)) return fail(SFA_E_INVALID, "scale must be finite and > 0");
   const int rc = check_pages(pg, a->B);
   if (rc != SFA_OK) return rc;
-  if ((int64_t)pg->max_pages * pg->page_size > (int64_t)1 << 30)
-    return fail(SFA_E_UNSUPPORTED, "a table of more than 2^30 rows a sequence");
+  if ((int64_t)pg->max_pages * pg->page_size > (int64_t)1 << 29)
+    return fail(SFA_E_UNSUPPORTED, "a table of more than 2^29 rows a sequence");
   if ((int64_t)a->B * a->T * a->Hq > (int64_t)INT_MAX / 4) return fail(SFA_E_UNSUPPORTED, "more than 2^29 query rows");
   return SFA_OK;
 }
@@ -293,7 +293,7 @@ int sfa_rope_bwd(const sfa_rope_args* a, void* workspace, size_t workspace_bytes
 size_t sfa_tree_fwd_workspace_size(const sfa_tree_args* a, const sfa_kv_pages* pages) {
   if (check_tree(a, pages) != SFA_OK) return 0;
   const sfa::TreePlan pl = sfa::tree_plan(tree_params(a, pages), a->dtype, tree_vec(a));
-  return pl.part_o_bytes + pl.part_lse_bytes;
+  return pl.workspace();
 }
 
 int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
@@ -303,12 +303,13 @@ int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* worksp
   if (rc != SFA_OK) return rc;
   sfa::TreeParams p = tree_params(a, pages);
   const sfa::TreePlan pl = sfa::tree_plan(p, a->dtype, tree_vec(a));
-  const size_t need = pl.part_o_bytes + pl.part_lse_bytes;
+  const size_t need = pl.workspace();
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)
       return fail(SFA_E_WORKSPACE, "sfa_tree_fwd needs %zu workspace bytes (got %zu)", need, workspace_bytes);
     p.part_o = (float*)workspace;
     p.part_lse = (float*)((char*)workspace + pl.part_o_bytes);
+    p.seq_slots = (int32_t*)((char*)workspace + pl.part_o_bytes + pl.part_lse_bytes);
   }
   return done(sfa::launch_tree(p, pl, a->dtype, (hipStream_t)stream), "sfa_tree_fwd");
 }

@@ -81,17 +81,19 @@ struct TreeParams {
   float scale, scale_log2;
   int nrb;                   // row blocks per (sequence, kv head)
   // Key ranges ("slots"): the batch's keys are cut into about `want` ranges of one
-  // length (a multiple of tile, at least min_len), found on the device; a
-  // sequence of several leaves partials per slot.  want = 0: one a sequence.
-  int want, tile, min_len;
+  // length (two tiles or more; a tile is a power of two of keys), found on the
+  // device; a sequence of several leaves partials per slot.  want = 0: one a sequence.
+  int want, tile;
   float* part_o;             // [slots][T * Hq][Dv], normalised by the slot's own sum
   float* part_lse;           // [slots][T * Hq], base-2 (-inf: nothing seen)
+  int32_t* seq_slots;        // [B][2] first slot and slots of a sequence
 };
 struct TreePlan {
   int kernel;
   int rows;       // query rows (token, head) per workgroup
   int want, slots;
-  size_t part_o_bytes, part_lse_bytes;
+  size_t part_o_bytes, part_lse_bytes, seq_bytes;
+  size_t workspace() const { return part_o_bytes + part_lse_bytes + seq_bytes; }
 };
 TreePlan tree_plan(const TreeParams& p, int dtype, bool vec);
 hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, int dtype, hipStream_t s);

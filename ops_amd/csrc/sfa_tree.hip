@@ -13,6 +13,8 @@
 // even work; the ranges are found on the device from ctx_lens.  A sequence
 // of several slots leaves float32 partials that tree_combine_kernel joins.
 
+#include <utility>
+
 #include "sfa_lds.h"
 #include "sfa_mfma.h"
 #include "sfa_ops.h"
@@ -44,43 +46,49 @@ __device__ __forceinline__ SeqLens seq_lens(const TreeParams& p, int b) {
   return s;
 }
 
+// Sums over the 64 lanes (row rotations and lane swaps: no LDS trips).
+__device__ __forceinline__ int lanes_sum(int x) {
+  x += __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true);  // row_ror:8
+  x += __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x122, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x121, 0xf, 0xf, true);
+  const auto a = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+  x = (int)(a[0] + a[1]);
+  const auto c = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+  return (int)(c[0] + c[1]);
+}
+
 // A key range of the batch.
 struct Slot {
   int b;           // sequence, or -1: none
   int k0, k1;      // its keys
   int first, n;    // the sequence's first slot and how many it has
 };
-// Length of the ranges, and the sequence of a slot (or the slots of sequence
-// `slot` when BY_SEQ).  By one wave; every wave of a workgroup gets the same.
-template <bool BY_SEQ>
+// The range of a slot; every wave finds the same.  Lengths are multiples of
+// the tile: ceil(all tiles / want) of them first, which gives up to B ranges more
+// than wanted, then longer ones until they are `want` or fewer, so that all
+// run at once (a few steps come within a tile of the best).
 __device__ Slot find_slot(const TreeParams& p, int slot) {
-  const int lane = threadIdx.x & 63;
-  int len = 0x7fffffff;  // want = 0: one slot a sequence
+  const int lane = threadIdx.x & 63, shift = 31 - __builtin_clz(p.tile);
+  auto tiles_of = [&](int b) { return b < p.B ? (seq_lens(p, b).keys + p.tile - 1) >> shift : 0; };
+  const int mine = tiles_of(lane);  // (of the first 64 sequences)
+  int len = 0x7fffffff >> shift;    // in tiles; want = 0: one slot a sequence
   if (p.want > 0) {
-    int64_t sum = 0;
-    for (int b = lane; b < p.B; b += 64) sum += seq_lens(p, b).keys;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const int64_t l = (sum + p.want - 1) / p.want;
-    len = l < p.min_len ? p.min_len : (int)((l + p.tile - 1) / p.tile) * p.tile;
-    // ranges of that length are up to B more than wanted: longer ones, so that
-    // all of them run at once (a few steps come within a tile of the best)
+    int64_t sum = lanes_sum(mine);
+    for (int b0 = 64; b0 < p.B; b0 += 64) sum += lanes_sum(tiles_of(b0 + lane));
+    len = max(2, (int)((sum + p.want - 1) / p.want));
     for (int i = 0; i < 6 && p.want > p.B; ++i) {
-      int64_t n = 0;
-      for (int b = lane; b < p.B; b += 64) n += max(1, (int)(((int64_t)seq_lens(p, b).keys + len - 1) / len));
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+      auto ranges = [&](int t, int b) { return b < p.B ? max(1, (t + len - 1) / len) : 0; };
+      int n = lanes_sum(ranges(mine, lane));
+      for (int b0 = 64; b0 < p.B; b0 += 64) n += lanes_sum(ranges(tiles_of(b0 + lane), b0 + lane));
       if (n <= p.want) break;
-      const int64_t up = (len * n / p.want + p.tile - 1) / p.tile * p.tile;
-      len = (int)min((int64_t)0x7fffffff / p.tile * p.tile, up > len ? up : (int64_t)len + p.tile);
+      len = max(len + 1, (int)((int64_t)len * n / p.want));
     }
   }
   int before = 0;
-  Slot s{-1, 0, 0, 0, 0};
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int keys = b < p.B ? seq_lens(p, b).keys : 0;
-    int n = b < p.B ? max(1, (int)(((int64_t)keys + len - 1) / len)) : 0;
+    const int b = b0 + lane, t = b0 == 0 ? mine : tiles_of(b);
+    const int n = b < p.B ? max(1, (t + len - 1) / len) : 0;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -88,21 +96,22 @@ __device__ Slot find_slot(const TreeParams& p, int slot) {
       if (lane >= o) incl += y;
     }
     const int first = before + incl - n;
-    const bool mine = BY_SEQ ? b == slot : slot >= first && slot < first + n;
-    const uint64_t hit = __ballot(mine);
+    const uint64_t hit = __ballot(slot >= first && slot < first + n);
     if (hit != 0) {
       const int w = __builtin_ctzll(hit);
+      Slot s;
       s.b = b0 + w;
-      s.first = __shfl(first, w, 64);
-      s.n = __shfl(n, w, 64);
-      const int kk = __shfl(keys, w, 64), i = BY_SEQ ? 0 : slot - s.first;
-      s.k0 = (int)min((int64_t)i * len, (int64_t)kk);
-      s.k1 = (int)min((int64_t)s.k0 + len, (int64_t)kk);
+      s.first = __builtin_amdgcn_readlane(first, w);
+      s.n = __builtin_amdgcn_readlane(n, w);
+      const int keys = seq_lens(p, s.b).keys;
+      const int64_t k0 = (int64_t)(slot - s.first) * len << shift;
+      s.k0 = (int)min(k0, (int64_t)keys);
+      s.k1 = (int)min(k0 + ((int64_t)len << shift), (int64_t)keys);
       return s;
     }
-    before += __shfl(incl, 63, 64);
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
-  return s;
+  return Slot{-1, 0, 0, 0, 0};
 }
 
 // Element offset of key s of sequence b in a pool of these strides, or -1.
@@ -110,6 +119,14 @@ __device__ __forceinline__ int64_t key_row(const TreeParams& p, int b, int s, in
   const int pg = p.block_table[b * p.bt_sb + (s >> p.page_shift)];
   if (pg < 0 || pg >= p.num_pages) return -1;
   return (int64_t)pg * page_stride + (int64_t)(s & ((1 << p.page_shift) - 1)) * row_stride;
+}
+
+// A sequence's slots, for tree_combine_kernel.
+__device__ __forceinline__ void note_slots(const TreeParams& p, int slot, const Slot& sl) {
+  if (p.want > 0 && slot == sl.first && threadIdx.x == 0) {
+    p.seq_slots[2 * sl.b] = sl.first;
+    p.seq_slots[2 * sl.b + 1] = sl.n;
+  }
 }
 
 // ---- any head dims up to 1024, bf16 or float32: float32 products --------------
@@ -266,9 +283,10 @@ __global__ __launch_bounds__(256) void tree_generic_kernel(TreeParams p) {
   const int rb = wi % p.nrb;
   wi /= p.nrb;
   const int g = wi % p.Hkv, slot = wi / p.Hkv;
-  const Slot sl = find_slot<false>(p, slot);
+  const Slot sl = find_slot(p, slot);
   if (sl.b < 0) return;
   const int b = sl.b, nodes = seq_lens(p, b).nodes;
+  if (rb == 0 && g == 0) note_slots(p, slot, sl);
   const int64_t pr = (int64_t)slot * p.T * p.Hq;
   const bool partial = sl.n > 1;
   generic_rows<T>(
@@ -324,6 +342,16 @@ struct Swz {  // position of chunk c of row r: c ^ at(r)
   }
 };
 
+// f(integral_constant i) for i = 0 .. N - 1
+template <int... I, class F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(std::make_integer_sequence<int, N>{}, f);
+}
+
 // lane l: 16 (4) bytes from its address to dst + 16 l (4 l); not seen by the
 // compiler: the kernel waits for vmcnt itself
 __device__ __forceinline__ void dma16(const void* lds, uint64_t addr) {
@@ -334,14 +362,288 @@ __device__ __forceinline__ void dma4(const void* lds, uint64_t addr) {
   const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(d), "v"(addr) : "memory", "m0");
 }
+// ... from a wave-uniform base and 32-bit lane offsets
+__device__ __forceinline__ void dma16(const void* lds, uint64_t base, uint32_t off) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void* lds, uint64_t base, uint32_t off) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(d), "v"(off), "s"(base) : "memory", "m0");
+}
+// the wait states between the last MFMA that wrote any of these AGPRs and a VALU read
+__device__ __forceinline__ void drain_all(f32x4 (&c)[4]) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]));
+}
+__device__ __forceinline__ void drain_all(f32x4 (&c)[8]) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+               : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+}
 template <int N>
 __device__ __forceinline__ void wait_vm() {  // at most N of this wave's loads in flight, all its LDS reads done
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// ---- work item: the row blocks of one range and kv head on one XCD ------------
+struct WorkItem {
+  int b, g, rb, k0, k1, ctx, nodes, slot;
+  bool partial;
+};
+__device__ __forceinline__ bool work_item(const TreeParams& p, WorkItem& it) {
+  int wi = blockIdx.x;
+  const int nitems = gridDim.x / p.nrb;
+  if (nitems % 8 == 0) {
+    const int x = wi % 8, r = wi / 8;
+    it.rb = r % p.nrb;
+    wi = (r / p.nrb) * 8 + x;
+  } else {
+    it.rb = wi % p.nrb;
+    wi /= p.nrb;
+  }
+  it.g = wi % p.Hkv;
+  it.slot = wi / p.Hkv;
+  const Slot sl = find_slot(p, it.slot);
+  if (sl.b < 0) return false;
+  if (it.rb == 0 && it.g == 0) note_slots(p, it.slot, sl);
+  it.b = __builtin_amdgcn_readfirstlane(sl.b);
+  it.k0 = __builtin_amdgcn_readfirstlane(sl.k0);
+  it.k1 = __builtin_amdgcn_readfirstlane(sl.k1);
+  it.partial = sl.n > 1;
+  const SeqLens len = seq_lens(p, it.b);
+  it.ctx = __builtin_amdgcn_readfirstlane(len.ctx);
+  it.nodes = __builtin_amdgcn_readfirstlane(len.nodes);
+  return true;
+}
+
+// The rows of a wave row's tiles into LDS: lanes 0..31 hold the K row addresses
+// of a tile, lanes 32..63 the V rows', and hand them to the lanes that load.
+template <int D, int WR, int WK>
+struct TileLoads {
+  static constexpr int KT = 32, CH = D / 8, RPI = 64 / CH, ROWI = KT / RPI, NI = 2 * ROWI / WR;
+  uint64_t side_base;
+  int64_t page_bytes, row_bytes;
+  const int32_t* trow;
+  int key0, k1, last_key, page_shift, num_pages, wr, lane;
+  __device__ __forceinline__ TileLoads(const TreeParams& p, int b, int g, int k0, int k1_, int wr_, int wk, int lane_)
+      : k1(k1_), last_key(p.cap - 1), page_shift(p.page_shift), num_pages(p.num_pages), wr(wr_), lane(lane_) {
+    const bool vside = lane >= 32;
+    side_base = vside ? (uint64_t)(uintptr_t)p.v + (uint64_t)(2 * g * p.v_sh)
+                      : (uint64_t)(uintptr_t)p.k + (uint64_t)(2 * g * p.k_sh);
+    page_bytes = 2 * (vside ? p.v_sb : p.k_sb);
+    row_bytes = 2 * (vside ? p.v_ss : p.k_ss);
+    trow = p.block_table + b * p.bt_sb;
+    key0 = k0 + wk * KT + (lane & 31);
+  }
+  __device__ __forceinline__ uint64_t page_addr(int j) const {  // (past the range: any entry, not used)
+    return (uint64_t)(uintptr_t)(trow + (min(key0 + j * WK * KT, last_key) >> page_shift));
+  }
+  // rows of tile j with page ids pg to dst; returns the mask of rows that are there
+  __device__ __forceinline__ uint32_t load(int j, int pg, u32x4* dst) const {
+    const int s = key0 + j * WK * KT;
+    const bool ok = s < k1 && pg >= 0 && pg < num_pages;
+    const uint64_t a = ok ? side_base + (uint64_t)((int64_t)pg * page_bytes + (int64_t)(s & ((1 << page_shift) - 1)) * row_bytes)
+                          : (uint64_t)(uintptr_t)kZeroRow;
+    const uint32_t mask = (uint32_t)__ballot(ok);
+    const int lo = (int)(uint32_t)a, hi = (int)(uint32_t)(a >> 32);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int q = wr * NI + i, v = q >= ROWI ? 1 : 0;
+      const int row = (q - v * ROWI) * RPI + lane / CH;
+      const int src = v * 32 + row;
+      const uint64_t ra = ((uint64_t)(uint32_t)__shfl(hi, src, 64) << 32) | (uint32_t)__shfl(lo, src, 64);
+      dma16(dst + q * 64, ra + (uint64_t)(16 * ((lane % CH) ^ Swz<D>::at(row))));
+    }
+    return mask;
+  }
+};
+
+// The same where a tile lies within one page (pages of 32 rows or more): the
+// wave's rows have one base, and a load instruction costs one select.
+template <int D, int WR, int WK>
+struct PageLoads {
+  static constexpr int KT = 32, CH = D / 8, RPI = 64 / CH, ROWI = KT / RPI, NI = 2 * ROWI / WR;
+  uint64_t kbase, vbase;
+  int64_t kpage, vpage, krow, vrow;
+  const int32_t* trow;
+  uint32_t off[NI];  // lane offsets of the wave's instructions
+  int key0, k1, last_key, page_shift, num_pages, wr, lane;
+  // tile `next`, as begin() found it
+  uint64_t kb, vb;
+  bool ok;
+  __device__ __forceinline__ PageLoads(const TreeParams& p, int b, int g, int k0, int k1_, int wr_, int wk, int lane_)
+      : kbase((uint64_t)(uintptr_t)p.k + (uint64_t)(2 * g * p.k_sh)), vbase((uint64_t)(uintptr_t)p.v + (uint64_t)(2 * g * p.v_sh)),
+        kpage(2 * p.k_sb), vpage(2 * p.v_sb), krow(2 * p.k_ss), vrow(2 * p.v_ss), trow(p.block_table + b * p.bt_sb),
+        key0(k0 + wk * KT), k1(k1_), last_key(p.cap - 1), page_shift(p.page_shift), num_pages(p.num_pages), wr(wr_),
+        lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int q = wr * NI + i, v = q >= ROWI ? 1 : 0, row = (q - v * ROWI) * RPI + lane / CH;
+      off[i] = (uint32_t)(row * (int)(v ? vrow : krow)) + 16u * (uint32_t)((lane % CH) ^ Swz<D>::at(row));
+    }
+  }
+  // page id of tile j to ring slot dst (every lane the same one)
+  __device__ __forceinline__ void fetch_page(int j, int* dst) const {
+    dma4(dst, (uint64_t)(uintptr_t)(trow + (min(key0 + j * WK * KT, last_key) >> page_shift)), 0u);
+  }
+  // tile j with its page id; returns the mask of rows that are there
+  __device__ __forceinline__ uint32_t begin(int j, int pg) {
+    const int s = key0 + j * WK * KT, n = k1 - s, in = s & ((1 << page_shift) - 1);
+    ok = n > 0 && pg >= 0 && pg < num_pages;
+    const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+    kb = ok ? kbase + (uint64_t)(pg * kpage + in * krow) : zero;
+    vb = ok ? vbase + (uint64_t)(pg * vpage + in * vrow) : zero;
+    return !ok ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+  }
+  __device__ __forceinline__ void issue(int i, u32x4* dst) const {
+    const int q = wr * NI + i;
+    dma16(dst + q * 64, q >= ROWI ? vb : kb, ok ? off[i] : 16u * (uint32_t)lane);
+  }
+};
+
+// Bits of the 4 keys from `key` of a tile: there, and context or a node that the
+// row with tree mask tm sees (past: the tile's first key minus the context's length).
+template <bool TAIL>
+__device__ __forceinline__ uint32_t seen4(uint32_t mask, uint64_t tm, int key, int past) {
+  uint32_t seen = mask >> key;
+  if constexpr (TAIL) {
+    const int node = past + key, back = min(max(-node, 0), 4);
+    const uint32_t drafted = node > 63 ? 0u : (uint32_t)(tm >> (max(node, 0) & 63));
+    seen &= (drafted << back) | ((1u << back) - 1u);
+  }
+  return seen;
+}
+
+// Drafted rows of a V tile that hold infinities or NaN, as bits; they are
+// cleared in LDS (0 times them would reach rows that do not see them) and
+// added by add_bad_rows to the rows that do.
+template <int D, int WR>
+__device__ __forceinline__ uint32_t bad_rows(u32x4* vt, int base, int ctx, int wr, int lane) {
+  constexpr int KT = 32, CH = D / 8;
+  uint32_t x = 0, bad = 0;
+#pragma unroll
+  for (int c = 0; c < CH / 2; ++c) {
+    const u32x4 w = vt[(lane >> 1) * CH + (lane & 1) * (CH / 2) + c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x |= (w[e] & 0x7f80u) == 0x7f80u;
+      x |= (w[e] & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  uint64_t rows2 = __ballot(x != 0 && base + (lane >> 1) >= ctx);
+  for (; rows2 != 0; rows2 &= rows2 - 1) bad |= 1u << (__builtin_ctzll(rows2) >> 1);
+  if constexpr (WR > 1) wg_barrier();
+  if (bad != 0 && wr == 0) {
+    for (int i = lane; i < KT * CH; i += 64)
+      if ((bad >> (i / CH)) & 1) vt[i] = u32x4{0, 0, 0, 0};
+  }
+  if constexpr (WR > 1) wg_barrier();
+  return bad;
+}
+template <int D, int NG, class Add>
+__device__ __forceinline__ void add_bad_rows(const TreeParams& p, int b, int g, int base, uint32_t bad,
+                                             const bf16x8 (&pb)[NG], int lt, int hq, Add add) {
+  for (; bad != 0; bad &= bad - 1) {
+    const int key = __builtin_ctz(bad), i = 4 * (key >> 4) + (key & 3);
+    const int64_t vo = key_row(p, b, base + key, p.v_sb, p.v_ss);
+    if (vo < 0) continue;
+    const bf16* v = reinterpret_cast<const bf16*>(p.v) + vo + g * p.v_sh + 4 * hq;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const u32x4 w = __builtin_bit_cast(u32x4, pb[n]);
+      const uint32_t word = i < 2 ? w[0] : i < 4 ? w[1] : i < 6 ? w[2] : w[3];
+      const float e = __shfl(__uint_as_float(i & 1 ? word & 0xffff0000u : word << 16), lt + 16 * ((key & 15) >> 2), 64);
+#pragma unroll
+      for (int ot = 0; ot < D / 16; ++ot) {
+        const bf16x4 x = *reinterpret_cast<const bf16x4*>(v + 16 * ot);
+        // (rows that do not see the key keep its infinities out)
+        const f32x4 y = {e * (float)x[0], e * (float)x[1], e * (float)x[2], e * (float)x[3]};
+        add(n, ot, e != 0.f ? y : f32x4{});
+      }
+    }
+  }
+}
+
+// The wave rows' sums joined in halves through LDS, and the results.
+template <int D, int NG, int WR, int WK>
+__device__ __forceinline__ void finish_rows(const TreeParams& p, const WorkItem& it, int row0, u32x4* s_kv, float* s_ml,
+                                            f32x4 (&oacc)[NG][D / 16], float (&m_used)[NG], float (&l_part)[NG], int wave,
+                                            int lane) {
+  constexpr int OT = D / 16, WROWS = 16 * NG;
+  const int wr = wave % WR, wk = wave / WR, lt = lane & 15, hq = lane >> 4;
+  const int b = it.b, g = it.g, R = p.T * p.G;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    l_part[n] += __shfl_xor(l_part[n], 16, 64);
+    l_part[n] = xor32_sum(l_part[n]);
+  }
+#pragma unroll
+  for (int half = WK / 2; half > 0; half >>= 1) {
+    wg_barrier();
+    f32x4* mine = reinterpret_cast<f32x4*>(s_kv) + (size_t)((wk % half) * WR + wr) * (NG * OT * 64);
+    if (wk >= half && wk < 2 * half) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+#pragma unroll
+        for (int ot = 0; ot < OT; ++ot) mine[(n * OT + ot) * 64 + lane] = oacc[n][ot];
+        if (hq == 0) {
+          s_ml[(2 * wave + 0) * WROWS + 16 * n + lt] = m_used[n];
+          s_ml[(2 * wave + 1) * WROWS + 16 * n + lt] = l_part[n];
+        }
+      }
+    }
+    wg_barrier();
+    if (wk < half) {
+      const int other = wave + half * WR;
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const float m2 = s_ml[(2 * other + 0) * WROWS + 16 * n + lt], l2 = s_ml[(2 * other + 1) * WROWS + 16 * n + lt];
+        const float m = fmaxf(m_used[n], m2);
+        // (a row without a finite maximum has sums that are zero or NaN)
+        const float a1 = m_used[n] == kNegInf ? 1.f : exp2f(m_used[n] - m), a2 = m2 == kNegInf ? 1.f : exp2f(m2 - m);
+        l_part[n] = l_part[n] * a1 + l2 * a2;
+#pragma unroll
+        for (int ot = 0; ot < OT; ++ot) oacc[n][ot] = oacc[n][ot] * a1 + mine[(n * OT + ot) * 64 + lane] * a2;
+        m_used[n] = m;
+      }
+    }
+  }
+  if (wk != 0) return;
+
+  // ---- results: lane holds row lt, dims 16 ot + 4 hq + e ------------------------------
+  const int64_t pr = (int64_t)it.slot * p.T * p.Hq;
+  const bool partial = it.partial;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int r = row0 + wr * WROWS + 16 * n + lt;
+    if (r >= R) continue;
+    const RowOut ro = row_out(p, g, r);
+    const float m = m_used[n], l = l_part[n];
+    float f, lse;
+    if (partial) {
+      f = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+      lse = l > 0.f ? lse2_of(m, l) : l == 0.f ? kNegInf : l;
+      if (hq == 0) p.part_lse[pr + ro.r] = lse;
+    } else {
+      f = finish_row(p, ro.h, ro.t < it.nodes, m, l, lse);
+      if (hq == 0) p.lse[b * p.l_sb + ro.t * p.l_ss + ro.h * p.l_sh] = lse;
+    }
+#pragma unroll
+    for (int ot = 0; ot < OT; ++ot) {
+      const f32x4 of = oacc[n][ot] * f, o = f == 0.f ? f32x4{} : of;
+      if (partial) {
+        *reinterpret_cast<f32x4*>(p.part_o + (pr + ro.r) * D + 16 * ot + 4 * hq) = o;
+      } else {
+        const bf16x4 o4 = {(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + ro.t * p.o_ss + ro.h * p.o_sh + 16 * ot +
+                                   4 * hq) = o4;
+      }
+    }
+  }
+}
+
 template <int D, int NG, int WR, int WK, int PD>
-__global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p) {
+__global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(TreeParams p) {
   using M = Mfma<16>;
   typedef M::acc_t acc_t;
   static_assert(NG == 4 || WR == 1, "whole waves of rows");
@@ -363,25 +665,10 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
   const int wr = wave % WR, wk = wave / WR;
   const int lt = lane & 15, hq = lane >> 4;
 
-  // ---- work item: the row blocks of one range and kv head on one XCD ------------
-  int wi = blockIdx.x, rb;
-  const int nitems = gridDim.x / p.nrb;
-  if (nitems % 8 == 0) {
-    const int x = wi % 8, r = wi / 8;
-    rb = r % p.nrb;
-    wi = (r / p.nrb) * 8 + x;
-  } else {
-    rb = wi % p.nrb;
-    wi /= p.nrb;
-  }
-  const int g = wi % p.Hkv, slot = wi / p.Hkv;
-  const Slot sl = find_slot<false>(p, slot);
-  if (sl.b < 0) return;
-  const int b = __builtin_amdgcn_readfirstlane(sl.b);
-  const int k0 = __builtin_amdgcn_readfirstlane(sl.k0), k1 = __builtin_amdgcn_readfirstlane(sl.k1);
-  const SeqLens len = seq_lens(p, b);
-  const int ctx = __builtin_amdgcn_readfirstlane(len.ctx), nodes = __builtin_amdgcn_readfirstlane(len.nodes);
-  const int R = p.T * p.G, row0 = rb * WR * WROWS;
+  WorkItem it;
+  if (!work_item(p, it)) return;
+  const int b = it.b, g = it.g, k0 = it.k0, k1 = it.k1, ctx = it.ctx;
+  const int R = p.T * p.G, row0 = it.rb * WR * WROWS;
   const int niter = (k1 - k0 + WK * KT - 1) / (WK * KT);
 
   // ---- rows: Q^T operands (lane: row 16 n + lt, dims 32 s + 8 hq ..), tree masks ----
@@ -402,47 +689,16 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
     s_mask[i] = r < R ? (uint64_t)p.tree_mask[b * p.tm_sb + (r / p.G) * p.tm_ss] : 0;
   }
 
-  // ---- loads -------------------------------------------------------------------------
-  // lanes 0..31 hold the K row addresses of a tile, lanes 32..63 the V rows'
-  const bool vside = lane >= 32;
-  const uint64_t side_base = vside ? (uint64_t)(uintptr_t)p.v + (uint64_t)(2 * g * p.v_sh)
-                                   : (uint64_t)(uintptr_t)p.k + (uint64_t)(2 * g * p.k_sh);
-  const int64_t page_bytes = 2 * (vside ? p.v_sb : p.k_sb), row_bytes = 2 * (vside ? p.v_ss : p.k_ss);
-  const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
-  const int32_t* trow = p.block_table + b * p.bt_sb;
-  const int last_key = p.cap - 1;
-  auto key_of = [&](int j) { return k0 + (j * WK + wk) * KT + (lane & 31); };
-  auto page_addr = [&](int j) {  // (past the range: any entry, not used)
-    return (uint64_t)(uintptr_t)(trow + (min(key_of(j), last_key) >> p.page_shift));
-  };
-  // rows of tile j with page ids pg into stage st; returns the mask of rows that are there
-  auto load_tile = [&](int j, int pg, int st) -> uint32_t {
-    const int s = key_of(j);
-    const bool ok = s < k1 && pg >= 0 && pg < p.num_pages;
-    const uint64_t a = ok ? side_base + (uint64_t)((int64_t)pg * page_bytes + (int64_t)(s & ((1 << p.page_shift) - 1)) * row_bytes)
-                          : zero;
-    const uint32_t mask = (uint32_t)__ballot(ok);
-    const int lo = (int)(uint32_t)a, hi = (int)(uint32_t)(a >> 32);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int q = wr * NI + i, v = q >= ROWI ? 1 : 0;
-      const int row = (q - v * ROWI) * RPI + lane / CH;
-      const int src = v * 32 + row;
-      const uint64_t ra = ((uint64_t)(uint32_t)__shfl(hi, src, 64) << 32) | (uint32_t)__shfl(lo, src, 64);
-      dma16(&s_kv[(st * WK + wk) * TILE + q * 64], ra + (uint64_t)(16 * ((lane % CH) ^ Swz<D>::at(row))));
-    }
-    return mask;
-  };
-
+  TileLoads<D, WR, WK> ld(p, b, g, k0, k1, wr, wk, lane);
   uint32_t vm[NS];  // rows that are there, of tiles j, j + 1, ..
   {
     int pg[2 * PD];
 #pragma unroll
-    for (int j = 0; j < 2 * PD; ++j) pg[j] = *reinterpret_cast<const int32_t*>(page_addr(j));
+    for (int j = 0; j < 2 * PD; ++j) pg[j] = *reinterpret_cast<const int32_t*>(ld.page_addr(j));
 #pragma unroll
     for (int j = PD; j < 2 * PD; ++j) s_page[wave][(j % NS) * 64 + lane] = pg[j];
 #pragma unroll
-    for (int j = 0; j < PD; ++j) vm[j] = load_tile(j, pg[j], j);
+    for (int j = 0; j < PD; ++j) vm[j] = ld.load(j, pg[j], &s_kv[(j * WK + wk) * TILE]);
   }
   wait_vm<(PD - 1) * NI>();  // tile 0 (its page ids are not in the loop's count yet)
   wg_barrier();              // the masks are staged
@@ -464,46 +720,23 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
   }
 
   int st = 0, st_new = PD;  // stage of tile j, of tile j + PD
-  for (int j = 0; j < niter; ++j) {
+  auto step = [&](int j, auto with_drafts) {
+    constexpr bool TAIL = decltype(with_drafts)::value;
     wait_vm<(PD - 1) * (NI + 1)>();  // tile j and the page ids of tile j + PD have landed
     if constexpr (WR > 1) asm volatile("s_barrier" ::: "memory");  // ... for all its waves; stage st_new is read
     {
       const int pg = s_page[wave][st_new * 64 + lane];
       // (page ring: tile j + 2 PD takes the place of tile j + PD - 1, read at j - 1)
       const int ring = st_new == 0 ? NS - 1 : st_new - 1;
-      dma4(&s_page[wave][ring * 64], page_addr(j + 2 * PD));
-      vm[PD] = load_tile(j + PD, pg, st_new);
+      dma4(&s_page[wave][ring * 64], ld.page_addr(j + 2 * PD));
+      vm[PD] = ld.load(j + PD, pg, &s_kv[(st_new * WK + wk) * TILE]);
     }
-    const u32x4* kt = &s_kv[(st * WK + wk) * TILE];
-    const u32x4* vt = kt + KT * CH;
+    u32x4* kt = &s_kv[(st * WK + wk) * TILE];
+    u32x4* vt = kt + KT * CH;
     const int base = k0 + (j * WK + wk) * KT;
     const uint32_t mask = vm[0];
-    // drafted rows in this step's tiles (any of the workgroup's)
-    const bool tail = k0 + (j + 1) * WK * KT > ctx;
     uint32_t bad = 0;  // drafted rows whose V holds infinities or NaN: out of the product, added by hand
-    if (tail) {
-      uint32_t x = 0;
-#pragma unroll
-      for (int c = 0; c < CH / 2; ++c) {
-        const u32x4 w = vt[(lane >> 1) * CH + (lane & 1) * (CH / 2) + c];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x |= (w[e] & 0x7f80u) == 0x7f80u;
-          x |= (w[e] & 0x7f800000u) == 0x7f800000u;
-        }
-      }
-      const uint64_t rows2 = __ballot(x != 0 && base + (lane >> 1) >= ctx);
-      // (bit r: row r)
-      const uint64_t any2 = rows2 | (rows2 >> 1);
-      for (int r = 0; r < 32; ++r) bad |= (uint32_t)((any2 >> (2 * r)) & 1) << r;
-      if constexpr (WR > 1) wg_barrier();
-      if (bad != 0 && wr == 0) {
-        for (int i = lane; i < KT * CH; i += 64)
-          if ((bad >> (i / CH)) & 1) const_cast<u32x4*>(vt)[i] = u32x4{0, 0, 0, 0};
-      }
-      if constexpr (WR > 1) wg_barrier();
-    }
-    const bool plain = mask == 0xffffffffu && !tail;
+    if constexpr (TAIL) bad = bad_rows<D, WR>(vt, base, ctx, wr, lane);
 
     // by 16 keys (half the scores in registers): S^T, then its softmax; a lane
     // holds keys 16 mt + 4 hq + e of its row
@@ -517,15 +750,10 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
 #pragma unroll
         for (int n = 0; n < NG; ++n) sacc[n] = M::mma(kf, qb[n][s], s == 0 ? acc_t{} : sacc[n]);
       }
-      if (!plain) {
-        // bits of the lane's 4 keys: there, and context or a node the row sees
-        const int key = 16 * mt + 4 * hq, node = base + key - ctx, back = min(max(-node, 0), 4);
-        const uint32_t there = mask >> key;
+      if (TAIL || mask != 0xffffffffu) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const uint64_t tm = s_mask[wr * WROWS + 16 * n + lt];
-          const uint32_t drafted = node > 63 ? 0u : (uint32_t)(tm >> (max(node, 0) & 63));
-          const uint32_t seen = there & ((drafted << back) | ((1u << back) - 1u));
+          const uint32_t seen = seen4<TAIL>(mask, TAIL ? s_mask[wr * WROWS + 16 * n + lt] : 0, 16 * mt + 4 * hq, base - ctx);
           const float x0 = seen & 1u ? sacc[n][0] : kNegInf, x1 = seen & 2u ? sacc[n][1] : kNegInf;
           const float x2 = seen & 4u ? sacc[n][2] : kNegInf, x3 = seen & 8u ? sacc[n][3] : kNegInf;
           sacc[n] = acc_t{x0, x1, x2, x3};
@@ -562,21 +790,6 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
           pb[n][4 * mt + i] = (bf16)ex[i];
         }
         l_part[n] += (ex[0] + ex[1]) + (ex[2] + ex[3]);
-        for (uint32_t left = bad & (0xffffu << (16 * mt)); left != 0; left &= left - 1) {
-          const int key = __builtin_ctz(left);
-          float e = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e = (key & 3) == i ? ex[i] : e;
-          e = __shfl(e, lt + 16 * ((key & 15) >> 2), 64);
-          const int64_t vo = key_row(p, b, base + key, p.v_sb, p.v_ss);
-          if (vo < 0) continue;
-          const bf16* v = reinterpret_cast<const bf16*>(p.v) + vo + g * p.v_sh + 4 * hq;
-#pragma unroll
-          for (int ot = 0; ot < OT; ++ot)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (e != 0.f) oacc[n][ot][i] = fmaf(e, (float)v[16 * ot + i], oacc[n][ot][i]);
-        }
       }
     }
 
@@ -589,136 +802,382 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void tree_mfma_kernel(TreeParams p
 #pragma unroll
       for (int n = 0; n < NG; ++n) oacc[n][ot] = M::mma(a, pb[n], oacc[n][ot]);
     }
+    if constexpr (TAIL)
+      add_bad_rows<D, NG>(p, b, g, base, bad, pb, lt, hq, [&](int n, int ot, const acc_t& y) { oacc[n][ot] += y; });
 #pragma unroll
     for (int i = 0; i < PD; ++i) vm[i] = vm[i + 1];
     st = st + 1 == NS ? 0 : st + 1;
     st_new = st_new + 1 == NS ? 0 : st_new + 1;
-  }
+  };
+  // steps without a drafted row in any of the workgroup's tiles, then the others
+  const int whole = min(max(ctx - k0, 0) / (WK * KT), niter);
+  int j = 0;
+  for (; j < whole; ++j) step(j, std::false_type{});
+  for (; j < niter; ++j) step(j, std::true_type{});
   wait_vm<0>();  // the loads past the range have landed before LDS is used for anything else
 
-  // ---- row sums; the wave rows' results joined in halves ----------------------------
+  finish_rows<D, NG, WR, WK>(p, it, row0, s_kv, &s_ml[0][0][0], oacc, m_used, l_part, wave, lane);
+}
+
+// ---- more than 64 rows: two waves a SIMD, scores a tile ahead ---------------------
+// 32 rows a wave, and each wave overlaps its own work too: a step issues the
+// products S^T of tile j + 1 and O^T of tile j, and between them, one score
+// after every second product or so, the softmax of tile j, which depends on
+// neither.  Sums and Q stay in AGPRs (inline asm: the compiler would copy Q to
+// VGPRs for every product); sched_barrier keeps the order that is written here.
+// 16 sequences of 4K-32K keys, 256 rows (one of 128K keys, 8 kv heads): 122 (190) us.
+// 64 rows a wave read half as much from LDS and took 132 (198) us with one wave a
+// SIMD, 256 (406) us with two, which spill; without the overlap 163 (248) us.
+template <int D, int NG, int WR, int WK, int NS, bool PAGE>
+__global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_pipe_kernel(TreeParams p) {
+  using M = Mfma16A;
+  typedef M::acc_t acc_t;
+  constexpr int NW = WR * WK, KT = 32, CH = D / 8, KS = D / 32, OT = D / 16;
+  constexpr int RPI = 64 / CH, ROWI = KT / RPI, NI = 2 * ROWI / WR;
+  constexpr int TILE = 2 * KT * CH, WROWS = 16 * NG, RING = 4;  // NS stages of a K and V tile
+  constexpr int MERGE = WK > 1 ? (WK / 2) * WR * NG * OT * 64 : 0;
+  constexpr int SLOTS = NS * WK * TILE > MERGE ? NS * WK * TILE : MERGE;
+  static_assert(NG % 2 == 0, "drain_v4");
+  static_assert(NS >= 3 && NS <= RING + 1, "page ids of NS - 1 tiles are held");
+
+  __shared__ u32x4 s_kv[SLOTS];
+  __shared__ int s_page[NW][(RING + 1) * 64];  // (and one slot for ids that are not used)
+  __shared__ uint64_t s_mask[WR * WROWS];
+  __shared__ float s_ml[NW][2][WROWS];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  const int lt = lane & 15, hq = lane >> 4;
+
+  WorkItem it;
+  if (!work_item(p, it)) return;
+  const int b = it.b, g = it.g, k0 = it.k0, k1 = it.k1, ctx = it.ctx;
+  const int R = p.T * p.G, row0 = it.rb * WR * WROWS;
+  const int niter = (k1 - k0 + WK * KT - 1) / (WK * KT);
+
+  bf16x8 qb[NG][KS];
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
-    l_part[n] += __shfl_xor(l_part[n], 16, 64);
-    l_part[n] = xor32_sum(l_part[n]);
-  }
+    const int r = row0 + wr * WROWS + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
+    const bool live = r < R;
+    const bf16* q = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
 #pragma unroll
-  for (int half = WK / 2; half > 0; half >>= 1) {
-    wg_barrier();
-    f32x4* mine = reinterpret_cast<f32x4*>(s_kv) + (size_t)((wk % half) * WR + wr) * (NG * OT * 64);
-    if (wk >= half && wk < 2 * half) {
+    for (int s = 0; s < KS; ++s) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(q + 32 * s);
+      qb[n][s] = M::to_agpr(live ? x : bf16x8{});
+    }
+  }
+  for (int i = tid; i < WR * WROWS; i += 64 * NW) {
+    const int r = row0 + i;
+    s_mask[i] = r < R ? (uint64_t)p.tree_mask[b * p.tm_sb + (r / p.G) * p.tm_ss] : 0;
+  }
+
+  typedef typename std::conditional<PAGE, PageLoads<D, WR, WK>, TileLoads<D, WR, WK>>::type Loads;
+  Loads ld(p, b, g, k0, k1, wr, wk, lane);
+  // Loads go out in groups, tile t's page id for tile t + NS - 2 before its own rows;
+  // group t goes out in step t - NS (0 .. NS - 1 here).
+  uint32_t vm[NS + 1];  // rows that are there, of tiles j, j + 1, ..
+  auto group_page = [&](int t) {
+    int* ring = &s_page[wave][(t < 2 ? RING : (t + NS - 2) % RING) * 64];
+    if constexpr (PAGE) ld.fetch_page(t + NS - 2, ring);
+    else dma4(ring, ld.page_addr(t + NS - 2));
+  };
+  {
+    int pg[NS];
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      if constexpr (PAGE) pg[t] = ld.trow[min(ld.key0 + t * WK * KT, ld.last_key) >> ld.page_shift];
+      else pg[t] = *reinterpret_cast<const int32_t*>(ld.page_addr(t));
+    }
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      u32x4* dst = &s_kv[(t * WK + wk) * TILE];
+      group_page(t);
+      if constexpr (PAGE) {
+        vm[t] = ld.begin(t, __builtin_amdgcn_readfirstlane(pg[t]));
+#pragma unroll
+        for (int i = 0; i < NI; ++i) ld.issue(i, dst);
+      } else {
+        vm[t] = ld.load(t, pg[t], dst);
+      }
+    }
+    vm[NS] = 0;
+  }
+  wait_vm<(NS - 2) * (NI + 1)>();  // tiles 0 and 1
+  wg_barrier();
+
+  const uint32_t pitch = CH * 16;
+  const uint32_t ka = (uint32_t)lt * pitch + (uint32_t)((hq ^ Swz<D>::at(lt)) << 4);
+  const int rr = lt >> 2, cc = lt & 3, vr = 4 * hq + rr;
+  const uint32_t va = (uint32_t)vr * pitch + (uint32_t)(((cc >> 1) ^ Swz<D>::at(vr)) << 4) + (uint32_t)(cc & 1) * 8u;
+
+  acc_t oacc[NG][OT];
+  float m_used[NG], l_part[NG];
+  float thr[NG], moff[NG];  // the raw score that moves the maximum, and -maximum (0 while there is none)
+  const float inv_scale = 1.f / p.scale_log2;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    m_used[n] = thr[n] = kNegInf;
+    l_part[n] = moff[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < OT; ++i) {
+      acc_t z = acc_t{};
+      asm volatile("" : "+a"(z));
+      oacc[n][i] = z;
+    }
+  }
+
+  // S^T product i of a tile: contraction step i / 2 NG, keys 16 (i / NG % 2) .., rows 16 (i % NG) ..
+  constexpr int NSM = 2 * NG * KS, NPV = NG * OT, NM = NSM + NPV, NF = 2 * KS;
+  auto read_k = [&](const u32x4* kt, int f) {
+    return lds_read_b128(kt, (ka ^ (uint32_t)(64 * (f >> 1))) + (uint32_t)(16 * (f & 1)) * pitch);
+  };
+  acc_t sca[NG][2], scb[NG][2];
+  float tmax[NG];
+  {
+    const u32x4* kt = &s_kv[wk * TILE];
+    bf16x8 prev_k = {};
+    each<NSM>([&](auto ic) {
+      constexpr int i = decltype(ic)::value, s = i / (2 * NG), mt = (i / NG) & 1, n = i % NG;
+      const bf16x8 kf = read_k(kt, i / NG);
+      if constexpr (s == 0) M::mma_v0_ba(kf, qb[n][s], sca[n][mt], prev_k);
+      else M::mma_v_ba(kf, qb[n][s], sca[n][mt], prev_k);
+      prev_k = kf;
+    });
+    M::tail1(prev_k);
+#pragma unroll
+    for (int n = 0; n < NG; n += 2) M::drain_v4(sca[n][0], sca[n][1], sca[n + 1][0], sca[n + 1][1]);
+  }
+  constexpr int PK = NF < 3 ? NF : 3;  // K operands read ahead
+  bf16x8 kf[4];                        // the first of tile j + 1 at the start of step j
+#pragma unroll
+  for (int f = 0; f < PK; ++f) kf[f] = read_k(&s_kv[((1 % NS) * WK + wk) * TILE], f);
+  auto max_of = [&](const acc_t (&sc)[2]) {
+    return max_raw(max3_raw(max3_raw(sc[0][0], sc[0][1], sc[0][2]), sc[0][3], sc[1][0]), max3_raw(sc[1][1], sc[1][2], sc[1][3]));
+  };
+#pragma unroll
+  for (int n = 0; n < NG; ++n) tmax[n] = max_of(sca[n]);
+
+  int st = 0;
+  auto step = [&](int j, acc_t (&cur)[NG][2], acc_t (&nxt)[NG][2], auto with_drafts) {
+    constexpr bool TAIL = decltype(with_drafts)::value;
+    const int st1 = st + 1 == NS ? 0 : st + 1, st2 = st1 + 1 == NS ? 0 : st1 + 1;
+    u32x4* vt = &s_kv[(st * WK + wk) * TILE] + KT * CH;
+    const u32x4* kn = &s_kv[(st1 * WK + wk) * TILE];
+    const u32x4* kn2 = &s_kv[(st2 * WK + wk) * TILE];
+    u32x4* dst = &s_kv[(st * WK + wk) * TILE];
+    int pg = 0;
+    const int base = k0 + (j * WK + wk) * KT;
+    const uint32_t mask = vm[0];
+    uint32_t bad = 0;  // drafted rows whose V holds infinities or NaN: out of the product, added by hand
+    if constexpr (TAIL) bad = bad_rows<D, WR>(vt, base, ctx, wr, lane);
+    if (TAIL || mask != 0xffffffffu) {
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
+        const uint64_t tm = TAIL ? s_mask[wr * WROWS + 16 * n + lt] : 0;
 #pragma unroll
-        for (int ot = 0; ot < OT; ++ot) mine[(n * OT + ot) * 64 + lane] = oacc[n][ot];
-        if (hq == 0) {
-          s_ml[wave][0][16 * n + lt] = m_used[n];
-          s_ml[wave][1][16 * n + lt] = l_part[n];
+        for (int mt = 0; mt < 2; ++mt) {
+          const uint32_t seen = seen4<TAIL>(mask, tm, 16 * mt + 4 * hq, base - ctx);
+          const float x0 = seen & 1u ? cur[n][mt][0] : kNegInf, x1 = seen & 2u ? cur[n][mt][1] : kNegInf;
+          const float x2 = seen & 4u ? cur[n][mt][2] : kNegInf, x3 = seen & 8u ? cur[n][mt][3] : kNegInf;
+          cur[n][mt] = acc_t{x0, x1, x2, x3};
+        }
+        tmax[n] = max_of(cur[n]);
+      }
+    }
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) over |= tmax[n] > thr[n];
+    if (__any(over)) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const float m_new = fmaxf(m_used[n], xor32_max(xor16_max(tmax[n])) * p.scale_log2);
+        const float alpha = m_new == kNegInf ? 1.f : exp2f(m_used[n] - m_new);
+        l_part[n] *= alpha;
+        m_used[n] = m_new;
+        thr[n] = (m_new + 8.f) * inv_scale;
+        moff[n] = m_new == kNegInf ? 0.f : -m_new;
+        drain_all(oacc[n]);
+#pragma unroll
+        for (int i = 0; i < OT; ++i) {
+          acc_t x = oacc[n][i] * alpha;
+          asm volatile("" : "+a"(x));
+          oacc[n][i] = x;
         }
       }
     }
-    wg_barrier();
-    if (wk < half) {
-      const int other = wave + half * WR;
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        const float m2 = s_ml[other][0][16 * n + lt], l2 = s_ml[other][1][16 * n + lt];
-        const float m = fmaxf(m_used[n], m2);
-        const float a1 = m_used[n] == kNegInf ? 0.f : exp2f(m_used[n] - m), a2 = m2 == kNegInf ? 0.f : exp2f(m2 - m);
-        // (a row without a finite maximum has sums that are zero or NaN)
-        l_part[n] = (m_used[n] == kNegInf ? l_part[n] : l_part[n] * a1) + (m2 == kNegInf ? l2 : l2 * a2);
-#pragma unroll
-        for (int ot = 0; ot < OT; ++ot) {
-          const f32x4 o2 = mine[(n * OT + ot) * 64 + lane];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x1 = m_used[n] == kNegInf ? oacc[n][ot][i] : oacc[n][ot][i] * a1;
-            const float x2 = m2 == kNegInf ? o2[i] : o2[i] * a2;
-            oacc[n][ot][i] = x1 + x2;
+
+    bf16x8 vf[OT], pb[NG];
+    uint32_t pw[NG][4];
+    float ex[2] = {0.f, 0.f}, arg = fmaf(cur[0][0][0], p.scale_log2, moff[0]);
+    bf16x8 pa = {}, pp = {};
+    each<NM>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (i < NSM) {
+        constexpr int f = i / NG, s = f >> 1, mt = f & 1, n = i % NG;
+        if constexpr (s == 0) M::mma_v0_ba(kf[f & 3], qb[n][s], nxt[n][mt], pa);
+        else M::mma_v_ba(kf[f & 3], qb[n][s], nxt[n][mt], pa);
+        pa = kf[f & 3];
+        if constexpr (n == 1 && f + 3 < NF) kf[(f + 3) & 3] = read_k(kn, f + 3);
+        if constexpr (i % (NSM / OT) == (NSM / OT) / 2) {
+          constexpr int o = i / (NSM / OT);
+          const uint32_t off = va ^ (uint32_t)(32 * o);
+          const bf16x4 lo = lds_read_tr16(vt, off), hi = lds_read_tr16(vt, off + 16u * pitch);
+          vf[o] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+      } else {
+        constexpr int n = (i - NSM) / OT, o = (i - NSM) % OT;
+        if constexpr (o == 0) pb[n] = __builtin_bit_cast(bf16x8, u32x4{pw[n][0], pw[n][1], pw[n][2], pw[n][3]});
+        M::template mma<o == 0>(vf[o], pb[n], oacc[n][o], pa, pp);
+        pa = vf[o];
+        pp = pb[n];
+      }
+      // the softmax's scores, evenly over the products before the last row group's
+      constexpr int NE = 8 * NG;
+      each<NE>([&](auto ec) {
+        constexpr int e = decltype(ec)::value, n = e >> 3, k = e & 7;
+        if constexpr (e * (NM - OT) / NE == i) {
+          const float x = __builtin_amdgcn_exp2f(arg);
+          if constexpr (e < NE - 1) {
+            constexpr int n1 = (e + 1) >> 3, k1_ = (e + 1) & 7;
+            arg = fmaf(cur[n1][k1_ >> 2][k1_ & 3], p.scale_log2, moff[n1]);
+          }
+          l_part[n] += x;
+          ex[k & 1] = x;
+          if constexpr (k & 1) {
+            const bf16x2 w = {(bf16)ex[0], (bf16)ex[1]};
+            pw[n][k >> 1] = __builtin_bit_cast(uint32_t, w);
           }
         }
-        m_used[n] = m;
+      });
+      // Once tile j's operands are all in registers: wait for tile j + 2, let the
+      // other waves finish with tile j, then load tile j + NS over it and read
+      // the first K operands of tile j + 2.
+      constexpr int BAR = NM - 20 > NSM ? NM - 20 : NSM;
+      static_assert(BAR + 5 + NI <= NM, "the step's loads fit");
+      if constexpr (i == BAR) {
+        wait_vm<(NS - 3) * (NI + 1)>();
+        if constexpr (WR > 1) asm volatile("s_barrier" ::: "memory");
+        pg = s_page[wave][((j + NS) % RING) * 64 + lane];
       }
+      if constexpr (i > BAR && i - BAR - 1 < PK) kf[i - BAR - 1] = read_k(kn2, i - BAR - 1);
+      if constexpr (i == BAR + 4) {
+        group_page(j + NS);
+        if constexpr (PAGE) vm[NS] = ld.begin(j + NS, __builtin_amdgcn_readfirstlane(pg));
+        else vm[NS] = ld.load(j + NS, pg, dst);
+      }
+      if constexpr (PAGE) {
+        if constexpr (i > BAR + 4 && i - BAR - 5 < NI) ld.issue(i - BAR - 5, dst);
+      }
+      // ... and the next tile's maxima after them
+      if constexpr (i >= NM - OT && (i - (NM - OT)) % (OT / NG) == 0) {
+        constexpr int n = (i - (NM - OT)) / (OT / NG);
+        tmax[n] = max_of(nxt[n]);
+      }
+    });
+    M::tail(pa, pp);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (TAIL) {
+      add_bad_rows<D, NG>(p, b, g, base, bad, pb, lt, hq, [&](int n, int o, const acc_t& y) {
+        M::drain(oacc[n][o]);
+        acc_t x = oacc[n][o] + y;
+        asm volatile("" : "+a"(x));
+        oacc[n][o] = x;
+      });
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) vm[i] = vm[i + 1];
+    st = st1;
+  };
+  // steps without a drafted row in any of the workgroup's tiles, then the others
+  const int whole = min(max(ctx - k0, 0) / (WK * KT), niter);
+  int j = 0;
+  for (; j + 1 < whole; j += 2) {
+    step(j, sca, scb, std::false_type{});
+    step(j + 1, scb, sca, std::false_type{});
+  }
+  for (; j < niter; ++j) {
+    step(j, sca, scb, std::true_type{});
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      sca[n][0] = scb[n][0];
+      sca[n][1] = scb[n][1];
     }
   }
-  if (wk != 0) return;
-
-  // ---- results: lane holds row lt, dims 16 ot + 4 hq + e ------------------------------
-  const int64_t pr = (int64_t)slot * p.T * p.Hq;
-  const bool partial = sl.n > 1;
+  wait_vm<0>();  // the loads past the range have landed before LDS is used for anything else
 #pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    const int r = row0 + wr * WROWS + 16 * n + lt;
-    if (r >= R) continue;
-    const RowOut ro = row_out(p, g, r);
-    const float m = m_used[n], l = l_part[n];
-    float f, lse;
-    if (partial) {
-      f = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-      lse = l > 0.f ? lse2_of(m, l) : l == 0.f ? kNegInf : l;
-      if (hq == 0) p.part_lse[pr + ro.r] = lse;
-    } else {
-      f = finish_row(p, ro.h, ro.t < nodes, m, l, lse);
-      if (hq == 0) p.lse[b * p.l_sb + ro.t * p.l_ss + ro.h * p.l_sh] = lse;
-    }
-#pragma unroll
-    for (int ot = 0; ot < OT; ++ot) {
-      f32x4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = f == 0.f ? 0.f : oacc[n][ot][i] * f;
-      if (partial) {
-        *reinterpret_cast<f32x4*>(p.part_o + (pr + ro.r) * D + 16 * ot + 4 * hq) = o;
-      } else {
-        const bf16x4 o4 = {(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
-        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + ro.t * p.o_ss + ro.h * p.o_sh + 16 * ot +
-                                   4 * hq) = o4;
-      }
-    }
-  }
+  for (int n = 0; n < NG; ++n) drain_all(oacc[n]);
+  finish_rows<D, NG, WR, WK>(p, it, row0, s_kv, &s_ml[0][0][0], oacc, m_used, l_part, wave, lane);
 }
 
 // ---- joining the slots of a sequence -------------------------------------------
-// One wave a row; a slot in which the row sees nothing has LSE -inf.
-template <typename T>
+// One wave a row; LPR lanes hold the row (4 dims each), 64 / LPR slots at a
+// time.  A slot in which the row sees nothing has LSE -inf.
+template <typename T, int LPR>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), per = (int64_t)p.T * p.Hq;
   if (row >= p.B * per) return;
   const int b = (int)(row / per), r = (int)(row % per), h = r % p.Hq, t = r / p.Hq;
-  const Slot sl = find_slot<true>(p, b);
-  if (sl.n <= 1) return;
-  const float* pl = p.part_lse + sl.first * per + r;
-  const float* po = p.part_o + (sl.first * per + r) * p.Dv;
+  const int first = p.seq_slots[2 * b], ns = p.seq_slots[2 * b + 1];
+  if (ns <= 1) return;
+  const float* pl = p.part_lse + first * per + r;
+  const float* po = p.part_o + (first * per + r) * p.Dv;
   const bool live = t < seq_lens(p, b).nodes;
-  float m = kNegInf;
-  bool bad = false;
-  for (int i = lane; i < sl.n; i += 64) {
+  float m = kNegInf, nan = 0.f;
+  for (int i = lane; i < ns; i += 64) {
     const float x = pl[i * per];
-    bad |= x != x;
+    nan += x != x ? x : 0.f;
     m = fmaxf(m, x);
   }
   m = wave_max(m);
-  bad = __any(bad);
+  const float moff = m == kNegInf ? 0.f : m;
   float l = 0.f;
-  for (int i = lane; i < sl.n; i += 64) {
-    const float x = pl[i * per];
-    if (x != kNegInf) l += exp2f(x - m);
-  }
-  l = wave_sum(l);
-  if (bad) l = __builtin_nanf("");
+  for (int i = lane; i < ns; i += 64) l += exp2f(pl[i * per] - moff);
+  l = wave_sum(l + nan);
   float lse;
   const float f = finish_row(p, h, live, m, l, lse);
   if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
   T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
-  for (int d = lane; d < p.Dv; d += 64) {
-    float x = 0.f;
-    if (f != 0.f)
-      for (int i = 0; i < sl.n; ++i) {
-        const float e = pl[i * per];
-        if (e != kNegInf) x = fmaf(exp2f(e - m), po[i * per * p.Dv + d], x);
+  constexpr int NP = 64 / LPR;  // slots at a time
+  const int sub = lane / LPR;
+  for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
+    const int d = d0 + 4 * (lane % LPR);
+    f32x4 x = {};
+    if (f != 0.f) {
+#pragma unroll 4
+      for (int i = sub; i < ns; i += NP) {
+        const float e = exp2f(pl[i * per] - moff);
+        f32x4 v = {};
+        const float* at = po + i * per * p.Dv + d;
+        if (p.Dv % 4 == 0) {
+          if (d < p.Dv) v = *reinterpret_cast<const f32x4*>(at);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = d + k < p.Dv ? at[k] : 0.f;
+        }
+        x += v * e;
       }
-    o[d] = from_f32<T>(f == 0.f ? 0.f : x * f);
+    }
+#pragma unroll
+    for (int s = LPR; s < 64; s <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], s, 64);
+    if (sub == 0)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (d + k < p.Dv) o[d + k] = from_f32<T>(f == 0.f ? 0.f : x[k] * f);
   }
+}
+
+template <typename T>
+void launch_combine(const TreeParams& p, hipStream_t s) {
+  const unsigned grid = (unsigned)(((int64_t)p.B * p.T * p.Hq + 3) / 4);
+  if (p.Dv <= 64) tree_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p);
+  else if (p.Dv <= 128) tree_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p);
+  else tree_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p);
 }
 
 // Kernels by query rows per (sequence, kv head): rows a workgroup, tile keys, waves.
@@ -726,8 +1185,18 @@ enum { kGeneric = 0, kRows16, kRows32, kRows64, kRows128, kRows256 };
 struct KernelShape {
   int rows, tile;
 };
-constexpr KernelShape kShapes[] = {{kGR, kGK}, {16, 128}, {32, 128}, {64, 128}, {128, 128}, {256, 64}};
+constexpr KernelShape kShapes[] = {{kGR, kGK}, {16, 128}, {32, 128}, {64, 128}, {128, 64}, {256, 32}};
 constexpr int kWorkgroups = 256;  // key ranges are cut until about so many workgroups (one a CU) are in flight
+
+template <int D, int NG, int WR, int WK, int NS>
+void launch_pipe(const TreeParams& p, unsigned grid, hipStream_t s) {
+  // (a page's byte offsets fit the loads' 32 bits)
+  const int64_t row = 2 * (p.k_ss > p.v_ss ? p.k_ss : p.v_ss);
+  if (p.page_shift >= 5 && p.k_ss > 0 && p.v_ss > 0 && row < ((int64_t)1 << 25))
+    tree_pipe_kernel<D, NG, WR, WK, NS, true><<<grid, 64 * WR * WK, 0, s>>>(p);
+  else
+    tree_pipe_kernel<D, NG, WR, WK, NS, false><<<grid, 64 * WR * WK, 0, s>>>(p);
+}
 
 template <int D>
 void launch_mfma(const TreeParams& p, int kernel, unsigned grid, hipStream_t s) {
@@ -735,8 +1204,8 @@ void launch_mfma(const TreeParams& p, int kernel, unsigned grid, hipStream_t s) 
     case kRows16: tree_mfma_kernel<D, 1, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
     case kRows32: tree_mfma_kernel<D, 2, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
     case kRows64: tree_mfma_kernel<D, 4, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
-    case kRows128: tree_mfma_kernel<D, 4, 2, 4, 1><<<grid, 512, 0, s>>>(p); break;
-    default: tree_mfma_kernel<D, 4, 4, 2, 2><<<grid, 512, 0, s>>>(p);
+    case kRows128: launch_pipe<D, 2, 4, 2, 4>(p, grid, s); break;
+    default: launch_pipe<D, 2, 8, 1, 5>(p, grid, s);
   }
 }
 
@@ -758,6 +1227,7 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
     const size_t rows = (size_t)pl.slots * p.T * p.Hq;
     pl.part_o_bytes = (rows * p.Dv * sizeof(float) + 255) / 256 * 256;
     pl.part_lse_bytes = (rows * sizeof(float) + 255) / 256 * 256;
+    pl.seq_bytes = (size_t)2 * p.B * sizeof(int32_t);
   }
   return pl;
 }
@@ -766,7 +1236,6 @@ hipError_t launch_tree(const TreeParams& p0, const TreePlan& pl, int dtype, hipS
   TreeParams p = p0;
   p.want = pl.want;
   p.tile = kShapes[pl.kernel].tile;
-  p.min_len = 2 * p.tile;
   p.nrb = (p.T * p.G + pl.rows - 1) / pl.rows;
   const unsigned grid = (unsigned)((int64_t)pl.slots * p.Hkv * p.nrb);
   if (pl.kernel != kGeneric) {
@@ -778,9 +1247,8 @@ hipError_t launch_tree(const TreeParams& p0, const TreePlan& pl, int dtype, hipS
     tree_generic_kernel<bf16><<<grid, 256, 0, s>>>(p);
   }
   if (pl.want > 0) {
-    const unsigned cg = (unsigned)(((int64_t)p.B * p.T * p.Hq + 3) / 4);
-    if (dtype == SFA_DTYPE_F32) tree_combine_kernel<float><<<cg, 256, 0, s>>>(p);
-    else tree_combine_kernel<bf16><<<cg, 256, 0, s>>>(p);
+    if (dtype == SFA_DTYPE_F32) launch_combine<float>(p, s);
+    else launch_combine<bf16>(p, s);
   }
   return hipGetLastError();
 }
