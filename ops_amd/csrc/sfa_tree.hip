@@ -392,11 +392,14 @@ struct WorkItem {
 };
 __device__ __forceinline__ bool work_item(const TreeParams& p, WorkItem& it) {
   int wi = blockIdx.x;
-  const int nitems = gridDim.x / p.nrb;
+  const int nitems = gridDim.x / p.nrb, x = wi % 8;
   if (nitems % 8 == 0) {
-    const int x = wi % 8, r = wi / 8;
-    it.rb = r % p.nrb;
-    wi = (r / p.nrb) * 8 + x;
+    it.rb = (wi / 8) % p.nrb;
+    wi = wi / 8 / p.nrb * 8 + x;
+  } else if ((nitems == 1 || nitems == 2 || nitems == 4) && p.nrb % 8 == 0) {  // an item on 8 / nitems of them
+    const int per = 8 / nitems;
+    it.rb = wi / 8 * per + x % per;
+    wi = x / per;
   } else {
     it.rb = wi % p.nrb;
     wi /= p.nrb;
@@ -1112,6 +1115,367 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_pipe_kernel(Tr
   finish_rows<D, NG, WR, WK>(p, it, row0, s_kv, &s_ml[0][0][0], oacc, m_used, l_part, wave, lane);
 }
 
+// ---- latent rows: d_qk = 576, d_v = 512, V the first 512 dims of K, bf16 ----------
+// One workgroup of 8 waves takes 64 rows of one key range, in tiles of 64
+// keys (72 KB of LDS, two stages), and divides the two products differently:
+//  * S^T = K Q^T: wave (rh, kq) takes 32 rows x 16 keys, its Q in 144 AGPRs; a K
+//    operand read from LDS serves 32 rows;
+//  * P^T goes through LDS (8 KB) in the operand order, and
+//  * O^T = V^T P^T: wave w takes dims 64 w .. 64 w + 63 of all 64 rows (64
+//    accumulators), so each V element is read from LDS once.
+// Per tile LDS moves 356 KB (2785 clocks), the products take 2176 clocks of
+// every SIMD.  The next tile's rows are loaded during S^T, a load after every
+// fourth product.  The running maximum is shared: a row's scores are in four
+// waves, so a wave that finds one past the maximum by 8 (base 2) raises a flag,
+// and all of them move it together after the barrier that publishes P.
+struct MlaTree {
+  static constexpr int kDqk = 576, kDv = 512, kKeys = 64, kSteps = kDqk / 32;
+  static constexpr int kCh = kDv / 8, kCr = (kDqk - kDv) / 8;  // 16-byte chunks of the two parts of a row
+};
+
+__global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
+  typedef MlaTree C;
+  typedef Mfma16A MA;
+  typedef Mfma<16> M;
+  typedef f32x4 acc_t;
+  constexpr int CH = C::kCh, CR = C::kCr, KEYS = C::kKeys, STEPS = C::kSteps, RPW = KEYS / 8;
+
+  __shared__ u32x4 s_k[2][KEYS * CH];  // dims 0 .. 511 (K and V), swizzled as rows of 128
+  __shared__ u32x4 s_r[2][KEYS * CR];  // dims 512 .. 575, as rows of 64
+  __shared__ u32x4 s_p[2 * 64 * 4];  // [32-key half][hq][row] 8 keys
+  __shared__ u32x4 s_q[64 * 4];      // [hq][row] Q's last 32 dims
+  __shared__ u32x4 s_q1[32 * 4];     // [hq][16 rh + lt] the 32 before them, of row group 1
+  __shared__ uint64_t s_mask[64];
+  __shared__ float s_m[64];          // running maxima (base 2)
+  __shared__ float s_x[4][64];       // per key quarter: row maxima, then row sums
+  __shared__ int s_over[2];
+  __shared__ unsigned long long s_bad;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rh = wave & 1, kq = wave >> 1;
+  const int lt = lane & 15, hq = lane >> 4;
+
+  WorkItem it;
+  if (!work_item(p, it)) return;
+  const int b = it.b, g = it.g, k0 = it.k0, k1 = it.k1, ctx = it.ctx;
+  const int R = p.T * p.G, row0 = it.rb * 64;
+  const int ntiles = (k1 - k0 + KEYS - 1) / KEYS;
+
+  // ---- rows ----------------------------------------------------------------------
+  // (Q's last one and a half contraction steps in LDS: 128 AGPRs, and no VGPR to spare)
+  bf16x8 qa[2][16], q16;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int r = row0 + 32 * rh + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
+    const bool live = r < R;
+    const bf16* q = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(q + 32 * s), y = live ? x : bf16x8{};
+      if (s < 16) qa[n][s < 16 ? s : 0] = MA::to_agpr(y);
+      else if (s == 16 && n == 0) q16 = y;
+      else if (s == 16 && kq == 0) s_q1[hq * 32 + 16 * rh + lt] = __builtin_bit_cast(u32x4, y);
+      else if (s == 17 && kq == 0) s_q[hq * 64 + 32 * rh + 16 * n + lt] = __builtin_bit_cast(u32x4, y);
+    }
+  }
+  if (tid < 64) {
+    const int r = row0 + tid;
+    s_mask[tid] = r < R ? (uint64_t)p.tree_mask[b * p.tm_sb + (r / p.G) * p.tm_ss] : 0;
+    s_m[tid] = kNegInf;
+    if (tid < 2) s_over[tid] = 0;
+    if (tid == 2) s_bad = 0;
+  }
+
+  // ---- loads: the wave's 8 rows of a tile, one instruction each for their first
+  // 1024 bytes and one for the last 128 of all; lane l finds the address of row l
+  const uint64_t kbase = (uint64_t)(uintptr_t)p.k + 2 * (int64_t)g * p.k_sh;
+  const int32_t* trow = p.block_table + b * p.bt_sb;
+  const int last_key = p.cap - 1;
+  auto page_of = [&](int j, int ln) { return trow[min(k0 + j * KEYS + ln, last_key) >> p.page_shift]; };
+  auto row_addr = [&](int j, int pg, int ln, bool& ok) {
+    const int s = k0 + j * KEYS + ln;
+    ok = s < k1 && pg >= 0 && pg < p.num_pages;
+    const uint64_t a = kbase + (uint64_t)((int64_t)pg * (2 * p.k_sb) + (int64_t)(s & ((1 << p.page_shift) - 1)) * (2 * p.k_ss));
+    return ok ? a : (uint64_t)(uintptr_t)kZeroRow;
+  };
+  auto load_row = [&](int i, uint64_t ra, u32x4* dst, int ln) {
+    const int row = wave * RPW + i;
+    const uint64_t base = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(ra >> 32), row) << 32) |
+                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)ra, row);
+    dma16(dst + row * CH, base, 16u * (uint32_t)(ln ^ Swz<128>::at(row)));
+  };
+  auto load_tails = [&](uint64_t ra, u32x4* dst, int ln) {
+    const int row = wave * RPW + (ln >> 3);
+    const uint64_t a = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(ra >> 32), row, 64) << 32) |
+                       (uint32_t)__shfl((int)(uint32_t)ra, row, 64);
+    dma16(dst + wave * RPW * CR, a + (uint64_t)(16 * (CH + ((ln & 7) ^ Swz<64>::at(row)))));
+  };
+  uint64_t mask;  // the rows of tile j that are there
+  {
+    bool ok;
+    const uint64_t ra = row_addr(0, page_of(0, lane), lane, ok);
+    mask = __ballot(ok);
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) load_row(i, ra, s_k[0], lane);
+    load_tails(ra, s_r[0], lane);
+  }
+  int pg_next = page_of(1, lane);
+
+  acc_t oacc[4][4];  // [16 dims][16 rows]
+#pragma unroll
+  for (int o = 0; o < 4; ++o)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) oacc[o][n] = acc_t{};
+  float m_used[2] = {kNegInf, kNegInf}, l_part[2] = {0.f, 0.f};
+
+  auto step = [&](int j, auto with_drafts) {
+    constexpr bool TAIL = decltype(with_drafts)::value;
+    const u32x4 *kt = s_k[j & 1], *rt = s_r[j & 1];
+    // (lane constants are formed per tile: held across the loop they spill)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    int lt = ln & 15, hq = ln >> 4;
+    // operand addresses (rows are whole multiples of 128 bytes: a chunk's bits
+    // can be flipped in place)
+    const int krow = 16 * kq + lt, fr = Swz<128>::at(lt);
+    const uint32_t ka = (uint32_t)(krow * CH + (hq ^ fr)) * 16u;
+    const uint32_t kr = (uint32_t)(krow * CR + (hq ^ Swz<64>::at(lt))) * 16u;
+    // tile j has landed for all waves; tile j - 1 and its P are read
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // contraction steps in order, the one with Q in LDS first
+    auto order = [](int i) { return i == 0 ? STEPS - 1 : i - 1; };
+    bf16x8 kf[3], ql[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) ql[n] = lds_read_b128(s_q, (uint32_t)((hq * 64 + 32 * rh + 16 * n + lt) * 16));
+    auto read_k = [&](int s) {
+      return s < 16 ? lds_read_b128(kt, ka ^ (uint32_t)(64 * s)) : lds_read_b128(rt, kr ^ (uint32_t)(64 * (s - 16)));
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) kf[s] = read_k(order(s));
+    bool ok;
+    const uint64_t ra = row_addr(j + 1, pg_next, ln, ok);
+    const uint64_t mask_next = __ballot(ok);
+    if (tid == 0) s_over[(j + 1) & 1] = 0;
+
+    // S^T of 16 keys x 32 rows
+    acc_t sacc[2];
+    bf16x8 pk = {};
+    each<STEPS>([&](auto ic) {
+      constexpr int i = decltype(ic)::value, s = i - 1;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (i + 2 < STEPS) kf[(i + 2) % 3] = read_k(i + 1);
+      if constexpr (i == 0) {
+        MA::mma_v0(kf[0], ql[0], sacc[0], pk);
+        MA::mma_v0(kf[0], ql[1], sacc[1], pk);
+      } else if constexpr (s < 16) {
+        MA::mma_v_ba(kf[i % 3], qa[0][s], sacc[0], pk);
+        MA::mma_v_ba(kf[i % 3], qa[1][s], sacc[1], pk);
+      } else {
+        MA::mma_v(kf[i % 3], q16, sacc[0], pk);
+        MA::mma_v(kf[i % 3], ql[0], sacc[1], pk);
+      }
+      pk = kf[i % 3];
+      if constexpr (i == 14) ql[0] = lds_read_b128(s_q1, (uint32_t)((hq * 32 + 16 * rh + lt) * 16));
+      if constexpr (i % 2 == 1 && i / 2 < RPW) load_row(i / 2, ra, s_k[(j + 1) & 1], ln);
+      if constexpr (i == 17) load_tails(ra, s_r[(j + 1) & 1], ln);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    pg_next = page_of(j + 2, ln);
+    MA::tail1(pk);
+    MA::drain_v1(sacc[0]);
+    MA::drain_v1(sacc[1]);
+    asm volatile("" : "+v"(ln));  // (what the second half needs is formed now)
+    lt = ln & 15;
+    hq = ln >> 4;
+    const int rr = lt >> 2, cc = lt & 3, vrow = 4 * hq + rr;
+    const uint32_t va =
+        (uint32_t)(vrow * CH + ((8 * wave + (cc >> 1)) ^ Swz<128>::at(vrow))) * 16u + (uint32_t)(cc & 1) * 8u;
+    char* const pw = reinterpret_cast<char*>(s_p) + (((kq >> 1) * 4 + hq) * 64 + 32 * rh + lt) * 16 + (kq & 1) * 8;
+
+    // the lane's keys 16 kq + 4 hq + e of its rows
+    if (TAIL || mask != ~0ull) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t seen = seen4<TAIL>((uint32_t)(mask >> (16 * kq)), TAIL ? s_mask[32 * rh + 16 * n + lt] : 0, 4 * hq,
+                                          k0 + j * KEYS + 16 * kq - ctx);
+        const float x0 = seen & 1u ? sacc[n][0] : kNegInf, x1 = seen & 2u ? sacc[n][1] : kNegInf;
+        const float x2 = seen & 4u ? sacc[n][2] : kNegInf, x3 = seen & 8u ? sacc[n][3] : kNegInf;
+        sacc[n] = acc_t{x0, x1, x2, x3};
+      }
+    }
+    bool over = false;
+    float tmax[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      tmax[n] = max_raw(max3_raw(sacc[n][0], sacc[n][1], sacc[n][2]), sacc[n][3]);
+      over |= tmax[n] * p.scale_log2 > m_used[n] + 8.f;
+    }
+    if (__any(over) && lane == 0) s_over[j & 1] = 1;
+    auto weights = [&](float (&sum)[2]) {  // P^T of the lane's keys into LDS
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float moff = m_used[n] == kNegInf ? 0.f : -m_used[n];
+        float ex[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ex[e] = __builtin_amdgcn_exp2f(fmaf(sacc[n][e], p.scale_log2, moff));
+        const bf16x4 w = {(bf16)ex[0], (bf16)ex[1], (bf16)ex[2], (bf16)ex[3]};
+        *reinterpret_cast<bf16x4*>(pw + n * 16 * 16) = w;
+        sum[n] = (ex[0] + ex[1]) + (ex[2] + ex[3]);
+      }
+    };
+    float sum[2];
+    weights(sum);
+    if constexpr (TAIL) {
+      // drafted rows whose V holds infinities or NaN (the wave's 8 rows)
+      const int row = wave * RPW + (ln >> 3);
+      uint32_t x = 0;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        const u32x4 w = kt[row * CH + (ln & 7) * 8 + c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x |= (w[e] & 0x7f80u) == 0x7f80u;
+          x |= (w[e] & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+      if (x != 0 && k0 + j * KEYS + row >= ctx) atomicOr(&s_bad, 1ull << row);
+    }
+    wg_barrier();  // P, the flag (and the rows with infinities) are there
+    if (s_over[j & 1] != 0) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float t = xor32_max(xor16_max(tmax[n])) * p.scale_log2;
+        if (hq == 0) s_x[kq][32 * rh + 16 * n + lt] = t;
+      }
+      wg_barrier();
+      auto moved = [&](int row, float& alpha) {
+        const float m = s_m[row];
+        const float mn = fmaxf(fmaxf(m, fmaxf(s_x[0][row], s_x[1][row])), fmaxf(s_x[2][row], s_x[3][row]));
+        alpha = mn == kNegInf ? 1.f : exp2f(m - mn);
+        return mn;
+      };
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        float alpha;
+        moved(16 * n + lt, alpha);
+#pragma unroll
+        for (int o = 0; o < 4; ++o) oacc[o][n] *= alpha;
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float alpha;
+        m_used[n] = moved(32 * rh + 16 * n + lt, alpha);
+        l_part[n] *= alpha;
+      }
+      weights(sum);
+      wg_barrier();
+      if (kq == 0 && hq == 0) {
+        s_m[32 * rh + lt] = m_used[0];
+        s_m[32 * rh + 16 + lt] = m_used[1];
+      }
+    }
+    l_part[0] += sum[0];
+    l_part[1] += sum[1];
+
+    uint64_t bad = 0;
+    if constexpr (TAIL) {
+      bad = s_bad;
+      if (bad != 0) {  // out of the product: 0 times them would reach rows that do not see them
+        for (int i = ln; i < RPW * CH; i += 64)
+          if ((bad >> (wave * RPW + i / CH)) & 1) s_k[j & 1][wave * RPW * CH + i] = u32x4{0, 0, 0, 0};
+        wg_barrier();
+      }
+    }
+    // O^T += V^T P^T over the wave's 64 dims
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 pb[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) pb[n] = lds_read_b128(s_p, (uint32_t)(((kk * 4 + hq) * 64 + 16 * n + lt) * 16));
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        if (o % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        const uint32_t off = (va ^ (uint32_t)(32 * o)) + (uint32_t)(32 * kk * CH) * 16u;
+        const bf16x4 lo = lds_read_tr16(kt, off), hi = lds_read_tr16(kt, off + 16u * CH * 16u);
+        const bf16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) oacc[o][n] = M::mma(a, pb[n], oacc[o][n]);
+      }
+    }
+    if constexpr (TAIL) {
+      if (bad != 0) {  // the rows that see them
+        for (uint64_t left = bad; left != 0; left &= left - 1) {
+          const int key = __builtin_ctzll(left);
+          const int64_t vo = key_row(p, b, k0 + j * KEYS + key, p.k_sb, p.k_ss);
+          if (vo < 0) continue;
+          const bf16* v = reinterpret_cast<const bf16*>(p.k) + vo + g * p.k_sh + 64 * wave + 4 * hq;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            // (the key's place in the operand order: half, lane group, then 4 + 4)
+            const int at = (((key >> 5) * 4 + ((key & 15) >> 2)) * 64 + 16 * n + lt) * 8 + ((key >> 4) & 1) * 4 + (key & 3);
+            const float e = (float)reinterpret_cast<const bf16*>(s_p)[at];
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+              __builtin_amdgcn_sched_barrier(0);
+              const bf16x4 x = *reinterpret_cast<const bf16x4*>(v + 16 * o);
+              const acc_t y = {e * (float)x[0], e * (float)x[1], e * (float)x[2], e * (float)x[3]};
+              oacc[o][n] += e != 0.f ? y : acc_t{};
+            }
+          }
+        }
+        wg_barrier();
+        if (tid == 0) s_bad = 0;
+      }
+    }
+    mask = mask_next;
+  };
+  const int whole = min(max(ctx - k0, 0) / KEYS, ntiles);
+  int j = 0;
+  for (; j < whole; ++j) step(j, std::false_type{});
+  for (; j < ntiles; ++j) step(j, std::true_type{});
+  wait_vm<0>();
+
+  // ---- row sums over the key quarters; results ------------------------------------------
+  wg_barrier();
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    float l = l_part[n];
+    l += __shfl_xor(l, 16, 64);
+    l = xor32_sum(l);
+    if (hq == 0) s_x[kq][32 * rh + 16 * n + lt] = l;
+  }
+  wg_barrier();
+  const int64_t pr = (int64_t)it.slot * p.T * p.Hq;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int row = 16 * n + lt, r = row0 + row;
+    if (r >= R) continue;
+    const RowOut ro = row_out(p, g, r);
+    const float m = s_m[row], l = (s_x[0][row] + s_x[1][row]) + (s_x[2][row] + s_x[3][row]);
+    float f, lse;
+    if (it.partial) {
+      f = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+      lse = l > 0.f ? lse2_of(m, l) : l == 0.f ? kNegInf : l;
+      if (wave == 0 && hq == 0) p.part_lse[pr + ro.r] = lse;
+    } else {
+      f = finish_row(p, ro.h, ro.t < it.nodes, m, l, lse);
+      if (wave == 0 && hq == 0) p.lse[b * p.l_sb + ro.t * p.l_ss + ro.h * p.l_sh] = lse;
+    }
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const f32x4 of = oacc[o][n] * f, x = f == 0.f ? f32x4{} : of;
+      const int d = 64 * wave + 16 * o + 4 * hq;
+      if (it.partial) {
+        *reinterpret_cast<f32x4*>(p.part_o + (pr + ro.r) * C::kDv + d) = x;
+      } else {
+        const bf16x4 o4 = {(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + ro.t * p.o_ss + ro.h * p.o_sh + d) = o4;
+      }
+    }
+  }
+}
+
 // ---- joining the slots of a sequence -------------------------------------------
 // One wave a row; LPR lanes hold the row (4 dims each), 64 / LPR slots at a
 // time.  A slot in which the row sees nothing has LSE -inf.
@@ -1181,11 +1545,11 @@ void launch_combine(const TreeParams& p, hipStream_t s) {
 }
 
 // Kernels by query rows per (sequence, kv head): rows a workgroup, tile keys, waves.
-enum { kGeneric = 0, kRows16, kRows32, kRows64, kRows128, kRows256 };
+enum { kGeneric = 0, kRows16, kRows32, kRows64, kRows128, kRows256, kMla };
 struct KernelShape {
   int rows, tile;
 };
-constexpr KernelShape kShapes[] = {{kGR, kGK}, {16, 128}, {32, 128}, {64, 128}, {128, 64}, {256, 32}};
+constexpr KernelShape kShapes[] = {{kGR, kGK}, {16, 128}, {32, 128}, {64, 128}, {128, 64}, {256, 32}, {64, 64}};
 constexpr int kWorkgroups = 256;  // key ranges are cut until about so many workgroups (one a CU) are in flight
 
 template <int D, int NG, int WR, int WK, int NS>
@@ -1216,6 +1580,9 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
   const int64_t R = (int64_t)p.T * p.G;
   if (dtype == SFA_DTYPE_BF16 && vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
     pl.kernel = R <= 16 ? kRows16 : R <= 32 ? kRows32 : R <= 64 ? kRows64 : R <= 128 ? kRows128 : kRows256;
+  if (dtype == SFA_DTYPE_BF16 && vec && p.Dqk == 576 && p.Dv == 512 && p.v == p.k && p.v_sb == p.k_sb && p.v_ss == p.k_ss &&
+      p.v_sh == p.k_sh)
+    pl.kernel = kMla;
   pl.rows = kShapes[pl.kernel].rows;
   const int64_t nrb = (R + pl.rows - 1) / pl.rows, min_len = 2 * kShapes[pl.kernel].tile;
   int64_t want = (pl.kernel == kGeneric ? 4 : 1) * kWorkgroups / (p.Hkv * nrb);
@@ -1223,6 +1590,9 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
   if (want > most) want = most;
   pl.want = want > p.B ? (int)want : 0;
   pl.slots = p.B + pl.want;
+  // (whole eights of items: the row blocks of one meet in the L2 of one XCD)
+  if (nrb > 1 && (int64_t)pl.slots * p.Hkv > 4)
+    while (pl.slots * p.Hkv % 8 != 0) ++pl.slots;
   if (pl.want > 0) {
     const size_t rows = (size_t)pl.slots * p.T * p.Hq;
     pl.part_o_bytes = (rows * p.Dv * sizeof(float) + 255) / 256 * 256;
@@ -1238,7 +1608,9 @@ hipError_t launch_tree(const TreeParams& p0, const TreePlan& pl, int dtype, hipS
   p.tile = kShapes[pl.kernel].tile;
   p.nrb = (p.T * p.G + pl.rows - 1) / pl.rows;
   const unsigned grid = (unsigned)((int64_t)pl.slots * p.Hkv * p.nrb);
-  if (pl.kernel != kGeneric) {
+  if (pl.kernel == kMla) {
+    tree_mla_kernel<<<grid, 512, 0, s>>>(p);
+  } else if (pl.kernel != kGeneric) {
     if (p.Dqk == 64) launch_mfma<64>(p, pl.kernel, grid, s);
     else launch_mfma<128>(p, pl.kernel, grid, s);
   } else if (dtype == SFA_DTYPE_F32) {
