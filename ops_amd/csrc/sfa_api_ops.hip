@@ -122,7 +122,7 @@ bool rope_vec(const sfa_rope_args* a, const sfa::RopeParams& p, bool backward) {
   for (int i = 0; i < 2; ++i) {
     const sfa::RopeSide& s = p.side[i];
     if (s.H == 0) continue;
-    if (!mult(E, s.n, s.y_sb, s.y_ss, s.y_sh) || !al16(s.y)) return false;
+    if (!mult(E, s.n, s.y_sb, s.y_ss, s.y_sh) || !al16(s.y) || (s.n > 0 && !al16(s.w))) return false;
     if ((!backward || s.n > 0) && (!mult(E, s.x_sb, s.x_ss, s.x_sh) || !al16(s.x))) return false;
     if (backward && (!mult(E, s.dx_sb, s.dx_ss, s.dx_sh) || !al16(s.dx))) return false;
   }
@@ -263,14 +263,14 @@ int sfa_rope_fwd(const sfa_rope_args* a, const sfa_kv_pages* pages, void* stream
   if (rc != SFA_OK) return rc;
   sfa::RopeParams p = rope_params(a, pages);
   const bool vec = rope_vec(a, p, false);
-  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, vec, false);
+  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, vec);
   return done(sfa::launch_rope_fwd(p, a->dtype, vec, (hipStream_t)stream), "sfa_rope_fwd");
 }
 
 size_t sfa_rope_bwd_workspace_size(const sfa_rope_args* a) {
   if (check_rope(a, true, false) != SFA_OK) return 0;
   sfa::RopeParams p = rope_params(a, nullptr);
-  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, rope_vec(a, p, true), true);
+  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, rope_vec(a, p, true));
   return sfa::rope_bwd_workspace(p);
 }
 
@@ -280,7 +280,7 @@ int sfa_rope_bwd(const sfa_rope_args* a, void* workspace, size_t workspace_bytes
   if (rc != SFA_OK) return rc;
   sfa::RopeParams p = rope_params(a, nullptr);
   const bool vec = rope_vec(a, p, true);
-  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, vec, true);
+  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, vec);
   const size_t need = sfa::rope_bwd_workspace(p);
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)

@@ -4,9 +4,21 @@
 // points are in sfa_api_ops.hip.
 #pragma once
 
+#include <utility>
+
 #include "sfa_common.h"
 
 namespace sfa {
+
+// f(integral_constant i) for i = 0 .. N - 1
+template <int... I, class F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(std::make_integer_sequence<int, N>{}, f);
+}
 
 // Stores the message for sfa_last_error() and returns code (sfa_api.hip).
 int api_fail(int code, const char* msg);
@@ -50,11 +62,12 @@ struct RopeParams {
   int max_pages, page_shift, num_pages;
   // geometry (rope_geometry)
   int P, K, chunks;     // lanes a row, 16-byte chunks a lane, chunks a row
-  int groups, per, upt; // row groups a token, groups a unit, units a token
-  int64_t units;
+  int groups, per, upt; // row groups a token; in blocks of per, upt blocks a token
+  int64_t units;        // B * S * groups
+  int stream;           // store the results past the L2s
   float* part;          // backward: [2][workgroups][1024] partial dw, or nullptr
 };
-void rope_geometry(RopeParams& p, int esize, bool vec, bool backward);
+void rope_geometry(RopeParams& p, int esize, bool vec);
 int rope_bwd_wgs(const RopeParams& p);
 size_t rope_bwd_workspace(const RopeParams& p);
 hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);

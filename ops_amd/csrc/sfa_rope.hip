@@ -16,19 +16,20 @@
 // taken of that fraction.
 //
 // Bound: HBM, each row read once and written once (backward: x and dy read,
-// dx written).  So a row is held in registers, 16 bytes a lane, P lanes a
-// row (the power of two that covers it; 8 lanes of 9 chunks for the 576-dim
-// latent row), 64 / P heads of one token per wave; the token's angles are
-// computed once per wave for all the heads that it takes.  Rows that are not
-// whole 16-byte chunks (odd dims, strides, offsets) take the scalar kernels,
-// one wave a row.
+// dx written).  So a row is held in registers, in 16-byte chunks over P lanes
+// (half layout over the whole row: two chunks a lane, so that partners meet in
+// one lane and share their angles; 8 lanes of 9 chunks for the 576-dim latent
+// row), 64 / P heads of one token per wave; the token's angles are computed
+// once per wave for all the heads that it takes.  Rows that are not whole
+// 16-byte chunks (odd dims, strides, offsets) take the scalar kernels, one
+// wave a row.
 
 #include "sfa_ops.h"
 
 namespace sfa {
 namespace {
 
-constexpr double kInv2Pi = 0.15915494309189533576888376337251;
+constexpr double k2Pi4 = 0.63661977236758134307553505349006;  // 2 / pi: quarter turns per radian
 constexpr int kMaxD = 1024;
 constexpr int kScalarSteps = kMaxD / 64;
 
@@ -61,11 +62,27 @@ __device__ __forceinline__ int64_t load_int(const void* base, int64_t i, int is6
   return is64 ? reinterpret_cast<const int64_t*>(base)[i] : (int64_t) reinterpret_cast<const int32_t*>(base)[i];
 }
 
-// cos and sin of pos * f, the angle reduced to (-1/2, 1/2] turns in float64
+// cos and sin of pos * f.  The angle is reduced in float64 to quarter turns q
+// and a rest r of at most half a quarter; sin and cos of the rest, x = r pi / 2
+// with |x| <= pi / 4, are their Taylor polynomials (the first term left out is
+// x^11 / 11! < 2e-9 and x^12 / 12! < 2e-10).
 __device__ __forceinline__ void angle(double pos, double f, float& c, float& s) {
-  double t = pos * (f * kInv2Pi);
-  t -= rint(t);
-  sincospif((float)(2.0 * t), &s, &c);
+  const double u = pos * (f * k2Pi4);
+  const double q = rint(u);
+  const int n = (int)(q - 4.0 * rint(0.25 * q));  // the quarter, -2 .. 2
+  const float x = (float)(u - q) * 1.57079632679489662f, x2 = x * x;
+  float a = fmaf(x2, 1.f / 362880.f, -1.f / 5040.f);
+  a = fmaf(x2, a, 1.f / 120.f);
+  a = fmaf(x2, a, -1.f / 6.f);
+  const float sx = fmaf(x * x2, a, x);
+  float d = fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f);
+  d = fmaf(x2, d, -1.f / 720.f);
+  d = fmaf(x2, d, 1.f / 24.f);
+  d = fmaf(x2, d, -0.5f);
+  const float cx = fmaf(x2, d, 1.f);
+  const float s0 = n & 1 ? cx : sx, c0 = n & 1 ? sx : cx;
+  s = n & 2 ? -s0 : s0;
+  c = (n + 1) & 2 ? -c0 : c0;
 }
 
 template <typename T>
@@ -73,9 +90,25 @@ __device__ __forceinline__ float load_w(const RopeParams& p, const void* w, int 
   return p.w_f32 ? reinterpret_cast<const float*>(w)[d] : to_f32(reinterpret_cast<const T*>(w)[d]);
 }
 
-// Sum over the P lanes of a row (P a power of two, wave-uniform).
-__device__ __forceinline__ float row_sum(float x, int P) {
-  for (int o = P >> 1; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+// Sum over the P lanes of a row (lane permutations of the VALU, no LDS trips).
+template <int C>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), C, 0xf, 0xf, true));
+}
+template <int P>
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp<0xb1>(x);                          // lane ^ 1
+  x += dpp<0x4e>(x);                          // lane ^ 2
+  if constexpr (P >= 8) x += dpp<0x141>(x);   // mirror of 8
+  if constexpr (P >= 16) x += dpp<0x140>(x);  // mirror of 16
+  if constexpr (P >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (P >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return x;
 }
 
@@ -102,21 +135,14 @@ struct Turn {
     }
   }
   __device__ __forceinline__ void angles(const RopeParams& p, double pos, float (&cs)[E], float (&sn)[E]) const {
-    if (p.interleaved) {
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) angle(pos, on ? p.freq[i0 + e] : 0.0, cs[e], sn[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) angle(pos, on ? p.freq[i0 + e] : 0.0, cs[e], sn[e]);
-    }
-    const float s = p.rope_scale;
-    if (s != 1.f) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        cs[e] *= s;
-        sn[e] *= s;
-      }
-    }
+    const float sc = p.rope_scale;
+    each<E>([&](auto ec) {
+      constexpr int e = decltype(ec)::value;
+      float c = 1.f, s = 0.f;
+      if (e < E / 2 || !p.interleaved) angle(pos, on ? p.freq[i0 + e] : 0.0, c, s);
+      cs[e] = c * sc;
+      sn[e] = s * sc;
+    });
   }
   // u (own) and o (the partner chunk, half layout) turned by +-a (dir = 1, -1)
   __device__ __forceinline__ void apply(const RopeParams& p, float (&u)[E], const float (&o)[E], const float (&cs)[E],
@@ -154,280 +180,399 @@ __device__ __forceinline__ int64_t cache_row(const RopeParams& p, int b, int s, 
   return (int64_t)pg * page_stride + (slot & ((1 << p.page_shift) - 1)) * row_stride;
 }
 
-// Forward.  A wave takes `per` row groups of a token: first the q heads' (64 / P
-// rows a group), then the k heads', then (append) 64-chunk groups of the v row.
-template <typename T, int K>
-__global__ __launch_bounds__(256) void rope_fwd_kernel(RopeParams p) {
-  constexpr int E = Chunk<T>::E;
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= p.units) return;
-  const int64_t tok = unit / p.upt;
-  const int b = (int)(tok / p.S), s = (int)(tok % p.S);
-  const int P = p.P, rpw = 64 / P, l = lane & (P - 1), rr = lane / P;
-  const int g0 = (int)(unit % p.upt) * p.per, g1 = min(g0 + p.per, p.groups);
-  const double pos = (double)load_int(p.pos, b * p.pos_sb + s * p.pos_ss, p.pos_i64);
-
-  // the angles of the lane's chunk, for all its rows (rows of several chunks a
-  // lane: per chunk and row, where it is rotated)
-  const Turn<E> t0(p, l);
-  float cs[E], sn[E];
-  if constexpr (K == 1) t0.angles(p, pos, cs, sn);
-
-  int held = -1;
-  float w[E], wo[E];  // K = 1: the chunk's weights and its partner's
-  for (int g = g0; g < g1; ++g) {
-    const int si = g < p.side[0].groups ? 0 : g < p.side[0].groups + p.side[1].groups ? 1 : 2;
-    if (si == 2) {  // the v row: copied
-      const int i = (g - p.side[0].groups - p.side[1].groups) * 64 + lane, cpr = p.Dv / E;
-      const int64_t row = cache_row(p, b, s, p.vo_sb, p.vo_ss);
-      if (i < p.side[1].H * cpr && row >= 0) {
-        const int h = i / cpr, c = i % cpr;
-        const T* x = reinterpret_cast<const T*>(p.v) + b * p.v_sb + s * p.v_ss + h * p.v_sh + c * E;
-        *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(p.v_out) + row + h * p.vo_sh + c * E) =
-            *reinterpret_cast<const u32x4*>(x);
-      }
-      continue;
-    }
-    const RopeSide& sd = p.side[si];
-    const int h = (si == 0 ? g : g - p.side[0].groups) * rpw + rr;
-    const bool live = h < sd.H;
-    const T* x = reinterpret_cast<const T*>(sd.x) + b * sd.x_sb + s * sd.x_ss + (int64_t)(live ? h : 0) * sd.x_sh;
-    int64_t yo;
-    if (si == 1 && p.block_table != nullptr)
-      yo = cache_row(p, b, s, sd.y_sb, sd.y_ss);
-    else
-      yo = b * sd.y_sb + s * sd.y_ss;
-    T* y = reinterpret_cast<T*>(sd.y) + yo + (int64_t)(live ? h : 0) * sd.y_sh;
-    const bool put = live && yo >= 0;
-
-    u32x4 raw[K];
+// A row's chunks: lane l of its P lanes holds chunks l, l + P, ..  IN: half
+// layout over the whole row in two chunks a lane, so a lane holds both partners;
+// else partners are another lane's chunk (K = 1) or read again (K > 2).
+template <typename T, int P, int K, bool IN>
+struct Row {
+  static constexpr int E = Chunk<T>::E;
+  static constexpr bool kHeld = IN || K == 1;  // the lane's angles serve all its rows
+  u32x4 r[K];
+  __device__ __forceinline__ void load(const RopeParams& p, const T* x, int l, int n) {  // chunks below dim n
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int c = j * P + l;
-      raw[j] = c < p.chunks ? *reinterpret_cast<const u32x4*>(x + c * E) : u32x4{0, 0, 0, 0};
+      r[j] = c * E < n ? *reinterpret_cast<const u32x4*>(x + c * E) : u32x4{0, 0, 0, 0};
     }
-    u32x4 oth[K];  // partner chunks (half layout)
-    if (!p.interleaved) {
-      if constexpr (K == 1) {
-        oth[0] = shfl16(raw[0], (lane & ~(P - 1)) + t0.pair);
-      } else {
+  }
+  __device__ __forceinline__ void store(const RopeParams& p, T* y, int l) const {
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-          const Turn<E> t(p, j * P + l);
-          if (t.on) oth[j] = *reinterpret_cast<const u32x4*>(x + t.pair * E);
-        }
-      }
+    for (int j = 0; j < K; ++j) {
+      const int c = j * P + l;
+      if (c >= p.chunks) continue;
+      if (p.stream) __builtin_nontemporal_store(r[j], reinterpret_cast<u32x4*>(y + c * E));
+      else *reinterpret_cast<u32x4*>(y + c * E) = r[j];
     }
-    float r = 1.f;
-    if (sd.n > 0) {
-      float q = 0.f;
+  }
+  // u(j, own, partner) replaces chunk j by its turned values: pre() makes u of
+  // the raw chunk c of this row
+  template <class Pre, class Put>
+  __device__ __forceinline__ void turn(const RopeParams& p, const T* x, int lane, double pos, const float (&cs)[E],
+                                       const float (&sn)[E], float dir, Pre pre, Put put) const {
+    const int l = lane & (P - 1);
+    if constexpr (IN) {
+      float a[E], b[E];
+      Chunk<T>::unpack(r[0], a);
+      Chunk<T>::unpack(r[1], b);
+      pre(0, l, a);
+      pre(1, l + P, b);
+      float ya[E], yb[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float sd = dir * sn[e];
+        ya[e] = a[e] * cs[e] - b[e] * sd;
+        yb[e] = b[e] * cs[e] + a[e] * sd;
+      }
+      put(0, l, ya);
+      put(1, l + P, yb);
+    } else {
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        float f[E];
-        Chunk<T>::unpack(raw[j], f);
-        if ((j * P + l) * E < sd.n) {
+        if constexpr (K > 2) __builtin_amdgcn_sched_barrier(0);  // (chunk by chunk: registers)
+        const int c = j * P + l;
+        const Turn<E> t(p, c);
+        float u[E], o[E];
+        Chunk<T>::unpack(r[j], u);
+        pre(j, c, u);
+        u32x4 other = {0, 0, 0, 0};
+        if (!p.interleaved) {
+          if constexpr (K == 1) {
+            other = shfl16(r[0], (lane & ~(P - 1)) + t.pair);
+          } else {
+            if (t.on) other = *reinterpret_cast<const u32x4*>(x + t.pair * E);
+          }
+        }
+        Chunk<T>::unpack(other, o);
+        if (!p.interleaved && t.on) pre(K, t.pair, o);
+        if constexpr (K == 1) {
+          t.apply(p, u, o, cs, sn, dir);
+        } else if (t.on) {
+          float c2[E], s2[E];
+          t.angles(p, pos, c2, s2);
+          t.apply(p, u, o, c2, s2, dir);
+        }
+        put(j, c, u);
+      }
+    }
+  }
+};
+
+template <typename T, int P, bool IN>
+__device__ __forceinline__ void lane_angles(const RopeParams& p, int l, double pos, float (&cs)[Chunk<T>::E],
+                                            float (&sn)[Chunk<T>::E]) {
+  Turn<Chunk<T>::E>(p, l).angles(p, pos, cs, sn);
+}
+
+// The weights of a whole chunk.
+template <typename T>
+__device__ __forceinline__ void load_chunk_w(const RopeParams& p, const void* w, int c, float (&f)[Chunk<T>::E]) {
+  constexpr int E = Chunk<T>::E;
+  if (p.w_f32) {
+    const float* at = reinterpret_cast<const float*>(w) + c * E;
+#pragma unroll
+    for (int q = 0; q < E / 4; ++q) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(at + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * q + e] = x[e];
+    }
+  } else {
+    Chunk<T>::unpack(*reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(w) + c * E), f);
+  }
+}
+// The weights of the chunks a lane holds (index K: of its partner chunk); rows
+// of many chunks read them again for each row.
+template <typename T, int P, int K, bool IN>
+struct Weights {
+  static constexpr int E = Chunk<T>::E;
+  static constexpr bool kRegs = K <= 2;
+  float w[kRegs ? K + 1 : 1][E];
+  __device__ __forceinline__ void load(const RopeParams& p, const RopeSide& sd, int l) {
+    if constexpr (kRegs) {
+#pragma unroll
+      for (int j = 0; j < (IN ? K : K + 1); ++j) {
+        const int c = j < K ? j * P + l : Turn<E>(p, l).pair;
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[j][e] = 1.f;
+        if (c * E < sd.n) load_chunk_w<T>(p, sd.w, c, w[j]);
+      }
+    }
+  }
+  __device__ __forceinline__ void chunk(const RopeParams& p, const RopeSide& sd, int j, int c, float (&f)[E]) const {
+    if constexpr (kRegs) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = w[j][e];
+    } else {
+      load_chunk_w<T>(p, sd.w, c, f);
+    }
+  }
+};
+
+// A wave's walk over (token, row group) units: blocks of `per` groups of a
+// token (p.per, p.upt blocks a token), every nw-th block, so that the waves of the
+// card read one window of the tensor at a time (strided rows, 128 of 1152
+// bytes: 142 us with a contiguous run per wave).
+struct Walk {
+  uint32_t blk, nblk, nw;
+  int b, s, g, g1;
+  __device__ __forceinline__ void at(const RopeParams& p, int groups, int per, int upt) {
+    const uint32_t tok = blk / (uint32_t)upt;
+    b = (int)(tok / (uint32_t)p.S);
+    s = (int)(tok - (uint32_t)b * (uint32_t)p.S);
+    g = (int)(blk - tok * (uint32_t)upt) * per;
+    g1 = min(g + per, groups);
+  }
+  __device__ __forceinline__ bool live() const { return blk < nblk; }
+  // the next unit; fresh: of another block (another token's, perhaps)
+  __device__ __forceinline__ bool next(const RopeParams& p, int groups, int per, int upt) {
+    if (++g < g1) return false;
+    blk += nw;
+    if (blk < nblk) at(p, groups, per, upt);
+    return true;
+  }
+};
+
+// Forward.  The units are (token, row group): the q heads' groups (64 / P rows
+// each), the k heads', then (append) 64-chunk groups of the v row.  A wave
+// loads the next unit's rows before it works on this one's.
+template <typename T, int P, int K, bool IN>
+__global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kernel(RopeParams p) {
+  typedef Row<T, P, K, IN> R;
+  constexpr int E = R::E, rpw = 64 / P;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (P - 1), rr = lane / P;
+  Walk w;
+  w.nw = gridDim.x * 4;
+  w.blk = blockIdx.x * 4 + wave;
+  w.nblk = (uint32_t)p.B * (uint32_t)p.S * (uint32_t)p.upt;
+  if (!w.live()) return;
+  w.at(p, p.groups, p.per, p.upt);
+  const int gq = p.side[0].groups, gk = gq + p.side[1].groups;
+
+  struct Unit {
+    R x;
+    const T* px;
+    T* py;
+    int b, s, g;
+    bool put;
+  };
+  auto load = [&](Unit& u) {
+    if (u.g >= gk) return;  // a v group
+    const int si = u.g < gq ? 0 : 1;
+    const RopeSide& sd = p.side[si];
+    const int h = (si == 0 ? u.g : u.g - gq) * rpw + rr;
+    u.put = h < sd.H;
+    const int64_t hh = u.put ? h : 0;
+    u.px = reinterpret_cast<const T*>(sd.x) + u.b * sd.x_sb + u.s * sd.x_ss + hh * sd.x_sh;
+    u.x.load(p, u.px, l, p.D);
+    int64_t yo;
+    if (si == 1 && p.block_table != nullptr) yo = cache_row(p, u.b, u.s, sd.y_sb, sd.y_ss);
+    else yo = u.b * sd.y_sb + u.s * sd.y_ss;
+    u.py = reinterpret_cast<T*>(sd.y) + yo + hh * sd.y_sh;
+    u.put = u.put && yo >= 0;
+  };
+  Unit cur;
+  cur.b = w.b;
+  cur.s = w.s;
+  cur.g = w.g;
+  load(cur);
+  double pos = 0.0;
+  float cs[E], sn[E];
+  bool fresh = true;
+  int held = -1;
+  Weights<T, P, K, IN> wt;
+  while (true) {
+    if (fresh) {
+      pos = (double)load_int(p.pos, cur.b * p.pos_sb + cur.s * p.pos_ss, p.pos_i64);
+      if constexpr (R::kHeld) lane_angles<T, P, IN>(p, l, pos, cs, sn);
+    }
+    fresh = w.next(p, p.groups, p.per, p.upt);
+    const bool more = w.live();
+    Unit nxt;
+    nxt.b = w.b;
+    nxt.s = w.s;
+    nxt.g = w.g;
+    if constexpr (K <= 2) {
+      if (more) load(nxt);
+    }
+    if (cur.g >= gk) {  // the v row: copied
+      const int i = (cur.g - gk) * 64 + lane, cpr = p.Dv / E;
+      const int64_t row = cache_row(p, cur.b, cur.s, p.vo_sb, p.vo_ss);
+      if (i < p.side[1].H * cpr && row >= 0) {
+        const int h = i / cpr, c = i % cpr;
+        const T* v = reinterpret_cast<const T*>(p.v) + cur.b * p.v_sb + cur.s * p.v_ss + h * p.v_sh + c * E;
+        *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(p.v_out) + row + h * p.vo_sh + c * E) =
+            *reinterpret_cast<const u32x4*>(v);
+      }
+    } else {
+      const int si = cur.g < gq ? 0 : 1;
+      const RopeSide& sd = p.side[si];
+      float r = 1.f;
+      if (sd.n > 0) {
+        if (held != si) {
+          held = si;
+          wt.load(p, sd, l);
+        }
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          float f[E];
+          Chunk<T>::unpack(cur.x.r[j], f);
           float q4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int e = 0; e < E; ++e) q4[e & 3] = fmaf(f[e], f[e], q4[e & 3]);
-          q += (q4[0] + q4[1]) + (q4[2] + q4[3]);
+          if ((j * P + l) * E < sd.n) q += (q4[0] + q4[1]) + (q4[2] + q4[3]);
         }
+        r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
       }
-      r = 1.f / sqrtf(row_sum(q, P) / (float)sd.n + p.eps);
-      if (K == 1 && held != si) {
-        held = si;
+      cur.x.turn(
+          p, cur.px, lane, pos, cs, sn, 1.f,
+          [&](int j, int c, float (&v)[E]) {
+            if (c * E < sd.n) {
+              float wc[E];
+              wt.chunk(p, sd, j, c, wc);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          w[e] = l * E < sd.n ? load_w<T>(p, sd.w, l * E + e) : 1.f;
-          wo[e] = t0.pair * E < sd.n ? load_w<T>(p, sd.w, t0.pair * E + e) : 1.f;
-        }
-      }
+              for (int e = 0; e < E; ++e) v[e] = v[e] * r * wc[e];
+            }
+          },
+          [&](int j, int c, const float (&v)[E]) { cur.x.r[j] = Chunk<T>::pack(v); });
+      // (every value of the row has been read: y may be x)
+      if (cur.put) cur.x.store(p, cur.py, l);
     }
-    u32x4 res[K];
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int c = j * P + l;
-      const Turn<E> t(p, c);
-      float u[E], o[E];
-      Chunk<T>::unpack(raw[j], u);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      if (!p.interleaved && t.on) Chunk<T>::unpack(oth[j], o);
-      if (c * E < sd.n) {
-        const int cw = c;
-#pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = u[e] * r * (K == 1 ? w[e] : load_w<T>(p, sd.w, cw * E + e));
-      }
-      if (!p.interleaved && t.on && t.pair * E < sd.n) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * r * (K == 1 ? wo[e] : load_w<T>(p, sd.w, t.pair * E + e));
-      }
-      if constexpr (K == 1) {
-        t.apply(p, u, o, cs, sn, 1.f);
-      } else if (t.on) {
-        float c2[E], s2[E];
-        t.angles(p, pos, c2, s2);
-        t.apply(p, u, o, c2, s2, 1.f);
-      }
-      res[j] = Chunk<T>::pack(u);
-    }
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int c = j * P + l;
-      if (put && c < p.chunks) *reinterpret_cast<u32x4*>(y + c * E) = res[j];
+    if (!more) break;
+    if constexpr (K <= 2) {
+      cur = nxt;
+    } else {
+      cur.b = nxt.b;
+      cur.s = nxt.s;
+      cur.g = nxt.g;
+      load(cur);
     }
   }
 }
 
-// Backward: side.y is dy, side.dx receives dx.  A wave takes a contiguous run of
-// (token, row group) units and sums its rows' dw in registers; a workgroup
-// writes its sums to partial row blockIdx.x, which rope_dw_kernel adds up in order.
-template <typename T, int K>
+// Backward of one tensor (blockIdx.y: q or k): side.y is dy, side.dx receives
+// dx.  A wave walks over units as in the forward and sums its rows' dw in registers; a workgroup writes its sums to partial row blockIdx.x,
+// which rope_dw_kernel adds up in order.
+template <typename T, int P, int K, bool IN>
 __global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p) {
-  constexpr int E = Chunk<T>::E;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int P = p.P, rpw = 64 / P, l = lane & (P - 1), rr = lane / P;
-  const int64_t nw = (int64_t)gridDim.x * 4, wv = (int64_t)blockIdx.x * 4 + wave;
-  const int64_t u0 = p.units * wv / nw, u1 = p.units * (wv + 1) / nw;
-  const Turn<E> t0(p, l);
-  float cs[E], sn[E];
-  int64_t tok_held = -1;
-  int held = -1;
-  double pos = 0.0;
-  float w[E];
-  float dw[2][K][E];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int j = 0; j < K; ++j)
-#pragma unroll
-      for (int e = 0; e < E; ++e) dw[a][j][e] = 0.f;
+  typedef Row<T, P, K, IN> R;
+  constexpr int E = R::E, rpw = 64 / P;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (P - 1), rr = lane / P;
+  const int si = blockIdx.y;
+  const RopeSide& sd = p.side[si];
+  if (sd.H == 0) return;
+  const int per = p.per < sd.groups ? p.per : sd.groups, upt = (sd.groups + per - 1) / per;
+  Walk w;
+  w.nw = gridDim.x * 4;
+  w.blk = blockIdx.x * 4 + wave;
+  w.nblk = (uint32_t)p.B * (uint32_t)p.S * (uint32_t)upt;
+  if (w.live()) w.at(p, sd.groups, per, upt);
 
-  for (int64_t u = u0; u < u1; ++u) {
-    const int64_t tok = u / p.groups;
-    const int g = (int)(u % p.groups);
-    const int b = (int)(tok / p.S), s = (int)(tok % p.S);
-    if (tok != tok_held) {
-      tok_held = tok;
-      pos = (double)load_int(p.pos, b * p.pos_sb + s * p.pos_ss, p.pos_i64);
-      if constexpr (K == 1) t0.angles(p, pos, cs, sn);
-    }
-    const int si = g < p.side[0].groups ? 0 : 1;
-    const RopeSide& sd = p.side[si];
-    const int h = (si == 0 ? g : g - p.side[0].groups) * rpw + rr;
-    const bool live = h < sd.H;
-    const int64_t hh = live ? h : 0;
-    const T* dy = reinterpret_cast<const T*>(sd.y) + b * sd.y_sb + s * sd.y_ss + hh * sd.y_sh;
-    T* dx = reinterpret_cast<T*>(sd.dx) + b * sd.dx_sb + s * sd.dx_ss + hh * sd.dx_sh;
-    u32x4 raw[K], xr[K], oth[K];
+  Weights<T, P, K, IN> wt;
+  if (sd.n > 0) wt.load(p, sd, l);
+  float dw[K][E];
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int c = j * P + l;
-      raw[j] = c < p.chunks ? *reinterpret_cast<const u32x4*>(dy + c * E) : u32x4{0, 0, 0, 0};
-    }
-    if (sd.n > 0) {
-      const T* x = reinterpret_cast<const T*>(sd.x) + b * sd.x_sb + s * sd.x_ss + hh * sd.x_sh;
+  for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        const int c = j * P + l;
-        xr[j] = c * E < sd.n ? *reinterpret_cast<const u32x4*>(x + c * E) : u32x4{0, 0, 0, 0};
-      }
+    for (int e = 0; e < E; ++e) dw[j][e] = 0.f;
+
+  struct Unit {
+    R dy, x;
+    const T* py;
+    T* px;
+    bool live;
+  };
+  auto load = [&](Unit& u, int b, int s, int g) {
+    const int h = g * rpw + rr;
+    u.live = h < sd.H;
+    const int64_t hh = u.live ? h : 0;
+    u.py = reinterpret_cast<const T*>(sd.y) + b * sd.y_sb + s * sd.y_ss + hh * sd.y_sh;
+    u.px = reinterpret_cast<T*>(sd.dx) + b * sd.dx_sb + s * sd.dx_ss + hh * sd.dx_sh;
+    u.dy.load(p, u.py, l, p.D);
+    if (sd.n > 0) u.x.load(p, reinterpret_cast<const T*>(sd.x) + b * sd.x_sb + s * sd.x_ss + hh * sd.x_sh, l, sd.n);
+  };
+  Unit cur;
+  if (w.live()) load(cur, w.b, w.s, w.g);
+  double pos = 0.0;
+  float cs[E], sn[E];
+  bool fresh = true;
+  while (w.live()) {
+    if (fresh) {
+      pos = (double)load_int(p.pos, w.b * p.pos_sb + w.s * p.pos_ss, p.pos_i64);
+      if constexpr (R::kHeld) lane_angles<T, P, IN>(p, l, pos, cs, sn);
     }
-    if (!p.interleaved) {
-      if constexpr (K == 1) {
-        oth[0] = shfl16(raw[0], (lane & ~(P - 1)) + t0.pair);
-      } else {
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-          const Turn<E> t(p, j * P + l);
-          if (t.on) oth[j] = *reinterpret_cast<const u32x4*>(dy + t.pair * E);
-        }
-      }
-    }
-    if (K == 1 && sd.n > 0 && held != si) {
-      held = si;
-#pragma unroll
-      for (int e = 0; e < E; ++e) w[e] = l * E < sd.n ? load_w<T>(p, sd.w, l * E + e) : 1.f;
+    fresh = w.next(p, sd.groups, per, upt);
+    Unit nxt;
+    if constexpr (K <= 2) {
+      if (w.live()) load(nxt, w.b, w.s, w.g);
     }
     float du[K][E];
     float q = 0.f, gx = 0.f;  // sum x^2, sum (du w) x
+    cur.dy.turn(
+        p, cur.py, lane, pos, cs, sn, -1.f, [](int, int, float (&)[E]) {},
+        [&](int j, int c, const float (&v)[E]) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int c = j * P + l;
-      const Turn<E> t(p, c);
-      float o[E];
-      Chunk<T>::unpack(raw[j], du[j]);
+          for (int e = 0; e < E; ++e) du[j][e] = v[e];
+          if (c * E < sd.n) {
+            float x[E], wc[E];
+            Chunk<T>::unpack(cur.x.r[j], x);
+            wt.chunk(p, sd, j, c, wc);
+            float q2[2] = {0.f, 0.f}, g2[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      if (!p.interleaved && t.on) Chunk<T>::unpack(oth[j], o);
-      if constexpr (K == 1) {
-        t.apply(p, du[j], o, cs, sn, -1.f);
-      } else if (t.on) {
-        float c2[E], s2[E];
-        t.angles(p, pos, c2, s2);
-        t.apply(p, du[j], o, c2, s2, -1.f);
-      }
-      if (c * E < sd.n) {
-        float x[E];
-        Chunk<T>::unpack(xr[j], x);
-        float q2[2] = {0.f, 0.f}, g2[2] = {0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float gw = du[j][e] * (K == 1 ? w[e] : load_w<T>(p, sd.w, c * E + e));
-          q2[e & 1] = fmaf(x[e], x[e], q2[e & 1]);
-          g2[e & 1] = fmaf(gw, x[e], g2[e & 1]);
-        }
-        q += q2[0] + q2[1];
-        gx += g2[0] + g2[1];
-      }
-    }
+            for (int e = 0; e < E; ++e) {
+              q2[e & 1] = fmaf(x[e], x[e], q2[e & 1]);
+              g2[e & 1] = fmaf(v[e] * wc[e], x[e], g2[e & 1]);
+            }
+            q += q2[0] + q2[1];
+            gx += g2[0] + g2[1];
+          }
+        });
+    R res;
     float r = 0.f, m = 0.f;  // 1 / rms, mean of (du w) xhat
     if (sd.n > 0) {
-      r = 1.f / sqrtf(row_sum(q, P) / (float)sd.n + p.eps);
-      m = row_sum(gx, P) * r / (float)sd.n;
+      r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
+      m = row_sum<P>(gx) * r / (float)sd.n;
     }
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int c = j * P + l;
       if (c * E < sd.n) {
-        float x[E];
-        Chunk<T>::unpack(xr[j], x);
+        float x[E], wc[E];
+        Chunk<T>::unpack(cur.x.r[j], x);
+        wt.chunk(p, sd, j, c, wc);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float xh = x[e] * r, d = du[j][e];
-          const float gw = d * (K == 1 ? w[e] : load_w<T>(p, sd.w, c * E + e));
-          if (live) {
-            if (si == 0) dw[0][j][e] = fmaf(d, xh, dw[0][j][e]);
-            else dw[1][j][e] = fmaf(d, xh, dw[1][j][e]);
-          }
-          du[j][e] = r * (gw - xh * m);
+          dw[j][e] = fmaf(cur.live ? d : 0.f, xh, dw[j][e]);
+          du[j][e] = r * (d * wc[e] - xh * m);
         }
       }
-      if (live && c < p.chunks) *reinterpret_cast<u32x4*>(dx + c * E) = Chunk<T>::pack(du[j]);
+      res.r[j] = Chunk<T>::pack(du[j]);
+    }
+    if (cur.live) res.store(p, cur.px, l);
+    if constexpr (K <= 2) {
+      cur = nxt;
+    } else if (w.live()) {
+      load(cur, w.b, w.s, w.g);
     }
   }
 
-  if (p.part == nullptr) return;
+  if (p.part == nullptr || sd.n == 0) return;
   // dw of the workgroup: the row groups of a wave by shuffles, then the waves
   __shared__ float s_w[4][kMaxD];
-  for (int a = 0; a < 2; ++a) {
-    const int n = p.side[a].n;
-    if (n == 0) continue;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const int c = j * P + l;
+  for (int j = 0; j < K; ++j) {
+    const int c = j * P + l;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float x = a == 0 ? dw[0][j][e] : dw[1][j][e];
-        for (int o = P; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-        if (rr == 0 && c * E < n) s_w[wave][c * E + e] = x;
-      }
+    for (int e = 0; e < E; ++e) {
+      float x = dw[j][e];
+#pragma unroll
+      for (int o = P; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+      if (rr == 0 && c * E < sd.n) s_w[wave][c * E + e] = x;
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < n; d += 256)
-      p.part[((int64_t)a * gridDim.x + blockIdx.x) * kMaxD + d] = (s_w[0][d] + s_w[1][d]) + (s_w[2][d] + s_w[3][d]);
-    __syncthreads();
   }
+  __syncthreads();
+  for (int d = threadIdx.x; d < sd.n; d += 256)
+    p.part[((int64_t)si * gridDim.x + blockIdx.x) * kMaxD + d] = (s_w[0][d] + s_w[1][d]) + (s_w[2][d] + s_w[3][d]);
 }
 
 // dw [side][n]: the partial rows added in a fixed order, 16 dims and 64 runs of
@@ -593,21 +738,61 @@ __global__ __launch_bounds__(256) void rope_bwd_scalar_kernel(RopeParams p) {
   }
 }
 
+// Workgroups of 4 waves for so many units: no more than stay on the card.
+int rope_wgs(int64_t units) {
+  const int64_t w = (units + 3) / 4;
+  return (int)(w < 1 ? 1 : w > 1024 ? 1024 : w);
+}
+
+// The kernel of a geometry: f.template operator()<P, K, IN>()
+template <class F>
+void by_geometry(const RopeParams& p, F f) {
+  if (p.K == 2) {
+    if (p.P == 4) f.template run<4, 2, true>();
+    else if (p.P == 8) f.template run<8, 2, true>();
+    else if (p.P == 16) f.template run<16, 2, true>();
+    else f.template run<32, 2, true>();
+  } else if (p.K == 1) {
+    if (p.P == 8) f.template run<8, 1, false>();
+    else if (p.P == 16) f.template run<16, 1, false>();
+    else if (p.P == 32) f.template run<32, 1, false>();
+    else f.template run<64, 1, false>();
+  } else if (p.K == 9) {
+    f.template run<8, 9, false>();
+  } else {
+    f.template run<64, 4, false>();
+  }
+}
+template <typename T>
+struct Fwd {
+  const RopeParams& p;
+  hipStream_t s;
+  template <int P, int K, bool IN>
+  void run() const {
+    rope_fwd_kernel<T, P, K, IN><<<(unsigned)rope_wgs(p.units), 256, 0, s>>>(p);
+  }
+};
+template <typename T>
+struct Bwd {
+  const RopeParams& p;
+  int wgs;
+  hipStream_t s;
+  template <int P, int K, bool IN>
+  void run() const {
+    rope_bwd_kernel<T, P, K, IN><<<dim3((unsigned)wgs, p.side[1].H > 0 ? 2 : 1), 256, 0, s>>>(p);
+  }
+};
+
 template <typename T>
 void fwd(const RopeParams& p, bool vec, hipStream_t s) {
-  const dim3 grid((unsigned)((p.units + 3) / 4));
-  if (!vec) rope_fwd_scalar_kernel<T><<<grid, 256, 0, s>>>(p);
-  else if (p.K == 1) rope_fwd_kernel<T, 1><<<grid, 256, 0, s>>>(p);
-  else if (p.K == 9) rope_fwd_kernel<T, 9><<<grid, 256, 0, s>>>(p);
-  else rope_fwd_kernel<T, 4><<<grid, 256, 0, s>>>(p);
+  if (!vec) rope_fwd_scalar_kernel<T><<<(unsigned)((p.units + 3) / 4), 256, 0, s>>>(p);
+  else by_geometry(p, Fwd<T>{p, s});
 }
 
 template <typename T>
 void bwd(const RopeParams& p, bool vec, int wgs, hipStream_t s) {
   if (!vec) rope_bwd_scalar_kernel<T><<<wgs, 256, 0, s>>>(p);
-  else if (p.K == 1) rope_bwd_kernel<T, 1><<<wgs, 256, 0, s>>>(p);
-  else if (p.K == 9) rope_bwd_kernel<T, 9><<<wgs, 256, 0, s>>>(p);
-  else rope_bwd_kernel<T, 4><<<wgs, 256, 0, s>>>(p);
+  else by_geometry(p, Bwd<T>{p, wgs, s});
   const int n = p.side[0].n > p.side[1].n ? p.side[0].n : p.side[1].n;
   if (n > 0) rope_dw_kernel<T><<<dim3((unsigned)((n + 15) / 16), 2), 1024, 0, s>>>(p, wgs);
 }
@@ -615,19 +800,23 @@ void bwd(const RopeParams& p, bool vec, int wgs, hipStream_t s) {
 }  // namespace
 
 // Lanes per row, chunks per lane, row groups (see the kernels).
-void rope_geometry(RopeParams& p, int esize, bool vec, bool backward) {
+void rope_geometry(RopeParams& p, int esize, bool vec) {
   const int E = 16 / esize;
   p.chunks = p.D / E;
   p.P = 64;
   p.K = 1;
   if (vec) {
-    if (p.chunks == 72) {
+    const bool pow2 = (p.chunks & (p.chunks - 1)) == 0;
+    if (!p.interleaved && p.off == 0 && p.R == p.D && pow2 && p.chunks >= 8 && p.chunks <= 64) {
+      p.P = p.chunks / 2;  // both partners in one lane
+      p.K = 2;
+    } else if (p.chunks == 72) {
       p.P = 8;
       p.K = 9;
     } else if (p.chunks > 64) {
       p.K = 4;  // up to 256 chunks: float32 rows of 1024 dims
     } else {
-      p.P = 1;
+      p.P = 8;
       while (p.P < p.chunks) p.P *= 2;
     }
   }
@@ -636,24 +825,23 @@ void rope_geometry(RopeParams& p, int esize, bool vec, bool backward) {
   int vg = 0;
   if (p.v != nullptr) vg = vec ? (p.side[1].H * (p.Dv / E) + 63) / 64 : p.side[1].H;
   p.groups = p.side[0].groups + p.side[1].groups + vg;
-  const int64_t toks = (int64_t)p.B * p.S, all = toks * p.groups;
-  p.per = 1;
-  p.upt = p.groups;
-  p.units = all;
-  if (vec && !backward) {
-    // enough row groups per wave to share a token's angles, once there are 8192 waves
-    int64_t per = all / 8192;
-    p.per = (int)(per < 1 ? 1 : per > p.groups ? p.groups : per);
-    p.upt = (p.groups + p.per - 1) / p.per;
-    p.units = toks * p.upt;
-  }
+  p.units = (int64_t)p.B * p.S * p.groups;
+  // Results that pass the L2s (32 MB) are stored past them: forward and backward
+  // of 2 x 8192 tokens, 34 heads of 128 dims 97 + 121 -> 76 + 111 us (285 + 428 MB);
+  // 67 MB from strided rows 142 -> 126, from whole ones 55 -> 58 us.
+  p.stream = (int64_t)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * esize > ((int64_t)32 << 20);
+  // blocks of up to 8 groups (a token's angles serve them) once there are 4096 waves of them
+  const int64_t per = p.units / 4096;
+  p.per = (int)(per < 1 ? 1 : per > 8 ? 8 : per);
+  if (p.per > p.groups) p.per = p.groups;
+  p.upt = (p.groups + p.per - 1) / p.per;
 }
 
 // Workgroups of the backward: its partial dw rows are summed, so no more than
 // fill the card.
 int rope_bwd_wgs(const RopeParams& p) {
-  const int64_t w = (p.units + 3) / 4;
-  return (int)(w < 1 ? 1 : w > 1024 ? 1024 : w);
+  const int g = p.side[0].groups > p.side[1].groups ? p.side[0].groups : p.side[1].groups;
+  return rope_wgs((int64_t)p.B * p.S * g);
 }
 
 size_t rope_bwd_workspace(const RopeParams& p) {

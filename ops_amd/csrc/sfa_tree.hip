@@ -13,8 +13,6 @@
 // even work; the ranges are found on the device from ctx_lens.  A sequence
 // of several slots leaves float32 partials that tree_combine_kernel joins.
 
-#include <utility>
-
 #include "sfa_lds.h"
 #include "sfa_mfma.h"
 #include "sfa_ops.h"
@@ -341,16 +339,6 @@ struct Swz {  // position of chunk c of row r: c ^ at(r)
     else return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
   }
 };
-
-// f(integral_constant i) for i = 0 .. N - 1
-template <int... I, class F>
-__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void each(F&& f) {
-  each_of(std::make_integer_sequence<int, N>{}, f);
-}
 
 // lane l: 16 (4) bytes from its address to dst + 16 l (4 l); not seen by the
 // compiler: the kernel waits for vmcnt itself

@@ -165,17 +165,18 @@ class _NormRope(torch.autograd.Function):
         if q.numel() + (0 if k is None else k.numel()) > 0:
             a = c.args(q, k, qo, ko)
             call(q.device, _lib.load().sfa_rope_fwd, ctypes.byref(a), None)
-        # x itself is read again only where a norm has to be undone
+        # x itself is read again only where a norm has to be undone; the others
+        # are saved for autograd's check that nobody has written them since
         ctx.save_for_backward(q if c.wq is not None else None, k if c.wk is not None else None, q_weight, k_weight,
                               c.pos, c.freq)
-        ctx.opts = (eps, rope_offset, interleaved, rope_scale)
+        ctx.call = c
         ctx.set_materialize_grads(False)
         return qo, ko
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, pos, freq = ctx.saved_tensors
+        q, k, q_weight, k_weight, _, _ = ctx.saved_tensors
         need = ctx.needs_input_grad
         if not (need[0] or need[2]):
             gq = None
@@ -184,7 +185,7 @@ class _NormRope(torch.autograd.Function):
         any_g = gq if gq is not None else gk
         if any_g is None:
             return (None,) * 10
-        c = _Call(any_g, pos, freq, q_weight, k_weight, *ctx.opts)
+        c = ctx.call
         gq, gk = None if gq is None else rows(gq), None if gk is None else rows(gk)
         dq, dk = None if gq is None else _like(gq), None if gk is None else _like(gk)
         dwq = None if gq is None or c.wq is None else torch.empty_like(c.wq) if gq.numel() else torch.zeros_like(c.wq)
