@@ -1121,6 +1121,10 @@ struct MlaTree {
   static constexpr int kCh = kDv / 8, kCr = (kDqk - kDv) / 8;  // 16-byte chunks of the two parts of a row
 };
 
+// PAGE: tiles lie within one page (64 rows or more), whose rows have one base:
+// 250 us against 260 with an address per row (4 sequences of 8K to 32K keys, 8
+// tokens, 128 heads).
+template <bool PAGE>
 __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
   typedef MlaTree C;
   typedef Mfma16A MA;
@@ -1199,8 +1203,40 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
                        (uint32_t)__shfl((int)(uint32_t)ra, row, 64);
     dma16(dst + wave * RPW * CR, a + (uint64_t)(16 * (CH + ((ln & 7) ^ Swz<64>::at(row)))));
   };
+  // PAGE: the tile's base and row stride (a tile that is not there: zeros, stride 0)
+  const int64_t krow_bytes = 2 * p.k_ss;
+  struct TileBase {
+    uint64_t base;
+    int64_t row;
+    uint64_t mask;
+  };
+  auto page_tile = [&](int j, int pg) {
+    const int s = k0 + j * KEYS, n = k1 - s;
+    const bool ok = n > 0 && pg >= 0 && pg < p.num_pages;
+    TileBase t;
+    t.base = ok ? kbase + (uint64_t)((int64_t)pg * (2 * p.k_sb) + (int64_t)(s & ((1 << p.page_shift) - 1)) * krow_bytes)
+                : (uint64_t)(uintptr_t)kZeroRow;
+    t.row = ok ? krow_bytes : 0;
+    t.mask = !ok ? 0 : n >= KEYS ? ~0ull : (1ull << n) - 1;
+    return t;
+  };
+  auto page_row = [&](int i, const TileBase& t, u32x4* dst, int ln) {
+    const int row = wave * RPW + i;
+    dma16(dst + row * CH, t.base + (uint64_t)(row * t.row), 16u * (uint32_t)(ln ^ Swz<128>::at(row)));
+  };
+  auto page_tails = [&](const TileBase& t, u32x4* dst, int ln) {
+    const int row = wave * RPW + (ln >> 3);
+    dma16(dst + wave * RPW * CR, t.base + (uint64_t)(wave * RPW * t.row),
+          (uint32_t)((ln >> 3) * (int)t.row) + 16u * (uint32_t)(CH + ((ln & 7) ^ Swz<64>::at(row))));
+  };
   uint64_t mask;  // the rows of tile j that are there
-  {
+  if constexpr (PAGE) {
+    const TileBase t = page_tile(0, __builtin_amdgcn_readfirstlane(page_of(0, 0)));
+    mask = t.mask;
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) page_row(i, t, s_k[0], lane);
+    page_tails(t, s_r[0], lane);
+  } else {
     bool ok;
     const uint64_t ra = row_addr(0, page_of(0, lane), lane, ok);
     mask = __ballot(ok);
@@ -1208,7 +1244,7 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
     for (int i = 0; i < RPW; ++i) load_row(i, ra, s_k[0], lane);
     load_tails(ra, s_r[0], lane);
   }
-  int pg_next = page_of(1, lane);
+  int pg_next = page_of(1, PAGE ? 0 : lane);
 
   acc_t oacc[4][4];  // [16 dims][16 rows]
 #pragma unroll
@@ -1241,9 +1277,16 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
     };
 #pragma unroll
     for (int s = 0; s < 2; ++s) kf[s] = read_k(order(s));
-    bool ok;
-    const uint64_t ra = row_addr(j + 1, pg_next, ln, ok);
-    const uint64_t mask_next = __ballot(ok);
+    uint64_t ra = 0, mask_next;
+    TileBase tb = {};
+    if constexpr (PAGE) {
+      tb = page_tile(j + 1, __builtin_amdgcn_readfirstlane(pg_next));
+      mask_next = tb.mask;
+    } else {
+      bool ok;
+      ra = row_addr(j + 1, pg_next, ln, ok);
+      mask_next = __ballot(ok);
+    }
     if (tid == 0) s_over[(j + 1) & 1] = 0;
 
     // S^T of 16 keys x 32 rows
@@ -1265,11 +1308,17 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
       }
       pk = kf[i % 3];
       if constexpr (i == 14) ql[0] = lds_read_b128(s_q1, (uint32_t)((hq * 32 + 16 * rh + lt) * 16));
-      if constexpr (i % 2 == 1 && i / 2 < RPW) load_row(i / 2, ra, s_k[(j + 1) & 1], ln);
-      if constexpr (i == 17) load_tails(ra, s_r[(j + 1) & 1], ln);
+      // the next tile's rows
+      if constexpr (i % 2 == 1 && i / 2 < RPW) {
+        if constexpr (PAGE) page_row(i / 2, tb, s_k[(j + 1) & 1], ln);
+        else load_row(i / 2, ra, s_k[(j + 1) & 1], ln);
+      } else if constexpr (i == 17) {
+        if constexpr (PAGE) page_tails(tb, s_r[(j + 1) & 1], ln);
+        else load_tails(ra, s_r[(j + 1) & 1], ln);
+      }
     });
     __builtin_amdgcn_sched_barrier(0);
-    pg_next = page_of(j + 2, ln);
+    pg_next = page_of(j + 2, PAGE ? 0 : ln);
     MA::tail1(pk);
     MA::drain_v1(sacc[0]);
     MA::drain_v1(sacc[1]);
@@ -1597,7 +1646,9 @@ hipError_t launch_tree(const TreeParams& p0, const TreePlan& pl, int dtype, hipS
   p.nrb = (p.T * p.G + pl.rows - 1) / pl.rows;
   const unsigned grid = (unsigned)((int64_t)pl.slots * p.Hkv * p.nrb);
   if (pl.kernel == kMla) {
-    tree_mla_kernel<<<grid, 512, 0, s>>>(p);
+    // (row offsets of a tile fit the loads' 32 bits)
+    if (p.page_shift >= 6 && p.k_ss > 0 && p.k_ss < ((int64_t)1 << 24)) tree_mla_kernel<true><<<grid, 512, 0, s>>>(p);
+    else tree_mla_kernel<false><<<grid, 512, 0, s>>>(p);
   } else if (pl.kernel != kGeneric) {
     if (p.Dqk == 64) launch_mfma<64>(p, pl.kernel, grid, s);
     else launch_mfma<128>(p, pl.kernel, grid, s);
