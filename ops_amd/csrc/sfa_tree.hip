@@ -67,21 +67,20 @@ struct Slot {
 // than wanted, then longer ones until they are `want` or fewer, so that all
 // run at once (a few steps come within a tile of the best).
 __device__ Slot find_slot(const TreeParams& p, int slot) {
+  if (p.want == 0)  // one range a sequence
+    return slot < p.B ? Slot{slot, 0, seq_lens(p, slot).keys, slot, 1} : Slot{-1, 0, 0, 0, 0};
   const int lane = threadIdx.x & 63, shift = 31 - __builtin_clz(p.tile);
   auto tiles_of = [&](int b) { return b < p.B ? (seq_lens(p, b).keys + p.tile - 1) >> shift : 0; };
   const int mine = tiles_of(lane);  // (of the first 64 sequences)
-  int len = 0x7fffffff >> shift;    // in tiles; want = 0: one slot a sequence
-  if (p.want > 0) {
-    int64_t sum = lanes_sum(mine);
-    for (int b0 = 64; b0 < p.B; b0 += 64) sum += lanes_sum(tiles_of(b0 + lane));
-    len = max(2, (int)((sum + p.want - 1) / p.want));
-    for (int i = 0; i < 6 && p.want > p.B; ++i) {
-      auto ranges = [&](int t, int b) { return b < p.B ? max(1, (t + len - 1) / len) : 0; };
-      int n = lanes_sum(ranges(mine, lane));
-      for (int b0 = 64; b0 < p.B; b0 += 64) n += lanes_sum(ranges(tiles_of(b0 + lane), b0 + lane));
-      if (n <= p.want) break;
-      len = max(len + 1, (int)((int64_t)len * n / p.want));
-    }
+  int64_t sum = lanes_sum(mine);
+  for (int b0 = 64; b0 < p.B; b0 += 64) sum += lanes_sum(tiles_of(b0 + lane));
+  int len = max(2, (int)((sum + p.want - 1) / p.want));  // in tiles
+  for (int i = 0; i < 6; ++i) {
+    auto ranges = [&](int t, int b) { return b < p.B ? max(1, (t + len - 1) / len) : 0; };
+    int n = lanes_sum(ranges(mine, lane));
+    for (int b0 = 64; b0 < p.B; b0 += 64) n += lanes_sum(ranges(tiles_of(b0 + lane), b0 + lane));
+    if (n <= p.want) break;
+    len = max(len + 1, (int)((int64_t)len * n / p.want));
   }
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -1514,12 +1513,14 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
 }
 
 // ---- joining the slots of a sequence -------------------------------------------
-// One wave a row; LPR lanes hold the row (4 dims each), 64 / LPR slots at a
-// time.  A slot in which the row sees nothing has LSE -inf.
-template <typename T, int LPR>
-__global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), per = (int64_t)p.T * p.Hq;
+// WPR waves a row; LPR lanes hold the row (4 dims each), 64 / LPR slots at a time
+// and wave.  A slot in which the row sees nothing has LSE -inf.
+template <typename T, int LPR, int WPR>  // WPR: 1, or 4 and more
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void tree_combine_kernel(TreeParams p) {
+  constexpr int RPB = WPR > 4 ? 1 : 4 / WPR;  // rows a workgroup
+  __shared__ f32x4 s_x[WPR > 1 ? WPR - 1 : 1][LPR];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR, per = (int64_t)p.T * p.Hq;
   if (row >= p.B * per) return;
   const int b = (int)(row / per), r = (int)(row % per), h = r % p.Hq, t = r / p.Hq;
   const int first = p.seq_slots[2 * b], ns = p.seq_slots[2 * b + 1];
@@ -1540,16 +1541,16 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
   l = wave_sum(l + nan);
   float lse;
   const float f = finish_row(p, h, live, m, l, lse);
-  if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+  if (part == 0 && lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
   T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
-  constexpr int NP = 64 / LPR;  // slots at a time
+  constexpr int NP = 64 / LPR * WPR;  // slots at a time
   const int sub = lane / LPR;
   for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
     const int d = d0 + 4 * (lane % LPR);
     f32x4 x = {};
     if (f != 0.f) {
 #pragma unroll 4
-      for (int i = sub; i < ns; i += NP) {
+      for (int i = part * (64 / LPR) + sub; i < ns; i += NP) {
         const float e = exp2f(pl[i * per] - moff);
         f32x4 v = {};
         const float* at = po + i * per * p.Dv + d;
@@ -1566,19 +1567,35 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeParams p) {
     for (int s = LPR; s < 64; s <<= 1)
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], s, 64);
-    if (sub == 0)
+    if constexpr (WPR > 1) {  // (one row a workgroup: all of it comes here)
+      if (part > 0 && sub == 0) s_x[part - 1][lane] = x;
+      __syncthreads();
+      if (part == 0 && sub == 0)
+#pragma unroll
+        for (int w = 0; w < WPR - 1; ++w) x += s_x[w][lane];
+      __syncthreads();
+    }
+    if (part == 0 && sub == 0)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (d + k < p.Dv) o[d + k] = from_f32<T>(f == 0.f ? 0.f : x[k] * f);
   }
 }
 
+template <typename T, int WPR>
+void launch_combine(const TreeParams& p, hipStream_t s) {
+  const int64_t rows = (int64_t)p.B * p.T * p.Hq;
+  const unsigned grid = (unsigned)(WPR > 1 ? rows : (rows + 3) / 4), threads = WPR > 1 ? 64 * WPR : 256;
+  if (p.Dv <= 64) tree_combine_kernel<T, 16, WPR><<<grid, threads, 0, s>>>(p);
+  else if (p.Dv <= 128) tree_combine_kernel<T, 32, WPR><<<grid, threads, 0, s>>>(p);
+  else tree_combine_kernel<T, 64, WPR><<<grid, threads, 0, s>>>(p);
+}
 template <typename T>
 void launch_combine(const TreeParams& p, hipStream_t s) {
-  const unsigned grid = (unsigned)(((int64_t)p.B * p.T * p.Hq + 3) / 4);
-  if (p.Dv <= 64) tree_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p);
-  else if (p.Dv <= 128) tree_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p);
-  else tree_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p);
+  // Many slots of few rows are joined by eight waves a row (256 slots of 256
+  // rows: 13 us, 44 by one wave; 16 slots of 2048 rows: 10 by four, 8 by one).
+  if (p.want / p.B >= 32) launch_combine<T, 8>(p, s);
+  else launch_combine<T, 1>(p, s);
 }
 
 // Kernels by query rows per (sequence, kv head): rows a workgroup, tile keys, waves.
