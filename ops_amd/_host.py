@@ -28,6 +28,20 @@ def need_gpu(name: str, t: torch.Tensor, device: torch.device = None) -> None:
         raise ValueError(f"{name} must be on {device} (got {t.device})")
 
 
+def written(*tensors) -> None:
+    """The caller's tensors that a call is about to write: their elements must be
+    distinct in memory, and autograd is told, so that a graph that has saved one
+    raises instead of using what was written."""
+    for t in tensors:
+        if t is None:
+            continue
+        if 0 in t.stride() and any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
+            raise ValueError(f"a tensor that is written must not be expanded (shape {tuple(t.shape)}, strides {t.stride()})")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a tensor that is written must not require a gradient: call under torch.no_grad()")
+        torch.autograd.graph.increment_version(t)
+
+
 def rows(t: torch.Tensor) -> torch.Tensor:
     """The kernels need a unit stride on the feature dimension."""
     return t if t.stride(-1) == 1 else t.contiguous()

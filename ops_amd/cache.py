@@ -21,7 +21,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._host import call, int_vec, need_gpu
+from ._host import call, int_vec, need_gpu, written
 
 __all__ = ["cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path"]
 
@@ -35,6 +35,7 @@ def _state(name: str, t: torch.Tensor, dim: int, device) -> None:
     if t.dtype != torch.int32 or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
         raise ValueError(f"{name} must be a {dim}-D int32 tensor with unit stride (changed in place), got {t.dtype} "
                          f"{tuple(t.shape)}")
+    written(t)
 
 
 def _pools(caches: Sequence[torch.Tensor], device=None):
@@ -57,8 +58,11 @@ def _pools(caches: Sequence[torch.Tensor], device=None):
                              f"{c.device}")
         if not (c.is_contiguous() or c[0].is_contiguous()):
             raise ValueError("each page of a cache must be contiguous")
+        written(c)
         e = c.element_size()
         vals += (c.data_ptr(), c.stride(0) * e, c.numel() // num_pages * e)
+    if len(set(vals[::3])) != len(caches):
+        raise ValueError("a cache is listed twice")
     return struct.pack(f"@{len(vals)}q", *vals), len(caches), num_pages, page_size, device
 
 

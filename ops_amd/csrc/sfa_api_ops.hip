@@ -194,12 +194,14 @@ int check_cache(const sfa_cache* c, bool table, bool refs, bool lens, bool pools
     return fail(SFA_E_INVALID, "page_size must be a power of two (got %d)", c->page_size);
   if (c->num_pages <= 0 || (int64_t)c->num_pages * c->page_size > INT32_MAX)
     return fail(SFA_E_INVALID, "num_pages must be positive and num_pages * page_size below 2^31");
+  if (c->num_pages > 1 << 30) return fail(SFA_E_UNSUPPORTED, "more than 2^30 pages");
   if (table) {
     if (c->block_table == nullptr) return fail(SFA_E_INVALID, "null page table");
     if (c->B <= 0 || c->max_pages <= 0) return fail(SFA_E_INVALID, "B and max_pages must be positive");
     if ((int64_t)c->max_pages * c->page_size > INT32_MAX)
       return fail(SFA_E_INVALID, "max_pages * page_size must stay below 2^31");
     if (c->B > 1 && c->bt_sb < c->max_pages) return fail(SFA_E_INVALID, "block-table rows overlap");
+    if ((int64_t)c->B * c->max_pages > INT32_MAX) return fail(SFA_E_UNSUPPORTED, "a table of more than 2^31 entries");
   }
   if (refs && c->ref_counts == nullptr) return fail(SFA_E_INVALID, "null ref_counts");
   if (lens && c->kv_lens == nullptr) return fail(SFA_E_INVALID, "null kv_lens");

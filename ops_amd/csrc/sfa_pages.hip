@@ -304,17 +304,16 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(PagesParams p, con
     if (b < p.B && l == 0) s_need[b] = e1 < 0 ? -1 : need;
   }
   __syncthreads();
-  int want = 0;  // s_need[b] becomes the rank of b's first page; ok[b]: its count for now
+  int want = 0;  // (at most the table's entries) s_need[b] becomes the rank of b's first page; ok[b]: its count for now
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid, need = b < p.B ? s_need[b] : 0;
     int total;
-    const int64_t room = 0x7fffffff - want;
     const int at = block_scan(need > 0 ? need : 0, s_scan, total);
     if (b < p.B) {
       s_need[b] = want + at;
       ok[b] = need;
     }
-    want = total < room ? want + total : 0x7fffffff;
+    want += total;
   }
   int32_t* list = ws_pages(p, 0);
   const int found = find_free(p, want < p.num_pages ? want : p.num_pages, list, s_scan);

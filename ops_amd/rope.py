@@ -29,7 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import DTYPES, call, check_pool, int_rows, kv_pages, need_gpu, rows, table
+from ._host import DTYPES, call, check_pool, int_rows, kv_pages, need_gpu, rows, table, written
 
 __all__ = ["rope_frequencies", "rotary_embedding", "qk_norm_rope", "qk_norm_rope_append"]
 
@@ -208,7 +208,8 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     ``rope_scale``; ``positions`` ``[B, S]`` or ``[S]``, int32 or int64.
 
     Differentiable in ``x``.  With ``out`` (x's shape and type, unit feature
-    stride; ``x`` itself turns it in place) there is no gradient."""
+    stride; ``x`` itself turns it in place, any other memory must not overlap
+    x's) there is no gradient."""
     _check_rows("x", x)
     if out is None:
         return _NormRope.apply(x, None, None, None, positions, inv_freq, 0.0, rope_offset, interleaved, rope_scale)[0]
@@ -217,6 +218,7 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (x.numel() and out.stride(-1) != 1):
         raise ValueError(f"out must be a {list(x.shape)} {x.dtype} tensor on {x.device} with a unit feature stride")
     c = _Call(x, positions, inv_freq, None, None, 0.0, rope_offset, interleaved, rope_scale)
+    written(out)
     if x.numel() > 0:
         a = c.args(rows(x), None, out, None)
         call(x.device, _lib.load().sfa_rope_fwd, ctypes.byref(a), None)
@@ -288,6 +290,7 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
     if q is not None:
         q = rows(q)
         out = _like(q) if out is None else out
+    written(out, k_cache, v_cache)
     if k.numel() > 0:
         a = c.args(q, rows(k), out, k_cache, v, v_cache, slots)
         pg = kv_pages(bt, B, num_pages, page_size, dev)

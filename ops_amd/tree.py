@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._host import DTYPES, call, check_pool, int_vec, kv_pages, need_gpu, rows, table
+from ._host import DTYPES, call, check_pool, int_vec, kv_pages, need_gpu, rows, table, written
 
 __all__ = ["tree_attention_paged"]
 
@@ -40,7 +40,8 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     sees nothing gives zeros and ``lse = -inf`` (with ``attn_sink`` ``[Hq]``, which
     adds ``exp(sink)`` to each denominator: the sink), a token past
     ``tree_lens[b]`` zeros and ``-inf``.  ``out`` ``[B, T, Hq, Dv]`` in q's type and
-    ``lse`` ``[B, T, Hq]`` float32 may be preallocated.  No gradient."""
+    ``lse`` ``[B, T, Hq]`` float32 may be preallocated (memory of their own).  No
+    gradient."""
     if q.dim() != 4:
         raise ValueError(f"q must be 4-D (BSHD), got shape {tuple(q.shape)}")
     need_gpu("q", q)
@@ -80,6 +81,7 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         lse = torch.empty((B, T, Hq), dtype=torch.float32, device=dev)
     elif tuple(lse.shape) != (B, T, Hq) or lse.dtype != torch.float32 or lse.device != dev:
         raise ValueError(f"lse must be a {[B, T, Hq]} float32 tensor on {dev}")
+    written(out, lse)
     if B * T == 0:
         return out, lse
     lib = _lib.load()

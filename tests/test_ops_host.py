@@ -204,3 +204,28 @@ def test_rope_frequencies():
                 dict(rotary_dim=8, scaling="other"), dict(rotary_dim=2, scaling="ntk"), dict(rotary_dim=8, scaling="yarn")):
         with pytest.raises(ValueError):
             ops_amd.rope_frequencies(**bad)
+
+
+def test_sizes_past_the_counters_are_refused():
+    lib = _lib.load()
+    one = dict(num_pages=(1 << 30) + 1, page_size=1, npools=0)
+    assert lib.sfa_cache_free(ctypes.byref(_cache(**one)), P, None, 1, None) == _lib.SFA_E_UNSUPPORTED
+    many = dict(B=1 << 12, max_pages=1 << 20, bt_sb=1 << 20)
+    assert lib.sfa_cache_extend(ctypes.byref(_cache(**many)), P, P, P, 1 << 30, None) == _lib.SFA_E_UNSUPPORTED
+
+
+def test_tensors_that_are_written():
+    from ops_amd._host import written
+    t = torch.zeros(3, 4)
+    v = t._version
+    written(t, None, t[:1].expand(1, 4), t[:0].expand(0, 4))
+    assert t._version > v
+    with pytest.raises(ValueError, match="expanded"):
+        written(t[:1].expand(3, 4))
+    w = t.clone().requires_grad_(True)
+    with pytest.raises(ValueError, match="gradient"):
+        written(w)
+    with torch.no_grad():
+        written(w)
+    with torch.inference_mode():
+        written(torch.zeros(2))
