@@ -58,8 +58,15 @@ struct Chunk {
   }
 };
 
+// Positions, slots and tables through the scalar cache (no kernel here writes
+// them): a vector load would wait for all the rows in flight before it.
+template <typename I>
+__device__ __forceinline__ I load_const(const I* at) {
+  return *(const __attribute__((address_space(4))) I*)at;
+}
 __device__ __forceinline__ int64_t load_int(const void* base, int64_t i, int is64) {
-  return is64 ? reinterpret_cast<const int64_t*>(base)[i] : (int64_t) reinterpret_cast<const int32_t*>(base)[i];
+  return is64 ? load_const(reinterpret_cast<const int64_t*>(base) + i)
+              : (int64_t)load_const(reinterpret_cast<const int32_t*>(base) + i);
 }
 
 // cos and sin of pos * f.  The angle is reduced in float64 to quarter turns q
@@ -134,12 +141,19 @@ struct Turn {
       sgn = first ? -1.f : 1.f;
     }
   }
-  __device__ __forceinline__ void angles(const RopeParams& p, double pos, float (&cs)[E], float (&sn)[E]) const {
+  __device__ __forceinline__ void freqs(const RopeParams& p, double (&f)[E]) const {
+    each<E>([&](auto ec) {
+      constexpr int e = decltype(ec)::value;
+      f[e] = on && (e < E / 2 || !p.interleaved) ? p.freq[i0 + e] : 0.0;
+    });
+  }
+  __device__ __forceinline__ void angles(const RopeParams& p, double pos, const double (&f)[E], float (&cs)[E],
+                                         float (&sn)[E]) const {
     const float sc = p.rope_scale;
     each<E>([&](auto ec) {
       constexpr int e = decltype(ec)::value;
       float c = 1.f, s = 0.f;
-      if (e < E / 2 || !p.interleaved) angle(pos, on ? p.freq[i0 + e] : 0.0, c, s);
+      if (e < E / 2 || !p.interleaved) angle(pos, f[e], c, s);
       cs[e] = c * sc;
       sn[e] = s * sc;
     });
@@ -175,7 +189,7 @@ __device__ __forceinline__ u32x4 shfl16(const u32x4& x, int lane) {
 __device__ __forceinline__ int64_t cache_row(const RopeParams& p, int b, int s, int64_t page_stride, int64_t row_stride) {
   const int64_t slot = load_int(p.slots, b * p.slot_sb + s * p.slot_ss, p.slot_i64);
   if (slot < 0 || slot >= ((int64_t)p.max_pages << p.page_shift)) return -1;
-  const int pg = p.block_table[b * p.bt_sb + (slot >> p.page_shift)];
+  const int pg = load_const(p.block_table + b * p.bt_sb + (slot >> p.page_shift));
   if (pg < 0 || pg >= p.num_pages) return -1;
   return (int64_t)pg * page_stride + (slot & ((1 << p.page_shift) - 1)) * row_stride;
 }
@@ -188,11 +202,13 @@ struct Row {
   static constexpr int E = Chunk<T>::E;
   static constexpr bool kHeld = IN || K == 1;  // the lane's angles serve all its rows
   u32x4 r[K];
-  __device__ __forceinline__ void load(const RopeParams& p, const T* x, int l, int n) {  // chunks below dim n
+  // (chunks past dim n > 0: the first one again, so that the number of loads in
+  // flight does not depend on the lane)
+  __device__ __forceinline__ void load(const RopeParams& p, const T* x, int l, int n) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int c = j * P + l;
-      r[j] = c * E < n ? *reinterpret_cast<const u32x4*>(x + c * E) : u32x4{0, 0, 0, 0};
+      r[j] = *reinterpret_cast<const u32x4*>(x + (c * E < n ? c * E : 0));
     }
   }
   __device__ __forceinline__ void store(const RopeParams& p, T* y, int l) const {
@@ -247,8 +263,10 @@ struct Row {
         if constexpr (K == 1) {
           t.apply(p, u, o, cs, sn, dir);
         } else if (t.on) {
+          double f2[E];
           float c2[E], s2[E];
-          t.angles(p, pos, c2, s2);
+          t.freqs(p, f2);
+          t.angles(p, pos, f2, c2, s2);
           t.apply(p, u, o, c2, s2, dir);
         }
         put(j, c, u);
@@ -256,12 +274,6 @@ struct Row {
     }
   }
 };
-
-template <typename T, int P, bool IN>
-__device__ __forceinline__ void lane_angles(const RopeParams& p, int l, double pos, float (&cs)[Chunk<T>::E],
-                                            float (&sn)[Chunk<T>::E]) {
-  Turn<Chunk<T>::E>(p, l).angles(p, pos, cs, sn);
-}
 
 // The weights of a whole chunk.
 template <typename T>
@@ -309,8 +321,7 @@ struct Weights {
 
 // A wave's walk over (token, row group) units: blocks of `per` groups of a
 // token (p.per, p.upt blocks a token), every nw-th block, so that the waves of the
-// card read one window of the tensor at a time (strided rows, 128 of 1152
-// bytes: 142 us with a contiguous run per wave).
+// card read one window of the tensor at a time.
 struct Walk {
   uint32_t blk, nblk, nw;
   int b, s, g, g1;
@@ -322,23 +333,32 @@ struct Walk {
     g1 = min(g + per, groups);
   }
   __device__ __forceinline__ bool live() const { return blk < nblk; }
-  // the next unit; fresh: of another block (another token's, perhaps)
+  // the next unit; fresh: of another block (another token's, perhaps).  Past the
+  // last one the walk is not live and stays at it: its addresses remain good.
   __device__ __forceinline__ bool next(const RopeParams& p, int groups, int per, int upt) {
     if (++g < g1) return false;
     blk += nw;
     if (blk < nblk) at(p, groups, per, upt);
+    else g = g1 - 1;
     return true;
   }
 };
 
 // Forward.  The units are (token, row group): the q heads' groups (64 / P rows
-// each), the k heads', then (append) 64-chunk groups of the v row.  A wave
-// loads the next unit's rows before it works on this one's.
-template <typename T, int P, int K, bool IN>
+// each), the k heads', then (append) 64-chunk groups of the v row.  NB units are
+// in flight, each in registers of its own that are refilled as soon as its
+// results are stored: the next unit's rows handed on from register to register
+// are waited for at the copy.  So 8192 tokens of 128 rows of 64 dims take 91 us
+// for 162 (read past the caches; a copy of the same rows 81), 2 x 8192 tokens of
+// 34 normed heads of 128 dims 91 for 119 (285 MB).  More in flight gains nothing
+// (NB 4 and 6, or 3 of rows in two chunks: 93, 95 us; 112).  Calls of one unit a wave take
+// NB = 1 (8.8 us for 11, 64 tokens into the cache: less code to fetch).
+template <typename T, int P, int K, bool IN, int NB>
 __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kernel(RopeParams p) {
   typedef Row<T, P, K, IN> R;
   constexpr int E = R::E, rpw = 64 / P;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (P - 1), rr = lane / P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l = lane & (P - 1), rr = lane / P;
   Walk w;
   w.nw = gridDim.x * 4;
   w.blk = blockIdx.x * 4 + wave;
@@ -351,112 +371,126 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
     R x;
     const T* px;
     T* py;
-    int b, s, g;
-    bool put;
+    int64_t pos;
+    int g;
+    bool live, fresh, put;
   };
-  auto load = [&](Unit& u) {
-    if (u.g >= gk) return;  // a v group
+  bool fresh = true;
+  auto fill = [&](Unit& u) __attribute__((always_inline)) {  // the walk's unit (past its end: the last one, again)
+    u.live = w.live();
+    u.fresh = fresh;
+    u.g = w.g;
+    u.pos = load_int(p.pos, w.b * p.pos_sb + w.s * p.pos_ss, p.pos_i64);
+    int64_t yo;
+    if (w.g >= gk) {  // of the v row: 64 chunks
+      const int i = (w.g - gk) * 64 + lane, cpr = p.Dv / E;
+      const bool in = i < p.side[1].H * cpr;
+      const int h = in ? i / cpr : 0, c = in ? i % cpr : 0;
+      u.px = reinterpret_cast<const T*>(p.v) + w.b * p.v_sb + w.s * p.v_ss + h * p.v_sh + c * E;
+#pragma unroll
+      for (int j = 0; j < K; ++j) u.x.r[j] = *reinterpret_cast<const u32x4*>(u.px);
+      yo = cache_row(p, w.b, w.s, p.vo_sb, p.vo_ss);
+      u.put = in && yo >= 0;
+      u.py = reinterpret_cast<T*>(p.v_out) + yo + h * p.vo_sh + c * E;
+    } else {
+      const int si = w.g < gq ? 0 : 1;
+      const RopeSide& sd = p.side[si];
+      const int h = (si == 0 ? w.g : w.g - gq) * rpw + rr;
+      const int64_t hh = h < sd.H ? h : 0;
+      u.px = reinterpret_cast<const T*>(sd.x) + w.b * sd.x_sb + w.s * sd.x_ss + hh * sd.x_sh;
+      u.x.load(p, u.px, l, p.D);
+      if (si == 1 && p.block_table != nullptr) yo = cache_row(p, w.b, w.s, sd.y_sb, sd.y_ss);
+      else yo = w.b * sd.y_sb + w.s * sd.y_ss;
+      u.put = h < sd.H && yo >= 0;
+      u.py = reinterpret_cast<T*>(sd.y) + yo + hh * sd.y_sh;
+    }
+    if (u.live) fresh = w.next(p, p.groups, p.per, p.upt);
+  };
+  double freq[E];
+  float cs[E], sn[E];
+  const Turn<E> lt(p, l);
+  if constexpr (R::kHeld) lt.freqs(p, freq);
+  Weights<T, P, K, IN> wt[R::kHeld ? 2 : 1];
+  if constexpr (R::kHeld) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+      if (p.side[a].n > 0) wt[a].load(p, p.side[a], l);
+  }
+  auto work = [&](Unit& u) __attribute__((always_inline)) {
+    const double pos = (double)u.pos;
+    if constexpr (R::kHeld) {
+      if (u.fresh) lt.angles(p, pos, freq, cs, sn);
+    }
+    if (u.g >= gk) {  // v is copied
+      if (u.put) *reinterpret_cast<u32x4*>(u.py) = u.x.r[0];
+      return;
+    }
     const int si = u.g < gq ? 0 : 1;
     const RopeSide& sd = p.side[si];
-    const int h = (si == 0 ? u.g : u.g - gq) * rpw + rr;
-    u.put = h < sd.H;
-    const int64_t hh = u.put ? h : 0;
-    u.px = reinterpret_cast<const T*>(sd.x) + u.b * sd.x_sb + u.s * sd.x_ss + hh * sd.x_sh;
-    u.x.load(p, u.px, l, p.D);
-    int64_t yo;
-    if (si == 1 && p.block_table != nullptr) yo = cache_row(p, u.b, u.s, sd.y_sb, sd.y_ss);
-    else yo = u.b * sd.y_sb + u.s * sd.y_ss;
-    u.py = reinterpret_cast<T*>(sd.y) + yo + hh * sd.y_sh;
-    u.put = u.put && yo >= 0;
-  };
-  Unit cur;
-  cur.b = w.b;
-  cur.s = w.s;
-  cur.g = w.g;
-  load(cur);
-  double pos = 0.0;
-  float cs[E], sn[E];
-  bool fresh = true;
-  int held = -1;
-  Weights<T, P, K, IN> wt;
-  while (true) {
-    if (fresh) {
-      pos = (double)load_int(p.pos, cur.b * p.pos_sb + cur.s * p.pos_ss, p.pos_i64);
-      if constexpr (R::kHeld) lane_angles<T, P, IN>(p, l, pos, cs, sn);
-    }
-    fresh = w.next(p, p.groups, p.per, p.upt);
-    const bool more = w.live();
-    Unit nxt;
-    nxt.b = w.b;
-    nxt.s = w.s;
-    nxt.g = w.g;
-    if constexpr (K <= 2) {
-      if (more) load(nxt);
-    }
-    if (cur.g >= gk) {  // the v row: copied
-      const int i = (cur.g - gk) * 64 + lane, cpr = p.Dv / E;
-      const int64_t row = cache_row(p, cur.b, cur.s, p.vo_sb, p.vo_ss);
-      if (i < p.side[1].H * cpr && row >= 0) {
-        const int h = i / cpr, c = i % cpr;
-        const T* v = reinterpret_cast<const T*>(p.v) + cur.b * p.v_sb + cur.s * p.v_ss + h * p.v_sh + c * E;
-        *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(p.v_out) + row + h * p.vo_sh + c * E) =
-            *reinterpret_cast<const u32x4*>(v);
+    float r = 1.f;
+    if (sd.n > 0) {
+      float q = 0.f;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        float f[E];
+        Chunk<T>::unpack(u.x.r[j], f);
+        float q4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) q4[e & 3] = fmaf(f[e], f[e], q4[e & 3]);
+        if ((j * P + l) * E < sd.n) q += (q4[0] + q4[1]) + (q4[2] + q4[3]);
       }
-    } else {
-      const int si = cur.g < gq ? 0 : 1;
-      const RopeSide& sd = p.side[si];
-      float r = 1.f;
-      if (sd.n > 0) {
-        if (held != si) {
-          held = si;
-          wt.load(p, sd, l);
-        }
-        float q = 0.f;
+      r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
+    }
+    u.x.turn(
+        p, u.px, lane, pos, cs, sn, 1.f,
+        [&](int j, int c, float (&v)[E]) {
+          if (c * E < sd.n) {
+            float wc[E];
+            if constexpr (R::kHeld) {
+              float w0[E], w1[E];
+              wt[0].chunk(p, sd, j, c, w0);
+              wt[1].chunk(p, sd, j, c, w1);
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-          float f[E];
-          Chunk<T>::unpack(cur.x.r[j], f);
-          float q4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < E; ++e) q4[e & 3] = fmaf(f[e], f[e], q4[e & 3]);
-          if ((j * P + l) * E < sd.n) q += (q4[0] + q4[1]) + (q4[2] + q4[3]);
-        }
-        r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
-      }
-      cur.x.turn(
-          p, cur.px, lane, pos, cs, sn, 1.f,
-          [&](int j, int c, float (&v)[E]) {
-            if (c * E < sd.n) {
-              float wc[E];
-              wt.chunk(p, sd, j, c, wc);
-#pragma unroll
-              for (int e = 0; e < E; ++e) v[e] = v[e] * r * wc[e];
+              for (int e = 0; e < E; ++e) wc[e] = si == 0 ? w0[e] : w1[e];
+            } else {
+              wt[0].chunk(p, sd, j, c, wc);
             }
-          },
-          [&](int j, int c, const float (&v)[E]) { cur.x.r[j] = Chunk<T>::pack(v); });
-      // (every value of the row has been read: y may be x)
-      if (cur.put) cur.x.store(p, cur.py, l);
-    }
-    if (!more) break;
-    if constexpr (K <= 2) {
-      cur = nxt;
-    } else {
-      cur.b = nxt.b;
-      cur.s = nxt.s;
-      cur.g = nxt.g;
-      load(cur);
-    }
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = v[e] * r * wc[e];
+          }
+        },
+        [&](int j, int c, const float (&v)[E]) { u.x.r[j] = Chunk<T>::pack(v); });
+    // (every value of the row has been read: y may be x)
+    if (u.put) u.x.store(p, u.py, l);
+  };
+  Unit u[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) fill(u[i]);
+  bool more = true;
+  while (more) {
+    each<NB>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      more = more && u[i].live;
+      if (!more) return;
+      work(u[i]);
+      if (NB == 1 && !w.live()) more = false;
+      else fill(u[i]);
+    });
   }
 }
 
 // Backward of one tensor (blockIdx.y: q or k): side.y is dy, side.dx receives
-// dx.  A wave walks over units as in the forward and sums its rows' dw in registers; a workgroup writes its sums to partial row blockIdx.x,
-// which rope_dw_kernel adds up in order.
-template <typename T, int P, int K, bool IN>
+// dx.  A wave walks over units as in the forward, NB of them in flight, and sums
+// its rows' dw in registers; a workgroup writes its sums to partial row
+// blockIdx.x, which rope_dw_kernel adds up in order.  NORM: some side is normed.
+// (The sizes above: 54 us with NB = 2 for 64, and 110 us, 428 MB, with NB = 1,
+// where x and dy keep four loads a lane in flight, 124 with 2.)
+template <typename T, int P, int K, bool IN, bool NORM, int NB>
 __global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p) {
   typedef Row<T, P, K, IN> R;
   constexpr int E = R::E, rpw = 64 / P;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (P - 1), rr = lane / P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l = lane & (P - 1), rr = lane / P;
   const int si = blockIdx.y;
   const RopeSide& sd = p.side[si];
   if (sd.H == 0) return;
@@ -465,10 +499,13 @@ __global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p) {
   w.nw = gridDim.x * 4;
   w.blk = blockIdx.x * 4 + wave;
   w.nblk = (uint32_t)p.B * (uint32_t)p.S * (uint32_t)upt;
-  if (w.live()) w.at(p, sd.groups, per, upt);
 
   Weights<T, P, K, IN> wt;
   if (sd.n > 0) wt.load(p, sd, l);
+  double freq[E];
+  float cs[E], sn[E];
+  const Turn<E> lt(p, l);
+  if constexpr (R::kHeld) lt.freqs(p, freq);
   float dw[K][E];
 #pragma unroll
   for (int j = 0; j < K; ++j)
@@ -479,80 +516,95 @@ __global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p) {
     R dy, x;
     const T* py;
     T* px;
-    bool live;
+    int64_t pos;
+    bool on, fresh, live;  // on: a unit of the walk; live: the lane's row is one
   };
-  auto load = [&](Unit& u, int b, int s, int g) {
-    const int h = g * rpw + rr;
+  bool fresh = true;
+  auto fill = [&](Unit& u) __attribute__((always_inline)) {  // the walk's unit (past its end: the last one, again)
+    u.on = w.live();
+    u.fresh = fresh;
+    u.pos = load_int(p.pos, w.b * p.pos_sb + w.s * p.pos_ss, p.pos_i64);
+    const int h = w.g * rpw + rr;
     u.live = h < sd.H;
     const int64_t hh = u.live ? h : 0;
-    u.py = reinterpret_cast<const T*>(sd.y) + b * sd.y_sb + s * sd.y_ss + hh * sd.y_sh;
-    u.px = reinterpret_cast<T*>(sd.dx) + b * sd.dx_sb + s * sd.dx_ss + hh * sd.dx_sh;
+    u.py = reinterpret_cast<const T*>(sd.y) + w.b * sd.y_sb + w.s * sd.y_ss + hh * sd.y_sh;
+    u.px = reinterpret_cast<T*>(sd.dx) + w.b * sd.dx_sb + w.s * sd.dx_ss + hh * sd.dx_sh;
     u.dy.load(p, u.py, l, p.D);
-    if (sd.n > 0) u.x.load(p, reinterpret_cast<const T*>(sd.x) + b * sd.x_sb + s * sd.x_ss + hh * sd.x_sh, l, sd.n);
-  };
-  Unit cur;
-  if (w.live()) load(cur, w.b, w.s, w.g);
-  double pos = 0.0;
-  float cs[E], sn[E];
-  bool fresh = true;
-  while (w.live()) {
-    if (fresh) {
-      pos = (double)load_int(p.pos, w.b * p.pos_sb + w.s * p.pos_ss, p.pos_i64);
-      if constexpr (R::kHeld) lane_angles<T, P, IN>(p, l, pos, cs, sn);
+    if constexpr (NORM) {  // (a side without a norm: dy again)
+      const T* x = sd.n > 0 ? reinterpret_cast<const T*>(sd.x) + w.b * sd.x_sb + w.s * sd.x_ss + hh * sd.x_sh : u.py;
+      u.x.load(p, x, l, sd.n > 0 ? sd.n : p.D);
     }
-    fresh = w.next(p, sd.groups, per, upt);
-    Unit nxt;
-    if constexpr (K <= 2) {
-      if (w.live()) load(nxt, w.b, w.s, w.g);
+    if (u.on) fresh = w.next(p, sd.groups, per, upt);
+  };
+  auto work = [&](Unit& u) __attribute__((always_inline)) {
+    const double pos = (double)u.pos;
+    if constexpr (R::kHeld) {
+      if (u.fresh) lt.angles(p, pos, freq, cs, sn);
     }
     float du[K][E];
     float q = 0.f, gx = 0.f;  // sum x^2, sum (du w) x
-    cur.dy.turn(
-        p, cur.py, lane, pos, cs, sn, -1.f, [](int, int, float (&)[E]) {},
+    u.dy.turn(
+        p, u.py, lane, pos, cs, sn, -1.f, [](int, int, float (&)[E]) {},
         [&](int j, int c, const float (&v)[E]) {
 #pragma unroll
           for (int e = 0; e < E; ++e) du[j][e] = v[e];
-          if (c * E < sd.n) {
-            float x[E], wc[E];
-            Chunk<T>::unpack(cur.x.r[j], x);
-            wt.chunk(p, sd, j, c, wc);
-            float q2[2] = {0.f, 0.f}, g2[2] = {0.f, 0.f};
+          if constexpr (NORM) {
+            if (c * E < sd.n) {
+              float x[E], wc[E];
+              Chunk<T>::unpack(u.x.r[j], x);
+              wt.chunk(p, sd, j, c, wc);
+              float q2[2] = {0.f, 0.f}, g2[2] = {0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              q2[e & 1] = fmaf(x[e], x[e], q2[e & 1]);
-              g2[e & 1] = fmaf(v[e] * wc[e], x[e], g2[e & 1]);
+              for (int e = 0; e < E; ++e) {
+                q2[e & 1] = fmaf(x[e], x[e], q2[e & 1]);
+                g2[e & 1] = fmaf(v[e] * wc[e], x[e], g2[e & 1]);
+              }
+              q += q2[0] + q2[1];
+              gx += g2[0] + g2[1];
             }
-            q += q2[0] + q2[1];
-            gx += g2[0] + g2[1];
           }
         });
     R res;
     float r = 0.f, m = 0.f;  // 1 / rms, mean of (du w) xhat
-    if (sd.n > 0) {
+    if (NORM && sd.n > 0) {
       r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
       m = row_sum<P>(gx) * r / (float)sd.n;
     }
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       const int c = j * P + l;
-      if (c * E < sd.n) {
-        float x[E], wc[E];
-        Chunk<T>::unpack(cur.x.r[j], x);
-        wt.chunk(p, sd, j, c, wc);
+      if constexpr (NORM) {
+        if (c * E < sd.n) {
+          float x[E], wc[E];
+          Chunk<T>::unpack(u.x.r[j], x);
+          wt.chunk(p, sd, j, c, wc);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float xh = x[e] * r, d = du[j][e];
-          dw[j][e] = fmaf(cur.live ? d : 0.f, xh, dw[j][e]);
-          du[j][e] = r * (d * wc[e] - xh * m);
+          for (int e = 0; e < E; ++e) {
+            const float xh = x[e] * r, d = du[j][e];
+            dw[j][e] = fmaf(u.live ? d : 0.f, xh, dw[j][e]);
+            du[j][e] = r * (d * wc[e] - xh * m);
+          }
         }
       }
       res.r[j] = Chunk<T>::pack(du[j]);
     }
-    if (cur.live) res.store(p, cur.px, l);
-    if constexpr (K <= 2) {
-      cur = nxt;
-    } else if (w.live()) {
-      load(cur, w.b, w.s, w.g);
+    if (u.live) res.store(p, u.px, l);
+  };
+  if (w.live()) {
+    w.at(p, sd.groups, per, upt);
+    Unit u[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) fill(u[i]);
+    bool more = true;
+    while (more) {
+      each<NB>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        more = more && u[i].on;
+        if (!more) return;
+        work(u[i]);
+        if (NB == 1 && !w.live()) more = false;
+        else fill(u[i]);
+      });
     }
   }
 
@@ -739,9 +791,10 @@ __global__ __launch_bounds__(256) void rope_bwd_scalar_kernel(RopeParams p) {
 }
 
 // Workgroups of 4 waves for so many units: no more than stay on the card.
+constexpr int kWaves = 4096;
 int rope_wgs(int64_t units) {
   const int64_t w = (units + 3) / 4;
-  return (int)(w < 1 ? 1 : w > 1024 ? 1024 : w);
+  return (int)(w < 1 ? 1 : w > kWaves / 4 ? kWaves / 4 : w);
 }
 
 // The kernel of a geometry: f.template operator()<P, K, IN>()
@@ -769,7 +822,10 @@ struct Fwd {
   hipStream_t s;
   template <int P, int K, bool IN>
   void run() const {
-    rope_fwd_kernel<T, P, K, IN><<<(unsigned)rope_wgs(p.units), 256, 0, s>>>(p);
+    constexpr int NB = K == 1 ? 3 : K == 2 ? 2 : 1;
+    const unsigned grid = (unsigned)rope_wgs(p.units);
+    if (NB > 1 && p.units > kWaves) rope_fwd_kernel<T, P, K, IN, NB><<<grid, 256, 0, s>>>(p);
+    else rope_fwd_kernel<T, P, K, IN, 1><<<grid, 256, 0, s>>>(p);
   }
 };
 template <typename T>
@@ -777,9 +833,17 @@ struct Bwd {
   const RopeParams& p;
   int wgs;
   hipStream_t s;
+  template <int P, int K, bool IN, int NB>
+  void launch(dim3 grid) const {
+    if (p.side[0].n > 0 || p.side[1].n > 0) rope_bwd_kernel<T, P, K, IN, true, NB><<<grid, 256, 0, s>>>(p);
+    else rope_bwd_kernel<T, P, K, IN, false, NB><<<grid, 256, 0, s>>>(p);
+  }
   template <int P, int K, bool IN>
   void run() const {
-    rope_bwd_kernel<T, P, K, IN><<<dim3((unsigned)wgs, p.side[1].H > 0 ? 2 : 1), 256, 0, s>>>(p);
+    const dim3 grid((unsigned)wgs, p.side[1].H > 0 ? 2 : 1);
+    constexpr int NB = K == 1 ? 2 : 1;
+    if (NB > 1 && p.units > kWaves) launch<P, K, IN, NB>(grid);
+    else launch<P, K, IN, 1>(grid);
   }
 };
 
@@ -827,11 +891,11 @@ void rope_geometry(RopeParams& p, int esize, bool vec) {
   p.groups = p.side[0].groups + p.side[1].groups + vg;
   p.units = (int64_t)p.B * p.S * p.groups;
   // Results that pass the L2s (32 MB) are stored past them: forward and backward
-  // of 2 x 8192 tokens, 34 heads of 128 dims 97 + 121 -> 76 + 111 us (285 + 428 MB);
-  // 67 MB from strided rows 142 -> 126, from whole ones 55 -> 58 us.
+  // of 2 x 8192 tokens, 34 heads of 128 dims (285 + 428 MB) took 97 + 121 us with
+  // plain stores, 76 + 111 so.
   p.stream = (int64_t)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * esize > ((int64_t)32 << 20);
   // blocks of up to 8 groups (a token's angles serve them) once there are 4096 waves of them
-  const int64_t per = p.units / 4096;
+  const int64_t per = p.units / kWaves;
   p.per = (int)(per < 1 ? 1 : per > 8 ? 8 : per);
   if (p.per > p.groups) p.per = p.groups;
   p.upt = (p.groups + p.per - 1) / p.per;
