@@ -1593,8 +1593,8 @@ void launch_combine(const TreeParams& p, hipStream_t s) {
 template <typename T>
 void launch_combine(const TreeParams& p, hipStream_t s) {
   // Many slots of few rows are joined by eight waves a row (256 slots of 256
-  // rows: 13 us, 44 by one wave; 16 slots of 2048 rows: 10 by four, 8 by one).
-  if (p.want / p.B >= 32) launch_combine<T, 8>(p, s);
+  // rows: 13 us, 44 by one wave; 64 of 1024: 14 and 22; but 32 of 2048: 20 and 12).
+  if (p.want / p.B >= 32 && (int64_t)p.B * p.T * p.Hq <= 1024) launch_combine<T, 8>(p, s);
   else launch_combine<T, 1>(p, s);
 }
 
@@ -1632,8 +1632,14 @@ void launch_mfma(const TreeParams& p, int kernel, unsigned grid, hipStream_t s) 
 TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
   TreePlan pl{};
   const int64_t R = (int64_t)p.T * p.G;
+  // Few keys and heads: fewer rows a workgroup give more workgroups, whose key
+  // rows meet in the L2 (whole call, 1 sequence, d = 128, 128 rows: 2K keys 16 us with
+  // 16 rows, 22 with 128; 32K: 27, 26 with 32 rows, 33; 1024 rows: 4K 44, 29, 38, 16K
+  // 103, 45, 46).  fit: workgroups of the shortest ranges, 256 keys.
+  auto fit = [&](int rows) { return (int64_t)p.B * p.Hkv * ((R + rows - 1) / rows) * (((int64_t)p.cap + 255) / 256); };
   if (dtype == SFA_DTYPE_BF16 && vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
-    pl.kernel = R <= 16 ? kRows16 : R <= 32 ? kRows32 : R <= 64 ? kRows64 : R <= 128 ? kRows128 : kRows256;
+    pl.kernel = R <= 16 || fit(16) <= 2 * kWorkgroups ? kRows16 : R <= 32 || fit(32) <= 5 * kWorkgroups ? kRows32
+              : R <= 64 ? kRows64 : R <= 128 ? kRows128 : kRows256;
   if (dtype == SFA_DTYPE_BF16 && vec && p.Dqk == 576 && p.Dv == 512 && p.v == p.k && p.v_sb == p.k_sb && p.v_ss == p.k_ss &&
       p.v_sh == p.k_sh)
     pl.kernel = kMla;

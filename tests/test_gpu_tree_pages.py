@@ -9,7 +9,7 @@ import torch
 
 import ops_amd
 from tests import ops_ref as ref
-from tests.test_gpu_tree import BF16, DEV, F32, _check, _g, _masks, _pool
+from tests.test_gpu_tree import BF16, CASES, DEV, F32, _check, _g, _masks, _pool
 
 pytestmark = pytest.mark.gpu
 
@@ -21,10 +21,31 @@ KINDS = [("rows16", BF16, 4, 8, 2, 128, 128, False), ("rows32", BF16, 4, 8, 1, 6
          ("mla-200", BF16, 5, 40, 1, 576, 512, True), ("f32", F32, 4, 4, 2, 64, 64, False)]
 
 
+def _wide(bt, ps):
+    """The table with room for 2^17 rows: the kernels of many rows a workgroup,
+    which short tables leave to those of 16 and 32."""
+    return torch.cat((bt, torch.full((bt.shape[0], (1 << 17) // ps), -1, dtype=torch.int32, device=DEV)), 1)
+
+
+@pytest.mark.parametrize("c", CASES, ids=[c[0] for c in CASES])
+def test_wide_tables(c):
+    _, dt, T, Hq, Hkv, Dk, Dv, shared, ps, ctx, with_sink = c
+    g = _g(27)
+    B = len(ctx)
+    kc, vc, bt = _pool(g, B, (max(ctx) + T + ps - 1) // ps + 1, ps, Hkv, Dk, Dv, dt, shared)
+    q = (2 * torch.randn(B, T, Hq, Dk, generator=g, device=DEV)).to(dt)
+    mask, cl = _masks(B, T, 28), torch.tensor(ctx, dtype=torch.int32, device=DEV)
+    sink = torch.randn(Hq, generator=g, device=DEV) if with_sink else None
+    out, lse = ops_amd.tree_attention_paged(q, kc, vc, _wide(bt, ps), cl, mask, attn_sink=sink)
+    torch.cuda.synchronize()
+    _check(q, kc, vc, bt, ctx, mask, None, 1 / math.sqrt(Dk), sink, out, lse)
+
+
 @pytest.mark.parametrize("k", KINDS, ids=[k[0] for k in KINDS])
 @pytest.mark.parametrize("ps", [16, 32, 64, 256])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("bad", [math.nan, -math.inf])
-def test_unseen_rows_of_a_page_may_hold_anything(k, ps, bad):
+def test_unseen_rows_of_a_page_may_hold_anything(k, ps, wide, bad):
     _, dt, T, Hq, Hkv, Dk, Dv, shared = k
     g = _g(21)
     ctx = [37, 192, 700]
@@ -45,7 +66,7 @@ def test_unseen_rows_of_a_page_may_hold_anything(k, ps, bad):
     kc[ok] = bad
     if not shared:
         vc[ok] = bad
-    out, lse = ops_amd.tree_attention_paged(q, kc, vc, bt, cl, mask, nodes)
+    out, lse = ops_amd.tree_attention_paged(q, kc, vc, _wide(bt, ps) if wide else bt, cl, mask, nodes)
     torch.cuda.synchronize()
     rows = [t for t in range(T) if t != 1]
     out, lse, o, l, pv, mag = (x[:, rows].double() for x in (out, lse, o, l, pv, mag))
