@@ -823,9 +823,12 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
 // after every second product or so, the softmax of tile j, which depends on
 // neither.  Sums and Q stay in AGPRs (inline asm: the compiler would copy Q to
 // VGPRs for every product); sched_barrier keeps the order that is written here.
-// 16 sequences of 4K-32K keys, 256 rows (one of 128K keys, 8 kv heads): 122 (190) us.
+// 16 sequences of 4K-32K keys, 256 rows (one of 128K keys, 8 kv heads): 115 (180) us,
+// the matrix cores busy 0.35 (0.39) of the time, 4.5 VALU instructions a product.
 // 64 rows a wave read half as much from LDS and took 132 (198) us with one wave a
 // SIMD, 256 (406) us with two, which spill; without the overlap 163 (248) us.
+// PAGE: tiles of 32 keys lie within one page, whose rows have one base and stride
+// (198 us for 208 with an address per row, 128K keys, 64 rows a wave).
 template <int D, int NG, int WR, int WK, int NS, bool PAGE>
 __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_pipe_kernel(TreeParams p) {
   using M = Mfma16A;
@@ -1653,6 +1656,7 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
     pl.kernel = kMla;
   pl.rows = kShapes[pl.kernel].rows;
   const int64_t nrb = (R + pl.rows - 1) / pl.rows, min_len = 2 * kShapes[pl.kernel].tile;
+  // (the generic kernel's workgroups are four to a CU)
   int64_t want = (pl.kernel == kGeneric ? 4 : 1) * kWorkgroups / (p.Hkv * nrb);
   const int64_t most = ((int64_t)p.cap + min_len - 1) / min_len * p.B;
   if (want > most) want = most;
