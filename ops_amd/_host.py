@@ -22,7 +22,7 @@ def call(device: torch.device, fn, *args) -> None:
 
 
 def need_gpu(name: str, t: torch.Tensor, device: torch.device = None) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (got device {t.device})")
     if device is not None and t.device != device:
         raise ValueError(f"{name} must be on {device} (got {t.device})")

@@ -91,6 +91,10 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _weight(w: Optional[torch.Tensor], dtype: torch.dtype) -> Optional[torch.Tensor]:
+    return w if w is None or (w.dtype == dtype and w.is_contiguous()) else w.detach().to(dtype).contiguous()
+
+
 class _Call:
     """What the forward and the backward of one call share."""
     __slots__ = ("dtype", "B", "S", "D", "R", "off", "inter", "eps", "scale", "pos", "freq", "wq", "wk", "wdt")
@@ -120,8 +124,7 @@ class _Call:
             if w.dtype != x.dtype:
                 self.wdt = _lib.SFA_DTYPE_F32
         wt = torch.float32 if self.wdt == _lib.SFA_DTYPE_F32 else x.dtype
-        self.wq = None if q_weight is None else q_weight.detach().to(wt).contiguous()
-        self.wk = None if k_weight is None else k_weight.detach().to(wt).contiguous()
+        self.wq, self.wk = _weight(q_weight, wt), _weight(k_weight, wt)
 
     def args(self, q, k, q_out, k_out, v=None, v_out=None, slots=None, dq=None, dk=None, dwq=None, dwk=None):
         """``sfa_rope_args``; q_out None: no q, k_out None: no k."""
