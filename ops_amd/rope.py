@@ -71,7 +71,9 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "no
             return rotary_dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
         lo = max(0.0, math.floor(index(beta_fast)))
-        hi = min(rotary_dim / 2 - 1.0, math.ceil(index(beta_slow)))
+        # (past the last pair, up to the published bound, where even that one turns
+        # more than beta_slow times: it then stays on the ramp)
+        hi = min(rotary_dim - 1.0, math.ceil(index(beta_slow)))
         ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         f = f * (1.0 - ramp) + f / factor * ramp
     return f.to(device) if device is not None else f
