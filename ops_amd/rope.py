@@ -225,7 +225,8 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     c = _Call(x, positions, inv_freq, None, None, 0.0, rope_offset, interleaved, rope_scale)
     written(out)
     if x.numel() > 0:
-        a = c.args(rows(x), None, out, None)
+        x = rows(x)  # (held until the launch, as everything a call reads)
+        a = c.args(x, None, out, None)
         call(x.device, _lib.load().sfa_rope_fwd, ctypes.byref(a), None)
     return out
 
@@ -297,7 +298,8 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
         out = _like(q) if out is None else out
     written(out, k_cache, v_cache)
     if k.numel() > 0:
-        a = c.args(q, rows(k), out, k_cache, v, v_cache, slots)
+        k = rows(k)
+        a = c.args(q, k, out, k_cache, v, v_cache, slots)
         pg = kv_pages(bt, B, num_pages, page_size, dev)
         call(dev, _lib.load().sfa_rope_fwd, ctypes.byref(a), ctypes.byref(pg))
     return out
