@@ -268,6 +268,8 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
     _check_rows("k", k)
     B, S, Hkv, D = k.shape
     dev = k.device
+    if Hkv == 0:
+        raise ValueError("append needs k rows, got k without heads (rotary_embedding or qk_norm_rope turn q alone)")
     if q is not None:
         _check_rows("q", q, k)
         if q.shape[3] != D:
