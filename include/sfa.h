@@ -398,7 +398,7 @@ SFA_API int sfa_cache_free(const sfa_cache* c, const int32_t* rows, const int32_
 
 /* Free pages for rows kv_lens[b] .. new_lens[b] - 1 of every sequence where none
  * is mapped: all of a sequence's or none (ok[b] = 0), in order of b while they
- * last.  kv_lens is not changed. */
+ * last (a sequence that needs none is always ok).  kv_lens is not changed. */
 SFA_API int sfa_cache_extend(const sfa_cache* c, const int32_t* new_lens, int32_t* ok, void* workspace,
                              size_t workspace_bytes, void* stream);
 

@@ -159,7 +159,8 @@ def cache_extend(block_table: torch.Tensor, ref_counts: torch.Tensor, kv_lens: t
                  page_size: int) -> torch.Tensor:
     """Free pages mapped for the rows ``kv_lens[b] .. new_lens[b] - 1`` of every
     sequence that has none there: all that a sequence needs or none, in order of
-    b while they last.  Returns ``ok`` int32 ``[B]`` (0: it did not get them);
+    b while they last.  Returns ``ok`` int32 ``[B]`` (0: it did not get them, or its
+    rows do not fit the table; 1 also for a sequence that needs none);
     ``kv_lens`` is left to the caller."""
     _state("block_table", block_table, 2, None)
     dev, B = block_table.device, block_table.shape[0]

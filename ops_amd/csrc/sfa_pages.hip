@@ -278,7 +278,8 @@ __global__ __launch_bounds__(256) void free_kernel(PagesParams p, const int32_t*
 
 // ---- mapping pages for rows to come -------------------------------------------------
 // Sequence b gets pages for rows kv_lens[b] .. new_lens[b] - 1 where it has
-// none, all or none of them: in order of b, as long as free pages last.
+// none, all or none of them: in order of b, as long as free pages last (one
+// that needs none has what it needs, also behind the last free page).
 __global__ __launch_bounds__(kPlanThreads) void extend_kernel(PagesParams p, const int32_t* new_lens, int32_t* ok) {
   __shared__ int s_scan[kPlanWaves + 1];
   __shared__ int s_need[kMaxSeqs];
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(PagesParams p, con
     const int b = b0 + tid / 16;
     if (b >= p.B) continue;  // (whole groups of 16 lanes)
     const int need = ok[b], first = s_need[b];
-    const bool good = need >= 0 && (int64_t)first + need <= found;
+    const bool good = need == 0 || (need > 0 && (int64_t)first + need <= found);
     if (good && need > 0) {
       int e0, e1, at = first;
       range(b, e0, e1);
