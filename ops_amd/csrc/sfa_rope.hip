@@ -664,10 +664,12 @@ __device__ __forceinline__ bool turn_of(const RopeParams& p, int d, int& pd, int
   return true;
 }
 
+// (rows from unit `first` on; a loop over them in the kernel held 135 registers
+// and scratch for 88)
 template <typename T>
-__global__ __launch_bounds__(256) void rope_fwd_scalar_kernel(RopeParams p) {
+__global__ __launch_bounds__(256) void rope_fwd_scalar_kernel(RopeParams p, int64_t first) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t unit = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (unit >= p.units) return;
   const int64_t tok = unit / p.groups;
   int h = (int)(unit % p.groups);
@@ -849,8 +851,15 @@ struct Bwd {
 
 template <typename T>
 void fwd(const RopeParams& p, bool vec, hipStream_t s) {
-  if (!vec) rope_fwd_scalar_kernel<T><<<(unsigned)((p.units + 3) / 4), 256, 0, s>>>(p);
-  else by_geometry(p, Fwd<T>{p, s});
+  if (vec) {
+    by_geometry(p, Fwd<T>{p, s});
+    return;
+  }
+  constexpr int64_t kMost = (int64_t)1 << 23;  // workgroups: a launch has fewer than 2^32 threads
+  for (int64_t first = 0; first < p.units; first += 4 * kMost) {
+    const int64_t wgs = (p.units - first + 3) / 4;
+    rope_fwd_scalar_kernel<T><<<(unsigned)(wgs < kMost ? wgs : kMost), 256, 0, s>>>(p, first);
+  }
 }
 
 template <typename T>
