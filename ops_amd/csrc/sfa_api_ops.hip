@@ -295,7 +295,7 @@ int sfa_rope_bwd(const sfa_rope_args* a, void* workspace, size_t workspace_bytes
 size_t sfa_tree_fwd_workspace_size(const sfa_tree_args* a, const sfa_kv_pages* pages) {
   if (check_tree(a, pages) != SFA_OK) return 0;
   const sfa::TreePlan pl = sfa::tree_plan(tree_params(a, pages), a->dtype, tree_vec(a));
-  return pl.workspace();
+  return pl.fits() ? pl.workspace() : 0;
 }
 
 int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
@@ -305,6 +305,7 @@ int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* worksp
   if (rc != SFA_OK) return rc;
   sfa::TreeParams p = tree_params(a, pages);
   const sfa::TreePlan pl = sfa::tree_plan(p, a->dtype, tree_vec(a));
+  if (!pl.fits()) return fail(SFA_E_UNSUPPORTED, "more query rows than one launch holds (%lld workgroups)", (long long)pl.wgs);
   const size_t need = pl.workspace();
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)

@@ -105,6 +105,9 @@ struct TreePlan {
   int kernel;
   int rows;       // query rows (token, head) per workgroup
   int want, slots;
+  int64_t wgs;    // workgroups of `threads` threads
+  int threads;
+  bool fits() const { return wgs * threads < (int64_t)1 << 32; }  // one launch
   size_t part_o_bytes, part_lse_bytes, seq_bytes;
   size_t workspace() const { return part_o_bytes + part_lse_bytes + seq_bytes; }
 };

@@ -1609,12 +1609,13 @@ void launch_combine(const TreeParams& p, hipStream_t s) {
   else launch_combine<T, 1>(p, s);
 }
 
-// Kernels by query rows per (sequence, kv head): rows a workgroup, tile keys, waves.
+// Kernels by query rows per (sequence, kv head): rows a workgroup, tile keys, threads.
 enum { kGeneric = 0, kRows16, kRows32, kRows64, kRows128, kRows256, kMla };
 struct KernelShape {
-  int rows, tile;
+  int rows, tile, threads;
 };
-constexpr KernelShape kShapes[] = {{kGR, kGK}, {16, 128}, {32, 128}, {64, 128}, {128, 64}, {256, 32}, {64, 64}};
+constexpr KernelShape kShapes[] = {{kGR, kGK, 256}, {16, 128, 256}, {32, 128, 256}, {64, 128, 256},
+                                   {128, 64, 512},  {256, 32, 512}, {64, 64, 512}};
 constexpr int kWorkgroups = 256;  // key ranges are cut until about so many workgroups (one a CU) are in flight
 
 template <int D, int NG, int WR, int WK, int NS>
@@ -1665,6 +1666,8 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
   // (whole eights of items: the row blocks of one meet in the L2 of one XCD)
   if (nrb > 1 && (int64_t)pl.slots * p.Hkv > 4)
     while (pl.slots * p.Hkv % 8 != 0) ++pl.slots;
+  pl.wgs = (int64_t)pl.slots * p.Hkv * nrb;
+  pl.threads = kShapes[pl.kernel].threads;
   if (pl.want > 0) {
     const size_t rows = (size_t)pl.slots * p.T * p.Hq;
     pl.part_o_bytes = (rows * p.Dv * sizeof(float) + 255) / 256 * 256;
@@ -1679,7 +1682,7 @@ hipError_t launch_tree(const TreeParams& p0, const TreePlan& pl, int dtype, hipS
   p.want = pl.want;
   p.tile = kShapes[pl.kernel].tile;
   p.nrb = (p.T * p.G + pl.rows - 1) / pl.rows;
-  const unsigned grid = (unsigned)((int64_t)pl.slots * p.Hkv * p.nrb);
+  const unsigned grid = (unsigned)pl.wgs;
   if (pl.kernel == kMla) {
     // (row offsets of a tile fit the loads' 32 bits)
     if (p.page_shift >= 6 && p.k_ss > 0 && p.k_ss < ((int64_t)1 << 24)) tree_mla_kernel<true><<<grid, 512, 0, s>>>(p);

@@ -1,9 +1,12 @@
 """Calls of the operators around the attention that the host layer refuses, with
 the GPU's checks passed by CPU tensors.  CPU only."""
+import ctypes
+
 import pytest
 import torch
 
 import ops_amd
+from ops_amd import _lib
 from tests.host_calls import launches  # noqa: F401
 
 
@@ -16,3 +19,18 @@ def test_append_without_k_rows(launches):  # noqa: F811
     empty = ops_amd.qk_norm_rope_append(q[:0], q[:0], None, torch.randn(9, 16, 4, 64), None, bt[:0], pos, pos,
                                         ops_amd.rope_frequencies(64))
     assert empty.shape == (0, 3, 4, 64) and launches == []
+
+
+@pytest.mark.parametrize("kw", [dict(B=1 << 24, T=1, Hq=1, Hkv=1, Dqk=64, Dv=64), dict(B=1 << 22, T=1, Hq=4, Hkv=4, Dqk=128, Dv=128),
+                                dict(B=1 << 21, T=64, Hq=1, Hkv=1, Dqk=77, Dv=33),
+                                dict(B=1 << 23, T=1, Hq=1, Hkv=1, Dqk=576, Dv=512)])
+def test_tree_of_more_rows_than_a_launch_holds(kw):
+    """(2^32 threads; before any HIP call)"""
+    from tests.test_ops_host import _pages, _tree
+    lib = _lib.load()
+    a, pg = _tree(**kw), _pages(max_pages=4096, bt_sb=4096, page_size=64, num_pages=100)
+    if kw["Dqk"] == 576:
+        a.v = a.k
+    assert lib.sfa_tree_fwd(ctypes.byref(a), ctypes.byref(pg), 0x10000, 1 << 40, None) == _lib.SFA_E_UNSUPPORTED
+    assert b"launch" in lib.sfa_last_error()
+    assert lib.sfa_tree_fwd_workspace_size(ctypes.byref(a), ctypes.byref(pg)) == 0
