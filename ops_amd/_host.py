@@ -59,12 +59,19 @@ def int_rows(name: str, t: torch.Tensor, B: int, S: int, device: torch.device) -
     return t
 
 
+def int32(t: torch.Tensor) -> torch.Tensor:
+    """int64 ids and lengths as int32.  Those past its range stay past every pool
+    and table, which hold fewer than 2^31 rows: cut to 32 bits they would come
+    back as page 0 or as a short length."""
+    return t if t.dtype == torch.int32 else t.clamp(-1 << 31, (1 << 31) - 1).to(torch.int32)
+
+
 def int_vec(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
     """A contiguous int32 ``[n]`` tensor."""
     need_gpu(name, t, device)
     if t.dtype not in INTS or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be an integer [{n}] tensor, got {t.dtype} {tuple(t.shape)}")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else int32(t).contiguous()
 
 
 def check_pool(name: str, t: torch.Tensor, device: torch.device) -> None:
@@ -91,7 +98,7 @@ def table(block_table: torch.Tensor, B: int, device: torch.device) -> torch.Tens
     if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype not in INTS:
         raise ValueError(f"block_table must be an integer [B, max_pages] tensor with B = {B}, got {block_table.dtype} "
                          f"{tuple(block_table.shape)}")
-    bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    bt = int32(block_table)
     if bt.stride(1) != 1 or (B > 1 and bt.stride(0) < bt.shape[1]):
         bt = bt.contiguous()
     return bt

@@ -21,7 +21,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._host import call, int_vec, need_gpu, written
+from ._host import call, int32, int_vec, need_gpu, written
 
 __all__ = ["cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path"]
 
@@ -206,7 +206,7 @@ def cache_keep_path(caches: Sequence[torch.Tensor], block_table: torch.Tensor, c
     if path.dim() != 2 or path.shape[0] != B or path.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"path must be an integer [{B}, n] tensor, got {path.dtype} {tuple(path.shape)}")
     path = path if path.dtype == torch.int32 and (path.numel() == 0 or path.stride(1) == 1) \
-        else path.to(torch.int32).contiguous()
+        else int32(path).contiguous()
     if B == 0 or path.shape[1] == 0:
         return
     lib = _lib.load()
