@@ -70,11 +70,14 @@ def _cache(pools, npools, num_pages, page_size, block_table=None, ref_counts=Non
     """sfa_cache; ``pools`` (bytes or None) must outlive the call."""
     buf = None if pools is None else ctypes.c_char_p(pools)
     bt = block_table
-    a = _lib.Cache.from_buffer_copy(_CACHE.pack(
-        0 if buf is None else ctypes.cast(buf, ctypes.c_void_p).value, npools, 0 if bt is None else bt.shape[0],
-        0 if bt is None else bt.shape[1], page_size, num_pages, 0, 0 if bt is None else bt.data_ptr(),
-        0 if bt is None else bt.stride(0), 0 if ref_counts is None else ref_counts.data_ptr(),
-        0 if kv_lens is None else kv_lens.data_ptr()))
+    try:
+        a = _lib.Cache.from_buffer_copy(_CACHE.pack(
+            0 if buf is None else ctypes.cast(buf, ctypes.c_void_p).value, npools, 0 if bt is None else bt.shape[0],
+            0 if bt is None else bt.shape[1], page_size, num_pages, 0, 0 if bt is None else bt.data_ptr(),
+            0 if bt is None else bt.stride(0), 0 if ref_counts is None else ref_counts.data_ptr(),
+            0 if kv_lens is None else kv_lens.data_ptr()))
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"the call's arguments do not fit the kernels' interface: {e}") from None
     return a, buf
 
 

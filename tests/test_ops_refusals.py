@@ -34,3 +34,21 @@ def test_tree_of_more_rows_than_a_launch_holds(kw):
     assert lib.sfa_tree_fwd(ctypes.byref(a), ctypes.byref(pg), 0x10000, 1 << 40, None) == _lib.SFA_E_UNSUPPORTED
     assert b"launch" in lib.sfa_last_error()
     assert lib.sfa_tree_fwd_workspace_size(ctypes.byref(a), ctypes.byref(pg)) == 0
+
+
+def test_sizes_that_do_not_fit_the_interface(launches):  # noqa: F811
+    """A ValueError as for every other argument, and no size cut to 32 bits."""
+    i = torch.zeros(2, dtype=torch.int32)
+    bt = torch.zeros(2, 2, dtype=torch.int32)
+    for size in (1 << 31, 1 << 40, 1 << 70):
+        with pytest.raises(ValueError, match="interface"):
+            ops_amd.cache_extend(bt, i, i, i, size)
+        with pytest.raises(ValueError, match="interface"):
+            ops_amd.cache_free(bt, i, i, i, page_size=size)
+    wide = torch.zeros(1, 16, 1, 64).expand((1 << 32) + 1, 16, 1, 64)
+    x, pos, mask = torch.zeros(2, 3, 1, 64), torch.arange(3), torch.ones(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="past 2\\^31"):
+        ops_amd.tree_attention_paged(x, wide, wide, bt, i, mask)
+    with pytest.raises(ValueError, match="expanded"):
+        ops_amd.qk_norm_rope_append(None, x, None, wide, None, bt, pos, pos, ops_amd.rope_frequencies(64))
+    assert launches == []
