@@ -52,3 +52,28 @@ def test_sizes_that_do_not_fit_the_interface(launches):  # noqa: F811
     with pytest.raises(ValueError, match="expanded"):
         ops_amd.qk_norm_rope_append(None, x, None, wide, None, bt, pos, pos, ops_amd.rope_frequencies(64))
     assert launches == []
+
+
+def test_forms_without_a_gradient_refuse_inputs_that_want_one(launches):  # noqa: F811
+    q, pool, sink = torch.randn(2, 3, 4, 64), torch.randn(9, 16, 2, 64), torch.zeros(4)
+    bt, ctx, mask = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.ones(2, 3, dtype=torch.int64)
+    pos, freq = torch.arange(3), ops_amd.rope_frequencies(64)
+
+    def leaf(t):
+        return t.clone().requires_grad_(True)
+
+    def tree(q=q, k=pool, v=pool, sink=sink):
+        return ops_amd.tree_attention_paged(q, k, v, bt, ctx, mask, attn_sink=sink)
+
+    calls = [lambda: tree(q=leaf(q)), lambda: tree(k=leaf(pool)), lambda: tree(v=leaf(pool)), lambda: tree(sink=leaf(sink)),
+             lambda: ops_amd.qk_norm_rope_append(leaf(q), q[:, :, :2], q[:, :, :2], pool, pool.clone(), bt, pos, pos, freq),
+             lambda: ops_amd.rotary_embedding(leaf(q), pos, freq, out=torch.empty_like(q))]
+    for c in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            c()
+    assert launches == []
+    tree()
+    with torch.no_grad():
+        for c in calls:
+            c()
+    assert len(launches) == 1 + len(calls)
