@@ -311,13 +311,14 @@ __global__ __launch_bounds__(256) void tree_generic_kernel(TreeParams p) {
 }
 
 // ---- head dims 64 and 128 on the matrix cores, bf16 ------------------------------
-// A workgroup of WR x WK waves takes 64 WR rows (wave column wr its NG groups
-// of 16; NG < 4 only for WR = 1) of one key range; wave row wk takes every
-// WK-th tile of 32 keys.  So a tile is read from HBM once for up to 256 rows,
-// and a short row set still spreads its keys over the waves of a CU:
-//  * K and V rows go straight into LDS (16 bytes a lane, PD tiles ahead), in
+// tree_mfma_kernel: a workgroup of four waves takes 16 NG rows of one key range,
+// wave w every fourth tile of 32 keys, so that a short row set still spreads its
+// keys over a CU.  tree_pipe_kernel (below): WR x WK waves, wave column wr with
+// rows 16 NG wr .., wave row wk with every WK-th tile, which is read from HBM once
+// for up to 256 rows.  In both
+//  * K and V rows go straight into LDS (16 bytes a lane, a tile or more ahead), in
 //    an order of chunks that both operand reads find without bank conflicts
-//    (Swz); the page ids go the same way, 2 PD tiles ahead, so that the loop has
+//    (Swz); the page ids go the same way, further ahead, so that the loop has
 //    no load that the compiler would wait for;
 //  * S^T = K Q^T, 16 keys x 16 rows a product (16x16x32), Q in registers: a K
 //    operand read from LDS serves 16 NG rows.  A lane holds 8 keys of a row;
@@ -325,9 +326,11 @@ __global__ __launch_bounds__(256) void tree_generic_kernel(TreeParams p) {
 //    passes it by 8 (2^8 more at most in a float32 sum), so that a tile needs no
 //    maximum across lanes; P^T in bf16 is already the operand of
 //    O^T = V^T P^T, whose V^T operands are transposing reads.
-// Unmapped rows and rows past the range read zeros.  Rounding P to bf16 adds
-// 2^-9 sum p |v| / sqrt(keys) or so, as much as the result's own rounding;
-// sums, maxima and partials are float32.
+// Unmapped rows and rows past the range read zeros.  Sums, maxima and partials
+// are float32.  P is rounded to bf16 for the product: tree_mfma_kernel multiplies
+// what that left in a second one (2^-16 of a weight), tree_pipe_kernel does not
+// (2^-8, which adds 2^-9 sum p |v| / sqrt(keys) or so, as much as the result's own
+// rounding).
 
 template <int D>
 struct Swz {  // position of chunk c of row r: c ^ at(r)
@@ -632,40 +635,36 @@ __device__ __forceinline__ void finish_rows(const TreeParams& p, const WorkItem&
   }
 }
 
-template <int D, int NG, int WR, int WK, int PD>
-__global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(TreeParams p) {
+template <int D, int NG>
+__global__ __launch_bounds__(256, 1) void tree_mfma_kernel(TreeParams p) {
   using M = Mfma<16>;
   typedef M::acc_t acc_t;
-  static_assert(NG == 4 || WR == 1, "whole waves of rows");
-  constexpr int NW = WR * WK, KT = 32, CH = D / 8, KS = D / 32, OT = D / 16;
-  constexpr int RPI = 64 / CH, ROWI = KT / RPI;        // rows per load instruction, instructions per K (or V) tile
-  constexpr int NI = 2 * ROWI / WR;                    // instructions per wave and tile
-  constexpr int TILE = 2 * KT * CH, NS = PD + 1;       // 16-byte slots of a K and V tile, stages
-  constexpr int WROWS = 16 * NG;
-  constexpr int MERGE = WK > 1 ? (WK / 2) * WR * NG * OT * 64 : 0;
+  constexpr int WK = 4, KT = 32, CH = D / 8, KS = D / 32, OT = D / 16;
+  constexpr int TILE = 2 * KT * CH, NS = 2;  // 16-byte slots of a K and V tile, stages
+  constexpr int ROWS = 16 * NG;
+  constexpr int MERGE = (WK / 2) * NG * OT * 64;
   constexpr int SLOTS = NS * WK * TILE > MERGE ? NS * WK * TILE : MERGE;
 
   __shared__ u32x4 s_kv[SLOTS];
-  __shared__ int s_page[NW][NS * 64];
-  __shared__ uint64_t s_mask[WR * WROWS];
-  __shared__ float s_ml[NW][2][WROWS];
+  __shared__ int s_page[WK][NS * 64];
+  __shared__ uint64_t s_mask[ROWS];
+  __shared__ float s_ml[WK][2][ROWS];
 
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = wave % WR, wk = wave / WR;
+  const int wk = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lt = lane & 15, hq = lane >> 4;
 
   WorkItem it;
   if (!work_item(p, it)) return;
   const int b = it.b, g = it.g, k0 = it.k0, k1 = it.k1, ctx = it.ctx;
-  const int R = p.T * p.G, row0 = it.rb * WR * WROWS;
+  const int R = p.T * p.G, row0 = it.rb * ROWS;
   const int niter = (k1 - k0 + WK * KT - 1) / (WK * KT);
 
   // ---- rows: Q^T operands (lane: row 16 n + lt, dims 32 s + 8 hq ..), tree masks ----
   bf16x8 qb[NG][KS];
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
-    const int r = row0 + wr * WROWS + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
+    const int r = row0 + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
     const bool live = r < R;
     const bf16* q = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
 #pragma unroll
@@ -674,24 +673,20 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
       qb[n][s] = live ? x : bf16x8{};
     }
   }
-  for (int i = tid; i < WR * WROWS; i += 64 * NW) {
+  for (int i = tid; i < ROWS; i += 256) {
     const int r = row0 + i;
     s_mask[i] = r < R ? (uint64_t)p.tree_mask[b * p.tm_sb + (r / p.G) * p.tm_ss] : 0;
   }
 
-  TileLoads<D, WR, WK> ld(p, b, g, k0, k1, wr, wk, lane);
-  uint32_t vm[NS];  // rows that are there, of tiles j, j + 1, ..
+  TileLoads<D, 1, WK> ld(p, b, g, k0, k1, 0, wk, lane);
+  uint32_t mask;  // rows of tile j that are there
   {
-    int pg[2 * PD];
-#pragma unroll
-    for (int j = 0; j < 2 * PD; ++j) pg[j] = *reinterpret_cast<const int32_t*>(ld.page_addr(j));
-#pragma unroll
-    for (int j = PD; j < 2 * PD; ++j) s_page[wave][(j % NS) * 64 + lane] = pg[j];
-#pragma unroll
-    for (int j = 0; j < PD; ++j) vm[j] = ld.load(j, pg[j], &s_kv[(j * WK + wk) * TILE]);
+    const int pg = *reinterpret_cast<const int32_t*>(ld.page_addr(0)), pg1 = *reinterpret_cast<const int32_t*>(ld.page_addr(1));
+    s_page[wk][64 + lane] = pg1;
+    mask = ld.load(0, pg, &s_kv[wk * TILE]);
   }
-  wait_vm<(PD - 1) * NI>();  // tile 0 (its page ids are not in the loop's count yet)
-  wg_barrier();              // the masks are staged
+  wait_vm<0>();
+  wg_barrier();  // the masks are staged
 
   // ---- operand addresses ---------------------------------------------------------------
   const uint32_t pitch = CH * 16;
@@ -709,24 +704,19 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
     for (int i = 0; i < OT; ++i) oacc[n][i] = acc_t{};
   }
 
-  int st = 0, st_new = PD;  // stage of tile j, of tile j + PD
+  int st = 0;  // stage of tile j; tile j + 1 goes to the other
   auto step = [&](int j, auto with_drafts) {
     constexpr bool TAIL = decltype(with_drafts)::value;
-    wait_vm<(PD - 1) * (NI + 1)>();  // tile j and the page ids of tile j + PD have landed
-    if constexpr (WR > 1) asm volatile("s_barrier" ::: "memory");  // ... for all its waves; stage st_new is read
-    {
-      const int pg = s_page[wave][st_new * 64 + lane];
-      // (page ring: tile j + 2 PD takes the place of tile j + PD - 1, read at j - 1)
-      const int ring = st_new == 0 ? NS - 1 : st_new - 1;
-      dma4(&s_page[wave][ring * 64], ld.page_addr(j + 2 * PD));
-      vm[PD] = ld.load(j + PD, pg, &s_kv[(st_new * WK + wk) * TILE]);
-    }
+    wait_vm<0>();  // tile j and the page ids of tile j + 1 have landed (a wave loads what it alone reads)
+    // (the page ids of tile j + 2 take the place of tile j's, read at j - 1)
+    const int pg = s_page[wk][(st ^ 1) * 64 + lane];
+    dma4(&s_page[wk][st * 64], ld.page_addr(j + 2));
+    const uint32_t mask_next = ld.load(j + 1, pg, &s_kv[((st ^ 1) * WK + wk) * TILE]);
     u32x4* kt = &s_kv[(st * WK + wk) * TILE];
     u32x4* vt = kt + KT * CH;
     const int base = k0 + (j * WK + wk) * KT;
-    const uint32_t mask = vm[0];
     uint32_t bad = 0;  // drafted rows whose V holds infinities or NaN: out of the product, added by hand
-    if constexpr (TAIL) bad = bad_rows<D, WR>(vt, base, ctx, wr, lane);
+    if constexpr (TAIL) bad = bad_rows<D, 1>(vt, base, ctx, 0, lane);
 
     // by 16 keys (half the scores in registers): S^T, then its softmax; a lane
     // holds keys 16 mt + 4 hq + e of its row
@@ -746,7 +736,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
       if (TAIL || mask != 0xffffffffu) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const uint32_t seen = seen4<TAIL>(mask, TAIL ? s_mask[wr * WROWS + 16 * n + lt] : 0, 16 * mt + 4 * hq, base - ctx);
+          const uint32_t seen = seen4<TAIL>(mask, TAIL ? s_mask[16 * n + lt] : 0, 16 * mt + 4 * hq, base - ctx);
           const float x0 = seen & 1u ? sacc[n][0] : kNegInf, x1 = seen & 2u ? sacc[n][1] : kNegInf;
           const float x2 = seen & 4u ? sacc[n][2] : kNegInf, x3 = seen & 8u ? sacc[n][3] : kNegInf;
           sacc[n] = acc_t{x0, x1, x2, x3};
@@ -802,10 +792,8 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
     }
     if constexpr (TAIL)
       add_bad_rows<D, NG>(p, b, g, base, bad, pb, lt, hq, [&](int n, int ot, const acc_t& y) { oacc[n][ot] += y; });
-#pragma unroll
-    for (int i = 0; i < PD; ++i) vm[i] = vm[i + 1];
-    st = st + 1 == NS ? 0 : st + 1;
-    st_new = st_new + 1 == NS ? 0 : st_new + 1;
+    mask = mask_next;
+    st ^= 1;
   };
   // steps without a drafted row in any of the workgroup's tiles, then the others
   const int whole = min(max(ctx - k0, 0) / (WK * KT), niter);
@@ -814,7 +802,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_mfma_kernel(Tr
   for (; j < niter; ++j) step(j, std::true_type{});
   wait_vm<0>();  // the loads past the range have landed before LDS is used for anything else
 
-  finish_rows<D, NG, WR, WK>(p, it, row0, s_kv, &s_ml[0][0][0], oacc, m_used, l_part, wave, lane);
+  finish_rows<D, NG, 1, WK>(p, it, row0, s_kv, &s_ml[0][0][0], oacc, m_used, l_part, wk, lane);
 }
 
 // ---- more than 64 rows: two waves a SIMD, scores a tile ahead ---------------------
@@ -1526,9 +1514,9 @@ __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
 // ---- joining the slots of a sequence -------------------------------------------
 // WPR waves a row; LPR lanes hold the row (4 dims each), 64 / LPR slots at a time
 // and wave.  A slot in which the row sees nothing has LSE -inf.
-template <typename T, int LPR, int WPR>  // WPR: 1, or 4 and more
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void tree_combine_kernel(TreeParams p) {
-  constexpr int RPB = WPR > 4 ? 1 : 4 / WPR;  // rows a workgroup
+template <typename T, int LPR, int WPR>
+__global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void tree_combine_kernel(TreeParams p) {
+  constexpr int RPB = WPR > 1 ? 1 : 4;  // rows a workgroup
   __shared__ f32x4 s_x[WPR > 1 ? WPR - 1 : 1][LPR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR, per = (int64_t)p.T * p.Hq;
@@ -1631,9 +1619,9 @@ void launch_pipe(const TreeParams& p, unsigned grid, hipStream_t s) {
 template <int D>
 void launch_mfma(const TreeParams& p, int kernel, unsigned grid, hipStream_t s) {
   switch (kernel) {
-    case kRows16: tree_mfma_kernel<D, 1, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
-    case kRows32: tree_mfma_kernel<D, 2, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
-    case kRows64: tree_mfma_kernel<D, 4, 1, 4, 1><<<grid, 256, 0, s>>>(p); break;
+    case kRows16: tree_mfma_kernel<D, 1><<<grid, 256, 0, s>>>(p); break;
+    case kRows32: tree_mfma_kernel<D, 2><<<grid, 256, 0, s>>>(p); break;
+    case kRows64: tree_mfma_kernel<D, 4><<<grid, 256, 0, s>>>(p); break;
     case kRows128: launch_pipe<D, 2, 4, 2, 4>(p, grid, s); break;
     default: launch_pipe<D, 2, 8, 1, 5>(p, grid, s);
   }
