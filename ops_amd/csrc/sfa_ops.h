@@ -64,7 +64,6 @@ struct RopeParams {
   int P, K, chunks;     // lanes a row, 16-byte chunks a lane, chunks a row
   int groups, per, upt; // row groups a token; in blocks of per, upt blocks a token
   int64_t units;        // B * S * groups
-  int stream;           // store the results past the L2s
   float* part;          // backward: [2][workgroups][1024] partial dw, or nullptr
 };
 void rope_geometry(RopeParams& p, int esize, bool vec);

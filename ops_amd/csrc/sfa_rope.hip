@@ -216,8 +216,7 @@ struct Row {
     for (int j = 0; j < K; ++j) {
       const int c = j * P + l;
       if (c >= p.chunks) continue;
-      if (p.stream) __builtin_nontemporal_store(r[j], reinterpret_cast<u32x4*>(y + c * E));
-      else *reinterpret_cast<u32x4*>(y + c * E) = r[j];
+      *reinterpret_cast<u32x4*>(y + c * E) = r[j];
     }
   }
   // u(j, own, partner) replaces chunk j by its turned values: pre() makes u of
@@ -899,10 +898,6 @@ void rope_geometry(RopeParams& p, int esize, bool vec) {
   if (p.v != nullptr) vg = vec ? (p.side[1].H * (p.Dv / E) + 63) / 64 : p.side[1].H;
   p.groups = p.side[0].groups + p.side[1].groups + vg;
   p.units = (int64_t)p.B * p.S * p.groups;
-  // Results that pass the L2s (32 MB) are stored past them: forward and backward
-  // of 2 x 8192 tokens, 34 heads of 128 dims (285 + 428 MB) took 97 + 121 us with
-  // plain stores, 76 + 111 so.
-  p.stream = (int64_t)p.B * p.S * (p.side[0].H + p.side[1].H) * p.D * esize > ((int64_t)32 << 20);
   // blocks of up to 8 groups (a token's angles serve them) once there are 4096 waves of them
   const int64_t per = p.units / kWaves;
   p.per = (int)(per < 1 ? 1 : per > 8 ? 8 : per);
