@@ -86,7 +86,7 @@ def check_pool(name: str, t: torch.Tensor, device: torch.device) -> None:
 def kv_pages(block_table: torch.Tensor, B: int, num_pages: int, page_size: int, device: torch.device) -> _lib.KvPages:
     """``sfa_kv_pages`` of an int32 table with unit column stride, which must
     outlive the call."""
-    if max(num_pages, block_table.shape[1], page_size) >= 1 << 31:
+    if (num_pages | block_table.shape[1] | page_size) >> 31:
         raise ValueError(f"a pool of {num_pages} pages of {page_size} rows or a table of {block_table.shape[1]} pages a sequence "
                          "is past 2^31")
     pg = _lib.KvPages()

@@ -42,7 +42,8 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``tree_lens[b]`` zeros and ``-inf``.  ``out`` ``[B, T, Hq, Dv]`` in q's type and
     ``lse`` ``[B, T, Hq]`` float32 may be preallocated (memory of their own).  No
     gradient: inputs that ask for one are refused outside of ``torch.no_grad()``."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k_cache, v_cache, attn_sink)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                    or (attn_sink is not None and attn_sink.requires_grad)):
         raise ValueError("the attention of drafted tokens records no gradient: call it under torch.no_grad()")
     if q.dim() != 4:
         raise ValueError(f"q must be 4-D (BSHD), got shape {tuple(q.shape)}")
