@@ -56,7 +56,7 @@ int check_rope(const sfa_rope_args* a, bool backward, bool append) {
   if (a->w_dtype != SFA_DTYPE_F32 && a->w_dtype != a->dtype)
     return fail(SFA_E_INVALID, "weights must be float32 or of the rows' type");
   if (a->flags != 0) return fail(SFA_E_INVALID, "flags must be 0");
-  if (a->B <= 0 || a->S <= 0 || a->Hq < 0 || a->Hkv < 0 || a->Hq + a->Hkv <= 0)
+  if (a->B <= 0 || a->S <= 0 || a->Hq < 0 || a->Hkv < 0 || (a->Hq == 0 && a->Hkv == 0))
     return fail(SFA_E_INVALID, "B, S and the heads must be positive");
   if (a->D <= 0 || a->D > kMaxHeadDim) return fail(SFA_E_INVALID, "the head dim must be in [1, %d]", kMaxHeadDim);
   if (a->rotary_dim < 0 || a->rotary_dim % 2 != 0 || a->rope_offset < 0 || a->rotary_dim > a->D ||
@@ -80,8 +80,8 @@ int check_rope(const sfa_rope_args* a, bool backward, bool append) {
     if (a->Dv < 0 || a->Dv > kMaxHeadDim) return fail(SFA_E_INVALID, "the v head dim must be in [0, %d]", kMaxHeadDim);
     if (a->Dv > 0 && (!a->v || !a->v_out)) return fail(SFA_E_INVALID, "null tensor pointer");
   }
-  // rows and units are counted in 32 bits per launch dimension
-  if ((int64_t)a->B * a->S * ((int64_t)a->Hq + 2 * (int64_t)a->Hkv) > (int64_t)INT_MAX)
+  // rows and units are counted in 32 bits per launch dimension (and the product itself in 64)
+  if ((int64_t)a->B * a->S > INT_MAX / ((int64_t)a->Hq + 2 * (int64_t)a->Hkv))
     return fail(SFA_E_UNSUPPORTED, "more than 2^31 rows");
   return SFA_OK;
 }
@@ -149,7 +149,7 @@ int check_tree(const sfa_tree_args* a, const sfa_kv_pages* pg) {
   if (rc != SFA_OK) return rc;
   if ((int64_t)pg->max_pages * pg->page_size > (int64_t)1 << 29)
     return fail(SFA_E_UNSUPPORTED, "a table of more than 2^29 rows a sequence");
-  if ((int64_t)a->B * a->T * a->Hq > (int64_t)INT_MAX / 4) return fail(SFA_E_UNSUPPORTED, "more than 2^29 query rows");
+  if ((int64_t)a->B * a->T > (int64_t)INT_MAX / 4 / a->Hq) return fail(SFA_E_UNSUPPORTED, "more than 2^29 query rows");
   return SFA_OK;
 }
 

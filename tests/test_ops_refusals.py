@@ -77,3 +77,15 @@ def test_forms_without_a_gradient_refuse_inputs_that_want_one(launches):  # noqa
         for c in calls:
             c()
     assert len(launches) == 1 + len(calls)
+
+
+def test_row_counts_past_64_bits():
+    """Their product would come back negative and pass for small; before any HIP call."""
+    from tests.test_ops_host import _pages, _rope, _tree
+    lib, top = _lib.load(), (1 << 31) - 1
+    for kw in (dict(B=top, S=top), dict(B=top, S=top, Hq=2, Hkv=1), dict(B=top, S=2, Hq=top, Hkv=top), dict(B=1, S=top, Hq=1, Hkv=1)):
+        assert lib.sfa_rope_fwd(ctypes.byref(_rope(**kw)), None, None) == _lib.SFA_E_UNSUPPORTED
+        assert lib.sfa_rope_bwd(ctypes.byref(_rope(**kw)), 0x10000, 1 << 40, None) == _lib.SFA_E_UNSUPPORTED
+    for kw in (dict(B=top, T=64, Hq=top - 1, Hkv=2), dict(B=top, T=2, Hq=1 << 30, Hkv=1)):
+        a, pg = _tree(**kw), _pages(bt_sb=4)
+        assert lib.sfa_tree_fwd(ctypes.byref(a), ctypes.byref(pg), 0x10000, 1 << 40, None) == _lib.SFA_E_UNSUPPORTED
