@@ -19,10 +19,11 @@
 // dx written).  So a row is held in registers, in 16-byte chunks over P lanes
 // (half layout over the whole row: two chunks a lane, so that partners meet in
 // one lane and share their angles; 8 lanes of 9 chunks for the 576-dim latent
-// row), 64 / P heads of one token per wave; the token's angles are computed
-// once per wave for all the heads that it takes.  Rows that are not whole
-// 16-byte chunks (odd dims, strides, offsets) take the scalar kernels, one
-// wave a row.
+// row), 64 / P heads of one token per wave.  With one or two
+// chunks a lane the token's angles are computed once per wave for all the heads
+// that it takes (rows of 4 or 9 chunks a lane form them again for every row and
+// rotated chunk: registers).  Rows that are not whole 16-byte chunks (odd dims,
+// strides, offsets) take the scalar kernels, one wave a row.
 
 #include "sfa_ops.h"
 
@@ -347,9 +348,10 @@ struct Walk {
 // each), the k heads', then (append) 64-chunk groups of the v row.  NB units are
 // in flight, each in registers of its own that are refilled as soon as its
 // results are stored: the next unit's rows handed on from register to register
-// are waited for at the copy.  So 8192 tokens of 128 rows of 64 dims take 91 us
-// for 162 (read past the caches; a copy of the same rows 81), 2 x 8192 tokens of
-// 34 normed heads of 128 dims 91 for 119 (285 MB).  More in flight gains nothing
+// are waited for at the copy.  So 8192 tokens of 128 rows of 64 dims take 90 us
+// for 162 (caches flushed before the call; a copy of the same rows 81), 2 x 8192
+// tokens of 34 normed heads of 128 dims 91 for 119 (285 MB); on inputs that the
+// last pass left in the caches 73 and 70.  More in flight gains nothing
 // (NB 4 and 6, or 3 of rows in two chunks: 93, 95 us; 112).  Calls of one unit a wave take
 // NB = 1 (8.8 us for 11, 64 tokens into the cache: less code to fetch).
 template <typename T, int P, int K, bool IN, int NB>
@@ -482,8 +484,9 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
 // dx.  A wave walks over units as in the forward, NB of them in flight, and sums
 // its rows' dw in registers; a workgroup writes its sums to partial row
 // blockIdx.x, which rope_dw_kernel adds up in order.  NORM: some side is normed.
-// (The sizes above: 54 us with NB = 2 for 64, and 110 us, 428 MB, with NB = 1,
-// where x and dy keep four loads a lane in flight, 124 with 2.)
+// (The sizes above, caches flushed: 54 us with NB = 2 for 64, and 109 us, 428 MB,
+// with NB = 1, where x and dy keep four loads a lane in flight, 124 with 2; warm
+// 49 and 102.)
 template <typename T, int P, int K, bool IN, bool NORM, int NB>
 __global__ __launch_bounds__(256) void rope_bwd_kernel(RopeParams p) {
   typedef Row<T, P, K, IN> R;

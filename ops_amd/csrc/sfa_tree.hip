@@ -132,8 +132,10 @@ constexpr int kGK = 64;    // keys per tile
 constexpr int kGD = 1024;  // largest head dim
 
 // The rows row0 .. row0 + kGR - 1 of (b, g) over keys [k0, k1), by a workgroup of
-// 256 threads; emit(i, d, o, l) gets the unnormalised sums and fin(i, m, l) the
-// row's maximum (base 2) and sum.
+// 256 threads; fin(i, m, l) gets a row's maximum (base 2) and sum, emit(i, d, o, m, l)
+// its unnormalised sum of dim d with them.  Far from its floor: the keys are read
+// again for every 8 rows, and a score is a scalar product of four threads (4 x 4K
+// float32 keys of 128 dims, 8 tokens, 16 / 4 heads: 188 us, the bytes alone 15).
 struct GenericScratch {
   float q[kGR][kGD];
   float s[kGR][kGK + 1];
@@ -1114,6 +1116,9 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_pipe_kernel(Tr
 // fourth product.  The running maximum is shared: a row's scores are in four
 // waves, so a wave that finds one past the maximum by 8 (base 2) raises a flag,
 // and all of them move it together after the barrier that publishes P.
+// P is rounded to bf16 once (2^-8 of a weight; results 0.0019 rms from float64 where
+// float32 weights leave the result's own 0.0017): what that left would make half of
+// the products again and needs 8 KB that LDS, 163.6 KB full, does not have.
 struct MlaTree {
   static constexpr int kDqk = 576, kDv = 512, kKeys = 64, kSteps = kDqk / 32;
   static constexpr int kCh = kDv / 8, kCr = (kDqk - kDv) / 8;  // 16-byte chunks of the two parts of a row
@@ -1591,8 +1596,8 @@ void launch_combine(const TreeParams& p, hipStream_t s) {
 }
 template <typename T>
 void launch_combine(const TreeParams& p, hipStream_t s) {
-  // Many slots of few rows are joined by eight waves a row (256 slots of 256
-  // rows: 13 us, 44 by one wave; 64 of 1024: 14 and 22; but 32 of 2048: 20 and 12).
+  // Many slots of few rows are joined by eight waves a row (d = 128, 256 slots of
+  // 256 rows: 13 us, 45 by one wave; 64 of 1024: 17 both ways; 32 of 2048: 17 and 13).
   if (p.want / p.B >= 32 && (int64_t)p.B * p.T * p.Hq <= 1024) launch_combine<T, 8>(p, s);
   else launch_combine<T, 1>(p, s);
 }
@@ -1633,9 +1638,11 @@ TreePlan tree_plan(const TreeParams& p, int dtype, bool vec) {
   TreePlan pl{};
   const int64_t R = (int64_t)p.T * p.G;
   // Few keys and heads: fewer rows a workgroup give more workgroups, whose key
-  // rows meet in the L2 (whole call, 1 sequence, d = 128, 128 rows: 2K keys 16 us with
-  // 16 rows, 22 with 128; 32K: 27, 26 with 32 rows, 33; 1024 rows: 4K 44, 29, 38, 16K
-  // 103, 45, 46).  fit: workgroups of the shortest ranges, 256 keys.
+  // rows meet in the L2 (kernel and join, 1 sequence, d = 128, us by rows a workgroup;
+  // 128 query rows: 2K keys 17 with 16, 19 with 32, 23 with 128; 32K: 28, 26, 33; 1024
+  // query rows: 4K 45 with 16, 28 with 32, 38 with 256; 16K 111, 49, 46).  By the
+  // table's width, the lengths being on the device: 128 rows on 2K keys of a table of
+  // 128K take 20 us a call for 18.  fit: workgroups of the shortest ranges, 256 keys.
   auto fit = [&](int rows) { return (int64_t)p.B * p.Hkv * ((R + rows - 1) / rows) * (((int64_t)p.cap + 255) / 256); };
   if (dtype == SFA_DTYPE_BF16 && vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
     pl.kernel = R <= 16 || fit(16) <= 2 * kWorkgroups ? kRows16 : R <= 32 || fit(32) <= 5 * kWorkgroups ? kRows32
