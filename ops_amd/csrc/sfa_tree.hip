@@ -818,7 +818,9 @@ __global__ __launch_bounds__(256, 1) void tree_mfma_kernel(TreeParams p) {
 // 64 rows a wave read half as much from LDS and took 132 (198) us with one wave a
 // SIMD, 256 (406) us with two, which spill; without the overlap 163 (248) us.
 // PAGE: tiles of 32 keys lie within one page, whose rows have one base and stride
-// (198 us for 208 with an address per row, 128K keys, 64 rows a wave).
+// (198 us for 208 with an address per row, 128K keys, 64 rows a wave; with 32 rows a
+// wave it is 112 and 181 us in pages of 64 rows, 108 and 188 with an address per row
+// in pages of 16, which spills one register).
 template <int D, int NG, int WR, int WK, int NS, bool PAGE>
 __global__ __launch_bounds__(64 * WR * WK, WR * WK / 4) void tree_pipe_kernel(TreeParams p) {
   using M = Mfma16A;
@@ -1124,9 +1126,9 @@ struct MlaTree {
   static constexpr int kCh = kDv / 8, kCr = (kDqk - kDv) / 8;  // 16-byte chunks of the two parts of a row
 };
 
-// PAGE: tiles lie within one page (64 rows or more), whose rows have one base:
-// 250 us against 260 with an address per row (4 sequences of 8K to 32K keys, 8
-// tokens, 128 heads).
+// PAGE: tiles lie within one page (64 rows or more), whose rows have one base: 245 to
+// 252 us, with an address per row 245 to 256 in pages of 16 and 32 rows (4 sequences
+// of 8K to 32K keys, 8 tokens, 128 heads).
 template <bool PAGE>
 __global__ __launch_bounds__(512, 2) void tree_mla_kernel(TreeParams p) {
   typedef MlaTree C;
