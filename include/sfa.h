@@ -244,6 +244,65 @@ typedef struct sfa_tree_args {
   int32_t flags;                                   /* reserved, must be 0             */
 } sfa_tree_args;
 
+/* ---- dense attention: a chunk of new tokens over a paged cache, or a sequence --
+ * Token t < lens[b] of sequence b stands at row pos = ctx_lens[b] + t and sees the
+ * rows j <= pos with j < first or pos - j < window (window 0: all of them); rows of
+ * unmapped pages, and rows past the table, are not seen.  With pages the k and v
+ * rows are the cache's (the chunk's own among them), else k and v are [B, S, Hkv, D]
+ * and ctx_lens NULL.  A token t >= lens[b] gives out = 0 and lse = -inf, as does
+ * one that sees nothing (with a sink its lse is the sink).
+ * kv_dtype: dtype, or with pages SFA_DTYPE_FP8_E4M3: a row of a head stands for its
+ * e4m3 values times 2^(e - 127), e its exponent byte in k_scale / v_scale
+ * [num_pages, page_size, Hkv] (255: NaN). */
+typedef struct sfa_dense_args {
+  int32_t dtype, kv_dtype;
+  int32_t B, S, Hq, Hkv, Dqk, Dv;                  /* head dims <= 1024               */
+  int32_t window, first;
+  float scale;                                     /* > 0                             */
+  const void* q;  int64_t q_sb, q_ss, q_sh;        /* [B, S, Hq, Dqk]                 */
+  const void* k;  int64_t k_sb, k_ss, k_sh;        /* pools: page, row, head strides  */
+  const void* v;  int64_t v_sb, v_ss, v_sh;        /* (v may be the first Dv dims of k) */
+  const uint8_t* k_scale; int64_t ks_sb, ks_ss, ks_sh;
+  const uint8_t* v_scale; int64_t vs_sb, vs_ss, vs_sh;
+  const int32_t* ctx_lens;                         /* [B], or NULL: 0                 */
+  const int32_t* lens;                             /* [B], or NULL: S                 */
+  const float* sink;                               /* [Hq] or NULL                    */
+  void* out;      int64_t o_sb, o_ss, o_sh;        /* [B, S, Hq, Dv]                  */
+  float* lse;     int64_t l_sb, l_ss, l_sh;        /* [B, S, Hq]                      */
+  int32_t flags;                                   /* reserved, must be 0             */
+} sfa_dense_args;
+/* Its backward, without pages: out and lse as the forward left them. */
+typedef struct sfa_dense_bwd_args {
+  sfa_dense_args fwd;
+  const void* dout; int64_t do_sb, do_ss, do_sh;
+  void* dq;       int64_t dq_sb, dq_ss, dq_sh;
+  void* dk;       int64_t dk_sb, dk_ss, dk_sh;
+  void* dv;       int64_t dv_sb, dv_ss, dv_sh;
+  const float* dlse;                               /* lse's strides, or NULL          */
+  float* dsink;                                    /* [Hq], or NULL                   */
+  int32_t flags;                                   /* reserved, must be 0             */
+} sfa_dense_bwd_args;
+
+/* Exponent bytes of the pools that sfa_rope_append_fp8 writes, with page, row and
+ * head strides. */
+typedef struct sfa_kv_scales {
+  uint8_t* k; int64_t k_sb, k_ss, k_sh;
+  uint8_t* v; int64_t v_sb, v_ss, v_sh;            /* NULL without v rows             */
+} sfa_kv_scales;
+
+/* Rows of a paged cache, in order: out[b, i] is row starts[b] + i of sequence b, zeros
+ * where that is negative, at or past lens[b], or on an unmapped page. */
+typedef struct sfa_cache_read_args {
+  int32_t dtype, cache_dtype;                      /* of out; of the pool: F32, BF16 or FP8_E4M3 */
+  int32_t B, N, H, D;
+  const void* cache; int64_t c_sb, c_ss, c_sh;     /* [num_pages, page_size, H, D]    */
+  const uint8_t* scale; int64_t s_sb, s_ss, s_sh;  /* FP8_E4M3: exponent bytes        */
+  const int32_t* starts;                           /* [B], or NULL: 0                 */
+  const int32_t* lens;                             /* [B]                             */
+  void* out; int64_t o_sb, o_ss, o_sh;             /* [B, N, H, D]                    */
+  int32_t flags;                                   /* reserved, must be 0             */
+} sfa_cache_read_args;
+
 /* ---- pages of a cache -------------------------------------------------------
  * block_table [B, max_pages] as in sfa_kv_pages (-1: none), ref_counts
  * [num_pages] the number of entries that map a page: a page is free iff its
@@ -362,6 +421,14 @@ SFA_API int sfa_bwd(const sfa_bwd_args* a, void* workspace, size_t workspace_byt
  * cache row leave one of them there, which is not specified. */
 SFA_API int sfa_rope_fwd(const sfa_rope_args* a, const sfa_kv_pages* pages, void* stream);
 
+/* sfa_rope_fwd with pages whose pools hold e4m3 bytes: the k rows (normed and turned,
+ * float32) and the v rows of a's type are quantised as they are written.  Each row
+ * of a head is divided by the smallest power of two 2^(e - 127), 16 <= e, that
+ * brings its largest finite magnitude to 448 or less, and rounded to the nearest
+ * e4m3 value; infinities and NaN become NaN.  k_out / v_out and scales: bytes. */
+SFA_API int sfa_rope_append_fp8(const sfa_rope_args* a, const sfa_kv_pages* pages, const sfa_kv_scales* scales,
+                                void* stream);
+
 /* dq, dk and the weights' gradients (summed in a fixed order) from the results'
  * gradients in q_out / k_out.  Workspace: 8 KiB per workgroup, up to 8 MiB, with
  * a norm; 0 without. */
@@ -373,6 +440,20 @@ SFA_API int sfa_rope_bwd(const sfa_rope_args* a, void* workspace, size_t workspa
 SFA_API size_t sfa_tree_fwd_workspace_size(const sfa_tree_args* a, const sfa_kv_pages* pages);
 SFA_API int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
                          void* stream);
+
+/* Dense attention.  Workspace: float32 partials where the keys of few query rows are
+ * cut into ranges.  pages NULL: contiguous k and v. */
+SFA_API size_t sfa_dense_fwd_workspace_size(const sfa_dense_args* a, const sfa_kv_pages* pages);
+SFA_API int sfa_dense_fwd(const sfa_dense_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* Its gradients (every sum in a fixed order).  Workspace: two floats a query row, and
+ * float32 partials of key blocks that many rows see. */
+SFA_API size_t sfa_dense_bwd_workspace_size(const sfa_dense_bwd_args* a);
+SFA_API int sfa_dense_bwd(const sfa_dense_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of a paged cache as contiguous ones of a's dtype. */
+SFA_API int sfa_cache_read(const sfa_cache_read_args* a, const sfa_kv_pages* pages, void* stream);
 
 /* Workspace of the sfa_cache_* calls on n pairs (or sequences). */
 SFA_API size_t sfa_cache_workspace_size(const sfa_cache* c, int32_t n);

@@ -13,15 +13,18 @@ Top-k index producer (scores + selection that create ``topk_idxs``):
 
 Around the attention: rotary positions and per-head norms (``ops_amd.rotary_embedding``,
 ``ops_amd.qk_norm_rope``, and ``ops_amd.qk_norm_rope_append`` into a cache's pages),
-drafted trees over the cache (``ops_amd.tree_attention_paged``), and its pages
-(``ops_amd.cache_extend``, ``cache_fork``, ``cache_free``, ``cache_compact``,
-``cache_copy_pages``, ``cache_keep_path``).
+dense attention of chunks over the cache (``ops_amd.chunk_attention_paged``) and of
+whole sequences (``ops_amd.window_attention``), drafted trees over the cache
+(``ops_amd.tree_attention_paged``), and its pages (``ops_amd.cache_extend``,
+``cache_fork``, ``cache_free``, ``cache_compact``, ``cache_copy_pages``,
+``cache_keep_path``, ``cache_read``).
 
 The HIP kernels live in ``libsfa.so`` (``python -m ops_amd.build``), reached
 through the C ABI declared in ``include/sfa.h``.
 """
 from .cache import (cache_compact, cache_copy_pages, cache_extend, cache_fork, cache_free,
-                    cache_keep_path)
+                    cache_keep_path, cache_read)
+from .dense import chunk_attention_paged, window_attention
 from .indexer import indexer_topk
 from .rope import qk_norm_rope, qk_norm_rope_append, rope_frequencies, rotary_embedding
 from .sfa import (SparseFlashAttention, SparseFlashAttentionSBHD, SparseFlashAttentionTriton, sfa_backward,
@@ -31,4 +34,5 @@ from .tree import tree_attention_paged
 __all__ = ["SparseFlashAttention", "sparse_flash_attention", "sfa_forward", "sfa_backward", "sfa_forward_paged",
            "SparseFlashAttentionSBHD", "SparseFlashAttentionTriton", "indexer_topk",
            "rope_frequencies", "rotary_embedding", "qk_norm_rope", "qk_norm_rope_append", "tree_attention_paged",
-           "cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path"]
+           "chunk_attention_paged", "window_attention",
+           "cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path", "cache_read"]

@@ -105,3 +105,28 @@ def table(block_table: torch.Tensor, B: int, device: torch.device) -> torch.Tens
     if bt.stride(1) != 1 or (B > 1 and bt.stride(0) < bt.shape[1]):
         bt = bt.contiguous()
     return bt
+
+
+SCALES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def check_scales(name: str, scales: torch.Tensor, cache: torch.Tensor, device: torch.device) -> None:
+    """The exponent bytes of an e4m3 pool ``[num_pages, page_size, H, D]``."""
+    if scales is None:
+        raise ValueError(f"an e4m3 cache needs its {name}")
+    need_gpu(name, scales, device)
+    if scales.dtype not in SCALES or scales.shape != cache.shape[:3]:
+        raise ValueError(f"{name} must be a uint8 or float8_e8m0fnu {list(cache.shape[:3])} tensor, got {scales.dtype} "
+                         f"{tuple(scales.shape)}")
+
+
+def strides4(t: torch.Tensor) -> tuple:
+    """Pointer and the three leading strides; zeros for None."""
+    return (0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:3])
+
+
+def count32(name: str, n: int, least: int) -> int:
+    """A whole number that the kernels hold in 32 bits."""
+    if int(n) != n or not least <= n < 1 << 31:
+        raise ValueError(f"{name} must be a whole number in [{least}, 2^31), got {n}")
+    return int(n)

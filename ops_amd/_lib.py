@@ -48,6 +48,12 @@ EXPORTED_SYMBOLS = (
     "sfa_rope_bwd",
     "sfa_tree_fwd_workspace_size",
     "sfa_tree_fwd",
+    "sfa_rope_append_fp8",
+    "sfa_dense_fwd_workspace_size",
+    "sfa_dense_fwd",
+    "sfa_dense_bwd_workspace_size",
+    "sfa_dense_bwd",
+    "sfa_cache_read",
     "sfa_cache_workspace_size",
     "sfa_cache_copy",
     "sfa_cache_fork",
@@ -165,6 +171,63 @@ class TreeArgs(ctypes.Structure):
     ]
 
 
+class DenseArgs(ctypes.Structure):
+    """Mirror of ``sfa_dense_args``."""
+    _fields_ = [
+        ("dtype", _i32), ("kv_dtype", _i32),
+        ("B", _i32), ("S", _i32), ("Hq", _i32), ("Hkv", _i32), ("Dqk", _i32), ("Dv", _i32),
+        ("window", _i32), ("first", _i32),
+        ("scale", ctypes.c_float),
+        ("q", _vp), ("q_sb", _i64), ("q_ss", _i64), ("q_sh", _i64),
+        ("k", _vp), ("k_sb", _i64), ("k_ss", _i64), ("k_sh", _i64),
+        ("v", _vp), ("v_sb", _i64), ("v_ss", _i64), ("v_sh", _i64),
+        ("k_scale", _vp), ("ks_sb", _i64), ("ks_ss", _i64), ("ks_sh", _i64),
+        ("v_scale", _vp), ("vs_sb", _i64), ("vs_ss", _i64), ("vs_sh", _i64),
+        ("ctx_lens", _vp),
+        ("lens", _vp),
+        ("sink", _vp),
+        ("out", _vp), ("o_sb", _i64), ("o_ss", _i64), ("o_sh", _i64),
+        ("lse", _vp), ("l_sb", _i64), ("l_ss", _i64), ("l_sh", _i64),
+        ("flags", _i32),
+    ]
+
+
+class DenseBwdArgs(ctypes.Structure):
+    """Mirror of ``sfa_dense_bwd_args``."""
+    _fields_ = [
+        ("fwd", DenseArgs),
+        ("dout", _vp), ("do_sb", _i64), ("do_ss", _i64), ("do_sh", _i64),
+        ("dq", _vp), ("dq_sb", _i64), ("dq_ss", _i64), ("dq_sh", _i64),
+        ("dk", _vp), ("dk_sb", _i64), ("dk_ss", _i64), ("dk_sh", _i64),
+        ("dv", _vp), ("dv_sb", _i64), ("dv_ss", _i64), ("dv_sh", _i64),
+        ("dlse", _vp),
+        ("dsink", _vp),
+        ("flags", _i32),
+    ]
+
+
+class KvScales(ctypes.Structure):
+    """Mirror of ``sfa_kv_scales``."""
+    _fields_ = [
+        ("k", _vp), ("k_sb", _i64), ("k_ss", _i64), ("k_sh", _i64),
+        ("v", _vp), ("v_sb", _i64), ("v_ss", _i64), ("v_sh", _i64),
+    ]
+
+
+class CacheReadArgs(ctypes.Structure):
+    """Mirror of ``sfa_cache_read_args``."""
+    _fields_ = [
+        ("dtype", _i32), ("cache_dtype", _i32),
+        ("B", _i32), ("N", _i32), ("H", _i32), ("D", _i32),
+        ("cache", _vp), ("c_sb", _i64), ("c_ss", _i64), ("c_sh", _i64),
+        ("scale", _vp), ("s_sb", _i64), ("s_ss", _i64), ("s_sh", _i64),
+        ("starts", _vp),
+        ("lens", _vp),
+        ("out", _vp), ("o_sb", _i64), ("o_ss", _i64), ("o_sh", _i64),
+        ("flags", _i32),
+    ]
+
+
 class CachePool(ctypes.Structure):
     """Mirror of ``sfa_cache_pool``."""
     _fields_ = [("base", _vp), ("page_stride", _i64), ("page_bytes", _i64)]
@@ -234,6 +297,12 @@ def load() -> ctypes.CDLL:
                 ("sfa_rope_bwd", ctypes.c_int, [ptr(RopeArgs), _vp, size, _vp]),
                 ("sfa_tree_fwd_workspace_size", size, [ptr(TreeArgs), ptr(KvPages)]),
                 ("sfa_tree_fwd", ctypes.c_int, [ptr(TreeArgs), ptr(KvPages), _vp, size, _vp]),
+                ("sfa_rope_append_fp8", ctypes.c_int, [ptr(RopeArgs), ptr(KvPages), ptr(KvScales), _vp]),
+                ("sfa_dense_fwd_workspace_size", size, [ptr(DenseArgs), ptr(KvPages)]),
+                ("sfa_dense_fwd", ctypes.c_int, [ptr(DenseArgs), ptr(KvPages), _vp, size, _vp]),
+                ("sfa_dense_bwd_workspace_size", size, [ptr(DenseBwdArgs)]),
+                ("sfa_dense_bwd", ctypes.c_int, [ptr(DenseBwdArgs), _vp, size, _vp]),
+                ("sfa_cache_read", ctypes.c_int, [ptr(CacheReadArgs), ptr(KvPages), _vp]),
                 ("sfa_cache_workspace_size", size, [ptr(Cache), _i32]),
                 ("sfa_cache_copy", ctypes.c_int, [ptr(Cache), _vp, _vp, _i32, _vp, size, _vp]),
                 ("sfa_cache_fork", ctypes.c_int, [ptr(Cache), _vp, _vp, _i32, _vp, _vp, size, _vp]),

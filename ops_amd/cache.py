@@ -1,5 +1,5 @@
 """Pages of a paged KV cache on MI355X: mapping, forking, freeing, compacting
-and copying them, all on the device.
+and copying them, all on the device, and reading their rows back.
 
 The state is the caller's: ``block_table`` int32 ``[B, max_pages]`` (the page of
 each sequence's i-th run of ``page_size`` rows, -1: none) as the paged forwards
@@ -21,12 +21,15 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._host import call, int32, int_vec, need_gpu, written
+from ._host import (DTYPES, call, check_pool, check_scales, count32, int32, int_vec, kv_pages, need_gpu, strides4, table,
+                    written)
 
-__all__ = ["cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path"]
+__all__ = ["cache_copy_pages", "cache_fork", "cache_free", "cache_extend", "cache_compact", "cache_keep_path", "cache_read"]
 
 _CACHE = struct.Struct("@P6iPqPP")
 assert _CACHE.size == ctypes.sizeof(_lib.Cache)
+_READ = struct.Struct("@6i" + 2 * "P3q" + "2P" + "P3q" + "i4x")
+assert _READ.size == ctypes.sizeof(_lib.CacheReadArgs)
 
 
 def _state(name: str, t: torch.Tensor, dim: int, device) -> None:
@@ -216,3 +219,58 @@ def cache_keep_path(caches: Sequence[torch.Tensor], block_table: torch.Tensor, c
     a, keep = _cache(pools, n, num_pages, page_size, block_table)
     call(dev, lib.sfa_cache_keep_path, ctypes.byref(a), ctx_lens.data_ptr(), path.data_ptr(), path.stride(0),
          path.shape[1])
+
+
+def cache_read(cache: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, length: int,
+               starts: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None,
+               dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rows of a cache ``[num_pages, page_size, H, D]`` in order, ``[B, length, H,
+    D]``: row ``i`` of sequence ``b`` is its row ``starts[b] + i`` (None: from 0), zeros
+    past ``lens[b]`` and on unmapped pages.  What an e4m3 cache's bytes stand for,
+    with its exponent bytes ``scales``, is exact in bfloat16 and float32
+    (``dtype``; None: the cache's own, bfloat16 for e4m3, or ``out``'s).  ``out`` may be
+    preallocated (unit feature stride, not part of the cache).  No gradient."""
+    if cache.requires_grad and torch.is_grad_enabled():
+        raise ValueError("reading a cache records no gradient: call it under torch.no_grad()")
+    need_gpu("cache", cache)
+    dev = cache.device
+    check_pool("cache", cache, dev)
+    fp8 = cache.dtype == torch.float8_e4m3fn
+    if not fp8 and cache.dtype not in DTYPES:
+        raise ValueError(f"unsupported cache dtype {cache.dtype}; expected bfloat16, float32 or float8_e4m3fn")
+    if fp8:
+        check_scales("scales", scales, cache, dev)
+    elif scales is not None:
+        raise ValueError("scales are those of an e4m3 cache")
+    num_pages, page_size, H, D = cache.shape
+    if cache.stride(3) != 1:
+        raise ValueError("the cache needs a unit feature stride")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [B, max_pages], got {tuple(block_table.shape)}")
+    B, N = block_table.shape[0], count32("length", length, 0)
+    bt = table(block_table, B, dev)
+    lens = int_vec("lens", lens, B, dev)
+    if starts is not None:
+        starts = int_vec("starts", starts, B, dev)
+    if dtype is None:
+        dtype = out.dtype if out is not None else torch.bfloat16 if fp8 else cache.dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}; expected bfloat16 or float32")
+    if out is None:
+        out = torch.empty((B, N, H, D), dtype=dtype, device=dev)
+    elif tuple(out.shape) != (B, N, H, D) or out.dtype != dtype or out.device != dev or (out.numel() and out.stride(3) != 1):
+        raise ValueError(f"out must be a {[B, N, H, D]} {dtype} tensor on {dev} with a unit feature stride")
+    written(out)
+    if out.numel() == 0:
+        return out
+    if num_pages == 0 or bt.shape[1] == 0:
+        return out.zero_()
+    try:
+        a = _lib.CacheReadArgs.from_buffer_copy(_READ.pack(
+            DTYPES[dtype], _lib.SFA_DTYPE_FP8_E4M3 if fp8 else DTYPES[cache.dtype], B, N, H, D, *strides4(cache),
+            *strides4(scales), 0 if starts is None else starts.data_ptr(), lens.data_ptr(), *strides4(out), 0))
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"the call's arguments do not fit the kernels' interface: {e}") from None
+    pg = kv_pages(bt, B, num_pages, page_size, dev)
+    call(dev, _lib.load().sfa_cache_read, ctypes.byref(a), ctypes.byref(pg))
+    return out

@@ -183,6 +183,95 @@ bool tree_vec(const sfa_tree_args* a) {
               a->o_sh) && al16(a->q) && al16(a->k) && al16(a->v) && al16(a->out);
 }
 
+// ---- dense attention -----------------------------------------------------------------
+
+int check_dense(const sfa_dense_args* a, const sfa_kv_pages* pg) {
+  if (a == nullptr) return fail(SFA_E_INVALID, "null argument struct");
+  if (a->dtype != SFA_DTYPE_F32 && a->dtype != SFA_DTYPE_BF16) return fail(SFA_E_INVALID, "unknown dtype %d", a->dtype);
+  const bool fp8 = a->kv_dtype == SFA_DTYPE_FP8_E4M3;
+  if (!fp8 && a->kv_dtype != a->dtype) return fail(SFA_E_INVALID, "k and v must have q's type or be e4m3 (got %d)", a->kv_dtype);
+  if (a->flags != 0) return fail(SFA_E_INVALID, "flags must be 0");
+  if (a->B <= 0 || a->S <= 0 || a->Hq <= 0 || a->Hkv <= 0) return fail(SFA_E_INVALID, "B, S, Hq, Hkv must be positive");
+  if (a->Hq % a->Hkv != 0) return fail(SFA_E_INVALID, "Hq (%d) must be a multiple of Hkv (%d)", a->Hq, a->Hkv);
+  if (a->Dqk <= 0 || a->Dv <= 0 || a->Dqk > kMaxHeadDim || a->Dv > kMaxHeadDim)
+    return fail(SFA_E_INVALID, "head dims must be in [1, %d]", kMaxHeadDim);
+  if (a->window < 0 || a->first < 0) return fail(SFA_E_INVALID, "window and first must not be negative");
+  if (!a->q || !a->k || !a->v || !a->out || !a->lse) return fail(SFA_E_INVALID, "null tensor pointer");
+  if (fp8 && (!a->k_scale || !a->v_scale)) return fail(SFA_E_INVALID, "e4m3 rows need their scales");
+  if (!(a->scale > 0.f) || isinf(a->scale)) return fail(SFA_E_INVALID, "scale must be finite and > 0");
+  if (pg != nullptr) {
+    const int rc = check_pages(pg, a->B);
+    if (rc != SFA_OK) return rc;
+    if (a->ctx_lens == nullptr) return fail(SFA_E_INVALID, "pages need ctx_lens");
+    if ((int64_t)pg->max_pages * pg->page_size > (int64_t)1 << 29)
+      return fail(SFA_E_UNSUPPORTED, "a table of more than 2^29 rows a sequence");
+  } else {
+    if (fp8) return fail(SFA_E_INVALID, "e4m3 rows are those of pages");
+    if (a->ctx_lens != nullptr) return fail(SFA_E_INVALID, "ctx_lens needs pages");
+    if (a->S > 1 << 29) return fail(SFA_E_UNSUPPORTED, "more than 2^29 tokens");
+  }
+  if ((int64_t)a->B * a->S > (int64_t)INT_MAX / 4 / a->Hq) return fail(SFA_E_UNSUPPORTED, "more than 2^29 query rows");
+  return SFA_OK;
+}
+
+sfa::DenseParams dense_params(const sfa_dense_args* a, const sfa_kv_pages* pg) {
+  constexpr int kNone = 1 << 30;  // a window past every row
+  sfa::DenseParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q; p.k = a->k; p.v = a->v; p.ks = a->k_scale; p.vs = a->v_scale;
+  p.ctx_lens = a->ctx_lens; p.lens = a->lens; p.sink = a->sink;
+  p.out = a->out; p.lse = a->lse;
+  p.q_sb = a->q_sb; p.q_ss = a->q_ss; p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb; p.k_ss = a->k_ss; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_ss = a->v_ss; p.v_sh = a->v_sh;
+  p.ks_sb = a->ks_sb; p.ks_ss = a->ks_ss; p.ks_sh = a->ks_sh;
+  p.vs_sb = a->vs_sb; p.vs_ss = a->vs_ss; p.vs_sh = a->vs_sh;
+  p.o_sb = a->o_sb; p.o_ss = a->o_ss; p.o_sh = a->o_sh;
+  p.l_sb = a->l_sb; p.l_ss = a->l_ss; p.l_sh = a->l_sh;
+  p.B = a->B; p.S = a->S; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv;
+  p.Dqk = a->Dqk; p.Dv = a->Dv;
+  p.window = a->window == 0 || a->window > kNone ? kNone : a->window;
+  p.first = a->first;
+  p.cap = a->S;
+  if (pg != nullptr) {
+    p.block_table = pg->block_table; p.bt_sb = pg->bt_sb;
+    p.num_pages = pg->num_pages;
+    p.page_shift = __builtin_ctz((unsigned)pg->page_size);
+    p.cap = pg->max_pages * pg->page_size;
+  }
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * sfa::kLog2e;
+  // rows and strides of whole 16-byte units (8 bytes of an 8-bit row)
+  const int E = a->dtype == SFA_DTYPE_F32 ? 4 : 8;
+  p.vec = mult(E, a->Dqk, a->Dv, a->q_sb, a->q_ss, a->q_sh, a->k_sb, a->k_ss, a->k_sh, a->v_sb, a->v_ss, a->v_sh, a->o_sb,
+               a->o_ss, a->o_sh) && al16(a->q) && al16(a->k) && al16(a->v) && al16(a->out);
+  return p;
+}
+
+int check_dense_bwd(const sfa_dense_bwd_args* a) {
+  if (a == nullptr) return fail(SFA_E_INVALID, "null argument struct");
+  const int rc = check_dense(&a->fwd, nullptr);
+  if (rc != SFA_OK) return rc;
+  if (a->flags != 0) return fail(SFA_E_INVALID, "flags must be 0");
+  if (!a->dout || !a->dq || !a->dk || !a->dv) return fail(SFA_E_INVALID, "null gradient pointer");
+  if (a->dsink != nullptr && a->fwd.sink == nullptr) return fail(SFA_E_INVALID, "dsink without a sink");
+  return SFA_OK;
+}
+
+sfa::DenseParams dense_bwd_params(const sfa_dense_bwd_args* a) {
+  sfa::DenseParams p = dense_params(&a->fwd, nullptr);
+  p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  p.do_sb = a->do_sb; p.do_ss = a->do_ss; p.do_sh = a->do_sh;
+  p.dq_sb = a->dq_sb; p.dq_ss = a->dq_ss; p.dq_sh = a->dq_sh;
+  p.dk_sb = a->dk_sb; p.dk_ss = a->dk_ss; p.dk_sh = a->dk_sh;
+  p.dv_sb = a->dv_sb; p.dv_ss = a->dv_ss; p.dv_sh = a->dv_sh;
+  p.dlse = a->dlse; p.dsink = a->dsink;
+  const int E = a->fwd.dtype == SFA_DTYPE_F32 ? 4 : 8;
+  p.vec = p.vec && mult(E, a->do_sb, a->do_ss, a->do_sh, a->dq_sb, a->dq_ss, a->dq_sh, a->dk_sb, a->dk_ss, a->dk_sh, a->dv_sb,
+                        a->dv_ss, a->dv_sh) && al16(a->dout) && al16(a->dq) && al16(a->dk) && al16(a->dv);
+  return p;
+}
+
 // ---- pages ---------------------------------------------------------------------------
 
 constexpr int kMaxPools = 1024;
@@ -269,6 +358,23 @@ int sfa_rope_fwd(const sfa_rope_args* a, const sfa_kv_pages* pages, void* stream
   return done(sfa::launch_rope_fwd(p, a->dtype, vec, (hipStream_t)stream), "sfa_rope_fwd");
 }
 
+int sfa_rope_append_fp8(const sfa_rope_args* a, const sfa_kv_pages* pages, const sfa_kv_scales* scales, void* stream) {
+  sfa::api_clear();
+  int rc = check_rope(a, false, true);
+  if (rc == SFA_OK) rc = check_pages(pages, a->B);
+  if (rc != SFA_OK) return rc;
+  if (scales == nullptr || !scales->k || (a->Dv > 0 && !scales->v)) return fail(SFA_E_INVALID, "null scales");
+  sfa::RopeParams p = rope_params(a, pages);
+  p.ks = scales->k; p.ks_sb = scales->k_sb; p.ks_ss = scales->k_ss; p.ks_sh = scales->k_sh;
+  if (p.v != nullptr) {
+    p.vs = scales->v; p.vs_sb = scales->v_sb; p.vs_ss = scales->v_ss; p.vs_sh = scales->v_sh;
+  }
+  // (the v rows go through the lanes of the k rows)
+  const bool vec = rope_vec(a, p, false) && (p.v == nullptr || p.Dv == p.D);
+  sfa::rope_geometry(p, a->dtype == SFA_DTYPE_F32 ? 4 : 2, vec);
+  return done(sfa::launch_rope_fwd(p, a->dtype, vec, (hipStream_t)stream), "sfa_rope_append_fp8");
+}
+
 size_t sfa_rope_bwd_workspace_size(const sfa_rope_args* a) {
   if (check_rope(a, true, false) != SFA_OK) return 0;
   sfa::RopeParams p = rope_params(a, nullptr);
@@ -315,6 +421,84 @@ int sfa_tree_fwd(const sfa_tree_args* a, const sfa_kv_pages* pages, void* worksp
     p.seq_slots = (int32_t*)((char*)workspace + pl.part_o_bytes + pl.part_lse_bytes);
   }
   return done(sfa::launch_tree(p, pl, a->dtype, (hipStream_t)stream), "sfa_tree_fwd");
+}
+
+size_t sfa_dense_fwd_workspace_size(const sfa_dense_args* a, const sfa_kv_pages* pages) {
+  if (check_dense(a, pages) != SFA_OK) return 0;
+  const sfa::DensePlan pl = sfa::dense_plan(dense_params(a, pages), a->dtype, a->kv_dtype);
+  return pl.fits() ? pl.workspace() : 0;
+}
+
+int sfa_dense_fwd(const sfa_dense_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  sfa::api_clear();
+  const int rc = check_dense(a, pages);
+  if (rc != SFA_OK) return rc;
+  sfa::DenseParams p = dense_params(a, pages);
+  const sfa::DensePlan pl = sfa::dense_plan(p, a->dtype, a->kv_dtype);
+  if (!pl.fits()) return fail(SFA_E_UNSUPPORTED, "more query rows than one launch holds (%lld workgroups)", (long long)pl.wgs);
+  const size_t need = pl.workspace();
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(SFA_E_WORKSPACE, "sfa_dense_fwd needs %zu workspace bytes (got %zu)", need, workspace_bytes);
+    p.part_o = (float*)workspace;
+    p.part_lse = (float*)((char*)workspace + pl.part_o_bytes);
+    p.unit_slots = (int32_t*)((char*)workspace + pl.part_o_bytes + pl.part_lse_bytes);
+  }
+  return done(sfa::launch_dense(p, pl, a->dtype, a->kv_dtype, (hipStream_t)stream), "sfa_dense_fwd");
+}
+
+size_t sfa_dense_bwd_workspace_size(const sfa_dense_bwd_args* a) {
+  if (check_dense_bwd(a) != SFA_OK) return 0;
+  const sfa::DenseBwdPlan pl = sfa::dense_bwd_plan(dense_bwd_params(a), a->fwd.dtype);
+  return pl.fits ? pl.workspace() : 0;
+}
+
+int sfa_dense_bwd(const sfa_dense_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  sfa::api_clear();
+  const int rc = check_dense_bwd(a);
+  if (rc != SFA_OK) return rc;
+  sfa::DenseParams p = dense_bwd_params(a);
+  const sfa::DenseBwdPlan pl = sfa::dense_bwd_plan(p, a->fwd.dtype);
+  if (!pl.fits) return fail(SFA_E_UNSUPPORTED, "more rows than one launch holds");
+  const size_t need = pl.workspace();
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(SFA_E_WORKSPACE, "sfa_dense_bwd needs %zu workspace bytes (got %zu)", need, workspace_bytes);
+  p.row_lse = (float*)workspace;
+  p.row_delta = (float*)((char*)workspace + pl.row_bytes / 2);
+  p.dkv_part = (float*)((char*)workspace + pl.row_bytes);
+  return done(sfa::launch_dense_bwd(p, pl, a->fwd.dtype, (hipStream_t)stream), "sfa_dense_bwd");
+}
+
+int sfa_cache_read(const sfa_cache_read_args* a, const sfa_kv_pages* pages, void* stream) {
+  sfa::api_clear();
+  if (a == nullptr) return fail(SFA_E_INVALID, "null argument struct");
+  if (a->dtype != SFA_DTYPE_F32 && a->dtype != SFA_DTYPE_BF16) return fail(SFA_E_INVALID, "unknown dtype %d", a->dtype);
+  const bool fp8 = a->cache_dtype == SFA_DTYPE_FP8_E4M3;
+  if (!fp8 && a->cache_dtype != SFA_DTYPE_F32 && a->cache_dtype != SFA_DTYPE_BF16)
+    return fail(SFA_E_INVALID, "unknown cache dtype %d", a->cache_dtype);
+  if (a->flags != 0) return fail(SFA_E_INVALID, "flags must be 0");
+  if (a->B <= 0 || a->N <= 0 || a->H <= 0 || a->D <= 0) return fail(SFA_E_INVALID, "B, N, H, D must be positive");
+  if (a->B > kMaxGridYZ) return fail(SFA_E_UNSUPPORTED, "more than %d sequences", kMaxGridYZ);
+  if (!a->cache || !a->lens || !a->out) return fail(SFA_E_INVALID, "null tensor pointer");
+  if (fp8 && !a->scale) return fail(SFA_E_INVALID, "e4m3 rows need their scales");
+  const int rc = check_pages(pages, a->B);
+  if (rc != SFA_OK) return rc;
+  if ((int64_t)a->H * a->D > INT_MAX / 8) return fail(SFA_E_UNSUPPORTED, "rows of more than 2^28 elements");
+  if (a->N > 1 << 25) return fail(SFA_E_UNSUPPORTED, "more than 2^25 rows a sequence");
+  sfa::ReadParams p;
+  memset(&p, 0, sizeof(p));
+  p.cache = a->cache; p.scale = a->scale; p.starts = a->starts; p.lens = a->lens; p.out = a->out;
+  p.block_table = pages->block_table; p.bt_sb = pages->bt_sb;
+  p.max_pages = pages->max_pages; p.num_pages = pages->num_pages;
+  p.page_shift = __builtin_ctz((unsigned)pages->page_size);
+  p.c_sb = a->c_sb; p.c_ss = a->c_ss; p.c_sh = a->c_sh;
+  p.s_sb = a->s_sb; p.s_ss = a->s_ss; p.s_sh = a->s_sh;
+  p.o_sb = a->o_sb; p.o_ss = a->o_ss; p.o_sh = a->o_sh;
+  p.B = a->B; p.N = a->N; p.H = a->H; p.D = a->D;
+  // units of 8 elements: 8, 16 or 32 bytes
+  const bool vec = mult(8, a->D, a->c_sb, a->c_ss, a->c_sh, a->o_sb, a->o_ss, a->o_sh) && al16(a->cache) && al16(a->out);
+  return done(sfa::launch_cache_read(p, a->dtype, a->cache_dtype, vec, (hipStream_t)stream), "sfa_cache_read");
 }
 
 size_t sfa_cache_workspace_size(const sfa_cache* c, int32_t n) {

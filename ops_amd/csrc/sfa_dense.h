@@ -1,0 +1,195 @@
+// Dense attention (no index rows): a chunk of new tokens over a paged cache, or
+// a whole sequence, both through an optional window.  Shared by its kernels
+// (sfa_dense_*.hip).
+//
+// Token t < n_b of sequence b stands at row pos = ctx_b + t and sees the rows j <=
+// pos with j < first or pos - j < window.  The query rows of a (sequence, kv head)
+// are r = t G + h, h < G = Hq / Hkv: its keys serve all G heads.
+#pragma once
+
+#include "sfa_lds.h"
+#include "sfa_mfma.h"
+#include "sfa_ops.h"
+
+namespace sfa {
+
+// Base-2 log-sum-exp of 2^m2 l (the logarithm of l's mantissa: its own whole
+// part would round the sum once more), and the natural one.
+__device__ __forceinline__ float dense_lse2(float m2, float l) {
+  int e;
+  const float f = frexpf(l, &e);
+  return m2 + ((float)e + log2f(f));
+}
+__device__ __forceinline__ float dense_lse(float m2, float l) {
+  int e;
+  const float f = frexpf(l, &e);
+  return fmaf(m2, kLn2, fmaf((float)e, kLn2, logf(f)));
+}
+
+struct DenseSeq {
+  int ctx, n;  // rows before the first token, tokens
+};
+__device__ __forceinline__ DenseSeq dense_seq(const DenseParams& p, int b) {
+  DenseSeq s;
+  s.ctx = p.ctx_lens != nullptr ? min(max(p.ctx_lens[b], 0), p.cap) : 0;
+  s.n = p.lens != nullptr ? min(max(p.lens[b], 0), p.S) : p.S;
+  return s;
+}
+
+__device__ __forceinline__ bool dense_seen(const DenseParams& p, int j, int pos) {
+  return j <= pos && (j < p.first || pos - j < p.window);
+}
+
+// The key tiles of 2^shift keys that some row of a block sees: the first ones,
+// then those of the window; tile(v) is the v-th.
+struct KeyTiles {
+  int head, from, n;
+  __device__ __forceinline__ int tile(int v) const { return v < head ? v : v - head + from; }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const DenseParams& p, const DenseSeq& s, int row0, int rows, int shift) {
+  KeyTiles k{0, 0, 0};
+  const int t0 = row0 / p.G, t1 = min((row0 + rows - 1) / p.G, s.n - 1);
+  if (t0 > t1) return k;
+  const int hi = min(s.ctx + t1 + 1, p.cap), lo = max(0, s.ctx + t0 - p.window + 1), one = (1 << shift) - 1;
+  const int end = (hi + one) >> shift;
+  k.head = lo > 0 ? min((min(p.first, hi) + one) >> shift, end) : 0;
+  k.from = max(lo >> shift, k.head);
+  k.n = k.head + max(end - k.from, 0);
+  return k;
+}
+
+// Element offset of key j of sequence b, or -1: rows of unmapped pages and
+// (contiguous) of none.
+__device__ __forceinline__ int64_t dense_row(const DenseParams& p, int b, int j, int64_t sb, int64_t ss) {
+  if (j >= p.cap) return -1;
+  if (p.block_table == nullptr) return b * sb + j * ss;
+  const int pg = p.block_table[b * p.bt_sb + (j >> p.page_shift)];
+  if (pg < 0 || pg >= p.num_pages) return -1;
+  return (int64_t)pg * sb + (int64_t)(j & ((1 << p.page_shift) - 1)) * ss;
+}
+
+// The value of a scale's exponent byte.
+__device__ __forceinline__ float scale_of(uint8_t e) {
+  // (2^-127 is no normal number, 255 stands for NaN)
+  return __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : (uint32_t)e << 23);
+}
+
+// ---- key ranges of a launch ("slots") ---------------------------------------------
+// A unit is a (sequence, row block).  The units' tiles are cut into ranges of one
+// length, found on the device as the lengths are there; each unit has one at least.
+struct DenseSlot {
+  int unit;       // or -1: none
+  int v0, v1;     // its tiles, as KeyTiles counts them
+  int first, n;   // the unit's first slot and how many it has
+};
+__device__ __forceinline__ int dense_lanes_sum(int x) {
+  x += __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true);  // row_ror:8
+  x += __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x122, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x121, 0xf, 0xf, true);
+  const auto a = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+  x = (int)(a[0] + a[1]);
+  const auto c = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+  return (int)(c[0] + c[1]);
+}
+__device__ __forceinline__ int unit_tiles(const DenseParams& p, int u) {
+  const int b = u / p.nrb, rb = u - b * p.nrb;
+  return key_tiles(p, dense_seq(p, b), rb * p.rows, p.rows, p.tile_shift).n;
+}
+__device__ __forceinline__ DenseSlot dense_slot(const DenseParams& p, int slot) {
+  const int units = p.B * p.nrb;
+  if (p.want == 0) {
+    if (slot >= units) return DenseSlot{-1, 0, 0, 0, 0};
+    return DenseSlot{slot, 0, unit_tiles(p, slot), slot, 1};
+  }
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](int u) { return u < units ? unit_tiles(p, u) : 0; };
+  const int mine = tiles_of(lane);  // (of the first 64 units)
+  int64_t sum = dense_lanes_sum(mine);
+  for (int u0 = 64; u0 < units; u0 += 64) sum += dense_lanes_sum(tiles_of(u0 + lane));
+  const int len = max(p.min_len, (int)((sum + p.want - 1) / p.want));
+  int before = 0;
+  for (int u0 = 0; u0 < units; u0 += 64) {
+    const int u = u0 + lane, t = u0 == 0 ? mine : tiles_of(u);
+    const int n = u < units ? max(1, (t + len - 1) / len) : 0;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    const int first = before + incl - n;
+    const uint64_t hit = __ballot(slot >= first && slot < first + n);
+    if (hit != 0) {
+      const int w = __builtin_ctzll(hit);
+      DenseSlot s;
+      s.unit = u0 + w;
+      s.first = __builtin_amdgcn_readlane(first, w);
+      s.n = __builtin_amdgcn_readlane(n, w);
+      const int tiles = __builtin_amdgcn_readlane(t, w);
+      // (even ranges: the unit's tiles over its own number of slots)
+      const int i = slot - s.first;
+      s.v0 = (int)((int64_t)tiles * i / s.n);
+      s.v1 = (int)((int64_t)tiles * (i + 1) / s.n);
+      return s;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return DenseSlot{-1, 0, 0, 0, 0};
+}
+
+// A workgroup's share of a launch.
+struct DenseItem {
+  int b, g, rb, row0;
+  DenseSeq s;
+  KeyTiles tiles;
+  int v0, v1;
+  int64_t part;   // row of the partial results of the block's first row
+  bool partial;
+};
+__device__ __forceinline__ bool dense_item(const DenseParams& p, int slot, int g, DenseItem& it) {
+  const DenseSlot sl = dense_slot(p, slot);
+  if (sl.unit < 0) return false;
+  const int unit = __builtin_amdgcn_readfirstlane(sl.unit);
+  it.b = unit / p.nrb;
+  it.rb = unit - it.b * p.nrb;
+  it.g = g;
+  it.row0 = it.rb * p.rows;
+  it.s = dense_seq(p, it.b);
+  it.tiles = key_tiles(p, it.s, it.row0, p.rows, p.tile_shift);
+  it.v0 = __builtin_amdgcn_readfirstlane(sl.v0);
+  it.v1 = __builtin_amdgcn_readfirstlane(sl.v1);
+  it.part = ((int64_t)slot * p.Hkv + g) * p.rows;
+  it.partial = sl.n > 1;
+  if (p.want > 0 && slot == sl.first && g == 0 && threadIdx.x == 0) {
+    p.unit_slots[2 * unit] = sl.first;
+    p.unit_slots[2 * unit + 1] = sl.n;
+  }
+  return true;
+}
+
+// The factor and LSE of a finished row of head h with maximum m (base 2) and sum l.
+__device__ __forceinline__ float dense_finish(const DenseParams& p, int h, bool live, float m, float l, float& lse) {
+  if (!live) {
+    lse = kNegInf;
+    return 0.f;
+  }
+  if (l == 0.f) {  // nothing seen
+    lse = p.sink ? p.sink[h] : kNegInf;
+    return 0.f;
+  }
+  const float sink2 = p.sink ? p.sink[h] * kLog2e : kNegInf;
+  const float mm = fmaxf(m, sink2);
+  const float f = m == kNegInf ? 0.f : exp2f(m - mm);
+  float x = l * f;
+  if (p.sink && mm != kNegInf) x += exp2f(sink2 - mm);
+  lse = x > 0.f ? dense_lse(mm, x) : x == 0.f ? kNegInf : x;
+  return x > 0.f ? f / x : x == 0.f ? 0.f : x;
+}
+// ... of a partial one: its own sum, base-2 LSE
+__device__ __forceinline__ float dense_part(float m, float l, float& lse2) {
+  lse2 = l > 0.f ? dense_lse2(m, l) : l == 0.f ? kNegInf : l;
+  return l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+}
+
+}  // namespace sfa

@@ -1,0 +1,219 @@
+// gfx950 dense attention through a window (sfa_dense.h): the choice of kernels,
+// the joining of key ranges, and the backward's row sums.
+
+#include "sfa_dense.h"
+
+namespace sfa {
+namespace {
+
+// ---- joining the ranges of a row block -------------------------------------------
+// One wave a row; LPR lanes hold it (4 dims each), 64 / LPR ranges at a time.  A range
+// in which the row sees nothing has LSE -inf.
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t i = (int64_t)blockIdx.x * 4 + wave;
+  const int row = (int)(i % p.rows);
+  i /= p.rows;
+  const int g = (int)(i % p.Hkv), u = (int)(i / p.Hkv);
+  if (u >= p.B * p.nrb) return;
+  const int b = u / p.nrb, r = (u - b * p.nrb) * p.rows + row;
+  if (r >= p.S * p.G) return;
+  const int first = p.unit_slots[2 * u], ns = p.unit_slots[2 * u + 1];
+  if (ns <= 1) return;
+  const int t = r / p.G, h = g * p.G + r % p.G;
+  const int64_t per = (int64_t)p.Hkv * p.rows, at0 = ((int64_t)first * p.Hkv + g) * p.rows + row;
+  const float* pl = p.part_lse + at0;
+  const float* po = p.part_o + at0 * p.Dv;
+  const bool live = t < dense_seq(p, b).n;
+  float m = kNegInf, nan = 0.f;
+  for (int k = lane; k < ns; k += 64) {
+    const float x = pl[k * per];
+    nan += x != x ? x : 0.f;
+    m = fmaxf(m, x);
+  }
+  m = wave_max(m);
+  const float moff = m == kNegInf ? 0.f : m;
+  float l = 0.f;
+  for (int k = lane; k < ns; k += 64) l += exp2f(pl[k * per] - moff);
+  l = wave_sum(l + nan);
+  float lse;
+  const float f = dense_finish(p, h, live, m, l, lse);
+  if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+  T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
+  const int sub = lane / LPR;
+  for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
+    const int d = d0 + 4 * (lane % LPR);
+    f32x4 x = {};
+    if (f != 0.f) {
+#pragma unroll 4
+      for (int k = sub; k < ns; k += 64 / LPR) {
+        const float e = exp2f(pl[k * per] - moff);
+        f32x4 v = {};
+        const float* at = po + k * per * p.Dv + d;
+        if (p.Dv % 4 == 0) {
+          if (d < p.Dv) v = *reinterpret_cast<const f32x4*>(at);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = d + q < p.Dv ? at[q] : 0.f;
+        }
+        x += v * e;
+      }
+    }
+#pragma unroll
+    for (int s = LPR; s < 64; s <<= 1)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] += __shfl_xor(x[q], s, 64);
+    if (sub == 0)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (d + q < p.Dv) o[d + q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+  }
+}
+template <typename T>
+void combine(const DenseParams& p, hipStream_t s) {
+  const unsigned grid = (unsigned)(((int64_t)p.B * p.nrb * p.Hkv * p.rows + 3) / 4);
+  if (p.Dv <= 64) dense_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p);
+  else if (p.Dv <= 128) dense_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p);
+  else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p);
+}
+
+// ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse ------------
+// 16 lanes a row.  Rows that see nothing get +inf, which makes every weight 0.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
+  const int64_t rr = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 15, R = p.S * p.G;
+  if (rr >= (int64_t)p.B * p.Hkv * R) return;
+  const int b = (int)(rr / ((int64_t)p.Hkv * R)), x = (int)(rr - (int64_t)b * p.Hkv * R), g = x / R, r = x - g * R;
+  const int t = r / p.G, h = g * p.G + r % p.G;
+  const bool live = t < dense_seq(p, b).n;
+  float sum = 0.f;
+  if (live) {
+    const T* o = reinterpret_cast<const T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
+    const T* go = reinterpret_cast<const T*>(p.dout) + b * p.do_sb + t * p.do_ss + h * p.do_sh;
+    if (p.vec && sizeof(T) == 2) {
+      for (int d = 8 * lane; d < p.Dv; d += 128) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(o + d), c = *reinterpret_cast<const bf16x8*>(go + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf((float)a[e], (float)c[e], sum);
+      }
+    } else {
+      for (int d = lane; d < p.Dv; d += 16) sum = fmaf(to_f32(o[d]), to_f32(go[d]), sum);
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) sum += __shfl_xor(sum, s, 64);
+  if (lane != 0) return;
+  const int64_t li = b * p.l_sb + t * p.l_ss + h * p.l_sh;
+  const float lse = live ? p.lse[li] : kNegInf;
+  p.row_lse[rr] = lse == kNegInf ? -kNegInf : lse * kLog2e;
+  p.row_delta[rr] = live ? sum - (p.dlse != nullptr ? p.dlse[li] : 0.f) : 0.f;
+}
+
+// dsink[h] = -sum over the rows of exp(sink - lse) delta, a workgroup a head, in a fixed order.
+__global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
+  __shared__ float s_x[1024];
+  const int h = blockIdx.x, g = h / p.G, hl = h % p.G;
+  const float sink = p.sink[h] * kLog2e;
+  float sum = 0.f;
+  for (int b = 0; b < p.B; ++b) {
+    const int64_t base = ((int64_t)b * p.Hkv + g) * p.S * p.G;
+    const int n = dense_seq(p, b).n;
+    for (int t = threadIdx.x; t < n; t += 1024) {
+      const int64_t rr = base + (int64_t)t * p.G + hl;
+      const float l = p.row_lse[rr];
+      sum += l == -kNegInf ? 0.f : exp2f(sink - l) * p.row_delta[rr];
+    }
+  }
+  s_x[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) s_x[threadIdx.x] += s_x[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.dsink[h] = -s_x[0];
+}
+
+enum { kAny = 0 };
+struct KernelShape {
+  int rows, tile_shift, threads;
+};
+constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256}};
+
+void set_launch(DenseParams& p, const DensePlan& pl) {
+  p.rows = pl.rows;
+  p.tile_shift = pl.tile_shift;
+  p.nrb = (int)(((int64_t)p.S * p.G + pl.rows - 1) / pl.rows);
+  p.want = pl.want;
+  p.min_len = pl.min_len;
+  p.slots = pl.slots;
+}
+
+}  // namespace
+
+DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
+  DensePlan pl{};
+  pl.kernel = kAny;
+  const KernelShape& k = kShapes[pl.kernel];
+  pl.rows = k.rows;
+  pl.tile_shift = k.tile_shift;
+  pl.threads = k.threads;
+  const int64_t nrb = ((int64_t)p.S * p.G + pl.rows - 1) / pl.rows, units = p.B * nrb;
+  const int64_t dims = pl.kernel == kAny ? (p.Dv + kAnyDims - 1) / kAnyDims : 1;
+  // Key ranges are cut while the row blocks are too few to fill the card evenly.
+  constexpr int64_t kWorkgroups = 1024;
+  pl.min_len = 4;
+  int64_t want = kWorkgroups / (p.Hkv * dims);
+  const int64_t most = (((int64_t)p.cap >> pl.tile_shift) + pl.min_len) / pl.min_len * units;
+  if (want > most) want = most;
+  pl.want = want > units ? (int)want : 0;
+  pl.slots = (int)(units + pl.want);
+  pl.wgs = (units + pl.want) * p.Hkv * dims;
+  if (pl.want > 0) {
+    const size_t rows = (size_t)pl.slots * p.Hkv * pl.rows;
+    pl.part_o_bytes = (rows * p.Dv * sizeof(float) + 255) / 256 * 256;
+    pl.part_lse_bytes = (rows * sizeof(float) + 255) / 256 * 256;
+    pl.unit_bytes = (size_t)2 * units * sizeof(int32_t);
+  }
+  return pl;
+}
+
+hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s) {
+  DenseParams p = p0;
+  set_launch(p, pl);
+  launch_dense_any(p, dtype, kv_dtype, s);
+  if (pl.want > 0) {
+    if (dtype == SFA_DTYPE_F32) combine<float>(p, s);
+    else combine<bf16>(p, s);
+  }
+  return hipGetLastError();
+}
+
+DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
+  DenseBwdPlan pl{};
+  const size_t rows = (size_t)p.B * p.Hkv * p.S * p.G;
+  pl.row_bytes = 2 * ((rows * sizeof(float) + 255) / 256 * 256);
+  const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
+  const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows;
+  pl.fits = p.B * nrb * p.Hkv * dims * 256 < (int64_t)1 << 32 && p.B * (((int64_t)p.S + 63) / 64) * p.Hkv * dims * 256 < (int64_t)1 << 32;
+  return pl;
+}
+
+hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int dtype, hipStream_t s) {
+  DenseParams p = p0;
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.S * p.G;
+  const unsigned grid = (unsigned)((rows + 15) / 16);
+  if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p);
+  else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
+  if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
+  DensePlan q{};
+  q.rows = kAnyRows;
+  q.tile_shift = kAnyShift;
+  q.slots = p.B * (int)(((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows);
+  set_launch(p, q);
+  launch_dense_bwd_any(p, dtype, s);
+  return hipGetLastError();
+}
+
+}  // namespace sfa

@@ -60,6 +60,9 @@ struct RopeParams {
   int64_t slot_sb, slot_ss;
   int slot_i64;
   int max_pages, page_shift, num_pages;
+  // append to 8-bit pools (y and v_out of side k are bytes): the rows' exponent bytes
+  uint8_t *ks, *vs;
+  int64_t ks_sb, ks_ss, ks_sh, vs_sb, vs_ss, vs_sh;
   // geometry (rope_geometry)
   int P, K, chunks;     // lanes a row, 16-byte chunks a lane, chunks a row
   int groups, per, upt; // row groups a token; in blocks of per, upt blocks a token
@@ -69,7 +72,7 @@ struct RopeParams {
 void rope_geometry(RopeParams& p, int esize, bool vec);
 int rope_bwd_wgs(const RopeParams& p);
 size_t rope_bwd_workspace(const RopeParams& p);
-hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);
+hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);  // p.ks: to 8-bit pools
 hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);
 
 // ---- attention of a tree of drafted tokens over a paged cache ----
@@ -112,6 +115,85 @@ struct TreePlan {
 };
 TreePlan tree_plan(const TreeParams& p, int dtype, bool vec);
 hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, int dtype, hipStream_t s);
+
+// ---- dense attention through a window: a chunk over a paged cache, a sequence ----
+struct DenseParams {
+  const void* q;
+  const void* k;             // pages: pools, else [B, cap]
+  const void* v;
+  const uint8_t* ks;         // 8-bit pools: exponent bytes, [pages, page, Hkv]
+  const uint8_t* vs;
+  const int32_t* block_table;  // nullptr: contiguous
+  const int32_t* ctx_lens;   // [B] or nullptr: 0
+  const int32_t* lens;       // [B] or nullptr: S
+  const float* sink;
+  void* out;
+  float* lse;
+  int64_t q_sb, q_ss, q_sh;
+  int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;  // (pools: page, row, head)
+  int64_t ks_sb, ks_ss, ks_sh, vs_sb, vs_ss, vs_sh;
+  int64_t o_sb, o_ss, o_sh, l_sb, l_ss, l_sh;
+  int64_t bt_sb;
+  int B, S, Hq, Hkv, G, Dqk, Dv;
+  int window, first;         // window: 2^30 stands for none
+  int page_shift, num_pages, cap;  // cap: rows a sequence can have
+  float scale, scale_log2;
+  bool vec;                  // rows are whole 16-byte units (8-bit: 8)
+  // a launch: row blocks of `rows` query rows, nrb a (sequence, kv head); key tiles of 2^tile_shift
+  int rows, nrb, tile_shift;
+  int want, min_len;         // key ranges wanted a kv head (0: one a row block), tiles of the shortest
+  int slots;                 // of the launch, a kv head
+  float* part_o;             // [slots][Hkv][rows][Dv], normalised by the slot's own sum
+  float* part_lse;           // [slots][Hkv][rows], base-2 (-inf: nothing seen)
+  int32_t* unit_slots;       // [B nrb][2] first slot and slots of a unit
+  // backward
+  const void* dout;
+  void *dq, *dk, *dv;
+  int64_t do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+  const float* dlse;         // lse's strides, or nullptr
+  float* dsink;              // [Hq] or nullptr
+  float* row_lse;            // [B][Hkv][S G] base-2 LSE, +inf for rows that see nothing
+  float* row_delta;          // [B][Hkv][S G] sum o do - dlse
+  float* dkv_part;           // partial dK | dV rows of key blocks cut in chunks of query rows
+  int chunk;                 // query rows a chunk
+};
+struct DensePlan {
+  int kernel;
+  int rows, tile_shift, want, min_len, slots;
+  int64_t wgs;               // workgroups of `threads` threads
+  int threads;
+  bool fits() const { return wgs * threads < (int64_t)1 << 32; }  // one launch
+  size_t part_o_bytes, part_lse_bytes, unit_bytes;
+  size_t workspace() const { return part_o_bytes + part_lse_bytes + unit_bytes; }
+};
+DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype);
+hipError_t launch_dense(const DenseParams& p, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s);
+struct DenseBwdPlan {
+  size_t row_bytes, dkv_bytes;  // row_lse + row_delta; partial dK | dV
+  int chunk;
+  bool mfma, fits;
+  size_t workspace() const { return row_bytes + dkv_bytes; }
+};
+DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype);
+hipError_t launch_dense_bwd(const DenseParams& p, const DenseBwdPlan& pl, int dtype, hipStream_t s);
+// any types and head dims (sfa_dense_any.hip)
+constexpr int kAnyRows = 64, kAnyShift = 5, kAnyDims = 128;
+void launch_dense_any(const DenseParams& p, int dtype, int kv_dtype, hipStream_t s);
+void launch_dense_bwd_any(const DenseParams& p, int dtype, hipStream_t s);
+
+// ---- rows of a cache as contiguous ones (sfa_read.hip) ----
+struct ReadParams {
+  const void* cache;
+  const uint8_t* scale;
+  const int32_t* block_table;
+  const int32_t* starts;  // nullptr: 0
+  const int32_t* lens;
+  void* out;
+  int64_t c_sb, c_ss, c_sh, s_sb, s_ss, s_sh, o_sb, o_ss, o_sh, bt_sb;
+  int B, N, H, D;
+  int max_pages, page_shift, num_pages;
+};
+hipError_t launch_cache_read(const ReadParams& p, int dtype, int cache_dtype, bool vec, hipStream_t s);
 
 // ---- pages of a cache ----
 constexpr int kPoolsPerLaunch = 48;

@@ -24,6 +24,11 @@
 // that it takes (rows of 4 or 9 chunks a lane form them again for every row and
 // rotated chunk: registers).  Rows that are not whole 16-byte chunks (odd dims,
 // strides, offsets) take the scalar kernels, one wave a row.
+//
+// 8-bit pools: a k or v row becomes e4m3 bytes times a power of two, the smallest that
+// brings its largest finite magnitude to 448 or less, from the float32 values (one
+// rounding).  Such a scale makes the division exact and costs e4m3 no precision
+// but at the small end of its range; what the row stands for is exact in bf16.
 
 #include "sfa_ops.h"
 
@@ -195,6 +200,73 @@ __device__ __forceinline__ int64_t cache_row(const RopeParams& p, int b, int s, 
   return (int64_t)pg * page_stride + (slot & ((1 << p.page_shift) - 1)) * row_stride;
 }
 
+// ---- 8-bit rows ----
+// Page and row in it of the cache row that token (b, s) goes to.
+__device__ __forceinline__ bool cache_place(const RopeParams& p, int b, int s, int& pg, int& in) {
+  const int64_t slot = load_int(p.slots, b * p.slot_sb + s * p.slot_ss, p.slot_i64);
+  if (slot < 0 || slot >= ((int64_t)p.max_pages << p.page_shift)) return false;
+  pg = load_const(p.block_table + b * p.bt_sb + (slot >> p.page_shift));
+  in = (int)slot & ((1 << p.page_shift) - 1);
+  return pg >= 0 && pg < p.num_pages;
+}
+// A value's part in its row's largest magnitude: infinities and NaN have none.
+__device__ __forceinline__ float finite_mag(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+// Exponent byte e of the smallest power of two 2^(e - 127) with amax <= 448 2^(e - 127)
+// = 1.75 2^(e - 119); at least 16, so that no value it makes is below float32's
+// normal range (amax of all zeros: 16).
+__device__ __forceinline__ int scale_byte(float amax) {
+  return max((int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8, 16);
+}
+__device__ __forceinline__ float inverse_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
+// Four values as e4m3 bytes (rounded to nearest, ties to even).
+__device__ __forceinline__ uint32_t e4m3x4(const float* x, float inv) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = fabsf(x[i]) <= 3.402823466e38f ? x[i] * inv : __uint_as_float(0x7fc00000u);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+}
+template <int P>
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, dpp<0xb1>(x));
+  x = fmaxf(x, dpp<0x4e>(x));
+  if constexpr (P >= 8) x = fmaxf(x, dpp<0x141>(x));
+  if constexpr (P >= 16) x = fmaxf(x, dpp<0x140>(x));
+  if constexpr (P >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if constexpr (P >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return x;
+}
+// The row in chunks l, l + P, .. of its lanes, quantised to y and its exponent to scale.
+template <int P, int K, int E>
+__device__ __forceinline__ void store_e4m3(const RopeParams& p, const float (&f)[K][E], int l, bool put, uint8_t* y,
+                                           uint8_t* scale) {
+  float a = 0.f;
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+#pragma unroll
+    for (int e = 0; e < E; ++e) a = j * P + l < p.chunks ? fmaxf(a, finite_mag(f[j][e])) : a;
+  const int se = scale_byte(row_max<P>(a));
+  const float inv = inverse_scale(se);
+  if (!put) return;
+  if (l == 0) *scale = (uint8_t)se;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int c = j * P + l;
+    if (c >= p.chunks) continue;
+    if constexpr (E == 8) *reinterpret_cast<u32x2*>(y + c * 8) = u32x2{e4m3x4(f[j], inv), e4m3x4(f[j] + 4, inv)};
+    else *reinterpret_cast<uint32_t*>(y + c * 4) = e4m3x4(f[j], inv);
+  }
+}
+
 // A row's chunks: lane l of its P lanes holds chunks l, l + P, ..  IN: half
 // layout over the whole row in two chunks a lane, so a lane holds both partners;
 // else partners are another lane's chunk (K = 1) or read again (K > 2).
@@ -354,7 +426,8 @@ struct Walk {
 // last pass left in the caches 73 and 70.  More in flight gains nothing
 // (NB 4 and 6, or 3 of rows in two chunks: 93, 95 us; 112).  Calls of one unit a wave take
 // NB = 1 (8.8 us for 11, 64 tokens into the cache: less code to fetch).
-template <typename T, int P, int K, bool IN, int NB>
+// FP8: the k rows, and the v rows in groups like theirs, go to 8-bit pools.
+template <typename T, int P, int K, bool IN, int NB, bool FP8 = false>
 __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kernel(RopeParams p) {
   typedef Row<T, P, K, IN> R;
   constexpr int E = R::E, rpw = 64 / P;
@@ -375,6 +448,7 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
     int64_t pos;
     int g;
     bool live, fresh, put;
+    uint8_t *pb, *ps;  // FP8: the row's bytes and its scale
   };
   bool fresh = true;
   auto fill = [&](Unit& u) __attribute__((always_inline)) {  // the walk's unit (past its end: the last one, again)
@@ -383,6 +457,24 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
     u.g = w.g;
     u.pos = load_int(p.pos, w.b * p.pos_sb + w.s * p.pos_ss, p.pos_i64);
     int64_t yo;
+    if constexpr (FP8) {
+      if (w.g >= gq) {  // rows of k, then of v
+        const bool isv = w.g >= gk;
+        const RopeSide& sd = p.side[1];
+        const int h = (isv ? w.g - gk : w.g - gq) * rpw + rr;
+        const int64_t hh = h < sd.H ? h : 0;
+        u.px = reinterpret_cast<const T*>(isv ? p.v : sd.x) + (isv ? w.b * p.v_sb + w.s * p.v_ss + hh * p.v_sh
+                                                                   : w.b * sd.x_sb + w.s * sd.x_ss + hh * sd.x_sh);
+        u.x.load(p, u.px, l, p.D);
+        int pg = 0, in = 0;
+        u.put = cache_place(p, w.b, w.s, pg, in) && h < sd.H;
+        u.pb = reinterpret_cast<uint8_t*>(isv ? p.v_out : sd.y) +
+               (isv ? pg * p.vo_sb + in * p.vo_ss + hh * p.vo_sh : pg * sd.y_sb + in * sd.y_ss + hh * sd.y_sh);
+        u.ps = isv ? p.vs + (pg * p.vs_sb + in * p.vs_ss + hh * p.vs_sh) : p.ks + (pg * p.ks_sb + in * p.ks_ss + hh * p.ks_sh);
+        if (u.live) fresh = w.next(p, p.groups, p.per, p.upt);
+        return;
+      }
+    }
     if (w.g >= gk) {  // of the v row: 64 chunks
       const int i = (w.g - gk) * 64 + lane, cpr = p.Dv / E;
       const bool in = i < p.side[1].H * cpr;
@@ -422,7 +514,14 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
     if constexpr (R::kHeld) {
       if (u.fresh) lt.angles(p, pos, freq, cs, sn);
     }
-    if (u.g >= gk) {  // v is copied
+    if (u.g >= gk) {  // v is copied, or quantised
+      if constexpr (FP8) {
+        float f[K][E];
+#pragma unroll
+        for (int j = 0; j < K; ++j) Chunk<T>::unpack(u.x.r[j], f[j]);
+        store_e4m3<P, K, E>(p, f, l, u.put, u.pb, u.ps);
+        return;
+      }
       if (u.put) *reinterpret_cast<u32x4*>(u.py) = u.x.r[0];
       return;
     }
@@ -442,6 +541,7 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
       }
       r = 1.f / sqrtf(row_sum<P>(q) / (float)sd.n + p.eps);
     }
+    float y8[FP8 ? K : 1][E];
     u.x.turn(
         p, u.px, lane, pos, cs, sn, 1.f,
         [&](int j, int c, float (&v)[E]) {
@@ -460,7 +560,22 @@ __global__ __launch_bounds__(256, K == 9 ? 2 : K > 2 ? 3 : 4) void rope_fwd_kern
             for (int e = 0; e < E; ++e) v[e] = v[e] * r * wc[e];
           }
         },
-        [&](int j, int c, const float (&v)[E]) { u.x.r[j] = Chunk<T>::pack(v); });
+        [&](int j, int c, const float (&v)[E]) {
+          if constexpr (FP8) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y8[j][e] = v[e];
+          } else {
+            u.x.r[j] = Chunk<T>::pack(v);
+          }
+        });
+    if constexpr (FP8) {
+      if (si == 1) {
+        store_e4m3<P, K, E>(p, y8, l, u.put, u.pb, u.ps);
+        return;
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j) u.x.r[j] = Chunk<T>::pack(y8[j]);
+    }
     // (every value of the row has been read: y may be x)
     if (u.put) u.x.store(p, u.py, l);
   };
@@ -668,7 +783,7 @@ __device__ __forceinline__ bool turn_of(const RopeParams& p, int d, int& pd, int
 
 // (rows from unit `first` on; a loop over them in the kernel held 135 registers
 // and scratch for 88)
-template <typename T>
+template <typename T, bool FP8>
 __global__ __launch_bounds__(256) void rope_fwd_scalar_kernel(RopeParams p, int64_t first) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -678,6 +793,55 @@ __global__ __launch_bounds__(256) void rope_fwd_scalar_kernel(RopeParams p, int6
   const int b = (int)(tok / p.S), s = (int)(tok % p.S);
   int si = 0;
   while (si < 2 && h >= p.side[si].groups) h -= p.side[si++].groups;
+  if constexpr (FP8) {
+    if (si >= 1) {  // one k or v head to 8-bit pools
+      const bool isv = si == 2;
+      const RopeSide& sd = p.side[1];
+      int pg, in;
+      if (!cache_place(p, b, s, pg, in)) return;
+      const T* x = reinterpret_cast<const T*>(isv ? p.v : sd.x) +
+                   (isv ? b * p.v_sb + s * p.v_ss + h * p.v_sh : b * sd.x_sb + s * sd.x_ss + h * sd.x_sh);
+      uint8_t* y = reinterpret_cast<uint8_t*>(isv ? p.v_out : sd.y) +
+                   (isv ? pg * p.vo_sb + in * p.vo_ss + h * p.vo_sh : pg * sd.y_sb + in * sd.y_ss + h * sd.y_sh);
+      uint8_t* ys = isv ? p.vs + (pg * p.vs_sb + in * p.vs_ss + h * p.vs_sh) : p.ks + (pg * p.ks_sb + in * p.ks_ss + h * p.ks_sh);
+      const int D = isv ? p.Dv : p.D, n = isv ? 0 : sd.n;
+      const double pos = (double)load_int(p.pos, b * p.pos_sb + s * p.pos_ss, p.pos_i64);
+      float v[kScalarSteps], q = 0.f, a = 0.f;
+#pragma unroll
+      for (int k = 0; k < kScalarSteps; ++k) {
+        const int d = lane + 64 * k;
+        v[k] = d < D ? to_f32(x[d]) : 0.f;
+        if (d < n) q = fmaf(v[k], v[k], q);
+      }
+      const float r = n > 0 ? 1.f / sqrtf(wave_sum(q) / (float)n + p.eps) : 1.f;
+#pragma unroll
+      for (int k = 0; k < kScalarSteps; ++k) {
+        const int d = lane + 64 * k;
+        if (d >= D) continue;
+        if (d < n) v[k] = v[k] * r * load_w<T>(p, sd.w, d);
+        int pd, i;
+        float sgn;
+        if (!isv && turn_of(p, d, pd, i, sgn)) {
+          float uo = to_f32(x[pd]), c, sn;
+          if (pd < n) uo = uo * r * load_w<T>(p, sd.w, pd);
+          angle(pos, p.freq[i], c, sn);
+          v[k] = v[k] * (c * p.rope_scale) + sgn * (uo * (sn * p.rope_scale));
+        }
+        a = fmaxf(a, finite_mag(v[k]));
+      }
+      const int se = scale_byte(wave_max(a));
+      const float inv = inverse_scale(se);
+      if (lane == 0) *ys = (uint8_t)se;
+#pragma unroll
+      for (int k = 0; k < kScalarSteps; ++k) {
+        const int d = lane + 64 * k;
+        if (d >= D) continue;
+        const float one[4] = {v[k], 0.f, 0.f, 0.f};
+        y[d] = (uint8_t)e4m3x4(one, inv);
+      }
+      return;
+    }
+  }
   if (si == 2) {  // one v head
     const int64_t row = cache_row(p, b, s, p.vo_sb, p.vo_ss);
     const T* x = reinterpret_cast<const T*>(p.v) + b * p.v_sb + s * p.v_ss + h * p.v_sh;
@@ -828,6 +992,13 @@ struct Fwd {
   void run() const {
     constexpr int NB = K == 1 ? 3 : K == 2 ? 2 : 1;
     const unsigned grid = (unsigned)rope_wgs(p.units);
+    if (p.ks != nullptr) {
+      // (two units of one or two chunks in flight: with their bytes' addresses three spill)
+      constexpr int NQ = K <= 2 ? 2 : 1;
+      if (NQ > 1 && p.units > kWaves) rope_fwd_kernel<T, P, K, IN, NQ, true><<<grid, 256, 0, s>>>(p);
+      else rope_fwd_kernel<T, P, K, IN, 1, true><<<grid, 256, 0, s>>>(p);
+      return;
+    }
     if (NB > 1 && p.units > kWaves) rope_fwd_kernel<T, P, K, IN, NB><<<grid, 256, 0, s>>>(p);
     else rope_fwd_kernel<T, P, K, IN, 1><<<grid, 256, 0, s>>>(p);
   }
@@ -860,7 +1031,9 @@ void fwd(const RopeParams& p, bool vec, hipStream_t s) {
   constexpr int64_t kMost = (int64_t)1 << 23;  // workgroups: a launch has fewer than 2^32 threads
   for (int64_t first = 0; first < p.units; first += 4 * kMost) {
     const int64_t wgs = (p.units - first + 3) / 4;
-    rope_fwd_scalar_kernel<T><<<(unsigned)(wgs < kMost ? wgs : kMost), 256, 0, s>>>(p, first);
+    const unsigned grid = (unsigned)(wgs < kMost ? wgs : kMost);
+    if (p.ks != nullptr) rope_fwd_scalar_kernel<T, true><<<grid, 256, 0, s>>>(p, first);
+    else rope_fwd_scalar_kernel<T, false><<<grid, 256, 0, s>>>(p, first);
   }
 }
 
@@ -898,7 +1071,7 @@ void rope_geometry(RopeParams& p, int esize, bool vec) {
   const int rpw = vec ? 64 / p.P : 1;
   for (int a = 0; a < 2; ++a) p.side[a].groups = (p.side[a].H + rpw - 1) / rpw;
   int vg = 0;
-  if (p.v != nullptr) vg = vec ? (p.side[1].H * (p.Dv / E) + 63) / 64 : p.side[1].H;
+  if (p.v != nullptr) vg = !vec ? p.side[1].H : p.vs != nullptr ? p.side[1].groups : (p.side[1].H * (p.Dv / E) + 63) / 64;
   p.groups = p.side[0].groups + p.side[1].groups + vg;
   p.units = (int64_t)p.B * p.S * p.groups;
   // blocks of up to 8 groups (a token's angles serve them) once there are 4096 waves of them

@@ -29,7 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import DTYPES, call, check_pool, int_rows, kv_pages, need_gpu, rows, table, written
+from ._host import DTYPES, call, check_pool, check_scales, int_rows, kv_pages, need_gpu, rows, strides4, table, written
 
 __all__ = ["rope_frequencies", "rotary_embedding", "qk_norm_rope", "qk_norm_rope_append"]
 
@@ -251,7 +251,8 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
                         v_cache: Optional[torch.Tensor], block_table: torch.Tensor, slots: torch.Tensor,
                         positions: torch.Tensor, inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                         k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, rope_offset: int = 0,
-                        interleaved: bool = False, rope_scale: float = 1.0, out: Optional[torch.Tensor] = None):
+                        interleaved: bool = False, rope_scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                        k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None):
     """:func:`qk_norm_rope` for serving: returns the turned q (into ``out``, which
     may be ``q``; None without q), writes each token's k row to row
     ``slots[b, s]`` of sequence ``b`` in ``k_cache`` ``[num_pages, page_size, Hkv,
@@ -262,7 +263,13 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
     ``positions`` (drafted tokens of one depth share a position, not a row).
     A slot outside the table (e.g. -1: a padded token) or on an unmapped page is
     not written.  Slots of one call must differ; of two tokens with the same
-    cache row, either's values may be left there.  No gradient."""
+    cache row, either's values may be left there.  No gradient.
+
+    ``float8_e4m3fn`` pools take the rows quantised, each head's row on its own: its
+    exponent ``e`` goes to ``k_scales`` / ``v_scales`` (uint8 or float8_e8m0fnu
+    ``[num_pages, page_size, Hkv]``) and the row stands for its bytes' values times
+    ``2^(e - 127)``, the smallest power of two, down to ``2^-111``, that leaves the
+    row's largest finite magnitude at 448 or less; infinities become NaN."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight)):
         raise ValueError("appending to a cache records no gradient: call it under torch.no_grad()")
     _check_rows("k", k)
@@ -276,18 +283,27 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
             raise ValueError(f"q and k must have one head dim, got {q.shape[3]} and {D}")
     check_pool("k_cache", k_cache, dev)
     num_pages, page_size = k_cache.shape[:2]
-    if tuple(k_cache.shape[2:]) != (Hkv, D) or k_cache.dtype != k.dtype or k_cache.stride(3) != 1:
-        raise ValueError(f"k_cache must be a [num_pages, page_size, {Hkv}, {D}] {k.dtype} pool with a unit feature stride")
+    fp8 = k_cache.dtype == torch.float8_e4m3fn
+    pool_type = torch.float8_e4m3fn if fp8 else k.dtype
+    if tuple(k_cache.shape[2:]) != (Hkv, D) or k_cache.dtype != pool_type or k_cache.stride(3) != 1:
+        raise ValueError(f"k_cache must be a [num_pages, page_size, {Hkv}, {D}] {k.dtype} or float8_e4m3fn pool with a unit "
+                         "feature stride")
     if (v is None) != (v_cache is None):
         raise ValueError("v and v_cache go together")
     if v is not None:
         _check_rows("v", v, k)
         check_pool("v_cache", v_cache, dev)
         if v.shape[2] != Hkv or tuple(v_cache.shape) != (num_pages, page_size, Hkv, v.shape[3]) \
-                or v_cache.dtype != v.dtype or v_cache.stride(3) != 1:
-            raise ValueError(f"v_cache must be a [{num_pages}, {page_size}, {Hkv}, {v.shape[3]}] {k.dtype} pool with a "
+                or v_cache.dtype != pool_type or v_cache.stride(3) != 1:
+            raise ValueError(f"v_cache must be a [{num_pages}, {page_size}, {Hkv}, {v.shape[3]}] {pool_type} pool with a "
                              "unit feature stride, v [B, S, Hkv, Dv]")
         v = rows(v)
+    if fp8:
+        check_scales("k_scales", k_scales, k_cache, dev)
+        if v is not None:
+            check_scales("v_scales", v_scales, v_cache, dev)
+    if (k_scales is not None and not fp8) or (v_scales is not None and (v is None or not fp8)):
+        raise ValueError("scales are those of float8_e4m3fn pools")
     c = _Call(k, positions, inv_freq, q_weight if q is not None else None, k_weight, eps, rope_offset, interleaved,
               rope_scale)
     bt = table(block_table, B, dev)
@@ -298,10 +314,14 @@ def qk_norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: Optional[
     if q is not None:
         q = rows(q)
         out = _like(q) if out is None else out
-    written(out, k_cache, v_cache)
+    written(out, k_cache, v_cache, k_scales, v_scales)
     if k.numel() > 0:
         k = rows(k)
         a = c.args(q, k, out, k_cache, v, v_cache, slots)
         pg = kv_pages(bt, B, num_pages, page_size, dev)
-        call(dev, _lib.load().sfa_rope_fwd, ctypes.byref(a), ctypes.byref(pg))
+        if fp8:
+            sc = _lib.KvScales(*strides4(k_scales), *strides4(v_scales))
+            call(dev, _lib.load().sfa_rope_append_fp8, ctypes.byref(a), ctypes.byref(pg), ctypes.byref(sc))
+        else:
+            call(dev, _lib.load().sfa_rope_fwd, ctypes.byref(a), ctypes.byref(pg))
     return out
