@@ -135,11 +135,11 @@ __global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
   if (threadIdx.x == 0) p.dsink[h] = -s_x[0];
 }
 
-enum { kAny = 0 };
+enum { kAny = 0, kWide };
 struct KernelShape {
   int rows, tile_shift, threads;
 };
-constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256}};
+constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256}, {kWideRows, 6, 512}};
 
 void set_launch(DenseParams& p, const DensePlan& pl) {
   p.rows = pl.rows;
@@ -155,6 +155,8 @@ void set_launch(DenseParams& p, const DensePlan& pl) {
 DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   DensePlan pl{};
   pl.kernel = kAny;
+  const int64_t R = (int64_t)p.S * p.G;
+  if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) && R > 64) pl.kernel = kWide;
   const KernelShape& k = kShapes[pl.kernel];
   pl.rows = k.rows;
   pl.tile_shift = k.tile_shift;
@@ -182,7 +184,8 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
 hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s) {
   DenseParams p = p0;
   set_launch(p, pl);
-  launch_dense_any(p, dtype, kv_dtype, s);
+  if (pl.kernel == kWide) launch_dense_wide(p, kv_dtype, s);
+  else launch_dense_any(p, dtype, kv_dtype, s);
   if (pl.want > 0) {
     if (dtype == SFA_DTYPE_F32) combine<float>(p, s);
     else combine<bf16>(p, s);

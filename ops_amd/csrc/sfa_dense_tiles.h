@@ -1,0 +1,270 @@
+// Key tiles of the bf16 dense attention kernels in LDS: 64 rows of K and of V, from
+// contiguous tensors, pages, or pages of e4m3 rows.
+#pragma once
+
+#include "sfa_dense.h"
+
+namespace sfa {
+
+constexpr int kWideKeys = 64;
+
+// A tile is written 1024 bytes (4 rows of 128 dims, 8 of 64) at a time, with 16 bytes
+// between, and chunk c (16 bytes) of row r goes to place c ^ at(r) of its row.  So
+// lanes that read one chunk of 16 consecutive rows (K) meet all 16 bank groups, as
+// do those that read four consecutive rows of an aligned group of four chunks (V,
+// transposed), and rows 8 further lie at a constant distance.
+template <int D>
+struct Tile {
+  static constexpr int CH = D / 8, RPI = 64 / CH, GROUP = 65;  // chunks a row, rows a group, chunks from group to group
+  static constexpr int SLOTS = kWideKeys / RPI * GROUP;
+  static __device__ __forceinline__ int at(int r) {
+    if constexpr (D == 128) return (r & 3) << 2;
+    else return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
+  }
+  static constexpr int rows(int n) { return n / RPI * GROUP * 16; }  // bytes to a row n further, n a multiple of 8
+  static __device__ __forceinline__ int slot(int r, int c) { return r / RPI * GROUP + r % RPI * CH + (c ^ at(r)); }
+};
+
+// Lane l: 16 bytes from base + its offset to dst + 16 l; not seen by the compiler:
+// the kernel waits for vmcnt itself.
+__device__ __forceinline__ void dense_dma16(const void* lds, uint64_t base, uint32_t off) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(d), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dense_dma16(const void* lds, uint64_t addr) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(d), "v"(addr) : "memory", "m0");
+}
+__device__ __forceinline__ void dense_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Reads at an LDS address and a constant.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(p); }
+__device__ __forceinline__ bf16x8 lds_b128_at(uint32_t a) {
+  return *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)a;
+}
+__device__ __forceinline__ bf16x4 lds_tr16_at(uint32_t a) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)a);
+}
+
+enum { kSrcTile, kSrcRows, kSrcFp8 };
+// kSrcTile: a tile's rows have one base and stride (contiguous tensors, pages of 64
+// rows or more) and 32-bit offsets.
+inline int dense_tile_source(const DenseParams& p) {
+  const int64_t row = 2 * (p.k_ss > p.v_ss ? p.k_ss : p.v_ss);
+  const bool one = p.block_table == nullptr || p.page_shift >= 6;
+  return one && p.k_ss >= 0 && p.v_ss >= 0 && row < (int64_t)1 << 25 ? kSrcTile : kSrcRows;
+}
+
+__device__ __forceinline__ int dense_load_const(const int32_t* at) {
+  return *(const __attribute__((address_space(4))) int32_t*)at;
+}
+
+// Tiles of 64 keys for NW waves.  ids(i, j0): the page ids of the tile at key j0 are
+// fetched; load(j0, ..): that tile's rows are, to LDS (or, e4m3, to registers, and
+// from there by store()); returns the rows that are there.  on = false: zeros, so
+// that the number of loads in flight does not depend on the range.
+template <int D, int NW, int SRC>
+struct TileSource {
+  static constexpr int KT = kWideKeys, CH = D / 8, RPI = 64 / CH, NI = KT / RPI / NW;
+  static_assert(NI >= 1 && KT / 8 == NW, "whole load instructions and eight rows a wave");
+  uint64_t kbase, vbase;
+  int64_t kpage, vpage, krow, vrow;
+  const int32_t* trow;
+  int cap, page_shift, num_pages, wave, lane;
+  int pg, pgr;                  // page ids: of the tile, or of key j0 + lane; of the wave's row lane / 8
+
+  __device__ __forceinline__ TileSource(const DenseParams& p, int b, int g, int wave_, int lane_)
+      : cap(p.cap), page_shift(p.page_shift), num_pages(p.num_pages), wave(wave_), lane(lane_) {
+    const int64_t e = SRC == kSrcFp8 ? 1 : 2;
+    kbase = (uint64_t)(uintptr_t)p.k + (uint64_t)(e * g * p.k_sh);
+    vbase = (uint64_t)(uintptr_t)p.v + (uint64_t)(e * g * p.v_sh);
+    kpage = e * p.k_sb;
+    vpage = e * p.v_sb;
+    krow = e * p.k_ss;
+    vrow = e * p.v_ss;
+    trow = nullptr;
+    if (p.block_table != nullptr) {
+      trow = p.block_table + b * p.bt_sb;
+    } else {  // one page of all rows
+      kbase += (uint64_t)(b * kpage);
+      vbase += (uint64_t)(b * vpage);
+      page_shift = 30;
+      num_pages = 1;
+    }
+    if constexpr (SRC == kSrcFp8) {
+      ksc = p.ks + g * p.ks_sh;
+      vsc = p.vs + g * p.vs_sh;
+      ks_sb = p.ks_sb; ks_ss = p.ks_ss; vs_sb = p.vs_sb; vs_ss = p.vs_ss;
+    }
+  }
+  __device__ __forceinline__ int entry(int j) const { return trow == nullptr ? 0 : trow[min(j, cap - 1) >> page_shift]; }
+  __device__ __forceinline__ void ids(int j0) {
+    if constexpr (SRC == kSrcTile) {
+      pg = trow == nullptr ? 0 : dense_load_const(trow + (j0 >> page_shift));
+    } else {
+      pg = entry(j0 + lane);
+      if constexpr (SRC == kSrcFp8) pgr = entry(j0 + wave * 8 + (lane >> 3));
+    }
+  }
+  // at most n tiles of this wave in flight
+  template <int N>
+  __device__ __forceinline__ void wait() const {
+    if constexpr (SRC != kSrcFp8) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N * 2 * NI) : "memory");
+  }
+
+  __device__ __forceinline__ uint64_t load(int j0, bool on, u32x4* kt, u32x4* vt) {
+    const int in_page = (1 << page_shift) - 1;
+    if constexpr (SRC == kSrcTile) {
+      const int in = j0 & in_page, n = cap - j0, pgu = __builtin_amdgcn_readfirstlane(pg);
+      const bool ok = on && pgu >= 0 && pgu < num_pages;
+      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+      const uint64_t kb = ok ? kbase + (uint64_t)(pgu * kpage + in * krow) : zero;
+      const uint64_t vb = ok ? vbase + (uint64_t)(pgu * vpage + in * vrow) : zero;
+      // (lane constants are formed per tile: held across the loop they spill)
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      const int sub = ln / CH;
+      const uint32_t c = 16u * (uint32_t)((ln % CH) ^ Tile<D>::at(sub));
+      const uint32_t ko = (uint32_t)(sub * (int)krow) + c, vo = (uint32_t)(sub * (int)vrow) + c;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int q = wave * NI + i, left = ok ? n - q * RPI : 0;
+        // (rows past the last one read some row's chunks: no row of the result sees them)
+        const bool there = sub < left;
+        const uint64_t step = left > 0 ? (uint64_t)(q * RPI) : 0;
+        dense_dma16(kt + q * Tile<D>::GROUP, kb + step * (uint64_t)krow, there ? ko : c);
+        dense_dma16(vt + q * Tile<D>::GROUP, vb + step * (uint64_t)vrow, there ? vo : c);
+      }
+      return !ok ? 0 : n >= KT ? ~0ull : (1ull << n) - 1;
+    } else if constexpr (SRC == kSrcRows) {
+      const int j = j0 + lane;
+      const bool ok = on && j < cap && pg >= 0 && pg < num_pages;
+      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+      const uint64_t ka = ok ? kbase + (uint64_t)(pg * kpage + (j & in_page) * krow) : zero;
+      const uint64_t va = ok ? vbase + (uint64_t)(pg * vpage + (j & in_page) * vrow) : zero;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int q = wave * NI + i, row = q * RPI + lane / CH;
+        const uint64_t c = (uint64_t)(16 * ((lane % CH) ^ Tile<D>::at(row)));
+        dense_dma16(kt + q * Tile<D>::GROUP, from(ka, row) + c);
+        dense_dma16(vt + q * Tile<D>::GROUP, from(va, row) + c);
+      }
+      return __ballot(ok);
+    } else {
+      const int j = j0 + lane, jr = j0 + wave * 8 + (lane >> 3);
+      const bool ok = on && j < cap && pg >= 0 && pg < num_pages, okr = on && jr < cap && pgr >= 0 && pgr < num_pages;
+      const int in = jr & in_page;
+      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+      const uint64_t piece = (uint64_t)((lane & 7) * (D / 8));
+      kraw = *reinterpret_cast<const raw_t*>((okr ? kbase + (uint64_t)(pgr * kpage + in * krow) : zero) + piece);
+      vraw = *reinterpret_cast<const raw_t*>((okr ? vbase + (uint64_t)(pgr * vpage + in * vrow) : zero) + piece);
+      kexp = okr ? ksc[pgr * ks_sb + in * ks_ss] : 127;
+      vexp = okr ? vsc[pgr * vs_sb + in * vs_ss] : 127;
+      return __ballot(ok);
+    }
+  }
+  __device__ __forceinline__ void store(u32x4* kt, u32x4* vt) const {
+    if constexpr (SRC == kSrcFp8) {
+      const int row = wave * 8 + (lane >> 3), c0 = (lane & 7) * (D / 64);
+      const float sk = scale_of((uint8_t)kexp), sv = scale_of((uint8_t)vexp);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        kt[Tile<D>::slot(row, c0 + i)] = chunk(kraw, i, sk);
+        vt[Tile<D>::slot(row, c0 + i)] = chunk(vraw, i, sv);
+      }
+    }
+  }
+
+  // dims d .. d + 3 of the V row of key j, which is there
+  __device__ __forceinline__ void value4(int j, int d, float (&v)[4]) const {
+    const int id = entry(j), in = j & ((1 << page_shift) - 1);
+    const uint64_t a = vbase + (uint64_t)(id * vpage + in * vrow);
+    if constexpr (SRC == kSrcFp8) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(a + d);
+      const float s = scale_of(vsc[id * vs_sb + in * vs_ss]);
+      v[0] = __builtin_amdgcn_cvt_f32_fp8((int)x, 0) * s;
+      v[1] = __builtin_amdgcn_cvt_f32_fp8((int)x, 1) * s;
+      v[2] = __builtin_amdgcn_cvt_f32_fp8((int)x, 2) * s;
+      v[3] = __builtin_amdgcn_cvt_f32_fp8((int)x, 3) * s;
+    } else {
+      const bf16x4 x = *reinterpret_cast<const bf16x4*>(a + 2 * d);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = (float)x[q];
+    }
+  }
+
+ private:
+  typedef typename std::conditional<D == 128, u32x4, u32x2>::type raw_t;
+  const uint8_t *ksc, *vsc;
+  int64_t ks_sb, ks_ss, vs_sb, vs_ss;
+  raw_t kraw, vraw;
+  int kexp, vexp;
+  static __device__ __forceinline__ uint64_t from(uint64_t a, int lane) {
+    return ((uint64_t)(uint32_t)__shfl((int)(a >> 32), lane, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)a, lane, 64);
+  }
+  // bytes 8 i .. 8 i + 7 as bf16 times a power of two (exact)
+  static __device__ __forceinline__ u32x4 chunk(const raw_t& x, int i, float s) {
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      r[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * i + w], s, false));
+      r[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * i + w], s, true));
+    }
+    return r;
+  }
+};
+
+// Infinities and NaN of a V tile whose rows not every query row sees: noted as bits
+// (of s_bad, 0 before) and cleared in LDS, as 0 times them would reach the rows that
+// do not see them; add_bad adds them to those that do.
+__device__ __forceinline__ uint32_t bad16(uint32_t w) {  // halves of w that are no numbers: their masks
+  return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+template <int D, int NW>
+__device__ __forceinline__ uint64_t clear_bad(u32x4* vt, unsigned long long* s_bad, int wave, int lane) {
+  constexpr int CH = D / 8, PER = kWideKeys * CH / 64 / NW;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int q = wave * PER + i, at = q * Tile<D>::GROUP + lane;
+    const u32x4 w = vt[at];
+    u32x4 m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = bad16(w[e]);
+    if ((m[0] | m[1] | m[2] | m[3]) != 0) {
+      vt[at] = w & ~m;
+      atomicOr(s_bad, 1ull << (q * Tile<D>::RPI + lane / CH));
+    }
+  }
+  dense_barrier();
+  return *s_bad;
+}
+
+// Where the workgroup's share of a launch is: the row blocks of a (sequence, kv head)
+// on one XCD (workgroup i is on XCD i % 8), whose L2 their keys then stay in; the
+// longest ones, which are a sequence's last, first.
+__device__ __forceinline__ bool dense_place(const DenseParams& p, int& slot, int& g) {
+  int w = blockIdx.x;
+  if (p.want > 0) {
+    g = w % p.Hkv;
+    slot = w / p.Hkv;
+    return true;
+  }
+  const int groups = p.B * p.Hkv, x = w & 7;
+  int group, rb;
+  if (groups % 8 == 0) {
+    w >>= 3;
+    group = x + 8 * (w / p.nrb);
+    rb = w % p.nrb;
+  } else if (8 % groups == 0 && p.nrb % (8 / groups) == 0) {  // 1, 2 or 4: each on several
+    group = x % groups;
+    rb = (w >> 3) * (8 / groups) + x / groups;
+  } else {
+    group = w % groups;
+    rb = w / groups;
+  }
+  g = group % p.Hkv;
+  slot = group / p.Hkv * p.nrb + (p.nrb - 1 - rb);
+  return true;
+}
+
+}  // namespace sfa

@@ -1,0 +1,281 @@
+// gfx950 dense attention through a window (sfa_dense.h), head dims 64 and 128 in
+// bf16, many query rows: a chunk of a prompt, a training step's forward.
+//
+// Eight waves of 32 query rows share tiles of 64 keys in LDS.  S^T = K Q^T (32 keys x
+// 32 rows a product, 32x32x16, Q in registers) leaves a lane with 16 keys of
+// its row; in bf16 they are the second operand of O^T = V^T P^T as they are, whose
+// first is read from LDS transposed.  A step makes the scores of tile j + 1 beside
+// the softmax of tile j, then the sums of tile j.  The running maximum moves only
+// when a score passes it by 8 (base 2; 2^8 more at most in a float32 sum), so a tile
+// needs no maximum across lanes.  P is rounded to bf16 once for its product (2^-8 of
+// a weight, as much as the result's own rounding); sums and statistics are float32.
+
+#include "sfa_dense_tiles.h"
+
+namespace sfa {
+namespace {
+
+template <int D, int SRC>
+__global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
+  typedef Mfma<32> M;
+  typedef f32x16 acc_t;
+  constexpr int NW = 8, KT = kWideKeys, KS = D / 16, OT = D / 32, NS = 4;
+  __shared__ u32x4 s_kv[NS][2][Tile<D>::SLOTS];
+  __shared__ unsigned long long s_bad[2];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, hq = lane >> 5;
+
+  int slot, g;
+  if (!dense_place(p, slot, g)) return;
+  DenseItem it;
+  if (!dense_item(p, slot, g, it)) return;
+  const int b = it.b, row = 32 * wave + lr, r = it.row0 + row;
+  const int t = r / p.G, h = g * p.G + r % p.G;
+  const bool in = r < p.S * p.G, live = in && t < it.s.n;
+  const int pos = live ? it.s.ctx + t : -1;
+  // what all rows of the block see of a tile without a look at each
+  const int p0 = it.s.ctx + it.row0 / p.G, p1 = it.s.ctx + min((it.row0 + p.rows - 1) / p.G, it.s.n - 1);
+
+  bf16x8 qb[KS];
+  {
+    const bf16* q = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(q + 16 * s);
+      qb[s] = live ? x : bf16x8{};
+    }
+  }
+
+  TileSource<D, NW, SRC> src(p, b, g, wave, lane);
+  const int n = it.v1 - it.v0;
+  // first key of the i-th tile (past the range: the last one's, whose rows are not read again)
+  auto tile_at = [&](int i) { return it.tiles.tile(it.v0 + max(min(i, n - 1), 0)) * KT; };
+
+  acc_t oacc[OT];
+#pragma unroll
+  for (int o = 0; o < OT; ++o) oacc[o] = acc_t{};
+  float m_used = kNegInf, l_part = 0.f;
+  const float inv_scale = 1.f / p.scale_log2;
+
+  // Operand addresses.  K: row lr, chunk 2 s + hq; V: rows 4 hq + (lane % 16) / 4, 16 dims
+  // by lane / 16 % 2.  The places of a row's chunks differ by rows in bits 2 and 3 (D = 64: 1
+  // and 2) of the chunk's number, which a step flips in its copy of the address.
+  typedef Tile<D> L;
+  constexpr int FLIP = D == 128 ? 6 : 5;  // the first of those bits, in bytes
+  const int l16 = lane & 15, vrow = 4 * hq + (l16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+  const uint32_t kx = 16u * (uint32_t)L::at(lr), k0a = 16u * (uint32_t)(L::slot(lr, L::at(lr)) + hq);
+  const uint32_t vx = 16u * (uint32_t)(L::at(vrow) ^ vc) , v0a = 16u * (uint32_t)L::slot(vrow, L::at(vrow)) + (uint32_t)(l16 & 1) * 8u;
+
+  uint64_t mask[NS + 1];  // rows that are there, of tiles j, j + 1, ..
+  src.ids(tile_at(0));
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    mask[i] = src.load(tile_at(i), i < n, s_kv[i][0], s_kv[i][1]);
+    src.ids(tile_at(i + 1));
+    src.store(s_kv[i][0], s_kv[i][1]);
+  }
+  if (tid < 2) s_bad[tid] = 0;
+  src.template wait<0>();
+  dense_barrier();
+
+  // A step's products: NQ of the next tile's scores, 32 keys at a time, then the
+  // sums' by 16 keys; each takes one operand from LDS, read four products ahead.
+  constexpr int NQ = 2 * KS, NM = NQ + 4 * OT;
+  bf16x8 op[4];
+  // (a, x: the address of place 0 of the lane's row, the flips; i: the product)
+  auto read_k = [&](uint32_t a, uint32_t x, int i) {
+    const int c = i % KS, kb = i / KS;
+    return lds_b128_at(a + (x ^ ((uint32_t)(D == 128 ? c >> 1 : c) << FLIP)) + (uint32_t)((D == 128 ? 32 * (c & 1) : 0) + L::rows(32 * kb)));
+  };
+  auto read_v = [&](uint32_t a, uint32_t x, int i) {
+    const uint32_t at = a + (x ^ (uint32_t)(64 * (i % OT)));
+    const bf16x4 lo = lds_tr16_at(at + (uint32_t)L::rows(16 * (i / OT))), hi = lds_tr16_at(at + (uint32_t)L::rows(16 * (i / OT) + 8));
+    return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto max_of = [&](const acc_t (&c)[2]) {
+    float x = max3_raw(c[0][0], c[0][1], c[0][2]), y = max3_raw(c[1][0], c[1][1], c[1][2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) {
+      x = max3_raw(x, c[0][e], c[0][e + 1]);
+      y = max3_raw(y, c[1][e], c[1][e + 1]);
+    }
+    return max3_raw(max_raw(x, c[0][15]), y, c[1][15]);
+  };
+  acc_t sa[2], sb[2];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    sa[kb] = acc_t{};
+#pragma unroll
+    for (int c = 0; c < KS; ++c) sa[kb] = M::mma(read_k(lds_addr(s_kv[0][0]) + k0a, kx, kb * KS + c), qb[c], sa[kb]);
+  }
+  M::drain_v1(sa[0]);  // (max_of reads them in inline asm: a step's come many products later)
+  M::drain_v1(sa[1]);
+  float tmax = max_of(sa);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) op[i] = read_k(lds_addr(s_kv[1][0]) + k0a, kx, i);
+
+  // (a lane's key e of block kb is 32 kb + 8 (e / 4) + 4 hq + e % 4)
+  auto add_bad = [&](uint64_t bad, int j0, const bf16x8 (&pb)[4]) {
+    for (; bad != 0; bad &= bad - 1) {
+      const int key = __builtin_ctzll(bad), e = 4 * ((key & 31) >> 3) + (key & 3);
+      uint32_t word = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4 x = __builtin_bit_cast(u32x4, pb[k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word = 8 * k + 2 * i == ((key >> 5) * 16 + e) - (e & 1) ? x[i] : word;
+      }
+      const float own = __uint_as_float(e & 1 ? word & 0xffff0000u : word << 16);
+      const float w = __shfl(own, lr + 32 * ((key >> 2) & 1), 64);
+#pragma unroll
+      for (int o = 0; o < OT; ++o)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[4];
+          src.value4(j0 + key, 32 * o + 8 * i + 4 * hq, v);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (w != 0.f && !(fabsf(v[q]) <= 3.402823466e38f)) oacc[o][4 * i + q] += w * v[q];
+        }
+    }
+  };
+  int st = 0, nbad = 0;
+  auto step = [&](int j, acc_t (&cur)[2], acc_t (&nxt)[2]) {
+    const int j0 = tile_at(j);
+    const int st1 = (st + 1) & (NS - 1), st2 = (st + 2) & (NS - 1);
+    // (opaque: the flipped addresses are formed at their reads, not held)
+    uint32_t kf = kx, vf = vx;
+    asm volatile("" : "+v"(kf), "+v"(vf));
+    const uint32_t kn = lds_addr(s_kv[st1][0]) + k0a, kn2 = lds_addr(s_kv[st2][0]) + k0a, vt = lds_addr(s_kv[st][1]) + v0a;
+    const bool whole = mask[0] == ~0ull && j0 + KT - 1 <= p0 && (j0 + KT <= p.first || p1 - j0 < p.window);
+    uint64_t bad = 0;
+    if (!whole) {
+      // (two words in turn: the other one's readers have passed a step's barrier)
+      bad = clear_bad<D, NW>(s_kv[st][1], &s_bad[nbad & 1], wave, lane);
+      ++nbad;
+      if (tid == 0) s_bad[nbad & 1] = 0;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const uint32_t there = (uint32_t)(mask[0] >> (32 * kb));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = 8 * (e >> 2) + 4 * hq + (e & 3);
+          const bool ok = ((there >> key) & 1) && dense_seen(p, j0 + 32 * kb + key, pos);
+          cur[kb][e] = ok ? cur[kb][e] : kNegInf;
+        }
+      }
+      tmax = max_of(cur);
+    }
+    if (__any(tmax * p.scale_log2 > m_used + 8.f)) {
+      const float mn = fmaxf(m_used, xor32_max(tmax * p.scale_log2));
+      const float alpha = mn == kNegInf ? 1.f : exp2f(m_used - mn);
+      l_part *= alpha;
+#pragma unroll
+      for (int o = 0; o < OT; ++o) oacc[o] *= alpha;
+      m_used = mn;
+    }
+    const float moff = m_used == kNegInf ? 0.f : -m_used;
+
+    bf16x8 pb[4];
+    float ex = 0.f;
+    each<NM>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (i < NQ) {
+        constexpr int kb = i / KS, c = i % KS;
+        nxt[kb] = M::mma(op[i & 3], qb[c], c == 0 ? acc_t{} : nxt[kb]);
+      } else {
+        constexpr int k = (i - NQ) / OT, o = (i - NQ) % OT;
+        oacc[o] = M::mma(op[i & 3], pb[k], oacc[o]);
+      }
+      if constexpr (i == NM - 4) {
+        // This tile's V and the next one's K are read: once tile j + 2 has landed (of those in
+        // flight the last but one that was asked for), tile j + 4 may take this one's place.
+        src.template wait<1>();
+        dense_barrier();
+      }
+      if constexpr (i + 4 < NQ) op[i & 3] = read_k(kn, kf, i + 4);
+      else if constexpr (i + 4 < NM) op[i & 3] = read_v(vt, vf, i + 4 - NQ);
+      else op[i & 3] = read_k(kn2, kf, i + 4 - NM);
+      // the weights, evenly before the last keys' sums
+      each<32>([&](auto ec) {
+        constexpr int e = decltype(ec)::value, kb = e >> 4, ee = e & 15;
+        if constexpr (e * (NM - OT) / 32 == i) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(cur[kb][ee], p.scale_log2, moff));
+          l_part += x;
+          asm volatile("" : "+v"(l_part));  // (added here: all weights held for one sum at the end spill)
+          if constexpr (e & 1) {
+            pb[e >> 3][(e & 7) - 1] = (bf16)ex;
+            pb[e >> 3][e & 7] = (bf16)x;
+          }
+          ex = x;
+        }
+      });
+      if constexpr (i == NM - 2) {
+        mask[NS] = src.load(tile_at(j + 4), j + 4 < n, s_kv[st][0], s_kv[st][1]);
+        src.ids(tile_at(j + 5));
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    tmax = max_of(nxt);
+    if (bad != 0) add_bad(bad, j0, pb);
+    src.store(s_kv[st][0], s_kv[st][1]);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) mask[i] = mask[i + 1];
+    st = st1;
+  };
+  int j = 0;
+  for (; j + 1 < n; j += 2) {
+    step(j, sa, sb);
+    step(j + 1, sb, sa);
+  }
+  if (j < n) step(j, sa, sb);
+  src.template wait<0>();
+
+  // ---- results: lane holds row lr, dims 32 o + 8 i + 4 hq + 0 .. 3 --------------------
+  const float l = xor32_sum(l_part);
+  if (!in) return;
+  float lse, f;
+  if (it.partial) {
+    f = dense_part(m_used, l, lse);
+    if (hq == 0) p.part_lse[it.part + row] = lse;
+  } else {
+    f = dense_finish(p, h, live, m_used, l, lse);
+    if (hq == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+  }
+#pragma unroll
+  for (int o = 0; o < OT; ++o)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = f == 0.f ? 0.f : oacc[o][4 * i + e] * f;
+      const int d = 32 * o + 8 * i + 4 * hq;
+      if (it.partial) {
+        *reinterpret_cast<f32x4*>(p.part_o + (it.part + row) * D + d) = x;
+      } else {
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + d) =
+            bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+      }
+    }
+}
+
+template <int D>
+void launch(const DenseParams& p, int src, unsigned grid, hipStream_t s) {
+  if (src == kSrcTile) dense_wide_kernel<D, kSrcTile><<<grid, 512, 0, s>>>(p);
+  else if (src == kSrcRows) dense_wide_kernel<D, kSrcRows><<<grid, 512, 0, s>>>(p);
+  else dense_wide_kernel<D, kSrcFp8><<<grid, 512, 0, s>>>(p);
+}
+
+}  // namespace
+
+void launch_dense_wide(const DenseParams& p, int kv_dtype, hipStream_t s) {
+  const int src = kv_dtype == SFA_DTYPE_FP8_E4M3 ? kSrcFp8 : dense_tile_source(p);
+  const unsigned grid = (unsigned)((int64_t)p.slots * p.Hkv);
+  if (p.Dqk == 64) launch<64>(p, src, grid, s);
+  else launch<128>(p, src, grid, s);
+}
+
+}  // namespace sfa

@@ -181,6 +181,10 @@ constexpr int kAnyRows = 64, kAnyShift = 5, kAnyDims = 128;
 void launch_dense_any(const DenseParams& p, int dtype, int kv_dtype, hipStream_t s);
 void launch_dense_bwd_any(const DenseParams& p, int dtype, hipStream_t s);
 
+// bf16 queries, head dims 64 and 128, many rows (sfa_dense_wide.hip)
+constexpr int kWideRows = 256;
+void launch_dense_wide(const DenseParams& p, int kv_dtype, hipStream_t s);
+
 // ---- rows of a cache as contiguous ones (sfa_read.hip) ----
 struct ReadParams {
   const void* cache;
