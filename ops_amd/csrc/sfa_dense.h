@@ -75,8 +75,11 @@ __device__ __forceinline__ float scale_of(uint8_t e) {
 }
 
 // ---- key ranges of a launch ("slots") ---------------------------------------------
-// A unit is a (sequence, row block).  The units' tiles are cut into ranges of one
-// length, found on the device as the lengths are there; each unit has one at least.
+// A unit is a (sequence, row block).  p.fit workgroups of a kv head run at once.  With
+// want > 0 (few units) the units' tiles are cut into ranges of up to one length, found
+// on the device as the lengths are there: the shortest that gives p.fit ranges or
+// fewer, or, where that leaves less work on the longest path, `want`, twice as many.
+// (Each unit has one at least.)
 struct DenseSlot {
   int unit;       // or -1: none
   int v0, v1;     // its tiles, as KeyTiles counts them
@@ -104,13 +107,46 @@ __device__ __forceinline__ DenseSlot dense_slot(const DenseParams& p, int slot) 
   }
   const int lane = threadIdx.x & 63;
   auto tiles_of = [&](int u) { return u < units ? unit_tiles(p, u) : 0; };
-  const int mine = tiles_of(lane);  // (of the first 64 units)
-  int64_t sum = dense_lanes_sum(mine);
-  for (int u0 = 64; u0 < units; u0 += 64) sum += dense_lanes_sum(tiles_of(u0 + lane));
-  const int len = max(p.min_len, (int)((sum + p.want - 1) / p.want));
+  int tiles[kDenseUnits / 64], sum = 0, most = 0;
+#pragma unroll
+  for (int i = 0; i < kDenseUnits / 64; ++i) {
+    tiles[i] = 64 * i < units ? tiles_of(64 * i + lane) : 0;
+    sum += tiles[i];
+    most = max(most, tiles[i]);
+  }
+  sum = dense_lanes_sum(sum);
+  most = wave_max_int(most);
+  auto ranges = [&](int len) {  // of up to len tiles
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kDenseUnits / 64; ++i)
+      if (64 * i < units) n += 64 * i + lane < units ? max(1, (tiles[i] + len - 1) / len) : 0;
+    return dense_lanes_sum(n);
+  };
+  auto shortest = [&](int slots) {  // (a few steps come within a tile of the best)
+    int len = max(p.min_len, (sum + slots - 1) / slots);
+    for (int i = 0; i < 6 && len < most; ++i) {
+      const int n = ranges(len);
+      if (n <= slots) return len;
+      len = max(len + 1, (int)((int64_t)len * n / slots));
+    }
+    return max(len, most);
+  };
+  int len = most;
+  if (units <= p.fit) len = shortest(p.fit);
+  if (len > p.min_len) {
+    const int l2 = shortest(p.want);
+    // (rounds of p.fit ranges; joining them costs a tenth or so)
+    const int rounds = units <= p.fit ? 1 : (units + p.fit - 1) / p.fit, r2 = (p.want + p.fit - 1) / p.fit;
+    if (l2 < most && 11 * r2 * l2 < 10 * rounds * len) len = l2;
+  }
+  len = max(len, 1);
   int before = 0;
   for (int u0 = 0; u0 < units; u0 += 64) {
-    const int u = u0 + lane, t = u0 == 0 ? mine : tiles_of(u);
+    const int u = u0 + lane;
+    int t = tiles[0];
+#pragma unroll
+    for (int i = 1; i < kDenseUnits / 64; ++i) t = u0 == 64 * i ? tiles[i] : t;
     const int n = u < units ? max(1, (t + len - 1) / len) : 0;
     int incl = n;
 #pragma unroll
@@ -126,11 +162,11 @@ __device__ __forceinline__ DenseSlot dense_slot(const DenseParams& p, int slot) 
       s.unit = u0 + w;
       s.first = __builtin_amdgcn_readlane(first, w);
       s.n = __builtin_amdgcn_readlane(n, w);
-      const int tiles = __builtin_amdgcn_readlane(t, w);
+      const int mine = __builtin_amdgcn_readlane(t, w);
       // (even ranges: the unit's tiles over its own number of slots)
       const int i = slot - s.first;
-      s.v0 = (int)((int64_t)tiles * i / s.n);
-      s.v1 = (int)((int64_t)tiles * (i + 1) / s.n);
+      s.v0 = (int)((int64_t)mine * i / s.n);
+      s.v1 = (int)((int64_t)mine * (i + 1) / s.n);
       return s;
     }
     before += __builtin_amdgcn_readlane(incl, 63);

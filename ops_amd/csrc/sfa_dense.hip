@@ -137,14 +137,15 @@ __global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
 
 enum { kAny = 0, kWide };
 struct KernelShape {
-  int rows, tile_shift, threads;
+  int rows, tile_shift, threads, per_cu;  // per_cu: workgroups on a CU at once
 };
-constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256}, {kWideRows, 6, 512}};
+constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256, 4}, {kWideRows, 6, 512, 1}};
 
 void set_launch(DenseParams& p, const DensePlan& pl) {
   p.rows = pl.rows;
   p.tile_shift = pl.tile_shift;
   p.nrb = (int)(((int64_t)p.S * p.G + pl.rows - 1) / pl.rows);
+  p.fit = pl.fit;
   p.want = pl.want;
   p.min_len = pl.min_len;
   p.slots = pl.slots;
@@ -163,15 +164,17 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   pl.threads = k.threads;
   const int64_t nrb = ((int64_t)p.S * p.G + pl.rows - 1) / pl.rows, units = p.B * nrb;
   const int64_t dims = pl.kernel == kAny ? (p.Dv + kAnyDims - 1) / kAnyDims : 1;
-  // Key ranges are cut while the row blocks are too few to fill the card evenly.
-  constexpr int64_t kWorkgroups = 1024;
+  // Few row blocks: their keys are cut into ranges that fill the card (sfa_dense.h).
+  constexpr int64_t kCus = 256;
   pl.min_len = 4;
-  int64_t want = kWorkgroups / (p.Hkv * dims);
-  const int64_t most = (((int64_t)p.cap >> pl.tile_shift) + pl.min_len) / pl.min_len * units;
+  const int64_t fit = kCus * k.per_cu / (p.Hkv * dims);
+  pl.fit = (int)(fit > 0 ? fit : 1);
+  int64_t want = 2 * ((units > pl.fit ? units : pl.fit));
+  const int64_t tiles = ((int64_t)p.cap >> pl.tile_shift) + 1, most = (tiles + pl.min_len - 1) / pl.min_len * units;
   if (want > most) want = most;
-  pl.want = want > units ? (int)want : 0;
-  pl.slots = (int)(units + pl.want);
-  pl.wgs = (units + pl.want) * p.Hkv * dims;
+  pl.want = units <= kDenseUnits && units <= 2 * pl.fit && want > units ? (int)want : 0;
+  pl.slots = (int)(pl.want > 0 ? pl.want : units);
+  pl.wgs = (int64_t)pl.slots * p.Hkv * dims;
   if (pl.want > 0) {
     const size_t rows = (size_t)pl.slots * p.Hkv * pl.rows;
     pl.part_o_bytes = (rows * p.Dv * sizeof(float) + 255) / 256 * 256;

@@ -46,125 +46,136 @@ __device__ __forceinline__ bf16x4 lds_tr16_at(uint32_t a) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)a);
 }
 
-enum { kSrcTile, kSrcRows, kSrcFp8 };
-// kSrcTile: a tile's rows have one base and stride (contiguous tensors, pages of 64
-// rows or more) and 32-bit offsets.
-inline int dense_tile_source(const DenseParams& p) {
-  const int64_t row = 2 * (p.k_ss > p.v_ss ? p.k_ss : p.v_ss);
-  const bool one = p.block_table == nullptr || p.page_shift >= 6;
-  return one && p.k_ss >= 0 && p.v_ss >= 0 && row < (int64_t)1 << 25 ? kSrcTile : kSrcRows;
+// Whether a tile's rows have one base and stride (contiguous tensors, pages of 64 rows
+// or more), with 32-bit offsets.
+inline bool dense_one_base(const DenseParams& p, int esize) {
+  const int64_t row = esize * (p.k_ss > p.v_ss ? p.k_ss : p.v_ss);
+  return (p.block_table == nullptr || p.page_shift >= 6) && p.k_ss >= 0 && p.v_ss >= 0 && row < (int64_t)1 << 25;
 }
 
-__device__ __forceinline__ int dense_load_const(const int32_t* at) {
-  return *(const __attribute__((address_space(4))) int32_t*)at;
-}
-
-// Tiles of 64 keys for NW waves.  ids(i, j0): the page ids of the tile at key j0 are
-// fetched; load(j0, ..): that tile's rows are, to LDS (or, e4m3, to registers, and
-// from there by store()); returns the rows that are there.  on = false: zeros, so
-// that the number of loads in flight does not depend on the range.
-template <int D, int NW, int SRC>
+// Tiles of 64 keys for NW waves.  at(i): the first key of the workgroup's i-th tile.
+// load(i, ..): that tile's rows go to LDS (e4m3: to registers, and from there by
+// store()); returns the rows that are there.  on = false: zeros, so that the number
+// of loads in flight does not depend on the range.  Calls of load come in order of i.
+// Page ids are held ahead of use, as a wait for one is a wait for every load before
+// it: ONE: those of 64 tiles by lane; else those of the next tile's rows.
+template <int D, int NW, bool FP8, bool ONE>
 struct TileSource {
   static constexpr int KT = kWideKeys, CH = D / 8, RPI = 64 / CH, NI = KT / RPI / NW;
   static_assert(NI >= 1 && KT / 8 == NW, "whole load instructions and eight rows a wave");
   uint64_t kbase, vbase;
   int64_t kpage, vpage, krow, vrow;
   const int32_t* trow;
+  KeyTiles tiles;
+  int v0, n;
   int cap, page_shift, num_pages, wave, lane;
-  int pg, pgr;                  // page ids: of the tile, or of key j0 + lane; of the wave's row lane / 8
+  int pg, pgr;  // page ids: of tiles by lane, or of the next tile's key `lane`; of its row that the lane loads (e4m3)
 
-  __device__ __forceinline__ TileSource(const DenseParams& p, int b, int g, int wave_, int lane_)
-      : cap(p.cap), page_shift(p.page_shift), num_pages(p.num_pages), wave(wave_), lane(lane_) {
-    const int64_t e = SRC == kSrcFp8 ? 1 : 2;
-    kbase = (uint64_t)(uintptr_t)p.k + (uint64_t)(e * g * p.k_sh);
-    vbase = (uint64_t)(uintptr_t)p.v + (uint64_t)(e * g * p.v_sh);
+  __device__ __forceinline__ TileSource(const DenseParams& p, const DenseItem& it, int wave_, int lane_)
+      : tiles(it.tiles), v0(it.v0), n(it.v1 - it.v0), cap(p.cap), page_shift(p.page_shift), num_pages(p.num_pages), wave(wave_),
+        lane(lane_) {
+    const int64_t e = FP8 ? 1 : 2;
+    kbase = (uint64_t)(uintptr_t)p.k + (uint64_t)(e * it.g * p.k_sh);
+    vbase = (uint64_t)(uintptr_t)p.v + (uint64_t)(e * it.g * p.v_sh);
     kpage = e * p.k_sb;
     vpage = e * p.v_sb;
     krow = e * p.k_ss;
     vrow = e * p.v_ss;
     trow = nullptr;
     if (p.block_table != nullptr) {
-      trow = p.block_table + b * p.bt_sb;
+      trow = p.block_table + it.b * p.bt_sb;
     } else {  // one page of all rows
-      kbase += (uint64_t)(b * kpage);
-      vbase += (uint64_t)(b * vpage);
+      kbase += (uint64_t)(it.b * kpage);
+      vbase += (uint64_t)(it.b * vpage);
       page_shift = 30;
       num_pages = 1;
     }
-    if constexpr (SRC == kSrcFp8) {
-      ksc = p.ks + g * p.ks_sh;
-      vsc = p.vs + g * p.vs_sh;
+    if constexpr (FP8) {
+      ksc = p.ks + it.g * p.ks_sh;
+      vsc = p.vs + it.g * p.vs_sh;
       ks_sb = p.ks_sb; ks_ss = p.ks_ss; vs_sb = p.vs_sb; vs_ss = p.vs_ss;
     }
+    ids(0);
   }
+  // (past the range: its last tile)
+  __device__ __forceinline__ int at(int i) const { return tiles.tile(v0 + max(min(i, n - 1), 0)) * KT; }
   __device__ __forceinline__ int entry(int j) const { return trow == nullptr ? 0 : trow[min(j, cap - 1) >> page_shift]; }
-  __device__ __forceinline__ void ids(int j0) {
-    if constexpr (SRC == kSrcTile) {
-      pg = trow == nullptr ? 0 : dense_load_const(trow + (j0 >> page_shift));
+  __device__ __forceinline__ void ids(int i) {
+    if constexpr (ONE) {
+      pg = entry(at(i + lane));
     } else {
-      pg = entry(j0 + lane);
-      if constexpr (SRC == kSrcFp8) pgr = entry(j0 + wave * 8 + (lane >> 3));
+      pg = entry(at(i) + lane);
+      if constexpr (FP8) pgr = entry(at(i) + wave * 8 + (lane >> 3));
     }
   }
-  // at most n tiles of this wave in flight
+  // at most N tiles of this wave in flight
   template <int N>
   __device__ __forceinline__ void wait() const {
-    if constexpr (SRC != kSrcFp8) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N * 2 * NI) : "memory");
+    if constexpr (!FP8) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N * 2 * NI) : "memory");
   }
 
-  __device__ __forceinline__ uint64_t load(int j0, bool on, u32x4* kt, u32x4* vt) {
-    const int in_page = (1 << page_shift) - 1;
-    if constexpr (SRC == kSrcTile) {
-      const int in = j0 & in_page, n = cap - j0, pgu = __builtin_amdgcn_readfirstlane(pg);
+  __device__ __forceinline__ uint64_t load(int i, u32x4* kt, u32x4* vt) {
+    const bool on = i < n;
+    const int j0 = at(i), in_page = (1 << page_shift) - 1;
+    const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+    uint64_t mask;
+    if constexpr (ONE) {
+      const int in = j0 & in_page, rows = cap - j0, pgu = __builtin_amdgcn_readlane(pg, i & 63);
       const bool ok = on && pgu >= 0 && pgu < num_pages;
-      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
       const uint64_t kb = ok ? kbase + (uint64_t)(pgu * kpage + in * krow) : zero;
       const uint64_t vb = ok ? vbase + (uint64_t)(pgu * vpage + in * vrow) : zero;
-      // (lane constants are formed per tile: held across the loop they spill)
-      int ln = lane;
-      asm volatile("" : "+v"(ln));
-      const int sub = ln / CH;
-      const uint32_t c = 16u * (uint32_t)((ln % CH) ^ Tile<D>::at(sub));
-      const uint32_t ko = (uint32_t)(sub * (int)krow) + c, vo = (uint32_t)(sub * (int)vrow) + c;
+      if constexpr (FP8) {
+        const int row = wave * 8 + (lane >> 3);
+        const bool there = ok && row < rows;
+        const uint32_t piece = (uint32_t)((lane & 7) * (D / 8));
+        raw(kb + (there ? (uint32_t)(row * (int)krow) : 0u) + piece, vb + (there ? (uint32_t)(row * (int)vrow) : 0u) + piece,
+            there, pgu, in + row);
+      } else {
+        // (lane constants are formed per tile: held across the loop they spill)
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int sub = ln / CH;
+        const uint32_t c = 16u * (uint32_t)((ln % CH) ^ Tile<D>::at(sub));
+        const uint32_t ko = (uint32_t)(sub * (int)krow) + c, vo = (uint32_t)(sub * (int)vrow) + c;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int q = wave * NI + i, left = ok ? n - q * RPI : 0;
-        // (rows past the last one read some row's chunks: no row of the result sees them)
-        const bool there = sub < left;
-        const uint64_t step = left > 0 ? (uint64_t)(q * RPI) : 0;
-        dense_dma16(kt + q * Tile<D>::GROUP, kb + step * (uint64_t)krow, there ? ko : c);
-        dense_dma16(vt + q * Tile<D>::GROUP, vb + step * (uint64_t)vrow, there ? vo : c);
+        for (int k = 0; k < NI; ++k) {
+          const int q = wave * NI + k, left = ok ? rows - q * RPI : 0;
+          // (rows past the last one read some row's chunks: no row of the result sees them)
+          const bool there = sub < left;
+          const uint64_t step = left > 0 ? (uint64_t)(q * RPI) : 0;
+          dense_dma16(kt + q * Tile<D>::GROUP, kb + step * (uint64_t)krow, there ? ko : c);
+          dense_dma16(vt + q * Tile<D>::GROUP, vb + step * (uint64_t)vrow, there ? vo : c);
+        }
       }
-      return !ok ? 0 : n >= KT ? ~0ull : (1ull << n) - 1;
-    } else if constexpr (SRC == kSrcRows) {
+      mask = !ok ? 0 : rows >= KT ? ~0ull : (1ull << rows) - 1;
+      if (((i + 1) & 63) == 0) ids(i + 1);
+    } else {
       const int j = j0 + lane;
       const bool ok = on && j < cap && pg >= 0 && pg < num_pages;
-      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
-      const uint64_t ka = ok ? kbase + (uint64_t)(pg * kpage + (j & in_page) * krow) : zero;
-      const uint64_t va = ok ? vbase + (uint64_t)(pg * vpage + (j & in_page) * vrow) : zero;
+      if constexpr (FP8) {
+        const int jr = j0 + wave * 8 + (lane >> 3), in = jr & in_page;
+        const bool there = on && jr < cap && pgr >= 0 && pgr < num_pages;
+        const uint64_t piece = (uint64_t)((lane & 7) * (D / 8));
+        raw((there ? kbase + (uint64_t)(pgr * kpage + in * krow) : zero) + piece,
+            (there ? vbase + (uint64_t)(pgr * vpage + in * vrow) : zero) + piece, there, pgr, in);
+      } else {
+        const uint64_t ka = ok ? kbase + (uint64_t)(pg * kpage + (j & in_page) * krow) : zero;
+        const uint64_t va = ok ? vbase + (uint64_t)(pg * vpage + (j & in_page) * vrow) : zero;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int q = wave * NI + i, row = q * RPI + lane / CH;
-        const uint64_t c = (uint64_t)(16 * ((lane % CH) ^ Tile<D>::at(row)));
-        dense_dma16(kt + q * Tile<D>::GROUP, from(ka, row) + c);
-        dense_dma16(vt + q * Tile<D>::GROUP, from(va, row) + c);
+        for (int k = 0; k < NI; ++k) {
+          const int q = wave * NI + k, row = q * RPI + lane / CH;
+          const uint64_t c = (uint64_t)(16 * ((lane % CH) ^ Tile<D>::at(row)));
+          dense_dma16(kt + q * Tile<D>::GROUP, from(ka, row) + c);
+          dense_dma16(vt + q * Tile<D>::GROUP, from(va, row) + c);
+        }
       }
-      return __ballot(ok);
-    } else {
-      const int j = j0 + lane, jr = j0 + wave * 8 + (lane >> 3);
-      const bool ok = on && j < cap && pg >= 0 && pg < num_pages, okr = on && jr < cap && pgr >= 0 && pgr < num_pages;
-      const int in = jr & in_page;
-      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
-      const uint64_t piece = (uint64_t)((lane & 7) * (D / 8));
-      kraw = *reinterpret_cast<const raw_t*>((okr ? kbase + (uint64_t)(pgr * kpage + in * krow) : zero) + piece);
-      vraw = *reinterpret_cast<const raw_t*>((okr ? vbase + (uint64_t)(pgr * vpage + in * vrow) : zero) + piece);
-      kexp = okr ? ksc[pgr * ks_sb + in * ks_ss] : 127;
-      vexp = okr ? vsc[pgr * vs_sb + in * vs_ss] : 127;
-      return __ballot(ok);
+      mask = __ballot(ok);
+      ids(i + 1);
     }
+    return mask;
   }
   __device__ __forceinline__ void store(u32x4* kt, u32x4* vt) const {
-    if constexpr (SRC == kSrcFp8) {
+    if constexpr (FP8) {
       const int row = wave * 8 + (lane >> 3), c0 = (lane & 7) * (D / 64);
       const float sk = scale_of((uint8_t)kexp), sv = scale_of((uint8_t)vexp);
 #pragma unroll
@@ -179,7 +190,7 @@ struct TileSource {
   __device__ __forceinline__ void value4(int j, int d, float (&v)[4]) const {
     const int id = entry(j), in = j & ((1 << page_shift) - 1);
     const uint64_t a = vbase + (uint64_t)(id * vpage + in * vrow);
-    if constexpr (SRC == kSrcFp8) {
+    if constexpr (FP8) {
       const uint32_t x = *reinterpret_cast<const uint32_t*>(a + d);
       const float s = scale_of(vsc[id * vs_sb + in * vs_ss]);
       v[0] = __builtin_amdgcn_cvt_f32_fp8((int)x, 0) * s;
@@ -199,6 +210,13 @@ struct TileSource {
   int64_t ks_sb, ks_ss, vs_sb, vs_ss;
   raw_t kraw, vraw;
   int kexp, vexp;
+  // the lane's bytes of row `in` of page id, and their exponents
+  __device__ __forceinline__ void raw(uint64_t ka, uint64_t va, bool there, int id, int in) {
+    kraw = *reinterpret_cast<const raw_t*>(ka);
+    vraw = *reinterpret_cast<const raw_t*>(va);
+    kexp = there ? ksc[id * ks_sb + in * ks_ss] : 127;
+    vexp = there ? vsc[id * vs_sb + in * vs_ss] : 127;
+  }
   static __device__ __forceinline__ uint64_t from(uint64_t a, int lane) {
     return ((uint64_t)(uint32_t)__shfl((int)(a >> 32), lane, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)a, lane, 64);
   }
@@ -213,6 +231,12 @@ struct TileSource {
     return r;
   }
 };
+
+// The rows of the tile at key j0 that a token at pos (-1: none) sees, as bits.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; }
+__device__ __forceinline__ uint64_t seen_of(const DenseParams& p, int pos, int j0) {
+  return low_bits(pos + 1 - j0) & (~low_bits(pos + 1 - p.window - j0) | low_bits(p.first - j0));
+}
 
 // Infinities and NaN of a V tile whose rows not every query row sees: noted as bits
 // (of s_bad, 0 before) and cleared in LDS, as 0 times them would reach the rows that

@@ -15,7 +15,7 @@
 namespace sfa {
 namespace {
 
-template <int D, int SRC>
+template <int D, bool FP8, bool ONE>
 __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   typedef Mfma<32> M;
   typedef f32x16 acc_t;
@@ -48,11 +48,8 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
     }
   }
 
-  TileSource<D, NW, SRC> src(p, b, g, wave, lane);
+  TileSource<D, NW, FP8, ONE> src(p, it, wave, lane);
   const int n = it.v1 - it.v0;
-  // first key of the i-th tile (past the range: the last one's, whose rows are not read again)
-  auto tile_at = [&](int i) { return it.tiles.tile(it.v0 + max(min(i, n - 1), 0)) * KT; };
-
   acc_t oacc[OT];
 #pragma unroll
   for (int o = 0; o < OT; ++o) oacc[o] = acc_t{};
@@ -69,11 +66,9 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   const uint32_t vx = 16u * (uint32_t)(L::at(vrow) ^ vc) , v0a = 16u * (uint32_t)L::slot(vrow, L::at(vrow)) + (uint32_t)(l16 & 1) * 8u;
 
   uint64_t mask[NS + 1];  // rows that are there, of tiles j, j + 1, ..
-  src.ids(tile_at(0));
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    mask[i] = src.load(tile_at(i), i < n, s_kv[i][0], s_kv[i][1]);
-    src.ids(tile_at(i + 1));
+    mask[i] = src.load(i, s_kv[i][0], s_kv[i][1]);
     src.store(s_kv[i][0], s_kv[i][1]);
   }
   if (tid < 2) s_bad[tid] = 0;
@@ -94,14 +89,15 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
     const bf16x4 lo = lds_tr16_at(at + (uint32_t)L::rows(16 * (i / OT))), hi = lds_tr16_at(at + (uint32_t)L::rows(16 * (i / OT) + 8));
     return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
+  // the largest of a lane's 32 scores, in 16 steps of two
+  auto max_step = [&](const acc_t (&c)[2], float (&x)[2], auto tc) {
+    constexpr int t = decltype(tc)::value, k = t & 1, e = 2 * (t >> 1);
+    x[k] = t < 2 ? max_raw(c[k][0], c[k][1]) : max3_raw(x[k], c[k][e], c[k][e + 1]);
+  };
   auto max_of = [&](const acc_t (&c)[2]) {
-    float x = max3_raw(c[0][0], c[0][1], c[0][2]), y = max3_raw(c[1][0], c[1][1], c[1][2]);
-#pragma unroll
-    for (int e = 3; e < 15; e += 2) {
-      x = max3_raw(x, c[0][e], c[0][e + 1]);
-      y = max3_raw(y, c[1][e], c[1][e + 1]);
-    }
-    return max3_raw(max_raw(x, c[0][15]), y, c[1][15]);
+    float x[2];
+    each<16>([&](auto tc) { max_step(c, x, tc); });
+    return max_raw(x[0], x[1]);
   };
   acc_t sa[2], sb[2];
 #pragma unroll
@@ -142,31 +138,33 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
     }
   };
   int st = 0, nbad = 0;
+  auto whole = [&](int j) {
+    const int j0 = src.at(j);
+    return j0 + KT - 1 <= p0 && (j0 + KT <= p.first || p1 - j0 < p.window);
+  };
   auto step = [&](int j, acc_t (&cur)[2], acc_t (&nxt)[2]) {
-    const int j0 = tile_at(j);
     const int st1 = (st + 1) & (NS - 1), st2 = (st + 2) & (NS - 1);
     // (opaque: the flipped addresses are formed at their reads, not held)
     uint32_t kf = kx, vf = vx;
     asm volatile("" : "+v"(kf), "+v"(vf));
     const uint32_t kn = lds_addr(s_kv[st1][0]) + k0a, kn2 = lds_addr(s_kv[st2][0]) + k0a, vt = lds_addr(s_kv[st][1]) + v0a;
-    const bool whole = mask[0] == ~0ull && j0 + KT - 1 <= p0 && (j0 + KT <= p.first || p1 - j0 < p.window);
     uint64_t bad = 0;
-    if (!whole) {
+    if (!(whole(j) && mask[0] == ~0ull)) {
       // (two words in turn: the other one's readers have passed a step's barrier)
       bad = clear_bad<D, NW>(s_kv[st][1], &s_bad[nbad & 1], wave, lane);
       ++nbad;
       if (tid == 0) s_bad[nbad & 1] = 0;
+      // the rows that the lane's row sees, as bits from its first key on
+      const uint64_t seen = seen_of(p, pos, src.at(j)) & mask[0];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const uint32_t there = (uint32_t)(mask[0] >> (32 * kb));
+        const uint32_t bits = (uint32_t)(seen >> (32 * kb)) >> (4 * hq);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = 8 * (e >> 2) + 4 * hq + (e & 3);
-          const bool ok = ((there >> key) & 1) && dense_seen(p, j0 + 32 * kb + key, pos);
-          cur[kb][e] = ok ? cur[kb][e] : kNegInf;
-        }
+        for (int e = 0; e < 16; ++e) cur[kb][e] = (bits >> (8 * (e >> 2) + (e & 3))) & 1 ? cur[kb][e] : kNegInf;
       }
       tmax = max_of(cur);
+      // (opaque: otherwise the other path copies each score to where this one left it)
+      asm volatile("" : "+v"(cur[0]), "+v"(cur[1]));
     }
     if (__any(tmax * p.scale_log2 > m_used + 8.f)) {
       const float mn = fmaxf(m_used, xor32_max(tmax * p.scale_log2));
@@ -179,7 +177,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
     const float moff = m_used == kNegInf ? 0.f : -m_used;
 
     bf16x8 pb[4];
-    float ex = 0.f;
+    float ex[2], arg = fmaf(cur[0][0], p.scale_log2, moff), mx[2];
     each<NM>([&](auto ic) {
       constexpr int i = decltype(ic)::value;
       __builtin_amdgcn_sched_barrier(0);
@@ -199,28 +197,38 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
       if constexpr (i + 4 < NQ) op[i & 3] = read_k(kn, kf, i + 4);
       else if constexpr (i + 4 < NM) op[i & 3] = read_v(vt, vf, i + 4 - NQ);
       else op[i & 3] = read_k(kn2, kf, i + 4 - NM);
-      // the weights, evenly before the last keys' sums
+      // the weights, evenly before the last keys' sums; each is used when the next one is made
       each<32>([&](auto ec) {
-        constexpr int e = decltype(ec)::value, kb = e >> 4, ee = e & 15;
+        constexpr int e = decltype(ec)::value;
         if constexpr (e * (NM - OT) / 32 == i) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(cur[kb][ee], p.scale_log2, moff));
-          l_part += x;
-          asm volatile("" : "+v"(l_part));  // (added here: all weights held for one sum at the end spill)
-          if constexpr (e & 1) {
-            pb[e >> 3][(e & 7) - 1] = (bf16)ex;
-            pb[e >> 3][e & 7] = (bf16)x;
+          const float x = __builtin_amdgcn_exp2f(arg);
+          if constexpr (e < 31) arg = fmaf(cur[(e + 1) >> 4][(e + 1) & 15], p.scale_log2, moff);
+          if constexpr (e > 0) l_part += ex[(e - 1) & 1];
+          if constexpr (e > 0 && e % 2 == 0) {
+            pb[(e - 2) >> 3][(e - 2) & 7] = (bf16)ex[0];
+            pb[(e - 2) >> 3][(e - 1) & 7] = (bf16)ex[1];
           }
-          ex = x;
+          ex[e & 1] = x;
+          if constexpr (e == 31) {
+            l_part += x;
+            pb[3][6] = (bf16)ex[0];
+            pb[3][7] = (bf16)ex[1];
+          }
+          asm volatile("" : "+v"(l_part));  // (added here: all weights held for one sum at the end spill)
         }
       });
+      // the next tile's maxima
+      each<16>([&](auto tc) {
+        constexpr int t = decltype(tc)::value, i0 = NQ + 3;
+        if constexpr (i0 + t * (NM - i0) / 16 == i) max_step(nxt, mx, tc);
+      });
       if constexpr (i == NM - 2) {
-        mask[NS] = src.load(tile_at(j + 4), j + 4 < n, s_kv[st][0], s_kv[st][1]);
-        src.ids(tile_at(j + 5));
+        mask[NS] = src.load(j + 4, s_kv[st][0], s_kv[st][1]);
       }
     });
     __builtin_amdgcn_sched_barrier(0);
-    tmax = max_of(nxt);
-    if (bad != 0) add_bad(bad, j0, pb);
+    tmax = max_raw(mx[0], mx[1]);
+    if (bad != 0) add_bad(bad, src.at(j), pb);
     src.store(s_kv[st][0], s_kv[st][1]);
 #pragma unroll
     for (int i = 0; i < NS; ++i) mask[i] = mask[i + 1];
@@ -263,19 +271,20 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
 }
 
 template <int D>
-void launch(const DenseParams& p, int src, unsigned grid, hipStream_t s) {
-  if (src == kSrcTile) dense_wide_kernel<D, kSrcTile><<<grid, 512, 0, s>>>(p);
-  else if (src == kSrcRows) dense_wide_kernel<D, kSrcRows><<<grid, 512, 0, s>>>(p);
-  else dense_wide_kernel<D, kSrcFp8><<<grid, 512, 0, s>>>(p);
+void launch(const DenseParams& p, bool fp8, unsigned grid, hipStream_t s) {
+  const bool one = dense_one_base(p, fp8 ? 1 : 2);
+  if (fp8 && one) dense_wide_kernel<D, true, true><<<grid, 512, 0, s>>>(p);
+  else if (fp8) dense_wide_kernel<D, true, false><<<grid, 512, 0, s>>>(p);
+  else if (one) dense_wide_kernel<D, false, true><<<grid, 512, 0, s>>>(p);
+  else dense_wide_kernel<D, false, false><<<grid, 512, 0, s>>>(p);
 }
 
 }  // namespace
 
 void launch_dense_wide(const DenseParams& p, int kv_dtype, hipStream_t s) {
-  const int src = kv_dtype == SFA_DTYPE_FP8_E4M3 ? kSrcFp8 : dense_tile_source(p);
   const unsigned grid = (unsigned)((int64_t)p.slots * p.Hkv);
-  if (p.Dqk == 64) launch<64>(p, src, grid, s);
-  else launch<128>(p, src, grid, s);
+  if (p.Dqk == 64) launch<64>(p, kv_dtype == SFA_DTYPE_FP8_E4M3, grid, s);
+  else launch<128>(p, kv_dtype == SFA_DTYPE_FP8_E4M3, grid, s);
 }
 
 }  // namespace sfa
