@@ -7,75 +7,80 @@ namespace sfa {
 namespace {
 
 // ---- joining the ranges of a row block -------------------------------------------
-// One wave a row; LPR lanes hold it (4 dims each), 64 / LPR ranges at a time.  A range
-// in which the row sees nothing has LSE -inf.
+// A workgroup takes jr rows of a unit, one wave a row; LPR lanes hold it (4 dims each),
+// 64 / LPR ranges at a time.  A range in which the row sees nothing has LSE -inf.
 template <typename T, int LPR>
-__global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p) {
+__global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p, int jr) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t i = (int64_t)blockIdx.x * 4 + wave;
-  const int row = (int)(i % p.rows);
-  i /= p.rows;
-  const int g = (int)(i % p.Hkv), u = (int)(i / p.Hkv);
-  if (u >= p.B * p.nrb) return;
-  const int b = u / p.nrb, r = (u - b * p.nrb) * p.rows + row;
-  if (r >= p.S * p.G) return;
+  const int chunks = (p.rows + jr - 1) / jr;
+  int wi = blockIdx.x;
+  const int row0 = wi % chunks * jr;
+  wi /= chunks;
+  const int g = wi % p.Hkv, u = wi / p.Hkv;
   const int first = p.unit_slots[2 * u], ns = p.unit_slots[2 * u + 1];
   if (ns <= 1) return;
-  const int t = r / p.G, h = g * p.G + r % p.G;
-  const int64_t per = (int64_t)p.Hkv * p.rows, at0 = ((int64_t)first * p.Hkv + g) * p.rows + row;
-  const float* pl = p.part_lse + at0;
-  const float* po = p.part_o + at0 * p.Dv;
-  const bool live = t < dense_seq(p, b).n;
-  float m = kNegInf, nan = 0.f;
-  for (int k = lane; k < ns; k += 64) {
-    const float x = pl[k * per];
-    nan += x != x ? x : 0.f;
-    m = fmaxf(m, x);
-  }
-  m = wave_max(m);
-  const float moff = m == kNegInf ? 0.f : m;
-  float l = 0.f;
-  for (int k = lane; k < ns; k += 64) l += exp2f(pl[k * per] - moff);
-  l = wave_sum(l + nan);
-  float lse;
-  const float f = dense_finish(p, h, live, m, l, lse);
-  if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
-  T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
-  const int sub = lane / LPR;
-  for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
-    const int d = d0 + 4 * (lane % LPR);
-    f32x4 x = {};
-    if (f != 0.f) {
-#pragma unroll 4
-      for (int k = sub; k < ns; k += 64 / LPR) {
-        const float e = exp2f(pl[k * per] - moff);
-        f32x4 v = {};
-        const float* at = po + k * per * p.Dv + d;
-        if (p.Dv % 4 == 0) {
-          if (d < p.Dv) v = *reinterpret_cast<const f32x4*>(at);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = d + q < p.Dv ? at[q] : 0.f;
-        }
-        x += v * e;
-      }
+  const int b = u / p.nrb;
+  for (int row = row0 + wave; row < min(row0 + jr, p.rows); row += 4) {
+    const int r = (u - b * p.nrb) * p.rows + row;
+    if (r >= p.S * p.G) return;
+    const int t = r / p.G, h = g * p.G + r % p.G;
+    const int64_t per = (int64_t)p.Hkv * p.rows, at0 = ((int64_t)first * p.Hkv + g) * p.rows + row;
+    const float* pl = p.part_lse + at0;
+    const float* po = p.part_o + at0 * p.Dv;
+    const bool live = t < dense_seq(p, b).n;
+    float m = kNegInf, nan = 0.f;
+    for (int k = lane; k < ns; k += 64) {
+      const float x = pl[k * per];
+      nan += x != x ? x : 0.f;
+      m = fmaxf(m, x);
     }
+    m = wave_max(m);
+    const float moff = m == kNegInf ? 0.f : m;
+    float l = 0.f;
+    for (int k = lane; k < ns; k += 64) l += exp2f(pl[k * per] - moff);
+    l = wave_sum(l + nan);
+    float lse;
+    const float f = dense_finish(p, h, live, m, l, lse);
+    if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+    T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
+    const int sub = lane / LPR;
+    for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
+      const int d = d0 + 4 * (lane % LPR);
+      f32x4 x = {};
+      if (f != 0.f) {
+#pragma unroll 4
+        for (int k = sub; k < ns; k += 64 / LPR) {
+          const float e = exp2f(pl[k * per] - moff);
+          f32x4 v = {};
+          const float* at = po + k * per * p.Dv + d;
+          if (p.Dv % 4 == 0) {
+            if (d < p.Dv) v = *reinterpret_cast<const f32x4*>(at);
+          } else {
 #pragma unroll
-    for (int s = LPR; s < 64; s <<= 1)
+            for (int q = 0; q < 4; ++q) v[q] = d + q < p.Dv ? at[q] : 0.f;
+          }
+          x += v * e;
+        }
+      }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] += __shfl_xor(x[q], s, 64);
-    if (sub == 0)
+      for (int s = LPR; s < 64; s <<= 1)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (d + q < p.Dv) o[d + q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+        for (int q = 0; q < 4; ++q) x[q] += __shfl_xor(x[q], s, 64);
+      if (sub == 0)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (d + q < p.Dv) o[d + q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+    }
   }
 }
 template <typename T>
 void combine(const DenseParams& p, hipStream_t s) {
-  const unsigned grid = (unsigned)(((int64_t)p.B * p.nrb * p.Hkv * p.rows + 3) / 4);
-  if (p.Dv <= 64) dense_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p);
-  else if (p.Dv <= 128) dense_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p);
-  else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p);
+  // (few rows: a wave each; many: their units often have one range, and then nothing is left to do)
+  const int jr = p.rows <= 64 ? 4 : 16;
+  const unsigned grid = (unsigned)((int64_t)p.B * p.nrb * p.Hkv * ((p.rows + jr - 1) / jr));
+  if (p.Dv <= 64) dense_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p, jr);
+  else if (p.Dv <= 128) dense_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p, jr);
+  else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p, jr);
 }
 
 // ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse ------------
@@ -135,11 +140,12 @@ __global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
   if (threadIdx.x == 0) p.dsink[h] = -s_x[0];
 }
 
-enum { kAny = 0, kWide };
+enum { kAny = 0, kWide, kFew16, kFew32, kFew64 };
 struct KernelShape {
   int rows, tile_shift, threads, per_cu;  // per_cu: workgroups on a CU at once
 };
-constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256, 4}, {kWideRows, 6, 512, 1}};
+constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256, 4}, {kWideRows, 6, 512, 1}, {16, 7, 256, 2}, {32, 7, 256, 2},
+                                   {64, 7, 256, 1}};
 
 void set_launch(DenseParams& p, const DensePlan& pl) {
   p.rows = pl.rows;
@@ -157,7 +163,8 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   DensePlan pl{};
   pl.kernel = kAny;
   const int64_t R = (int64_t)p.S * p.G;
-  if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) && R > 64) pl.kernel = kWide;
+  if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
+    pl.kernel = R <= 16 ? kFew16 : R <= 32 ? kFew32 : R <= 64 ? kFew64 : kWide;
   const KernelShape& k = kShapes[pl.kernel];
   pl.rows = k.rows;
   pl.tile_shift = k.tile_shift;
@@ -166,8 +173,11 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   const int64_t dims = pl.kernel == kAny ? (p.Dv + kAnyDims - 1) / kAnyDims : 1;
   // Few row blocks: their keys are cut into ranges that fill the card (sfa_dense.h).
   constexpr int64_t kCus = 256;
-  pl.min_len = 4;
-  const int64_t fit = kCus * k.per_cu / (p.Hkv * dims);
+  const bool few = pl.kernel >= kFew16;
+  pl.min_len = few ? 2 : 4;
+  // (LDS of the few rows' kernel: one workgroup a CU with bf16 rows of 128 dims)
+  const int per_cu = few && kv_dtype == SFA_DTYPE_BF16 && p.Dqk == 128 ? 1 : k.per_cu;
+  const int64_t fit = kCus * per_cu / (p.Hkv * dims);
   pl.fit = (int)(fit > 0 ? fit : 1);
   int64_t want = 2 * ((units > pl.fit ? units : pl.fit));
   const int64_t tiles = ((int64_t)p.cap >> pl.tile_shift) + 1, most = (tiles + pl.min_len - 1) / pl.min_len * units;
@@ -188,6 +198,7 @@ hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, i
   DenseParams p = p0;
   set_launch(p, pl);
   if (pl.kernel == kWide) launch_dense_wide(p, kv_dtype, s);
+  else if (pl.kernel >= kFew16) launch_dense_few(p, kv_dtype, s);
   else launch_dense_any(p, dtype, kv_dtype, s);
   if (pl.want > 0) {
     if (dtype == SFA_DTYPE_F32) combine<float>(p, s);

@@ -46,11 +46,11 @@ __device__ __forceinline__ bf16x4 lds_tr16_at(uint32_t a) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)a);
 }
 
-// Whether a tile's rows have one base and stride (contiguous tensors, pages of 64 rows
-// or more), with 32-bit offsets.
-inline bool dense_one_base(const DenseParams& p, int esize) {
+// Whether the 2^shift rows of a tile have one base and stride (contiguous tensors, pages of
+// so many rows or more), with 32-bit offsets.
+inline bool dense_one_base(const DenseParams& p, int esize, int shift) {
   const int64_t row = esize * (p.k_ss > p.v_ss ? p.k_ss : p.v_ss);
-  return (p.block_table == nullptr || p.page_shift >= 6) && p.k_ss >= 0 && p.v_ss >= 0 && row < (int64_t)1 << 25;
+  return (p.block_table == nullptr || p.page_shift >= shift) && p.k_ss >= 0 && p.v_ss >= 0 && row < (int64_t)1 << 25;
 }
 
 // Tiles of 64 keys for NW waves.  at(i): the first key of the workgroup's i-th tile.

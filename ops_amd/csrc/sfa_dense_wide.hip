@@ -272,7 +272,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
 
 template <int D>
 void launch(const DenseParams& p, bool fp8, unsigned grid, hipStream_t s) {
-  const bool one = dense_one_base(p, fp8 ? 1 : 2);
+  const bool one = dense_one_base(p, fp8 ? 1 : 2, 6);
   if (fp8 && one) dense_wide_kernel<D, true, true><<<grid, 512, 0, s>>>(p);
   else if (fp8) dense_wide_kernel<D, true, false><<<grid, 512, 0, s>>>(p);
   else if (one) dense_wide_kernel<D, false, true><<<grid, 512, 0, s>>>(p);

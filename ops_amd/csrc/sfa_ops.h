@@ -186,6 +186,9 @@ void launch_dense_bwd_any(const DenseParams& p, int dtype, hipStream_t s);
 constexpr int kWideRows = 256;
 void launch_dense_wide(const DenseParams& p, int kv_dtype, hipStream_t s);
 
+// ... and up to 64 rows a (sequence, kv head) (sfa_dense_few.hip): p.rows 16, 32 or 64
+void launch_dense_few(const DenseParams& p, int kv_dtype, hipStream_t s);
+
 // ---- rows of a cache as contiguous ones (sfa_read.hip) ----
 struct ReadParams {
   const void* cache;
