@@ -112,8 +112,14 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
   if (lane != 0) return;
   const int64_t li = b * p.l_sb + t * p.l_ss + h * p.l_sh;
   const float lse = live ? p.lse[li] : kNegInf;
-  p.row_lse[rr] = lse == kNegInf ? -kNegInf : lse * kLog2e;
-  p.row_delta[rr] = live ? sum - (p.dlse != nullptr ? p.dlse[li] : 0.f) : 0.f;
+  const float delta = live ? sum - (p.dlse != nullptr ? p.dlse[li] : 0.f) : 0.f;
+  if (p.row_neg) {
+    p.row_lse[rr] = lse == kNegInf ? kNegInf : -lse / p.scale;
+    p.row_delta[rr] = -delta;
+  } else {
+    p.row_lse[rr] = lse == kNegInf ? -kNegInf : lse * kLog2e;
+    p.row_delta[rr] = delta;
+  }
 }
 
 // dsink[h] = -sum over the rows of exp(sink - lse) delta, a workgroup a head, in a fixed order.
@@ -127,8 +133,8 @@ __global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
     const int n = dense_seq(p, b).n;
     for (int t = threadIdx.x; t < n; t += 1024) {
       const int64_t rr = base + (int64_t)t * p.G + hl;
-      const float l = p.row_lse[rr];
-      sum += l == -kNegInf ? 0.f : exp2f(sink - l) * p.row_delta[rr];
+      const float l = p.row_neg ? -p.row_lse[rr] * p.scale_log2 : p.row_lse[rr], d = p.row_delta[rr];
+      sum += l == -kNegInf ? 0.f : exp2f(sink - l) * (p.row_neg ? -d : d);
     }
   }
   s_x[threadIdx.x] = sum;
@@ -211,25 +217,66 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   DenseBwdPlan pl{};
   const size_t rows = (size_t)p.B * p.Hkv * p.S * p.G;
   pl.row_bytes = 2 * ((rows * sizeof(float) + 255) / 256 * 256);
-  const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
-  const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows;
-  pl.fits = p.B * nrb * p.Hkv * dims * 256 < (int64_t)1 << 32 && p.B * (((int64_t)p.S + 63) / 64) * p.Hkv * dims * 256 < (int64_t)1 << 32;
+  const int64_t groups = (int64_t)p.B * p.Hkv, most = (int64_t)1 << 32;
+  pl.mfma = dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) &&
+            p.k_ss >= 0 && p.v_ss >= 0 && p.k_ss < (int64_t)1 << 24 && p.v_ss < (int64_t)1 << 24;
+  if (!pl.mfma) {
+    const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
+    const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows;
+    pl.fits = groups * nrb * dims * 256 < most && groups * (((int64_t)p.S + 63) / 64) * dims * 256 < most;
+    return pl;
+  }
+  // Key blocks' rows in chunks, so that there are some units for every CU and none is much
+  // longer than the others: without a window the first keys are seen by all rows, the last
+  // by few, and the first tokens of a window by all of them.
+  const int64_t nkb = ((int64_t)p.S + kDkvKeys - 1) / kDkvKeys;
+  auto block_rows = [&](int64_t kb) {
+    const int64_t j0 = kb * kDkvKeys, t1 = j0 < p.first ? p.S : j0 + kDkvKeys - 1 + p.window;
+    return ((t1 < p.S ? t1 : (int64_t)p.S) - j0) * p.G;
+  };
+  int64_t total = 0;
+  for (int64_t kb = 0; kb < nkb; ++kb) total += block_rows(kb);
+  constexpr int64_t kUnits = 768, kLeast = 512;  // three a CU; a chunk of fewer rows is mostly its start
+  int64_t chunk = (total * groups / kUnits + 31) / 32 * 32;
+  if (chunk < kLeast) chunk = kLeast;
+  // (blocks up to a quarter over stay whole)
+  int64_t units = 0, parts = 0, widest = 0;
+  for (int64_t kb = 0; kb < nkb; ++kb) {
+    const int64_t r = block_rows(kb);
+    if (r <= chunk + chunk / 4 && r > widest) widest = r;
+  }
+  if (widest > chunk) chunk = (widest + 31) / 32 * 32;
+  for (int64_t kb = 0; kb < nkb; ++kb) {
+    const int64_t nc = (block_rows(kb) + chunk - 1) / chunk;
+    units += nc;
+    parts += nc > 1 ? nc : 0;
+  }
+  pl.chunk = (int)(chunk < (int64_t)1 << 30 ? chunk : (int64_t)1 << 30);
+  pl.units = (int)units;
+  pl.parts = (int)parts;
+  pl.dkv_bytes = (size_t)(groups * parts) * kDkvKeys * 2 * p.Dqk * sizeof(float);
+  const int64_t nrb = ((int64_t)p.S * p.G + kWideRows - 1) / kWideRows;
+  pl.fits = groups * nrb * 512 < most && groups * units * 256 < most && groups * nkb * 256 < most;
   return pl;
 }
 
 hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int dtype, hipStream_t s) {
   DenseParams p = p0;
+  p.row_neg = pl.mfma;
   const int64_t rows = (int64_t)p.B * p.Hkv * p.S * p.G;
   const unsigned grid = (unsigned)((rows + 15) / 16);
   if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p);
   else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
   if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
   DensePlan q{};
-  q.rows = kAnyRows;
-  q.tile_shift = kAnyShift;
-  q.slots = p.B * (int)(((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows);
+  q.rows = pl.mfma ? kWideRows : kAnyRows;
+  q.tile_shift = pl.mfma ? 6 : kAnyShift;
+  q.slots = p.B * (int)(((int64_t)p.S * p.G + q.rows - 1) / q.rows);
   set_launch(p, q);
-  launch_dense_bwd_any(p, dtype, s);
+  p.chunk = pl.chunk;
+  p.dkv_parts = pl.parts;
+  if (pl.mfma) launch_dense_bwd_mfma(p, pl.units, s);
+  else launch_dense_bwd_any(p, dtype, s);
   return hipGetLastError();
 }
 

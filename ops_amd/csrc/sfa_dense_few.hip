@@ -33,13 +33,6 @@ struct FewSwz {
   }
 };
 
-// lane l: 4 bytes (1 byte, as 4) from its address to dst + 4 l
-__device__ __forceinline__ void dense_dma4(const void* lds, uint64_t addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr(lds)), "v"(addr) : "memory", "m0");
-}
-__device__ __forceinline__ void dense_dma1(const void* lds, uint64_t addr) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds_addr(lds)), "v"(addr) : "memory", "m0");
-}
 __device__ __forceinline__ uint32_t bad8(uint32_t w) {  // bytes of w that are NaN: their masks
   uint32_t m = 0;
 #pragma unroll

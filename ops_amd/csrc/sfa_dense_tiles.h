@@ -35,6 +35,15 @@ __device__ __forceinline__ void dense_dma16(const void* lds, uint64_t addr) {
   const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(d), "v"(addr) : "memory", "m0");
 }
+// 4 bytes (1 byte, as 4) to dst + 4 l
+__device__ __forceinline__ void dense_dma4(const void* lds, uint64_t addr) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(d), "v"(addr) : "memory", "m0");
+}
+__device__ __forceinline__ void dense_dma1(const void* lds, uint64_t addr) {
+  const uint32_t d = (uint32_t)(uintptr_t)(lds_void*)const_cast<void*>(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_ubyte %1, off" ::"s"(d), "v"(addr) : "memory", "m0");
+}
 __device__ __forceinline__ void dense_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Reads at an LDS address and a constant.
@@ -261,6 +270,25 @@ __device__ __forceinline__ uint64_t clear_bad(u32x4* vt, unsigned long long* s_b
   }
   dense_barrier();
   return *s_bad;
+}
+
+// Elements of 32 rows from `row` on that are no numbers, cleared; a barrier on both sides
+// of what all waves do with them.
+template <int D, int NW>
+__device__ __forceinline__ void clear_rows(u32x4* t, int row, int wave, int lane) {
+  constexpr int N = 32 / Tile<D>::RPI;  // groups of 64 chunks
+#pragma unroll
+  for (int i = 0; i < (N + NW - 1) / NW; ++i) {
+    const int q = i * NW + wave;
+    if (N % NW != 0 && q >= N) break;
+    const int at = (row / Tile<D>::RPI + q) * Tile<D>::GROUP + lane;
+    const u32x4 w = t[at];
+    u32x4 m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = bad16(w[e]);
+    if ((m[0] | m[1] | m[2] | m[3]) != 0) t[at] = w & ~m;
+  }
+  dense_barrier();
 }
 
 // Where the workgroup's share of a launch is: the row blocks of a (sequence, kv head)

@@ -152,10 +152,13 @@ struct DenseParams {
   int64_t do_sb, do_ss, do_sh, dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
   const float* dlse;         // lse's strides, or nullptr
   float* dsink;              // [Hq] or nullptr
-  float* row_lse;            // [B][Hkv][S G] base-2 LSE, +inf for rows that see nothing
-  float* row_delta;          // [B][Hkv][S G] sum o do - dlse
-  float* dkv_part;           // partial dK | dV rows of key blocks cut in chunks of query rows
-  int chunk;                 // query rows a chunk
+  // [B][Hkv][S G]: base-2 LSE (+inf: nothing seen) and delta = sum o do - dlse; for the bf16
+  // matrix kernels (row_neg) -lse / scale and -delta, which their accumulators start from
+  float* row_lse;
+  float* row_delta;
+  bool row_neg;
+  float* dkv_part;           // [B Hkv][dkv_parts][kDkvKeys][2 D] partial dK | dV of key blocks cut in chunks
+  int chunk, dkv_parts;      // query rows a chunk; partials a kv head
 };
 constexpr int kDenseUnits = 256;  // row blocks of a launch that is cut into ranges, at most
 struct DensePlan {
@@ -169,9 +172,10 @@ struct DensePlan {
 };
 DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype);
 hipError_t launch_dense(const DenseParams& p, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s);
+constexpr int kDkvKeys = 128;  // keys a block of the dk / dv kernel
 struct DenseBwdPlan {
   size_t row_bytes, dkv_bytes;  // row_lse + row_delta; partial dK | dV
-  int chunk;
+  int chunk, units, parts;      // of the dk / dv kernel: rows a chunk, units and partials a kv head
   bool mfma, fits;
   size_t workspace() const { return row_bytes + dkv_bytes; }
 };
@@ -188,6 +192,8 @@ void launch_dense_wide(const DenseParams& p, int kv_dtype, hipStream_t s);
 
 // ... and up to 64 rows a (sequence, kv head) (sfa_dense_few.hip): p.rows 16, 32 or 64
 void launch_dense_few(const DenseParams& p, int kv_dtype, hipStream_t s);
+
+void launch_dense_bwd_mfma(const DenseParams& p, int units, hipStream_t s);  // (sfa_dense_bwd.hip)
 
 // ---- rows of a cache as contiguous ones (sfa_read.hip) ----
 struct ReadParams {
