@@ -114,12 +114,19 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
     const uint32_t kn2 = lds_addr(s_kv[st1][0]) + k0a, vn2 = lds_addr(s_kv[st1][1]) + k0a;
     const int j0 = src.at(j);
     const bool whole = mask[0] == ~0ull && j0 + KT - 1 <= p0 && (j0 + KT <= p.first || p1 - j0 < p.window);
-    uint32_t seen = ~0u;
     if (!whole) {
       // infinities and NaN of keys that not every row sees: 0 times them would reach those
       // that do not (those that do have weights that are no numbers)
       clear_rows<D, NW>(s_kv[st][0], 32 * H, wave, lane);
-      seen = (uint32_t)((seen_of(p, pos, j0) & mask[0]) >> (32 * H)) >> (4 * hq);
+      const uint32_t seen = (uint32_t)((seen_of(p, pos, j0) & mask[0]) >> (32 * H)) >> (4 * hq);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool ok = (seen >> (8 * (e >> 2) + (e & 3))) & 1;
+        cs[e] = ok ? cs[e] : kNegInf;
+        cd[e] = ok ? cd[e] : 0.f;
+      }
+      // (opaque: otherwise the other path copies each score to where this one left it)
+      asm volatile("" : "+v"(cs), "+v"(cd));
     }
     bf16x8 pb[2];
     float ex = 0.f;
@@ -146,8 +153,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
         constexpr int e = decltype(ec)::value;
         if constexpr (e * (NM - OT) / 16 == i) {
           const float w = __builtin_amdgcn_exp2f(fmaf(cs[e], p.scale_log2, moff));
-          float x = w * (cd[e] + ndelta);
-          x = (seen >> (8 * (e >> 2) + (e & 3))) & 1 ? x : 0.f;
+          const float x = w * (cd[e] + ndelta);
           if constexpr (e & 1) {
             pb[e >> 3][(e & 7) - 1] = (bf16)ex;
             pb[e >> 3][e & 7] = (bf16)x;
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
     }
 }
 
-// ---- dk and dv: four waves of 32 keys, tiles of 32 query rows of all heads ---------------
+// ---- dk and dv: 128 keys, tiles of 32 query rows of all heads ----------------------------
 // A key block's rows are one range of r = t G + h; blocks that many rows see are cut in
 // chunks of p.chunk rows, which leave partial sums that dense_dkv_join_kernel adds in order.
 struct DkvUnit {
@@ -234,18 +240,26 @@ __device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
   return DkvUnit{-1, 0, 0, 0, 0, 0};
 }
 
+// Waves 0 .. 3 make p and ds of 32 rows x 128 keys (each 16 rows x 64 keys, 16x16x32: an
+// operand of Q or dO read from LDS serves 64 keys) and leave them in LDS as bf16, in operand
+// order; waves 4 .. 7, one on each SIMD beside one of those, take the last step's for the
+// sums of 64 keys x half of the dims.  So no wave holds both the keys' rows and the
+// sums (all in one wave are 320 registers: 929 us at 8192 tokens, window 1024, 32 / 8
+// heads of 128), the products of one cover the weights of the other, and LDS moves 112 KB a
+// step of 1024 clocks' products.
 template <int D>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void dense_dkv_kernel(DenseParams p, int units) {
+__global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   typedef Tile<D> L;
-  constexpr int NW = 4, RT = 32, KS = D / 16, OT = D / 32, NS = 4, CH = D / 8, RPI = L::RPI, NI = RT / RPI / NW;
-  constexpr int SLOTS = RT / RPI * L::GROUP, LOADS = 2 * NI + 1;
-  static_assert(NI >= 1, "a load instruction a wave");
-  __shared__ u32x4 s_row[NS][2][SLOTS];     // Q, dO
-  __shared__ float s_c[NS][NW][2][RT];      // -lse / scale, -delta (a copy a wave)
+  typedef Mfma<16> M16;
+  constexpr int NW = 8, RT = 32, NS = 5, CH = D / 8, RPI = L::RPI;
+  constexpr int GROUPS = RT / RPI, PER = 2 * GROUPS / NW, LOADS = PER + 1;  // load instructions a tensor; a wave
+  constexpr int SLOTS = GROUPS * L::GROUP;
+  __shared__ u32x4 s_row[NS][2][SLOTS];        // Q, dO
+  __shared__ u32x4 s_pd[2][2][2][2][kDkvKeys]; // [step][p, ds][16 rows][lane half][key]: 8 rows
+  __shared__ float s_c[NS][NW][2][RT];         // -lse / scale, -delta (a copy a wave)
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 31, hq = lane >> 5;
   const int groups = p.B * p.Hkv, gi = blockIdx.x % groups;
   const int b = gi / p.Hkv, g = gi % p.Hkv;
   const DkvUnit un = dkv_unit(p, blockIdx.x / groups);
@@ -253,223 +267,251 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void dense_dkv_kernel(DenseP
   const int kb = __builtin_amdgcn_readfirstlane(un.kb);
   const DenseSeq sq = dense_seq(p, b);
   const int end = min(__builtin_amdgcn_readfirstlane(un.r1), sq.n * p.G), begin = __builtin_amdgcn_readfirstlane(un.r0);
-  const int j0 = kb * kDkvKeys, key = j0 + 32 * wave + lr;
+  const int j0 = kb * kDkvKeys;
   const int n = end > begin ? (end - begin + RT - 1) / RT : 0;
 
-  // ---- the keys' rows as second operands ----
-  bf16x8 kf[KS], vf[KS];
-  {
-    const bool live = key < sq.n;
-    const bf16* k = reinterpret_cast<const bf16*>(p.k) + b * p.k_sb + (live ? key * p.k_ss : 0) + g * p.k_sh + 8 * hq;
-    const bf16* v = reinterpret_cast<const bf16*>(p.v) + b * p.v_sb + (live ? key * p.v_ss : 0) + g * p.v_sh + 8 * hq;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const bf16x8 x = *reinterpret_cast<const bf16x8*>(k + 16 * s), y = *reinterpret_cast<const bf16x8*>(v + 16 * s);
-      kf[s] = live ? x : bf16x8{};
-      vf[s] = live ? y : bf16x8{};
-    }
-  }
-
   // ---- loads: rows begin + 32 i .. as (token, head) pairs that advance with the tiles ----
-  int lt[NI], lh[NI];
+  int lt_[PER], lh_[PER];
 #pragma unroll
-  for (int k = 0; k < NI; ++k) {
-    const int r = begin + (wave * NI + k) * RPI + lane / CH;
-    lt[k] = r / p.G;
-    lh[k] = r - lt[k] * p.G;
+  for (int k = 0; k < PER; ++k) {
+    const int r = begin + (wave * PER + k) % GROUPS * RPI + lane / CH;
+    lt_[k] = r / p.G;
+    lh_[k] = r - lt_[k] * p.G;
   }
-  const int dt = RT / p.G, dh = RT - dt * p.G;
-  const uint64_t qbase = (uint64_t)(uintptr_t)p.q + (uint64_t)(2 * (b * p.q_sb + g * p.G * p.q_sh));
-  const uint64_t obase = (uint64_t)(uintptr_t)p.dout + (uint64_t)(2 * (b * p.do_sb + g * p.G * p.do_sh));
+  const bool is_do = wave >= NW / 2;
+  const int dt = RT / p.G, dh_step = RT - dt * p.G;
+  const int64_t x_ss = 2 * (is_do ? p.do_ss : p.q_ss), x_sh = 2 * (is_do ? p.do_sh : p.q_sh);
+  const uint64_t xbase = is_do ? (uint64_t)(uintptr_t)p.dout + (uint64_t)(2 * (b * p.do_sb + g * p.G * p.do_sh))
+                               : (uint64_t)(uintptr_t)p.q + (uint64_t)(2 * (b * p.q_sb + g * p.G * p.q_sh));
   const int64_t r_all = ((int64_t)b * p.Hkv + g) * p.S * p.G;
   const int last_row = p.S * p.G - 1;
   auto load = [&](int i) {  // tile i, in order of i
-    const int st = i & (NS - 1);
+    const int st = i % NS;
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      const int q = wave * NI + k;
+    for (int k = 0; k < PER; ++k) {
+      const int q = (wave * PER + k) % GROUPS;
       const uint32_t c = 16u * (uint32_t)((lane % CH) ^ L::at(lane / CH));
-      const bool ok = i < n && lt[k] < sq.n;
-      const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
-      const uint64_t qa = ok ? qbase + (uint64_t)(2 * (lt[k] * p.q_ss + lh[k] * p.q_sh)) : zero;
-      const uint64_t oa = ok ? obase + (uint64_t)(2 * (lt[k] * p.do_ss + lh[k] * p.do_sh)) : zero;
-      dense_dma16(&s_row[st][0][q * L::GROUP], qa + c);
-      dense_dma16(&s_row[st][1][q * L::GROUP], oa + c);
-      lt[k] += dt;
-      lh[k] += dh;
-      if (lh[k] >= p.G) {
-        lh[k] -= p.G;
-        ++lt[k];
+      const bool ok = i < n && lt_[k] < sq.n;
+      const uint64_t a = ok ? xbase + (uint64_t)(lt_[k] * x_ss + lh_[k] * x_sh) : (uint64_t)(uintptr_t)kZeroRow;
+      dense_dma16(&s_row[st][is_do][q * L::GROUP], a + c);
+      lt_[k] += dt;
+      lh_[k] += dh_step;
+      if (lh_[k] >= p.G) {
+        lh_[k] -= p.G;
+        ++lt_[k];
       }
     }
     const int r = min(begin + i * RT + (lane & 31), last_row);
     dense_dma4(&s_c[st][wave][0][0], (uint64_t)(uintptr_t)((lane < 32 ? p.row_lse : p.row_delta) + r_all + r));
   };
-#pragma unroll
-  for (int i = 0; i < NS; ++i) load(i);
-
-  acc_t dk[OT], dv[OT];
-#pragma unroll
-  for (int o = 0; o < OT; ++o) dk[o] = dv[o] = acc_t{};
-
-  constexpr int FLIP = D == 128 ? 6 : 5;
-  const int l16 = lane & 15, trow = 4 * hq + (l16 >> 2), tc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-  const uint32_t kx = 16u * (uint32_t)L::at(lr), k0a = 16u * (uint32_t)(L::slot(lr, L::at(lr)) + hq);
-  const uint32_t tx = 16u * (uint32_t)(L::at(trow) ^ tc), t0a = 16u * (uint32_t)L::slot(trow, L::at(trow)) + (uint32_t)(l16 & 1) * 8u;
-  constexpr int NQ = 2 * KS, NM = NQ + 4 * OT;
-  // (i even: Q, odd: dO)
-  auto read_row = [&](uint32_t q, uint32_t o, uint32_t x, int i) {
-    const int c = i >> 1;
-    return lds_b128_at((i & 1 ? o : q) + (x ^ ((uint32_t)(D == 128 ? c >> 1 : c) << FLIP)) + (uint32_t)(D == 128 ? 32 * (c & 1) : 0));
+  // rows of tile i all see all keys of the block
+  auto whole = [&](int i) {
+    const int r0 = begin + i * RT, t0 = r0 / p.G, t1 = (r0 + RT - 1) / p.G;
+    return r0 + RT <= end && j0 + kDkvKeys - 1 <= t0 && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
   };
-  // dO transposed by 16 rows, then Q
-  auto read_t = [&](uint32_t q, uint32_t o, uint32_t x, int i) {
-    const uint32_t at = (i < 2 * OT ? o : q) + (x ^ (uint32_t)(64 * (i % OT))) + (uint32_t)L::rows(16 * (i / OT % 2));
-    const bf16x4 lo = lds_tr16_at(at), hi = lds_tr16_at(at + (uint32_t)L::rows(8));
-    return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-  // the accumulators' start values: the lane's rows 8 x + 4 hq + 0 .. 3 (no VALU for either)
-  auto start = [&](const float* c) {
-    acc_t a;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(c + 8 * x + 4 * hq);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[4 * x + e] = y[e];
+  // Between the steps: what the sums are about to read of a tile whose rows do not see all
+  // keys is cleared of infinities and NaN (0 times them would reach the keys they do not see).
+  auto clear = [&](int i) {
+    if (!whole(i)) {
+      clear_rows<D, NW>(s_row[i % NS][0], 0, wave, lane);
+      clear_rows<D, NW>(s_row[i % NS][1], 0, wave, lane);
     }
-    return a;
   };
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  dense_barrier();
-  acc_t sa, sb, da, db;
-  bf16x8 op[4];
-  {
-    const uint32_t q = lds_addr(s_row[0][0]) + k0a, o = lds_addr(s_row[0][1]) + k0a;
-    sa = start(s_c[0][wave][0]);
-    da = start(s_c[0][wave][1]);
+  auto next = [&]() {  // tile i + 2 has landed (behind it: i + 3), this step's are read
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    dense_barrier();
+  };
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const bf16x8 x = read_row(q, o, kx, i);
-      if (i & 1) da = M::mma(x, vf[i >> 1], da);
-      else sa = M::mma(x, kf[i >> 1], sa);
-    }
-    const uint32_t q1 = lds_addr(s_row[1][0]) + k0a, o1 = lds_addr(s_row[1][1]) + k0a;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) op[i] = read_row(q1, o1, kx, i);
-  }
+  for (int i = 0; i < 3; ++i) load(i);
 
-  auto step = [&](int i0, acc_t& cs, acc_t& cd, acc_t& ns, acc_t& nd) {
-    const int st = i0 & (NS - 1), st1 = (i0 + 1) & (NS - 1), st2 = (i0 + 2) & (NS - 1);
-    uint32_t xf = kx, tf = tx;
-    asm volatile("" : "+v"(xf), "+v"(tf));
-    const uint32_t qt = lds_addr(s_row[st][0]) + t0a, ot = lds_addr(s_row[st][1]) + t0a;
-    const uint32_t qn = lds_addr(s_row[st1][0]) + k0a, on = lds_addr(s_row[st1][1]) + k0a;
-    const uint32_t qn2 = lds_addr(s_row[st2][0]) + k0a, on2 = lds_addr(s_row[st2][1]) + k0a;
-    // rows that see all keys of the block, or not
-    const int r0 = begin + i0 * RT, t0 = r0 / p.G, t1 = (r0 + RT - 1) / p.G;
-    const bool whole = r0 + RT <= end && j0 + kDkvKeys - 1 <= t0 && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
-    uint32_t seen = ~0u;
-    if (!whole) {
-      clear_rows<D, NW>(s_row[st][0], 0, wave, lane);
-      clear_rows<D, NW>(s_row[st][1], 0, wave, lane);
-      // row 8 x + 4 hq + e of the tile sees the lane's key
-      seen = 0;
-      int t = (r0 + 4 * hq) / p.G, h = r0 + 4 * hq - t * p.G;
+  if (wave < 4) {
+    // ---- weights: rows 16 rh + .., keys 64 kg + .. ----
+    constexpr int KS = D / 32;
+    const int lt = lane & 15, hq = lane >> 4, kg = wave & 1, rh = wave >> 1;
+    bf16x8 kf[4][KS], vf[4][KS];
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const int r = r0 + 8 * (x >> 2) + 4 * hq + (x & 3);
-        seen |= (uint32_t)(r < end && dense_seen(p, key, t)) << (8 * (x >> 2) + (x & 3));
-        const int by = (x & 3) == 3 ? 5 : 1;
-        h += by;
-        while (h >= p.G) {
-          h -= p.G;
-          ++t;
+    for (int j = 0; j < 4; ++j) {
+      const int key = j0 + 64 * kg + 16 * j + lt;
+      const bool live = key < sq.n;
+      const bf16* k = reinterpret_cast<const bf16*>(p.k) + b * p.k_sb + (live ? key * p.k_ss : 0) + g * p.k_sh + 8 * hq;
+      const bf16* v = reinterpret_cast<const bf16*>(p.v) + b * p.v_sb + (live ? key * p.v_ss : 0) + g * p.v_sh + 8 * hq;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(k + 32 * s), y = *reinterpret_cast<const bf16x8*>(v + 32 * s);
+        kf[j][s] = live ? x : bf16x8{};
+        vf[j][s] = live ? y : bf16x8{};
+      }
+    }
+    const int row = 16 * rh + lt;
+    const uint32_t x0 = 16u * (uint32_t)(hq ^ L::at(row)), a0 = 16u * (uint32_t)L::slot(row, L::at(row));
+    f32x4 sa[4], da[4], sb[4], db[4];
+    auto products = [&](int i, f32x4 (&ns)[4], f32x4 (&nd)[4], auto between) {
+      const int st = i % NS;
+      const uint32_t q = lds_addr(s_row[st][0]) + a0, o = lds_addr(s_row[st][1]) + a0;
+      const f32x4 cs = *reinterpret_cast<const f32x4*>(&s_c[st][wave][0][16 * rh + 4 * hq]);
+      const f32x4 cd = *reinterpret_cast<const f32x4*>(&s_c[st][wave][1][16 * rh + 4 * hq]);
+      bf16x8 op[2][2];
+      op[0][0] = lds_b128_at(q + x0);
+      op[0][1] = lds_b128_at(o + x0);
+      each<8 * KS>([&](auto uc) {
+        constexpr int u = decltype(uc)::value, c = u / 8, w = (u >> 2) & 1, j = u & 3;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (u % 8 == 0 && c + 1 < KS) {
+          op[(c + 1) & 1][0] = lds_b128_at(q + (x0 ^ (uint32_t)(64 * (c + 1))));
+          op[(c + 1) & 1][1] = lds_b128_at(o + (x0 ^ (uint32_t)(64 * (c + 1))));
         }
-      }
-    }
-    bf16x8 pb[2], db2[2];
-    float ep = 0.f, es = 0.f;
-    ns = start(s_c[st1][wave][0]);
-    nd = start(s_c[st1][wave][1]);
-    each<NM>([&](auto ic) {
-      constexpr int i = decltype(ic)::value;
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (i < NQ) {
-        if constexpr (i & 1) nd = M::mma(op[i & 3], vf[i >> 1], nd);
-        else ns = M::mma(op[i & 3], kf[i >> 1], ns);
-      } else {
-        constexpr int u = i - NQ, o = u % OT, k = u / OT % 2;
-        if constexpr (u < 2 * OT) dv[o] = M::mma(op[i & 3], pb[k], dv[o]);
-        else dk[o] = M::mma(op[i & 3], db2[k], dk[o]);
-      }
-      if constexpr (i == NM - 4) {
-        // tile i0 + 2 has landed (behind it: i0 + 3), this one is read
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-        dense_barrier();
-      }
-      if constexpr (i + 4 < NQ) op[i & 3] = read_row(qn, on, xf, i + 4);
-      else if constexpr (i + 4 < NM) op[i & 3] = read_t(qt, ot, tf, i + 4 - NQ);
-      else op[i & 3] = read_row(qn2, on2, xf, i + 4 - NM);
-      // p and ds, evenly before the first sums
-      each<16>([&](auto ec) {
-        constexpr int e = decltype(ec)::value;
-        if constexpr (e * (NQ + OT) / 16 == i) {
-          const bool ok = (seen >> (8 * (e >> 2) + (e & 3))) & 1;
-          float w = __builtin_amdgcn_exp2f(cs[e] * p.scale_log2), x = w * cd[e];
-          w = ok ? w : 0.f;
-          x = ok ? x : 0.f;
-          if constexpr (e & 1) {
-            pb[e >> 3][(e & 7) - 1] = (bf16)ep;
-            pb[e >> 3][e & 7] = (bf16)w;
-            db2[e >> 3][(e & 7) - 1] = (bf16)es;
-            db2[e >> 3][e & 7] = (bf16)x;
-          }
-          ep = w;
-          es = x;
-        }
+        if constexpr (w == 0) ns[j] = M16::mma(op[c & 1][0], kf[j][c], c == 0 ? cs : ns[j]);
+        else nd[j] = M16::mma(op[c & 1][1], vf[j][c], c == 0 ? cd : nd[j]);
+        between(uc);
       });
-      if constexpr (i == NM - 2) load(i0 + 4);
-    });
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  int i = 0;
-  for (; i + 1 < n; i += 2) {
-    step(i, sa, da, sb, db);
-    step(i + 1, sb, db, sa, da);
-  }
-  if (i < n) step(i, sa, da, sb, db);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-
-  // ---- results: the lane's key, dims 32 o + 8 x + 4 hq + 0 .. 3 ----
-  if (un.nc > 1) {
-    float* out = p.dkv_part + (((int64_t)gi * p.dkv_parts + un.part + un.c) * kDkvKeys + 32 * wave + lr) * (2 * D);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    dense_barrier();
+    products(0, sa, da, [](auto) {});
+    auto step = [&](int i, f32x4 (&cs)[4], f32x4 (&cd)[4], f32x4 (&ns)[4], f32x4 (&nd)[4]) {
+      load(i + 3);
+      if (i > 0) clear(i - 1);
+      if (!whole(i)) {
+        int t = (begin + i * RT + 16 * rh + 4 * hq) / p.G, h = begin + i * RT + 16 * rh + 4 * hq - t * p.G;
 #pragma unroll
-    for (int o = 0; o < OT; ++o)
+        for (int e = 0; e < 4; ++e) {
+          const bool in = begin + i * RT + 16 * rh + 4 * hq + e < end;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int d = 32 * o + 8 * x + 4 * hq;
-        *reinterpret_cast<f32x4*>(out + d) = f32x4{dk[o][4 * x], dk[o][4 * x + 1], dk[o][4 * x + 2], dk[o][4 * x + 3]};
-        *reinterpret_cast<f32x4*>(out + D + d) = f32x4{dv[o][4 * x], dv[o][4 * x + 1], dv[o][4 * x + 2], dv[o][4 * x + 3]};
+          for (int j = 0; j < 4; ++j) {
+            const bool ok = in && dense_seen(p, j0 + 64 * kg + 16 * j + lt, t);
+            // (do.v that is no number makes the weight none: its row is cleared for the sums)
+            cs[j][e] = ok ? fmaf(0.f, cd[j][e], cs[j][e]) : kNegInf;
+            cd[j][e] = ok ? cd[j][e] : 0.f;
+          }
+          if (++h == p.G) {
+            h = 0;
+            ++t;
+          }
+        }
+        asm volatile("" : "+v"(cs[0]), "+v"(cs[1]), "+v"(cs[2]), "+v"(cs[3]), "+v"(cd[0]), "+v"(cd[1]), "+v"(cd[2]), "+v"(cd[3]));
       }
+      char* const out = reinterpret_cast<char*>(&s_pd[i & 1][0][rh][hq & 1][64 * kg + lt]) + 8 * (hq >> 1);
+      constexpr int WHICH = (int)sizeof(s_pd[0][0]);
+      bf16x4 pw, dw;
+      products(i + 1, ns, nd, [&](auto uc) {
+        constexpr int u = decltype(uc)::value, NU = 8 * KS;
+        each<16>([&](auto ec) {
+          constexpr int x = decltype(ec)::value, j = x >> 2, e = x & 3;
+          if constexpr (x * (NU - 2) / 16 == u) {
+            const float w = __builtin_amdgcn_exp2f(cs[j][e] * p.scale_log2);
+            pw[e] = (bf16)w;
+            dw[e] = (bf16)(w * cd[j][e]);
+            if constexpr (e == 3) {
+              *reinterpret_cast<bf16x4*>(out + 16 * 16 * j) = pw;
+              *reinterpret_cast<bf16x4*>(out + WHICH + 16 * 16 * j) = dw;
+            }
+          }
+        });
+      });
+      next();
+    };
+    int i = 0;
+    for (; i + 1 < n; i += 2) {
+      step(i, sa, da, sb, db);
+      step(i + 1, sb, db, sa, da);
+    }
+    if (i < n) step(i, sa, da, sb, db);
+    if (n > 0) clear(n - 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     return;
   }
-  if (key >= p.S) return;
-  bf16* ok = reinterpret_cast<bf16*>(p.dk) + b * p.dk_sb + key * p.dk_ss + g * p.dk_sh;
-  bf16* ov = reinterpret_cast<bf16*>(p.dv) + b * p.dv_sb + key * p.dv_ss + g * p.dv_sh;
+
+  // ---- sums: keys 64 kg + 32 m + .., dims DW dh + .. ----
+  constexpr int DW = D / 2, DT = DW / 32;
+  const int lr = lane & 31, hq = lane >> 5, kg = wave & 1, dh = (wave >> 1) & 1;
+  f32x16 dk[DT][2], dv[DT][2];
 #pragma unroll
-  for (int o = 0; o < OT; ++o)
+  for (int o = 0; o < DT; ++o)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      bf16x4 a, c;
+    for (int m = 0; m < 2; ++m) dk[o][m] = dv[o][m] = f32x16{};
+  const int l16 = lane & 15, trow = 4 * hq + (l16 >> 2), tc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+  const uint32_t tx = 16u * (uint32_t)(L::at(trow) ^ tc), t0a = 16u * (uint32_t)L::slot(trow, L::at(trow)) + (uint32_t)(l16 & 1) * 8u;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  dense_barrier();
+  for (int i = 0; i <= n; ++i) {  // (step 0 has no weights yet)
+    if (i < n) load(i + 3);
+    if (i > 0) {
+      clear(i - 1);
+      const int st = (i - 1) % NS;
+      const uint32_t q = lds_addr(s_row[st][0]) + t0a, o = lds_addr(s_row[st][1]) + t0a;
+      const uint32_t pd = lds_addr(&s_pd[(i - 1) & 1][0][0][hq][64 * kg + lr]);
+      constexpr int WHICH = (int)sizeof(s_pd[0][0]), HALF = (int)sizeof(s_pd[0][0][0]);
+      // products u: [dv, dk][16 rows][32 dims][32 keys]
+      constexpr int NU = 2 * 2 * DT;
+      auto read_t = [&](int u) {
+        const int which = u / (2 * DT), ks = u / DT % 2, t = u % DT;
+        const uint32_t at = (which ? q : o) + (tx ^ (uint32_t)(2 * (DW * dh + 32 * t))) + (uint32_t)L::rows(16 * ks);
+        const bf16x4 lo = lds_tr16_at(at), hi = lds_tr16_at(at + (uint32_t)L::rows(8));
+        return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+      auto read_w = [&](int u, int m) {
+        return lds_b128_at(pd + (uint32_t)(u / (2 * DT) * WHICH + u / DT % 2 * HALF + 32 * 16 * m));
+      };
+      bf16x8 a[3], w[2][2];
+      a[0] = read_t(0);
+      a[1] = read_t(1);
+      w[0][0] = read_w(0, 0);
+      w[0][1] = read_w(0, 1);
+      each<NU>([&](auto uc) {
+        constexpr int u = decltype(uc)::value, which = u / (2 * DT), t = u % DT, k = u / DT;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (u + 2 < NU) a[(u + 2) % 3] = read_t(u + 2);
+        if constexpr (t == 0 && u + DT < NU) {
+          w[(k + 1) & 1][0] = read_w(u + DT, 0);
+          w[(k + 1) & 1][1] = read_w(u + DT, 1);
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = (bf16)(dk[o][4 * x + e] * p.scale);
-        c[e] = (bf16)dv[o][4 * x + e];
-      }
-      const int d = 32 * o + 8 * x + 4 * hq;
-      *reinterpret_cast<bf16x4*>(ok + d) = a;
-      *reinterpret_cast<bf16x4*>(ov + d) = c;
+        for (int m = 0; m < 2; ++m) {
+          if constexpr (which == 0) dv[t][m] = M::mma(a[u % 3], w[k & 1][m], dv[t][m]);
+          else dk[t][m] = M::mma(a[u % 3], w[k & 1][m], dk[t][m]);
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (i < n) next();
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // ---- results: the lane's keys, dims DW dh + 32 o + 8 x + 4 hq + 0 .. 3 ----
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int in = 64 * kg + 32 * m + lr, key = j0 + in;
+    if (un.nc > 1) {
+      float* out = p.dkv_part + (((int64_t)gi * p.dkv_parts + un.part + un.c) * kDkvKeys + in) * (2 * D);
+#pragma unroll
+      for (int o = 0; o < DT; ++o)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int d = DW * dh + 32 * o + 8 * x + 4 * hq;
+          *reinterpret_cast<f32x4*>(out + d) = f32x4{dk[o][m][4 * x], dk[o][m][4 * x + 1], dk[o][m][4 * x + 2], dk[o][m][4 * x + 3]};
+          *reinterpret_cast<f32x4*>(out + D + d) = f32x4{dv[o][m][4 * x], dv[o][m][4 * x + 1], dv[o][m][4 * x + 2], dv[o][m][4 * x + 3]};
+        }
+      continue;
+    }
+    if (key >= p.S) continue;
+    bf16* ok = reinterpret_cast<bf16*>(p.dk) + b * p.dk_sb + key * p.dk_ss + g * p.dk_sh;
+    bf16* ov = reinterpret_cast<bf16*>(p.dv) + b * p.dv_sb + key * p.dv_ss + g * p.dv_sh;
+#pragma unroll
+    for (int o = 0; o < DT; ++o)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        bf16x4 a, c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = (bf16)(dk[o][m][4 * x + e] * p.scale);
+          c[e] = (bf16)dv[o][m][4 * x + e];
+        }
+        const int d = DW * dh + 32 * o + 8 * x + 4 * hq;
+        *reinterpret_cast<bf16x4*>(ok + d) = a;
+        *reinterpret_cast<bf16x4*>(ov + d) = c;
+      }
+  }
 }
 
 // The chunks of key blocks that have several, added in order: 4 dims of a key a lane.
@@ -507,7 +549,7 @@ __global__ __launch_bounds__(256) void dense_dkv_join_kernel(DenseParams p) {
 template <int D>
 void launch(const DenseParams& p, int units, hipStream_t s) {
   dense_dq_kernel<D><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv), 512, 0, s>>>(p);
-  dense_dkv_kernel<D><<<(unsigned)((int64_t)units * p.B * p.Hkv), 256, 0, s>>>(p, units);
+  dense_dkv_kernel<D><<<(unsigned)((int64_t)units * p.B * p.Hkv), 512, 0, s>>>(p);
   if (p.dkv_parts > 0)
     dense_dkv_join_kernel<D><<<dim3((unsigned)((p.S + kDkvKeys - 1) / kDkvKeys * p.B * p.Hkv), 4), 256, 0, s>>>(p);
 }
