@@ -226,32 +226,52 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
     pl.fits = groups * nrb * dims * 256 < most && groups * (((int64_t)p.S + 63) / 64) * dims * 256 < most;
     return pl;
   }
-  // Key blocks' rows in chunks, so that there are some units for every CU and none is much
-  // longer than the others: without a window the first keys are seen by all rows, the last
-  // by few, and the first tokens of a window by all of them.
+  // Key blocks' rows in chunks.  Without a window the first keys are seen by all rows, the
+  // last by few; with one, the first tokens by all of them.  Blocks stay whole where
+  // there are three or more for two CUs, but for some that are cut in five, for the units
+  // left over from whole rounds of 256 (8192 tokens, window 1024: 0.97 of the CUs' time
+  // used for 0.84); else every block is cut in chunks of half a CU's share (with the longest
+  // first 0.97).  A partial sum costs 128 keys of float32, written and read; a chunk of fewer
+  // than 512 rows is mostly its start.
   const int64_t nkb = ((int64_t)p.S + kDkvKeys - 1) / kDkvKeys;
   auto block_rows = [&](int64_t kb) {
     const int64_t j0 = kb * kDkvKeys, t1 = j0 < p.first ? p.S : j0 + kDkvKeys - 1 + p.window;
     return ((t1 < p.S ? t1 : (int64_t)p.S) - j0) * p.G;
   };
-  int64_t total = 0;
-  for (int64_t kb = 0; kb < nkb; ++kb) total += block_rows(kb);
-  constexpr int64_t kUnits = 768, kLeast = 512;  // three a CU; a chunk of fewer rows is mostly its start
-  int64_t chunk = (total * groups / kUnits + 31) / 32 * 32;
-  if (chunk < kLeast) chunk = kLeast;
-  // (blocks up to a quarter over stay whole)
-  int64_t units = 0, parts = 0, widest = 0;
+  constexpr int64_t kCus = 256, kLeast = 512;
+  auto up = [&](int64_t x) { return (x < kLeast ? kLeast : x + 31) / 32 * 32; };
+  int64_t total = 0, widest = 0;  // (of the blocks behind the first tokens)
   for (int64_t kb = 0; kb < nkb; ++kb) {
     const int64_t r = block_rows(kb);
-    if (r <= chunk + chunk / 4 && r > widest) widest = r;
+    total += r;
+    if (kb * kDkvKeys >= p.first && r > widest) widest = r;
   }
-  if (widest > chunk) chunk = (widest + 31) / 32 * 32;
-  for (int64_t kb = 0; kb < nkb; ++kb) {
-    const int64_t nc = (block_rows(kb) + chunk - 1) / chunk;
-    units += nc;
-    parts += nc > 1 ? nc : 0;
+  const int64_t share = total * groups / kCus;
+  const bool cut = 3 * widest > 2 * share;
+  const int64_t chunk = up(cut ? share / 2 : widest);
+  int64_t units = 0, parts = 0;
+  pl.cut0 = pl.cut1 = 0;
+  pl.cut_chunk = (int)up(chunk / 5);
+  auto count = [&]() {
+    units = parts = 0;
+    for (int64_t kb = 0; kb < nkb; ++kb) {
+      const int64_t c = kb >= pl.cut0 && kb < pl.cut1 ? pl.cut_chunk : chunk, nc = (block_rows(kb) + c - 1) / c;
+      units += nc;
+      parts += nc > 1 ? nc : 0;
+    }
+  };
+  count();
+  const int64_t left = units * groups % kCus;
+  if (!cut && left > 0 && 3 * left < 2 * kCus) {
+    const int64_t from = ((int64_t)p.first + kDkvKeys - 1) / kDkvKeys;
+    const int64_t blocks = (left + groups - 1) / groups;
+    if (from + blocks < nkb) {
+      pl.cut0 = (int)from;
+      pl.cut1 = (int)(from + blocks);
+      count();
+    }
   }
-  pl.chunk = (int)(chunk < (int64_t)1 << 30 ? chunk : (int64_t)1 << 30);
+  pl.chunk = (int)chunk;
   pl.units = (int)units;
   pl.parts = (int)parts;
   pl.dkv_bytes = (size_t)(groups * parts) * kDkvKeys * 2 * p.Dqk * sizeof(float);
@@ -274,6 +294,9 @@ hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int d
   q.slots = p.B * (int)(((int64_t)p.S * p.G + q.rows - 1) / q.rows);
   set_launch(p, q);
   p.chunk = pl.chunk;
+  p.cut0 = pl.cut0;
+  p.cut1 = pl.cut1;
+  p.cut_chunk = pl.cut_chunk;
   p.dkv_parts = pl.parts;
   if (pl.mfma) launch_dense_bwd_mfma(p, pl.units, s);
   else launch_dense_bwd_any(p, dtype, s);

@@ -200,12 +200,59 @@ struct DkvUnit {
 __device__ __forceinline__ int dkv_tokens(const DenseParams& p, int j0) {  // tokens that see a key of the block at j0
   return j0 < p.first ? p.S : (int)min((int64_t)p.S, (int64_t)j0 + kDkvKeys - 1 + p.window);
 }
-__device__ __forceinline__ int dkv_chunks(const DenseParams& p, int kb) {
-  const int j0 = kb * kDkvKeys;
-  const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
-  return (int)((rows + p.chunk - 1) / p.chunk);
+__device__ __forceinline__ int dkv_chunk(const DenseParams& p, int kb) {
+  return kb >= p.cut0 && kb < p.cut1 ? p.cut_chunk : p.chunk;
 }
-// of unit u of a (sequence, kv head)
+__device__ __forceinline__ int dkv_chunks(const DenseParams& p, int kb) {
+  const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
+  const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
+  return (int)((rows + chunk - 1) / chunk);
+}
+// Unit u of a (sequence, kv head): the longest first, so that the card's last ones are short
+// (up to 256 key blocks: a thread for each block's whole chunks and one for its rest).
+struct DkvSort {
+  int size[512], num[512], nc[256];
+  int unit[6];
+};
+__device__ __forceinline__ DkvUnit dkv_unit_sorted(const DenseParams& p, int u, DkvSort& sort) {
+  const int nkb = (p.S + kDkvKeys - 1) / kDkvKeys, tid = threadIdx.x, kb = tid >> 1;
+  int size = 0, num = 0, nc = 0;
+  if (kb < nkb) {
+    const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
+    const int rows = (dkv_tokens(p, j0) - j0) * p.G, whole = rows / chunk, rest = rows - whole * chunk;
+    nc = whole + (rest > 0 ? 1 : 0);
+    size = tid & 1 ? rest : chunk;
+    num = tid & 1 ? (rest > 0 ? 1 : 0) : whole;
+    if ((tid & 1) == 0) sort.nc[kb] = nc;
+  }
+  sort.size[tid] = size;
+  sort.num[tid] = num;
+  if (tid < 6) sort.unit[tid] = -1;
+  dense_barrier();
+  if (num > 0) {
+    int first = 0;
+    for (int i = 0; i < 2 * nkb; ++i) {
+      const int s = sort.size[i];
+      first += s > size || (s == size && i < tid) ? sort.num[i] : 0;
+    }
+    if (u >= first && u < first + num) {
+      int part = 0;
+      for (int k = 0; k < kb; ++k) part += sort.nc[k] > 1 ? sort.nc[k] : 0;
+      const int c = tid & 1 ? nc - 1 : u - first, j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
+      sort.unit[0] = kb;
+      sort.unit[1] = j0 * p.G + c * chunk;
+      sort.unit[2] = (int)min((int64_t)j0 * p.G + (int64_t)(c + 1) * chunk, (int64_t)dkv_tokens(p, j0) * p.G);
+      sort.unit[3] = part;
+      sort.unit[4] = nc;
+      sort.unit[5] = c;
+    }
+  }
+  dense_barrier();
+  const DkvUnit x{sort.unit[0], sort.unit[1], sort.unit[2], sort.unit[3], sort.unit[4], sort.unit[5]};
+  dense_barrier();  // (its place in LDS is loaded over)
+  return x;
+}
+// ... in order of the keys
 __device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
   const int lane = threadIdx.x & 63, nkb = (p.S + kDkvKeys - 1) / kDkvKeys;
   int before = 0, parts = 0;
@@ -230,8 +277,9 @@ __device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
       x.c = u - __builtin_amdgcn_readlane(first, w);
       x.part = __builtin_amdgcn_readlane(parts + pin - np, w);
       const int j0 = x.kb * kDkvKeys;
-      x.r0 = j0 * p.G + x.c * p.chunk;
-      x.r1 = (int)min((int64_t)x.r0 + p.chunk, (int64_t)dkv_tokens(p, j0) * p.G);
+      const int chunk = dkv_chunk(p, x.kb);
+      x.r0 = j0 * p.G + x.c * chunk;
+      x.r1 = (int)min((int64_t)x.r0 + chunk, (int64_t)dkv_tokens(p, j0) * p.G);
       return x;
     }
     before += __builtin_amdgcn_readlane(incl, 63);
@@ -251,22 +299,25 @@ template <int D>
 __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   typedef Tile<D> L;
   typedef Mfma<16> M16;
-  constexpr int NW = 8, RT = 32, NS = 5, CH = D / 8, RPI = L::RPI;
+  constexpr int NW = 8, RT = 32, NS = 7, CH = D / 8, RPI = L::RPI;
   constexpr int GROUPS = RT / RPI, PER = 2 * GROUPS / NW, LOADS = PER + 1;  // load instructions a tensor; a wave
   constexpr int SLOTS = GROUPS * L::GROUP;
   __shared__ u32x4 s_row[NS][2][SLOTS];        // Q, dO
   __shared__ u32x4 s_pd[2][2][2][2][kDkvKeys]; // [step][p, ds][16 rows][lane half][key]: 8 rows
-  __shared__ float s_c[NS][NW][2][RT];         // -lse / scale, -delta (a copy a wave)
+  __shared__ float s_c[NS][NW / 2][2][RT];     // -lse / scale, -delta (a copy for each wave of weights)
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = p.B * p.Hkv, gi = blockIdx.x % groups;
   const int b = gi / p.Hkv, g = gi % p.Hkv;
-  const DkvUnit un = dkv_unit(p, blockIdx.x / groups);
-  if (un.kb < 0) return;
+  static_assert(sizeof(DkvSort) <= sizeof(s_row), "the units are sorted where the rows come later");
+  const bool sorted = p.S <= 256 * kDkvKeys;
+  const DkvUnit un = sorted ? dkv_unit_sorted(p, blockIdx.x / groups, *reinterpret_cast<DkvSort*>(s_row)) : dkv_unit(p, blockIdx.x / groups);
   const int kb = __builtin_amdgcn_readfirstlane(un.kb);
+  if (kb < 0) return;
   const DenseSeq sq = dense_seq(p, b);
   const int end = min(__builtin_amdgcn_readfirstlane(un.r1), sq.n * p.G), begin = __builtin_amdgcn_readfirstlane(un.r0);
+  const int nc = __builtin_amdgcn_readfirstlane(un.nc), part = __builtin_amdgcn_readfirstlane(un.part + un.c);
   const int j0 = kb * kDkvKeys;
   const int n = end > begin ? (end - begin + RT - 1) / RT : 0;
 
@@ -285,8 +336,10 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
                                : (uint64_t)(uintptr_t)p.q + (uint64_t)(2 * (b * p.q_sb + g * p.G * p.q_sh));
   const int64_t r_all = ((int64_t)b * p.Hkv + g) * p.S * p.G;
   const int last_row = p.S * p.G - 1;
+  int ls = 0;               // the next tile's place
   auto load = [&](int i) {  // tile i, in order of i
-    const int st = i % NS;
+    const int st = ls;
+    ls = ls == NS - 1 ? 0 : ls + 1;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int q = (wave * PER + k) % GROUPS;
@@ -302,27 +355,47 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
       }
     }
     const int r = min(begin + i * RT + (lane & 31), last_row);
-    dense_dma4(&s_c[st][wave][0][0], (uint64_t)(uintptr_t)((lane < 32 ? p.row_lse : p.row_delta) + r_all + r));
+    dense_dma4(&s_c[st][wave & 3][0][0], (uint64_t)(uintptr_t)((lane < 32 ? p.row_lse : p.row_delta) + r_all + r));
   };
-  // rows of tile i all see all keys of the block
-  auto whole = [&](int i) {
-    const int r0 = begin + i * RT, t0 = r0 / p.G, t1 = (r0 + RT - 1) / p.G;
-    return r0 + RT <= end && j0 + kDkvKeys - 1 <= t0 && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
+  // The tile a step is at: its number, place, first row's token and head (divisions are long).
+  struct At {
+    int i, st, t, h;
+    bool whole;  // its rows all see all keys of the block
   };
+  const int dt31 = (RT - 1) / p.G, dh31 = RT - 1 - dt31 * p.G;
+  auto settle = [&](At& a) {
+    const int t1 = a.t + dt31 + (a.h + dh31 >= p.G ? 1 : 0);
+    a.whole = begin + a.i * RT + RT <= end && j0 + kDkvKeys - 1 <= a.t && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
+  };
+  auto advance = [&](At& a) {
+    ++a.i;
+    a.st = a.st == NS - 1 ? 0 : a.st + 1;
+    a.t += dt;
+    a.h += dh_step;
+    if (a.h >= p.G) {
+      a.h -= p.G;
+      ++a.t;
+    }
+    settle(a);
+  };
+  At at{0, 0, begin / p.G, 0, false};
+  at.h = begin - at.t * p.G;
+  settle(at);
   // Between the steps: what the sums are about to read of a tile whose rows do not see all
   // keys is cleared of infinities and NaN (0 times them would reach the keys they do not see).
-  auto clear = [&](int i) {
-    if (!whole(i)) {
-      clear_rows<D, NW>(s_row[i % NS][0], 0, wave, lane);
-      clear_rows<D, NW>(s_row[i % NS][1], 0, wave, lane);
+  auto clear = [&](int st, bool is_whole) {
+    if (!is_whole) {
+      clear_rows<D, NW>(s_row[st][0], 0, wave, lane);
+      clear_rows<D, NW>(s_row[st][1], 0, wave, lane);
     }
   };
-  auto next = [&]() {  // tile i + 2 has landed (behind it: i + 3), this step's are read
+  // At the end of step i: tile i + 3 has landed (behind it i + 4), what the step read is read.
+  auto next = [&]() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
     dense_barrier();
   };
 #pragma unroll
-  for (int i = 0; i < 3; ++i) load(i);
+  for (int i = 0; i < 4; ++i) load(i);
 
   if (wave < 4) {
     // ---- weights: rows 16 rh + .., keys 64 kg + .. ----
@@ -345,38 +418,50 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
     const int row = 16 * rh + lt;
     const uint32_t x0 = 16u * (uint32_t)(hq ^ L::at(row)), a0 = 16u * (uint32_t)L::slot(row, L::at(row));
     f32x4 sa[4], da[4], sb[4], db[4];
-    auto products = [&](int i, f32x4 (&ns)[4], f32x4 (&nd)[4], auto between) {
-      const int st = i % NS;
+    // the products of the tile at place st, whose first operands are in op; then those of the next
+    bf16x8 op[2][2];
+    f32x4 c0, c1;  // its rows' start values
+    auto first = [&](int st) {
+      op[0][0] = lds_b128_at(lds_addr(s_row[st][0]) + a0 + x0);
+      op[0][1] = lds_b128_at(lds_addr(s_row[st][1]) + a0 + x0);
+      c0 = *reinterpret_cast<const f32x4*>(&s_c[st][wave][0][16 * rh + 4 * hq]);
+      c1 = *reinterpret_cast<const f32x4*>(&s_c[st][wave][1][16 * rh + 4 * hq]);
+    };
+    auto products = [&](int st, f32x4 (&ns)[4], f32x4 (&nd)[4], auto between) {
+      uint32_t x = x0;
+      asm volatile("" : "+v"(x));
       const uint32_t q = lds_addr(s_row[st][0]) + a0, o = lds_addr(s_row[st][1]) + a0;
-      const f32x4 cs = *reinterpret_cast<const f32x4*>(&s_c[st][wave][0][16 * rh + 4 * hq]);
-      const f32x4 cd = *reinterpret_cast<const f32x4*>(&s_c[st][wave][1][16 * rh + 4 * hq]);
-      bf16x8 op[2][2];
-      op[0][0] = lds_b128_at(q + x0);
-      op[0][1] = lds_b128_at(o + x0);
       each<8 * KS>([&](auto uc) {
         constexpr int u = decltype(uc)::value, c = u / 8, w = (u >> 2) & 1, j = u & 3;
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (u % 8 == 0 && c + 1 < KS) {
-          op[(c + 1) & 1][0] = lds_b128_at(q + (x0 ^ (uint32_t)(64 * (c + 1))));
-          op[(c + 1) & 1][1] = lds_b128_at(o + (x0 ^ (uint32_t)(64 * (c + 1))));
+          op[(c + 1) & 1][0] = lds_b128_at(q + (x ^ (uint32_t)(64 * (c + 1))));
+          op[(c + 1) & 1][1] = lds_b128_at(o + (x ^ (uint32_t)(64 * (c + 1))));
         }
-        if constexpr (w == 0) ns[j] = M16::mma(op[c & 1][0], kf[j][c], c == 0 ? cs : ns[j]);
-        else nd[j] = M16::mma(op[c & 1][1], vf[j][c], c == 0 ? cd : nd[j]);
+        if constexpr (w == 0) ns[j] = M16::mma(op[c & 1][0], kf[j][c], c == 0 ? c0 : ns[j]);
+        else nd[j] = M16::mma(op[c & 1][1], vf[j][c], c == 0 ? c1 : nd[j]);
         between(uc);
       });
       __builtin_amdgcn_sched_barrier(0);
     };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     dense_barrier();
+    first(0);
     products(0, sa, da, [](auto) {});
-    auto step = [&](int i, f32x4 (&cs)[4], f32x4 (&cd)[4], f32x4 (&ns)[4], f32x4 (&nd)[4]) {
-      load(i + 3);
-      if (i > 0) clear(i - 1);
-      if (!whole(i)) {
-        int t = (begin + i * RT + 16 * rh + 4 * hq) / p.G, h = begin + i * RT + 16 * rh + 4 * hq - t * p.G;
+    first(1);
+    At ahead = at;  // (tile i + 1)
+    advance(ahead);
+    int prev_st = 0;
+    bool prev_whole = true;
+    auto step = [&](f32x4 (&cs)[4], f32x4 (&cd)[4], f32x4 (&ns)[4], f32x4 (&nd)[4]) {
+      load(at.i + 4);
+      if (at.i > 0) clear(prev_st, prev_whole);
+      if (!at.whole) {
+        const int r0 = begin + at.i * RT + 16 * rh + 4 * hq;
+        int t = r0 / p.G, h = r0 - t * p.G;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool in = begin + i * RT + 16 * rh + 4 * hq + e < end;
+          const bool in = r0 + e < end;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const bool ok = in && dense_seen(p, j0 + 64 * kg + 16 * j + lt, t);
@@ -391,10 +476,10 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
         }
         asm volatile("" : "+v"(cs[0]), "+v"(cs[1]), "+v"(cs[2]), "+v"(cs[3]), "+v"(cd[0]), "+v"(cd[1]), "+v"(cd[2]), "+v"(cd[3]));
       }
-      char* const out = reinterpret_cast<char*>(&s_pd[i & 1][0][rh][hq & 1][64 * kg + lt]) + 8 * (hq >> 1);
+      char* const out = reinterpret_cast<char*>(&s_pd[at.i & 1][0][rh][hq & 1][64 * kg + lt]) + 8 * (hq >> 1);
       constexpr int WHICH = (int)sizeof(s_pd[0][0]);
       bf16x4 pw, dw;
-      products(i + 1, ns, nd, [&](auto uc) {
+      products(ahead.st, ns, nd, [&](auto uc) {
         constexpr int u = decltype(uc)::value, NU = 8 * KS;
         each<16>([&](auto ec) {
           constexpr int x = decltype(ec)::value, j = x >> 2, e = x & 3;
@@ -409,15 +494,20 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
           }
         });
       });
+      prev_st = at.st;
+      prev_whole = at.whole;
+      at = ahead;
+      advance(ahead);
+      first(ahead.st);  // (tile i + 2, which had landed before this step)
       next();
     };
     int i = 0;
     for (; i + 1 < n; i += 2) {
-      step(i, sa, da, sb, db);
-      step(i + 1, sb, db, sa, da);
+      step(sa, da, sb, db);
+      step(sb, db, sa, da);
     }
-    if (i < n) step(i, sa, da, sb, db);
-    if (n > 0) clear(n - 1);
+    if (i < n) step(sa, da, sb, db);
+    if (n > 0) clear(prev_st, prev_whole);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     return;
   }
@@ -434,13 +524,13 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   const uint32_t tx = 16u * (uint32_t)(L::at(trow) ^ tc), t0a = 16u * (uint32_t)L::slot(trow, L::at(trow)) + (uint32_t)(l16 & 1) * 8u;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   dense_barrier();
-  for (int i = 0; i <= n; ++i) {  // (step 0 has no weights yet)
-    if (i < n) load(i + 3);
+  for (int i = 0; i <= n; ++i) {  // (step 0 has no weights yet; at: tile i - 1)
+    if (i < n) load(i + 4);
     if (i > 0) {
-      clear(i - 1);
-      const int st = (i - 1) % NS;
+      clear(at.st, at.whole);
+      const int st = at.st;
       const uint32_t q = lds_addr(s_row[st][0]) + t0a, o = lds_addr(s_row[st][1]) + t0a;
-      const uint32_t pd = lds_addr(&s_pd[(i - 1) & 1][0][0][hq][64 * kg + lr]);
+      const uint32_t pd = lds_addr(&s_pd[at.i & 1][0][0][hq][64 * kg + lr]);
       constexpr int WHICH = (int)sizeof(s_pd[0][0]), HALF = (int)sizeof(s_pd[0][0][0]);
       // products u: [dv, dk][16 rows][32 dims][32 keys]
       constexpr int NU = 2 * 2 * DT;
@@ -473,6 +563,7 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
         }
       });
       __builtin_amdgcn_sched_barrier(0);
+      advance(at);
     }
     if (i < n) next();
   }
@@ -482,8 +573,8 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     const int in = 64 * kg + 32 * m + lr, key = j0 + in;
-    if (un.nc > 1) {
-      float* out = p.dkv_part + (((int64_t)gi * p.dkv_parts + un.part + un.c) * kDkvKeys + in) * (2 * D);
+    if (nc > 1) {
+      float* out = p.dkv_part + (((int64_t)gi * p.dkv_parts + part) * kDkvKeys + in) * (2 * D);
 #pragma unroll
       for (int o = 0; o < DT; ++o)
 #pragma unroll

@@ -158,7 +158,8 @@ struct DenseParams {
   float* row_delta;
   bool row_neg;
   float* dkv_part;           // [B Hkv][dkv_parts][kDkvKeys][2 D] partial dK | dV of key blocks cut in chunks
-  int chunk, dkv_parts;      // query rows a chunk; partials a kv head
+  int chunk, cut0, cut1, cut_chunk;  // query rows a chunk; of the key blocks [cut0, cut1)
+  int dkv_parts;             // partials a kv head
 };
 constexpr int kDenseUnits = 256;  // row blocks of a launch that is cut into ranges, at most
 struct DensePlan {
@@ -175,7 +176,7 @@ hipError_t launch_dense(const DenseParams& p, const DensePlan& pl, int dtype, in
 constexpr int kDkvKeys = 128;  // keys a block of the dk / dv kernel
 struct DenseBwdPlan {
   size_t row_bytes, dkv_bytes;  // row_lse + row_delta; partial dK | dV
-  int chunk, units, parts;      // of the dk / dv kernel: rows a chunk, units and partials a kv head
+  int chunk, cut0, cut1, cut_chunk, units, parts;  // of the dk / dv kernel: as above; units and partials a kv head
   bool mfma, fits;
   size_t workspace() const { return row_bytes + dkv_bytes; }
 };
