@@ -216,7 +216,8 @@ hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, i
 DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   DenseBwdPlan pl{};
   const size_t rows = (size_t)p.B * p.Hkv * p.S * p.G;
-  pl.row_bytes = 2 * ((rows * sizeof(float) + 255) / 256 * 256);
+  // (each a row tile longer: the matrix kernels read whole tiles of them)
+  pl.row_bytes = 2 * ((rows * sizeof(float) + 128 + 255) / 256 * 256);
   const int64_t groups = (int64_t)p.B * p.Hkv, most = (int64_t)1 << 32;
   pl.mfma = dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) &&
             p.k_ss >= 0 && p.v_ss >= 0 && p.k_ss < (int64_t)1 << 24 && p.v_ss < (int64_t)1 << 24;

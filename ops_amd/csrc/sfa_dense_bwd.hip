@@ -208,11 +208,21 @@ __device__ __forceinline__ int dkv_chunks(const DenseParams& p, int kb) {
   const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
   return (int)((rows + chunk - 1) / chunk);
 }
-// Unit u of a (sequence, kv head): the longest first, so that the card's last ones are short
-// (up to 256 key blocks: a thread for each block's whole chunks and one for its rest).
+// Chunk c of key block kb.  Chunks are counted from the last row that sees the block, so
+// that without a window those of all blocks begin and end at the same rows.
+__device__ __forceinline__ void dkv_rows(const DenseParams& p, DkvUnit& x) {
+  const int j0 = x.kb * kDkvKeys, chunk = dkv_chunk(p, x.kb);
+  const int64_t first = (int64_t)j0 * p.G, last = (int64_t)dkv_tokens(p, j0) * p.G, end = last - (int64_t)x.c * chunk;
+  x.r1 = (int)end;
+  x.r0 = (int)max(first, end - chunk);
+}
+// Unit u of a (sequence, kv head): the longest first, so that the card's last ones are
+// short; those of a full chunk in order of the chunk, then of the block, so that what runs
+// at once reads the same rows (a block's chunks after one another: 0.26 of the reads in L2).
+// Up to 256 key blocks: a thread for each one's full chunks and one for its rest.
 struct DkvSort {
   int size[512], num[512], nc[256];
-  int unit[6];
+  int unit[4];  // block, chunk, first partial, chunks of the block
 };
 __device__ __forceinline__ DkvUnit dkv_unit_sorted(const DenseParams& p, int u, DkvSort& sort) {
   const int nkb = (p.S + kDkvKeys - 1) / kDkvKeys, tid = threadIdx.x, kb = tid >> 1;
@@ -227,28 +237,43 @@ __device__ __forceinline__ DkvUnit dkv_unit_sorted(const DenseParams& p, int u, 
   }
   sort.size[tid] = size;
   sort.num[tid] = num;
-  if (tid < 6) sort.unit[tid] = -1;
+  if (tid < 4) sort.unit[tid] = -1;
   dense_barrier();
-  if (num > 0) {
-    int first = 0;
+  // the full ones: thread c counts those of chunks 0 .. c - 1
+  int before = 0, here = 0, all = 0;
+  for (int i = 0; i < 2 * nkb; i += 2) {
+    const int m = sort.size[i] == p.chunk ? sort.num[i] : 0;
+    before += min(m, tid);
+    here += m > tid ? 1 : 0;
+    all += m;
+  }
+  if (u < all) {
+    if (u >= before && u < before + here) {
+      int k = u - before, i = 0;
+      for (; i < 2 * nkb; i += 2)
+        if (sort.size[i] == p.chunk && sort.num[i] > tid && k-- == 0) break;
+      sort.unit[0] = i >> 1;
+      sort.unit[1] = tid;
+      sort.unit[3] = sort.nc[i >> 1];
+    }
+  } else if (num > 0 && size < p.chunk) {
+    int first = all;
     for (int i = 0; i < 2 * nkb; ++i) {
       const int s = sort.size[i];
-      first += s > size || (s == size && i < tid) ? sort.num[i] : 0;
+      first += s < p.chunk && (s > size || (s == size && i < tid)) ? sort.num[i] : 0;
     }
     if (u >= first && u < first + num) {
-      int part = 0;
-      for (int k = 0; k < kb; ++k) part += sort.nc[k] > 1 ? sort.nc[k] : 0;
-      const int c = tid & 1 ? nc - 1 : u - first, j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
       sort.unit[0] = kb;
-      sort.unit[1] = j0 * p.G + c * chunk;
-      sort.unit[2] = (int)min((int64_t)j0 * p.G + (int64_t)(c + 1) * chunk, (int64_t)dkv_tokens(p, j0) * p.G);
-      sort.unit[3] = part;
-      sort.unit[4] = nc;
-      sort.unit[5] = c;
+      sort.unit[1] = tid & 1 ? nc - 1 : u - first;
+      sort.unit[3] = nc;
     }
   }
   dense_barrier();
-  const DkvUnit x{sort.unit[0], sort.unit[1], sort.unit[2], sort.unit[3], sort.unit[4], sort.unit[5]};
+  DkvUnit x{sort.unit[0], 0, 0, 0, sort.unit[3], sort.unit[1]};
+  if (x.kb >= 0) {
+    for (int k = 0; k < x.kb; ++k) x.part += sort.nc[k] > 1 ? sort.nc[k] : 0;
+    dkv_rows(p, x);
+  }
   dense_barrier();  // (its place in LDS is loaded over)
   return x;
 }
@@ -276,10 +301,7 @@ __device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
       x.nc = __builtin_amdgcn_readlane(nc, w);
       x.c = u - __builtin_amdgcn_readlane(first, w);
       x.part = __builtin_amdgcn_readlane(parts + pin - np, w);
-      const int j0 = x.kb * kDkvKeys;
-      const int chunk = dkv_chunk(p, x.kb);
-      x.r0 = j0 * p.G + x.c * chunk;
-      x.r1 = (int)min((int64_t)x.r0 + chunk, (int64_t)dkv_tokens(p, j0) * p.G);
+      dkv_rows(p, x);
       return x;
     }
     before += __builtin_amdgcn_readlane(incl, 63);
@@ -293,14 +315,16 @@ __device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
 // order; waves 4 .. 7, one on each SIMD beside one of those, take the last step's for the
 // sums of 64 keys x half of the dims.  So no wave holds both the keys' rows and the
 // sums (all in one wave are 320 registers: 929 us at 8192 tokens, window 1024, 32 / 8
-// heads of 128), the products of one cover the weights of the other, and LDS moves 112 KB a
-// step of 1024 clocks' products.
+// heads of 128, where this takes 525), the products of one cover the weights of the other, and
+// LDS moves 112 KB a step of 1024 clocks' products.  The waves of sums load the rows, five
+// tiles ahead: they have the registers for the addresses (by all waves it was 626, with
+// spills).
 template <int D>
 __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   typedef Tile<D> L;
   typedef Mfma<16> M16;
   constexpr int NW = 8, RT = 32, NS = 7, CH = D / 8, RPI = L::RPI;
-  constexpr int GROUPS = RT / RPI, PER = 2 * GROUPS / NW, LOADS = PER + 1;  // load instructions a tensor; a wave
+  constexpr int GROUPS = RT / RPI, PER = 2 * GROUPS / 4, LOADS = PER + 1;  // load instructions a tensor; a wave of sums
   constexpr int SLOTS = GROUPS * L::GROUP;
   __shared__ u32x4 s_row[NS][2][SLOTS];        // Q, dO
   __shared__ u32x4 s_pd[2][2][2][2][kDkvKeys]; // [step][p, ds][16 rows][lane half][key]: 8 rows
@@ -311,7 +335,7 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   const int groups = p.B * p.Hkv, gi = blockIdx.x % groups;
   const int b = gi / p.Hkv, g = gi % p.Hkv;
   static_assert(sizeof(DkvSort) <= sizeof(s_row), "the units are sorted where the rows come later");
-  const bool sorted = p.S <= 256 * kDkvKeys;
+  const bool sorted = p.S <= 256 * kDkvKeys && (int64_t)p.S * p.G <= 512 * (int64_t)p.chunk;
   const DkvUnit un = sorted ? dkv_unit_sorted(p, blockIdx.x / groups, *reinterpret_cast<DkvSort*>(s_row)) : dkv_unit(p, blockIdx.x / groups);
   const int kb = __builtin_amdgcn_readfirstlane(un.kb);
   if (kb < 0) return;
@@ -320,52 +344,59 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   const int nc = __builtin_amdgcn_readfirstlane(un.nc), part = __builtin_amdgcn_readfirstlane(un.part + un.c);
   const int j0 = kb * kDkvKeys;
   const int n = end > begin ? (end - begin + RT - 1) / RT : 0;
+  // Blocks that are whole go through their rows from a multiple of the chunk on and around, so
+  // that blocks that run at once and overlap read the same rows at a time.
+  const int turn = nc == 1 && p.window < p.S ? (p.chunk - begin % p.chunk) % p.chunk / RT : 0, from = turn < n ? turn : 0;
 
-  // ---- loads: rows begin + 32 i .. as (token, head) pairs that advance with the tiles ----
-  int lt_[PER], lh_[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int r = begin + (wave * PER + k) % GROUPS * RPI + lane / CH;
-    lt_[k] = r / p.G;
-    lh_[k] = r - lt_[k] * p.G;
-  }
-  const bool is_do = wave >= NW / 2;
+  // ---- loads (by the waves of sums, which have registers for it): addresses that advance ----
+  const int lw = wave & 3;
+  const bool is_do = lw >= 2;
   const int dt = RT / p.G, dh_step = RT - dt * p.G;
   const int64_t x_ss = 2 * (is_do ? p.do_ss : p.q_ss), x_sh = 2 * (is_do ? p.do_sh : p.q_sh);
   const uint64_t xbase = is_do ? (uint64_t)(uintptr_t)p.dout + (uint64_t)(2 * (b * p.do_sb + g * p.G * p.do_sh))
                                : (uint64_t)(uintptr_t)p.q + (uint64_t)(2 * (b * p.q_sb + g * p.G * p.q_sh));
-  const int64_t r_all = ((int64_t)b * p.Hkv + g) * p.S * p.G;
-  const int last_row = p.S * p.G - 1;
-  int ls = 0;               // the next tile's place
-  auto load = [&](int i) {  // tile i, in order of i
-    const int st = ls;
+  const uint64_t by = (uint64_t)(dt * x_ss + dh_step * x_sh), by_wrap = by + (uint64_t)(x_ss - p.G * x_sh);
+  uint64_t xa[PER];  // of the lane's rows of the next tile
+  int xh[PER];       // their heads
+  auto start_rows = [&](int tile) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int r = begin + tile * RT + (lw * PER + k) % GROUPS * RPI + lane / CH, t = r / p.G;
+      xh[k] = r - t * p.G;
+      xa[k] = xbase + (uint64_t)(t * x_ss + xh[k] * x_sh) + 16u * (uint32_t)((lane % CH) ^ L::at(lane / CH));
+    }
+  };
+  const uint64_t c_at = (uint64_t)(uintptr_t)((lane < 32 ? p.row_lse : p.row_delta) + ((int64_t)b * p.Hkv + g) * p.S * p.G + begin + (lane & 31));
+  int ls = 0, lpos = from;  // the next tile's place in LDS and among the unit's
+  auto load = [&](int i) {  // the i-th tile, in order of i
+    const int st = ls, left = i < n ? end - begin - lpos * RT : 0;
     ls = ls == NS - 1 ? 0 : ls + 1;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int q = (wave * PER + k) % GROUPS;
-      const uint32_t c = 16u * (uint32_t)((lane % CH) ^ L::at(lane / CH));
-      const bool ok = i < n && lt_[k] < sq.n;
-      const uint64_t a = ok ? xbase + (uint64_t)(lt_[k] * x_ss + lh_[k] * x_sh) : (uint64_t)(uintptr_t)kZeroRow;
-      dense_dma16(&s_row[st][is_do][q * L::GROUP], a + c);
-      lt_[k] += dt;
-      lh_[k] += dh_step;
-      if (lh_[k] >= p.G) {
-        lh_[k] -= p.G;
-        ++lt_[k];
-      }
+      const int q = (lw * PER + k) % GROUPS;
+      dense_dma16(&s_row[st][is_do][q * L::GROUP], q * RPI + lane / CH < left ? xa[k] : (uint64_t)(uintptr_t)kZeroRow);
+      xh[k] += dh_step;
+      const bool wrap = xh[k] >= p.G;
+      xh[k] -= wrap ? p.G : 0;
+      xa[k] += wrap ? by_wrap : by;
     }
-    const int r = min(begin + i * RT + (lane & 31), last_row);
-    dense_dma4(&s_c[st][wave & 3][0][0], (uint64_t)(uintptr_t)((lane < 32 ? p.row_lse : p.row_delta) + r_all + r));
+    // (up to 31 rows behind the last, whose tiles are masked: the array is that much longer)
+    dense_dma4(&s_c[st][lw][0][0], c_at + (uint64_t)(4 * RT) * (uint64_t)lpos);
+    if (++lpos >= n) {
+      lpos = 0;
+      start_rows(0);
+    }
   };
   // The tile a step is at: its number, place, first row's token and head (divisions are long).
   struct At {
-    int i, st, t, h;
+    int i, st, pos, t, h;
     bool whole;  // its rows all see all keys of the block
   };
+  const int tb = begin / p.G, hb = begin - tb * p.G;  // (of the first)
   const int dt31 = (RT - 1) / p.G, dh31 = RT - 1 - dt31 * p.G;
   auto settle = [&](At& a) {
     const int t1 = a.t + dt31 + (a.h + dh31 >= p.G ? 1 : 0);
-    a.whole = begin + a.i * RT + RT <= end && j0 + kDkvKeys - 1 <= a.t && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
+    a.whole = begin + a.pos * RT + RT <= end && j0 + kDkvKeys - 1 <= a.t && (j0 + kDkvKeys <= p.first || t1 - j0 < p.window);
   };
   auto advance = [&](At& a) {
     ++a.i;
@@ -376,10 +407,15 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
       a.h -= p.G;
       ++a.t;
     }
+    if (++a.pos == n) {
+      a.pos = 0;
+      a.t = tb;
+      a.h = hb;
+    }
     settle(a);
   };
-  At at{0, 0, begin / p.G, 0, false};
-  at.h = begin - at.t * p.G;
+  At at{0, 0, from, (begin + from * RT) / p.G, 0, false};
+  at.h = begin + from * RT - at.t * p.G;
   settle(at);
   // Between the steps: what the sums are about to read of a tile whose rows do not see all
   // keys is cleared of infinities and NaN (0 times them would reach the keys they do not see).
@@ -389,13 +425,9 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
       clear_rows<D, NW>(s_row[st][1], 0, wave, lane);
     }
   };
-  // At the end of step i: tile i + 3 has landed (behind it i + 4), what the step read is read.
-  auto next = [&]() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-    dense_barrier();
-  };
-#pragma unroll
-  for (int i = 0; i < 4; ++i) load(i);
+  // In step i the sums read tile i - 1, the weights are made of tile i and their next operands
+  // read of tile i + 1; tile i + 5 goes where tile i - 2 was.  At its end tile i + 2 has landed
+  // (behind it i + 3 .. i + 5), what the step read is read.
 
   if (wave < 4) {
     // ---- weights: rows 16 rh + .., keys 64 kg + .. ----
@@ -417,98 +449,95 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
     }
     const int row = 16 * rh + lt;
     const uint32_t x0 = 16u * (uint32_t)(hq ^ L::at(row)), a0 = 16u * (uint32_t)L::slot(row, L::at(row));
-    f32x4 sa[4], da[4], sb[4], db[4];
-    // the products of the tile at place st, whose first operands are in op; then those of the next
-    bf16x8 op[2][2];
+    // A tile's operands are held: 16 keys after 16 keys, their scores and do.v in turn, beside
+    // the weights of the 16 before.
+    bf16x8 op[2][KS];
     f32x4 c0, c1;  // its rows' start values
-    auto first = [&](int st) {
-      op[0][0] = lds_b128_at(lds_addr(s_row[st][0]) + a0 + x0);
-      op[0][1] = lds_b128_at(lds_addr(s_row[st][1]) + a0 + x0);
+    auto read_op = [&](int st, int w, int c) {
+      return lds_b128_at(lds_addr(s_row[st][w]) + a0 + (x0 ^ (uint32_t)(64 * c)));
+    };
+    auto read_c = [&](int st) {
       c0 = *reinterpret_cast<const f32x4*>(&s_c[st][wave][0][16 * rh + 4 * hq]);
       c1 = *reinterpret_cast<const f32x4*>(&s_c[st][wave][1][16 * rh + 4 * hq]);
     };
-    auto products = [&](int st, f32x4 (&ns)[4], f32x4 (&nd)[4], auto between) {
-      uint32_t x = x0;
-      asm volatile("" : "+v"(x));
-      const uint32_t q = lds_addr(s_row[st][0]) + a0, o = lds_addr(s_row[st][1]) + a0;
-      each<8 * KS>([&](auto uc) {
-        constexpr int u = decltype(uc)::value, c = u / 8, w = (u >> 2) & 1, j = u & 3;
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (u % 8 == 0 && c + 1 < KS) {
-          op[(c + 1) & 1][0] = lds_b128_at(q + (x ^ (uint32_t)(64 * (c + 1))));
-          op[(c + 1) & 1][1] = lds_b128_at(o + (x ^ (uint32_t)(64 * (c + 1))));
-        }
-        if constexpr (w == 0) ns[j] = M16::mma(op[c & 1][0], kf[j][c], c == 0 ? c0 : ns[j]);
-        else nd[j] = M16::mma(op[c & 1][1], vf[j][c], c == 0 ? c1 : nd[j]);
-        between(uc);
-      });
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     dense_barrier();
-    first(0);
-    products(0, sa, da, [](auto) {});
-    first(1);
-    At ahead = at;  // (tile i + 1)
-    advance(ahead);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      op[0][c] = read_op(0, 0, c);
+      op[1][c] = read_op(0, 1, c);
+    }
+    read_c(0);
     int prev_st = 0;
     bool prev_whole = true;
-    auto step = [&](f32x4 (&cs)[4], f32x4 (&cd)[4], f32x4 (&ns)[4], f32x4 (&nd)[4]) {
-      load(at.i + 4);
+    auto step = [&](auto masked) {
+      constexpr bool MASKED = decltype(masked)::value;
       if (at.i > 0) clear(prev_st, prev_whole);
-      if (!at.whole) {
-        const int r0 = begin + at.i * RT + 16 * rh + 4 * hq;
+      // tokens of the lane's rows (-1: none)
+      int tok[4];
+      if constexpr (MASKED) {
+        const int r0 = begin + at.pos * RT + 16 * rh + 4 * hq;
         int t = r0 / p.G, h = r0 - t * p.G;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool in = r0 + e < end;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool ok = in && dense_seen(p, j0 + 64 * kg + 16 * j + lt, t);
-            // (do.v that is no number makes the weight none: its row is cleared for the sums)
-            cs[j][e] = ok ? fmaf(0.f, cd[j][e], cs[j][e]) : kNegInf;
-            cd[j][e] = ok ? cd[j][e] : 0.f;
-          }
+          tok[e] = r0 + e < end ? t : -1;
           if (++h == p.G) {
             h = 0;
             ++t;
           }
         }
-        asm volatile("" : "+v"(cs[0]), "+v"(cs[1]), "+v"(cs[2]), "+v"(cs[3]), "+v"(cd[0]), "+v"(cd[1]), "+v"(cd[2]), "+v"(cd[3]));
       }
+      const int st1 = at.st == NS - 1 ? 0 : at.st + 1;
       char* const out = reinterpret_cast<char*>(&s_pd[at.i & 1][0][rh][hq & 1][64 * kg + lt]) + 8 * (hq >> 1);
-      constexpr int WHICH = (int)sizeof(s_pd[0][0]);
-      bf16x4 pw, dw;
-      products(ahead.st, ns, nd, [&](auto uc) {
-        constexpr int u = decltype(uc)::value, NU = 8 * KS;
-        each<16>([&](auto ec) {
-          constexpr int x = decltype(ec)::value, j = x >> 2, e = x & 3;
-          if constexpr (x * (NU - 2) / 16 == u) {
-            const float w = __builtin_amdgcn_exp2f(cs[j][e] * p.scale_log2);
-            pw[e] = (bf16)w;
-            dw[e] = (bf16)(w * cd[j][e]);
-            if constexpr (e == 3) {
-              *reinterpret_cast<bf16x4*>(out + 16 * 16 * j) = pw;
-              *reinterpret_cast<bf16x4*>(out + WHICH + 16 * 16 * j) = dw;
+      constexpr int WHICH = (int)sizeof(s_pd[0][0]), NJ = 2 * KS;  // products of 16 keys
+      f32x4 s[2], d[2], w;
+      bf16x4 dw;
+      // four weights in four stages, some products apart
+      auto weights = [&](int j, int stage) {
+        f32x4 &cs = s[j & 1], &cd = d[j & 1];
+        if (stage == 0) {
+          if constexpr (MASKED) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool ok = dense_seen(p, j0 + 64 * kg + 16 * j + lt, tok[e]);
+              // (do.v that is no number makes the weight none: its row is cleared for the sums)
+              cs[e] = ok ? fmaf(0.f, cd[e], cs[e]) : kNegInf;
+              cd[e] = ok ? cd[e] : 0.f;
             }
           }
-        });
+          w = cs * p.scale_log2;
+        } else if (stage == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(w[e]);
+        } else if (stage == 2) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dw[e] = (bf16)(w[e] * cd[e]);
+        } else {
+          *reinterpret_cast<bf16x4*>(out + 16 * 16 * j) = bf16x4{(bf16)w[0], (bf16)w[1], (bf16)w[2], (bf16)w[3]};
+          *reinterpret_cast<bf16x4*>(out + WHICH + 16 * 16 * j) = dw;
+        }
+      };
+      each<4 * NJ>([&](auto uc) {
+        constexpr int u = decltype(uc)::value, j = u / NJ, i = u % NJ, c = i >> 1;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (i & 1) d[j & 1] = M16::mma(op[1][c], vf[j][c], c == 0 ? c1 : d[j & 1]);
+        else s[j & 1] = M16::mma(op[0][c], kf[j][c], c == 0 ? c0 : s[j & 1]);
+        if constexpr (j == 3) op[i & 1][c] = read_op(st1, i & 1, c);
+        if constexpr (j > 0 && i % (NJ / 4) == 0) weights(j - 1, i / (NJ / 4));
       });
+      __builtin_amdgcn_sched_barrier(0);
+      read_c(st1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) weights(3, k);
       prev_st = at.st;
       prev_whole = at.whole;
-      at = ahead;
-      advance(ahead);
-      first(ahead.st);  // (tile i + 2, which had landed before this step)
-      next();
+      advance(at);
+      dense_barrier();
     };
-    int i = 0;
-    for (; i + 1 < n; i += 2) {
-      step(sa, da, sb, db);
-      step(sb, db, sa, da);
+    for (int i = 0; i < n; ++i) {
+      if (at.whole) step(std::false_type{});
+      else step(std::true_type{});
     }
-    if (i < n) step(sa, da, sb, db);
     if (n > 0) clear(prev_st, prev_whole);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     return;
   }
 
@@ -522,10 +551,13 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
     for (int m = 0; m < 2; ++m) dk[o][m] = dv[o][m] = f32x16{};
   const int l16 = lane & 15, trow = 4 * hq + (l16 >> 2), tc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
   const uint32_t tx = 16u * (uint32_t)(L::at(trow) ^ tc), t0a = 16u * (uint32_t)L::slot(trow, L::at(trow)) + (uint32_t)(l16 & 1) * 8u;
+  start_rows(from);
+#pragma unroll
+  for (int i = 0; i < 5; ++i) load(i);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   dense_barrier();
   for (int i = 0; i <= n; ++i) {  // (step 0 has no weights yet; at: tile i - 1)
-    if (i < n) load(i + 4);
+    if (i < n) load(i + 5);
     if (i > 0) {
       clear(at.st, at.whole);
       const int st = at.st;
@@ -565,7 +597,10 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
       __builtin_amdgcn_sched_barrier(0);
       advance(at);
     }
-    if (i < n) next();
+    if (i < n) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");
+      dense_barrier();
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
