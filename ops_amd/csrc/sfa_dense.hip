@@ -146,12 +146,12 @@ __global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
   if (threadIdx.x == 0) p.dsink[h] = -s_x[0];
 }
 
-enum { kAny = 0, kWide, kFew16, kFew32, kFew64 };
+enum { kAny = 0, kWide, kFew16, kFew32, kFew64, kLatent };
 struct KernelShape {
   int rows, tile_shift, threads, per_cu;  // per_cu: workgroups on a CU at once
 };
 constexpr KernelShape kShapes[] = {{kAnyRows, kAnyShift, 256, 4}, {kWideRows, 6, 512, 1}, {16, 7, 256, 2}, {32, 7, 256, 2},
-                                   {64, 7, 256, 1}};
+                                   {64, 7, 256, 1}, {kLatentRows, 6, 512, 1}};
 
 void set_launch(DenseParams& p, const DensePlan& pl) {
   p.rows = pl.rows;
@@ -171,6 +171,9 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   const int64_t R = (int64_t)p.S * p.G;
   if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
     pl.kernel = R <= 16 ? kFew16 : R <= 32 ? kFew32 : R <= 64 ? kFew64 : kWide;
+  if (dtype == SFA_DTYPE_BF16 && kv_dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == kLatentQK && p.Dv == kLatentV && p.v == p.k &&
+      p.v_sb == p.k_sb && p.v_ss == p.k_ss && p.v_sh == p.k_sh)
+    pl.kernel = kLatent;
   const KernelShape& k = kShapes[pl.kernel];
   pl.rows = k.rows;
   pl.tile_shift = k.tile_shift;
@@ -179,7 +182,7 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   const int64_t dims = pl.kernel == kAny ? (p.Dv + kAnyDims - 1) / kAnyDims : 1;
   // Few row blocks: their keys are cut into ranges that fill the card (sfa_dense.h).
   constexpr int64_t kCus = 256;
-  const bool few = pl.kernel >= kFew16;
+  const bool few = pl.kernel >= kFew16 && pl.kernel <= kFew64;
   pl.min_len = few ? 2 : 4;
   // (LDS of the few rows' kernel: one workgroup a CU with bf16 rows of 128 dims)
   const int per_cu = few && kv_dtype == SFA_DTYPE_BF16 && p.Dqk == 128 ? 1 : k.per_cu;
@@ -204,6 +207,7 @@ hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, i
   DenseParams p = p0;
   set_launch(p, pl);
   if (pl.kernel == kWide) launch_dense_wide(p, kv_dtype, s);
+  else if (pl.kernel == kLatent) launch_dense_mla(p, s);
   else if (pl.kernel >= kFew16) launch_dense_few(p, kv_dtype, s);
   else launch_dense_any(p, dtype, kv_dtype, s);
   if (pl.want > 0) {
