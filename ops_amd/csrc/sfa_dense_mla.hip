@@ -113,11 +113,12 @@ template <bool ONE>
 __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   typedef Mfma<16> M16;
   typedef Mfma<32> M;
-  constexpr int CH = kLatentCh, CR = kLatentCr, KT = kWideKeys, STEPS = kLatentQK / 32, QR = 17;  // steps of Q in registers
+  constexpr int CH = kLatentCh, CR = kLatentCr, KT = kWideKeys, STEPS = kLatentQK / 32, QR = 16;  // steps of Q in registers
   __shared__ u32x4 s_k[2][KT * CH];       // dims 0 .. 511 (K and V)
   __shared__ u32x4 s_r[2][KT * CR];       // dims 512 .. 575, Swz<64>
   __shared__ u32x4 s_p[4][2][kLatentRows];  // P of 16 keys: [lane half][row] keys 4 half + 0 .. 3, 8 + 4 half + 0 .. 3
   __shared__ u32x4 s_q[4][kLatentRows];   // Q's last 32 dims: [8 of them][row]
+  __shared__ u32x4 s_q1[4][32];           // the 32 before them, of rows 16 .. 31 and 48 .. 63
   __shared__ float s_m[kLatentRows];      // running maxima (base 2)
   __shared__ float s_x[4][kLatentRows];   // per key quarter: row maxima, then row sums
   __shared__ int s_over[2];
@@ -135,20 +136,20 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   // what all rows of the block see of a tile without a look at each
   const int p0 = it.s.ctx + it.row0 / p.G, p1 = it.s.ctx + min((it.row0 + p.rows - 1) / p.G, it.s.n - 1);
 
-  bf16x8 q[2][QR];
-  int pos[2];
+  bf16x8 q[2][QR], q16;  // (Q's last one and a half steps in LDS: there is no register to spare)
   {
     const int lt = lane & 15, hq = lane >> 4;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int r = it.row0 + 32 * rh + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
       const bool live = r < R && t < it.s.n;
-      pos[n] = live ? it.s.ctx + t : -1;
       const bf16* a = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         const bf16x8 x = *reinterpret_cast<const bf16x8*>(a + 32 * s), y = live ? x : bf16x8{};
         if (s < QR) q[n][s < QR ? s : 0] = y;
+        else if (s == QR && n == 0) q16 = y;
+        else if (kq == 0 && s == QR) s_q1[hq][16 * rh + lt] = __builtin_bit_cast(u32x4, y);
         else if (kq == 0) s_q[hq][32 * rh + 16 * n + lt] = __builtin_bit_cast(u32x4, y);
       }
     }
@@ -209,8 +210,10 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         if constexpr (i == 0) sc[n] = M16::mma(kf[0], ql[n], f32x4{});
-        else sc[n] = M16::mma(kf[i % 3], q[n][i > 0 ? i - 1 : 0], sc[n]);
+        else if constexpr (i <= QR) sc[n] = M16::mma(kf[i % 3], q[n][(i + QR - 1) % QR], sc[n]);
+        else sc[n] = M16::mma(kf[i % 3], n == 0 ? q16 : ql[0], sc[n]);
       }
+      if constexpr (i == 14) ql[0] = __builtin_bit_cast(bf16x8, s_q1[hq][16 * rh + lt]);
       // the next tile's rows
       if constexpr (i % 2 == 1 && i / 2 < 8) src.row(i / 2, kn, ln);
       else if constexpr (i == 17) src.rest(rn, ln);
@@ -224,7 +227,9 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     if (masked) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const uint32_t bits = (uint32_t)((seen_of(p, pos[n], j0) & mask) >> (16 * kq + 4 * hq));
+        // (formed here: held they spill)
+        const int r = it.row0 + 32 * rh + 16 * n + lt, t = r / p.G, pos = r < R && t < it.s.n ? it.s.ctx + t : -1;
+        const uint32_t bits = (uint32_t)((seen_of(p, pos, j0) & mask) >> (16 * kq + 4 * hq));
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = (bits >> e) & 1 ? sc[n][e] : kNegInf;
       }
