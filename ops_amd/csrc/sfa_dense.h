@@ -78,7 +78,8 @@ __device__ __forceinline__ float scale_of(uint8_t e) {
 // A unit is a (sequence, row block).  p.fit workgroups of a kv head run at once.  With
 // want > 0 (few units) the units' tiles are cut into ranges of up to one length, found
 // on the device as the lengths are there: the shortest that gives p.fit ranges or
-// fewer, or, where that leaves less work on the longest path, `want`, twice as many.
+// fewer, or, where that leaves less work on the longest path, `want`, twice as many.  To
+// write partial results and join them takes the time of p.join tiles.
 // (Each unit has one at least.)
 struct DenseSlot {
   int unit;       // or -1: none
@@ -133,12 +134,15 @@ __device__ __forceinline__ DenseSlot dense_slot(const DenseParams& p, int slot) 
     return max(len, most);
   };
   int len = most;
-  if (units <= p.fit) len = shortest(p.fit);
+  if (units <= p.fit) {
+    const int l1 = shortest(p.fit);
+    if (l1 + p.join < most) len = l1;
+  }
   if (len > p.min_len) {
     const int l2 = shortest(p.want);
-    // (rounds of p.fit ranges; joining them costs a tenth or so)
+    // (rounds of p.fit ranges; more of them cost a tenth or so)
     const int rounds = units <= p.fit ? 1 : (units + p.fit - 1) / p.fit, r2 = (p.want + p.fit - 1) / p.fit;
-    if (l2 < most && 11 * r2 * l2 < 10 * rounds * len) len = l2;
+    if (l2 < most && 11 * r2 * l2 + (len == most ? 10 * p.join : 0) < 10 * rounds * len) len = l2;
   }
   len = max(len, 1);
   int before = 0;

@@ -8,14 +8,16 @@ namespace {
 
 // ---- joining the ranges of a row block -------------------------------------------
 // A workgroup takes jr rows of a unit, one wave a row; LPR lanes hold it (4 dims each),
-// 64 / LPR ranges at a time.  A range in which the row sees nothing has LSE -inf.
+// 64 / LPR ranges at a time, jd dims.  A range in which the row sees nothing has LSE -inf.
 template <typename T, int LPR>
-__global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p, int jr) {
+__global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p, int jr, int jd) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int chunks = (p.rows + jr - 1) / jr;
   int wi = blockIdx.x;
   const int row0 = wi % chunks * jr;
   wi /= chunks;
+  const int nd = (p.Dv + jd - 1) / jd, dim0 = wi % nd * jd;
+  wi /= nd;
   const int g = wi % p.Hkv, u = wi / p.Hkv;
   const int first = p.unit_slots[2 * u], ns = p.unit_slots[2 * u + 1];
   if (ns <= 1) return;
@@ -41,14 +43,14 @@ __global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p, int j
     l = wave_sum(l + nan);
     float lse;
     const float f = dense_finish(p, h, live, m, l, lse);
-    if (lane == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+    if (lane == 0 && dim0 == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
     T* o = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
     const int sub = lane / LPR;
-    for (int d0 = 0; d0 < p.Dv; d0 += 4 * LPR) {
+    for (int d0 = dim0; d0 < min(dim0 + jd, p.Dv); d0 += 4 * LPR) {
       const int d = d0 + 4 * (lane % LPR);
       f32x4 x = {};
       if (f != 0.f) {
-#pragma unroll 4
+#pragma unroll 8
         for (int k = sub; k < ns; k += 64 / LPR) {
           const float e = exp2f(pl[k * per] - moff);
           f32x4 v = {};
@@ -66,21 +68,34 @@ __global__ __launch_bounds__(256) void dense_combine_kernel(DenseParams p, int j
       for (int s = LPR; s < 64; s <<= 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[q] += __shfl_xor(x[q], s, 64);
-      if (sub == 0)
+      if (sub == 0) {
+        if (p.vec && d < p.Dv) {
+          typedef T t4 __attribute__((ext_vector_type(4)));
+          t4 y;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (d + q < p.Dv) o[d + q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+          for (int q = 0; q < 4; ++q) y[q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+          *reinterpret_cast<t4*>(o + d) = y;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (d + q < p.Dv) o[d + q] = from_f32<T>(f == 0.f ? 0.f : x[q] * f);
+        }
+      }
     }
   }
 }
 template <typename T>
 void combine(const DenseParams& p, hipStream_t s) {
-  // (few rows: a wave each; many: their units often have one range, and then nothing is left to do)
+  // Few rows: a wave each (more than 128 dims: for each 128 of them; one row of 512 dims from
+  // 56 ranges 14.6 us for 41).  Many: their units often have one range, and then nothing is left
+  // to do; a wave takes all dims (8192 rows of 512 dims from 2 ranges: 18 us, 31 with 128 each).
   const int jr = p.rows <= 64 ? 4 : 16;
-  const unsigned grid = (unsigned)((int64_t)p.B * p.nrb * p.Hkv * ((p.rows + jr - 1) / jr));
-  if (p.Dv <= 64) dense_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p, jr);
-  else if (p.Dv <= 128) dense_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p, jr);
-  else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p, jr);
+  const int64_t rows = (int64_t)p.B * p.nrb * p.Hkv * p.rows;
+  const int jd = rows < 2048 ? 128 : (p.Dv + 127) / 128 * 128;
+  const unsigned grid = (unsigned)(rows / p.rows * ((p.Dv + jd - 1) / jd) * ((p.rows + jr - 1) / jr));
+  if (p.Dv <= 64) dense_combine_kernel<T, 16><<<grid, 256, 0, s>>>(p, jr, jd);
+  else if (jd <= 128) dense_combine_kernel<T, 32><<<grid, 256, 0, s>>>(p, jr, jd);
+  else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p, jr, jd);
 }
 
 // ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse ------------
@@ -160,6 +175,7 @@ void set_launch(DenseParams& p, const DensePlan& pl) {
   p.fit = pl.fit;
   p.want = pl.want;
   p.min_len = pl.min_len;
+  p.join = pl.join;
   p.slots = pl.slots;
 }
 
@@ -184,6 +200,9 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   constexpr int64_t kCus = 256;
   const bool few = pl.kernel >= kFew16 && pl.kernel <= kFew64;
   pl.min_len = few ? 2 : 4;
+  // A row block's partial results are 128 KB (wide, latent rows): with the joining launch as
+  // long as five tiles; of few rows it is the launch.
+  pl.join = pl.kernel == kWide || pl.kernel == kLatent ? (int)(R < pl.rows ? 1 + 4 * R / pl.rows : 5) : 1;
   // (LDS of the few rows' kernel: one workgroup a CU with bf16 rows of 128 dims)
   const int per_cu = few && kv_dtype == SFA_DTYPE_BF16 && p.Dqk == 128 ? 1 : k.per_cu;
   const int64_t fit = kCus * per_cu / (p.Hkv * dims);

@@ -136,23 +136,27 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   // what all rows of the block see of a tile without a look at each
   const int p0 = it.s.ctx + it.row0 / p.G, p1 = it.s.ctx + min((it.row0 + p.rows - 1) / p.G, it.s.n - 1);
 
-  bf16x8 q[2][QR], q16;  // (Q's last one and a half steps in LDS: there is no register to spare)
+  // The rows of Q come through LDS, where tile 1 goes later (straight from global memory each
+  // load touches 16 rows and four waves load the same: 6 us a workgroup).
   {
-    const int lt = lane & 15, hq = lane >> 4;
+    const int r0 = it.row0 + 8 * wave;
+    int t = r0 / p.G, h = r0 - t * p.G;
+    const uint64_t qbase = (uint64_t)(uintptr_t)p.q + (uint64_t)(2 * (b * p.q_sb + g * p.G * p.q_sh)), zero = (uint64_t)(uintptr_t)kZeroRow;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int r = it.row0 + 32 * rh + 16 * n + lt, t = r / p.G, h = g * p.G + r % p.G;
-      const bool live = r < R && t < it.s.n;
-      const bf16* a = reinterpret_cast<const bf16*>(p.q) + b * p.q_sb + (live ? t * p.q_ss + h * p.q_sh : 0) + 8 * hq;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(a + 32 * s), y = live ? x : bf16x8{};
-        if (s < QR) q[n][s < QR ? s : 0] = y;
-        else if (s == QR && n == 0) q16 = y;
-        else if (kq == 0 && s == QR) s_q1[hq][16 * rh + lt] = __builtin_bit_cast(u32x4, y);
-        else if (kq == 0) s_q[hq][32 * rh + 16 * n + lt] = __builtin_bit_cast(u32x4, y);
+    for (int k = 0; k < 8; ++k) {
+      const int row = 8 * wave + k;
+      const uint64_t a = r0 + k < R && t < it.s.n ? qbase + (uint64_t)(2 * (t * p.q_ss + h * p.q_sh)) : zero;
+      dense_dma16(&s_k[1][row * CH], a, 16u * (uint32_t)(lane ^ latent_at(row)));
+      if (++h == p.G) {
+        h = 0;
+        ++t;
       }
     }
+    const int row = 8 * wave + (lane >> 3), r = it.row0 + row;
+    t = r / p.G;
+    h = r - t * p.G;
+    const uint64_t a = r < R && t < it.s.n ? qbase + (uint64_t)(2 * (t * p.q_ss + h * p.q_sh)) : zero;
+    dense_dma16(&s_r[1][8 * wave * CR], a + (uint64_t)(16 * (CH + ((lane & 7) ^ latent_rest_at(row)))));
   }
   if (tid < kLatentRows) {
     s_m[tid] = kNegInf;
@@ -170,6 +174,26 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   for (int k = 0; k < 8; ++k) src.row(k, s_k[0], lane);
   src.rest(s_r[0], lane);
   if constexpr (!ONE) src.ids(1);
+
+  bf16x8 q[2][QR], q16;  // (Q's last one and a half steps in LDS: there is no register to spare)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  dense_barrier();
+  {
+    const int lt = lane & 15, hq = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int row = 32 * rh + 16 * n + lt;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const bf16x8 y = s < 16 ? __builtin_bit_cast(bf16x8, s_k[1][row * CH + ((4 * s + hq) ^ latent_at(lt))])
+                                : __builtin_bit_cast(bf16x8, s_r[1][row * CR + ((4 * (s - 16) + hq) ^ latent_rest_at(lt))]);
+        if (s < QR) q[n][s < QR ? s : 0] = y;
+        else if (s == QR && n == 0) q16 = y;
+        else if (kq == 0 && s == QR) s_q1[hq][16 * rh + lt] = __builtin_bit_cast(u32x4, y);
+        else if (kq == 0) s_q[hq][row] = __builtin_bit_cast(u32x4, y);
+      }
+    }
+  }
 
   f32x16 oacc[2][2];  // [32 dims][32 rows]
 #pragma unroll

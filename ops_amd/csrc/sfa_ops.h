@@ -141,7 +141,7 @@ struct DenseParams {
   bool vec;                  // rows are whole 16-byte units (8-bit: 8)
   // a launch: row blocks of `rows` query rows, nrb a (sequence, kv head); key tiles of 2^tile_shift
   int rows, nrb, tile_shift;
-  int fit, want, min_len;    // ranges a kv head that run at once; the most (0: one a row block); tiles of the shortest
+  int fit, want, min_len, join;  // ranges a kv head that run at once; the most (0: one a row block); tiles of the shortest; of a join
   int slots;                 // of the launch, a kv head
   float* part_o;             // [slots][Hkv][rows][Dv], normalised by the slot's own sum
   float* part_lse;           // [slots][Hkv][rows], base-2 (-inf: nothing seen)
@@ -164,7 +164,7 @@ struct DenseParams {
 constexpr int kDenseUnits = 256;  // row blocks of a launch that is cut into ranges, at most
 struct DensePlan {
   int kernel;
-  int rows, tile_shift, fit, want, min_len, slots;
+  int rows, tile_shift, fit, want, min_len, join, slots;
   int64_t wgs;               // workgroups of `threads` threads
   int threads;
   bool fits() const { return wgs * threads < (int64_t)1 << 32; }  // one launch
