@@ -175,17 +175,18 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
     half(j, std::integral_constant<int, 1>{}, sb, db, sa, da);
   }
   src.template wait<0>();
-  if (!in) return;
+  dense_barrier();  // the tiles are read
+  const RowsOut<D / 8> out{&s_kv[0][0][0] + wave * 32 * (D / 8)};
 #pragma unroll
   for (int o = 0; o < OT; ++o)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f32x4 x;
+      bf16x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dq[o][4 * i + e] * p.scale;
-      *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.dq) + b * p.dq_sb + t * p.dq_ss + h * p.dq_sh + 32 * o + 8 * i + 4 * hq) =
-          bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+      for (int e = 0; e < 4; ++e) x[e] = (bf16)(dq[o][4 * i + e] * p.scale);
+      out.put(lr, 32 * o + 8 * i + 4 * hq, x);
     }
+  out.store(0, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.dq) + b * p.dq_sb + t * p.dq_ss + h * p.dq_sh) : 0, lane);
 }
 
 // ---- dk and dv: 128 keys, tiles of 32 query rows of all heads ----------------------------

@@ -411,34 +411,41 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   }
   dense_barrier();
   const int lr = lane & 31, half = lane >> 5;
+  u32x4* const rows = &s_k[0][0];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int row = 32 * n + lr, r = it.row0 + row, t = r / p.G, h = g * p.G + r % p.G;
-    if (r >= R) continue;
+    const bool in = r < R, first = in && wave == 0 && half == 0;
     const float l = (s_x[0][row] + s_x[1][row]) + (s_x[2][row] + s_x[3][row]);
     float lse, f;
     if (it.partial) {
       f = dense_part(s_m[row], l, lse);
-      if (wave == 0 && half == 0) p.part_lse[it.part + row] = lse;
+      if (first) p.part_lse[it.part + row] = lse;
     } else {
-      f = dense_finish(p, h, t < it.s.n, s_m[row], l, lse);
-      if (wave == 0 && half == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+      f = dense_finish(p, h, in && t < it.s.n, s_m[row], l, lse);
+      if (first) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
     }
+    auto results = [&](auto put) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
+      for (int o = 0; o < 2; ++o)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 x;
+        for (int i = 0; i < 4; ++i) {
+          f32x4 x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = f == 0.f ? 0.f : oacc[o][n][4 * i + e] * f;
-        const int d = 64 * wave + 32 * o + 8 * i + 4 * half;
-        if (it.partial) {
-          *reinterpret_cast<f32x4*>(p.part_o + (it.part + row) * p.Dv + d) = x;
-        } else {
-          *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + d) =
-              bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+          for (int e = 0; e < 4; ++e) x[e] = f == 0.f ? 0.f : oacc[o][n][4 * i + e] * f;
+          put(32 * o + 8 * i + 4 * half, x);
         }
-      }
+    };
+    if (it.partial) {
+      const RowsOut<16> out{rows + wave * kLatentRows * 16};
+      results([&](int d, f32x4 x) { out.put(row, d, x); });
+      out.store(32 * n, in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * p.Dv + 64 * wave) : 0, lane);
+    } else {
+      const RowsOut<8> out{rows + wave * kLatentRows * 8};
+      results([&](int d, f32x4 x) { out.put(row, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
+      out.store(32 * n, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + 64 * wave) : 0,
+                lane);
+    }
   }
 }
 

@@ -22,6 +22,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   constexpr int NW = 8, KT = kWideKeys, KS = D / 16, OT = D / 32, NS = 4;
   __shared__ u32x4 s_kv[NS][2][Tile<D>::SLOTS];
   __shared__ unsigned long long s_bad[2];
+  static_assert(sizeof(s_kv) >= 256 * D * 4, "the results' rows");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -243,31 +244,43 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   src.template wait<0>();
 
   // ---- results: lane holds row lr, dims 32 o + 8 i + 4 hq + 0 .. 3 --------------------
-  const float l = xor32_sum(l_part);
-  if (!in) return;
-  float lse, f;
-  if (it.partial) {
-    f = dense_part(m_used, l, lse);
-    if (hq == 0) p.part_lse[it.part + row] = lse;
-  } else {
-    f = dense_finish(p, h, live, m_used, l, lse);
-    if (hq == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
-  }
-#pragma unroll
-  for (int o = 0; o < OT; ++o)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = f == 0.f ? 0.f : oacc[o][4 * i + e] * f;
-      const int d = 32 * o + 8 * i + 4 * hq;
-      if (it.partial) {
-        *reinterpret_cast<f32x4*>(p.part_o + (it.part + row) * D + d) = x;
-      } else {
-        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + d) =
-            bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
-      }
+  dense_barrier();  // the tiles are read
+  {  // (what follows is formed now: held across the loop it spills)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int lr = ln & 31, hq = ln >> 5, row = 32 * wave + lr, r = it.row0 + row, t = r / p.G, h = g * p.G + r % p.G;
+    const bool in = r < p.S * p.G, live = in && t < it.s.n;
+    const float l = xor32_sum(l_part);
+    float lse, f;
+    if (it.partial) {
+      f = dense_part(m_used, l, lse);
+      if (in && hq == 0) p.part_lse[it.part + row] = lse;
+    } else {
+      f = dense_finish(p, h, live, m_used, l, lse);
+      if (in && hq == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
     }
+    u32x4* const rows = &s_kv[0][0][0];
+    auto results = [&](auto put) {
+#pragma unroll
+      for (int o = 0; o < OT; ++o)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = f == 0.f ? 0.f : oacc[o][4 * i + e] * f;
+          put(32 * o + 8 * i + 4 * hq, x);
+        }
+    };
+    if (it.partial) {
+      const RowsOut<D / 4> out{rows + wave * 32 * (D / 4)};
+      results([&](int d, f32x4 x) { out.put(lr, d, x); });
+      out.store(0, in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * D) : 0, ln);
+    } else {
+      const RowsOut<D / 8> out{rows + wave * 32 * (D / 8)};
+      results([&](int d, f32x4 x) { out.put(lr, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
+      out.store(0, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh) : 0, ln);
+    }
+  }
 }
 
 template <int D>
