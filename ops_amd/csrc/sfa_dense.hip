@@ -246,8 +246,18 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
             p.k_ss >= 0 && p.v_ss >= 0 && p.k_ss < (int64_t)1 << 24 && p.v_ss < (int64_t)1 << 24;
   if (!pl.mfma) {
     const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
-    const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows;
-    pl.fits = groups * nrb * dims * 256 < most && groups * (((int64_t)p.S + 63) / 64) * dims * 256 < most;
+    const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows, nkb = ((int64_t)p.S + kAnyRows - 1) / kAnyRows;
+    // Few key blocks (two workgroups a CU): their rows in chunks, of four times as many
+    // workgroups in all (256 tokens, 32 heads on 2: 8 blocks of up to 4096 rows).
+    const int64_t blocks = groups * nkb * dims, widest = p.first > 0 || p.window >= p.S ? p.S : (int64_t)p.window + kAnyRows - 1;
+    const int64_t rows = (widest < p.S ? widest : p.S) * p.G;
+    int64_t chunk = rows;
+    if (blocks < 512) chunk = (rows * blocks / 1024 + 128) / 32 * 32;
+    if (chunk > rows) chunk = rows;
+    pl.chunk = (int)chunk;
+    pl.parts = (int)((rows + chunk - 1) / chunk);
+    pl.dkv_bytes = pl.parts > 1 ? (size_t)(groups * nkb * pl.parts) * kAnyRows * (p.Dqk + p.Dv) * sizeof(float) : 0;
+    pl.fits = groups * nrb * dims * 256 < most && blocks * pl.parts * 256 < most;
     return pl;
   }
   // Key blocks' rows in chunks.  Without a window the first keys are seen by all rows, the

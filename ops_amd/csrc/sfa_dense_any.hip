@@ -1,4 +1,4 @@
-// gfx950 dense attention through a window (sfa_dense.h), any head dims up to 1024,
+// gfx950 dense attention through a window (sfa_dense.h), any head dims from 129 up to 1024,
 // bf16, float32 or 8-bit pages: every product in float32 on the matrix cores.
 //
 //   s_ij = scale q_i.k_j,  p = softmax over the rows that i sees,  o_i = sum_j p_ij v_j
@@ -13,60 +13,14 @@
 // makes 128 dims of its result: wider heads take several, which make the scores again.
 // Bound: the float32 matrix rate (154 TFLOP/s), with all rows staged twice or more.
 
-#include "sfa_dense.h"
+#include "sfa_dense_f32.h"
 
 namespace sfa {
 namespace {
 
-constexpr int kE = 1 << kAnyShift;  // entries a tile
 constexpr int kC = 64;              // dims staged at a time
 constexpr int kPitch = kC + 4;      // (floats; 4 rows apart, the lanes' groups meet different banks)
-static_assert(kE == 32 && kAnyRows == 64 && kAnyDims == 2 * kC, "four waves of 16 columns, two 16-entry products");
-
-struct fp8_t {
-  uint8_t x;
-};
-template <typename T>
-__device__ __forceinline__ float value_of(T x) {
-  if constexpr (std::is_same<T, fp8_t>::value) return __builtin_amdgcn_cvt_f32_fp8((int)x.x, 0);
-  else return to_f32(x);
-}
-// dims d .. d + 3 of a row of D, zeros past its end
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int d, int D, bool vec) {
-  f32x4 r = {};
-  if (vec) {  // (whole rows of 4)
-    if (d < D) {
-      if constexpr (sizeof(T) == 4) {
-        r = *reinterpret_cast<const f32x4*>(p + d);
-      } else if constexpr (sizeof(T) == 2) {
-        const bf16x4 x = *reinterpret_cast<const bf16x4*>(p + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = (float)x[e];
-      } else {
-        const int x = *reinterpret_cast<const int*>(p + d);
-        r = f32x4{__builtin_amdgcn_cvt_f32_fp8(x, 0), __builtin_amdgcn_cvt_f32_fp8(x, 1), __builtin_amdgcn_cvt_f32_fp8(x, 2),
-                  __builtin_amdgcn_cvt_f32_fp8(x, 3)};
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < D) r[e] = value_of(p[d + e]);
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, int d, int D, bool vec, const f32x4& x) {
-  if (vec && d < D) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p + d) = x;
-    else *reinterpret_cast<bf16x4*>(p + d) = bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < D) p[d + e] = from_f32<T>(x[e]);
-  }
-}
+static_assert(kAnyDims == 2 * kC, "two halves of a workgroup's dims");
 
 // The entries of a tile: element offsets of their rows in two tensors (-1: none)
 // and the rows' scales.
@@ -105,41 +59,29 @@ __device__ __forceinline__ void stage(Entries& e, const T* base, int which, int 
   }
 }
 
-// The lanes' columns: their rows held (up to 128 dims) or read again for every tile.
-template <typename T, bool HELD>
+// The lanes' columns: their rows, read again for every tile.
+template <typename T>
 struct Column {
   const T* p;
   int D;
   bool vec;
-  float sc;
-  f32x4 r[HELD ? 8 : 1];
-  __device__ __forceinline__ void init(const T* p_, int D_, bool vec_, int hq, float sc_ = 1.f) {
-    p = p_;
-    D = D_;
-    vec = vec_;
-    sc = sc_;
-    if constexpr (HELD) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) r[c] = p != nullptr ? load4(p, 16 * c + 4 * hq, D, vec) * sc : f32x4{};
-    }
-  }
+  __device__ __forceinline__ Column(const T* p_, int D_, bool vec_) : p(p_), D(D_), vec(vec_) {}
   __device__ __forceinline__ f32x4 at(int c, int hq) const {
-    if constexpr (HELD) return r[c];
-    else return p != nullptr ? load4(p, 16 * c + 4 * hq, D, vec) * sc : f32x4{};
+    return p != nullptr ? load4(p, 16 * c + 4 * hq, D, vec) : f32x4{};
   }
 };
 
 // s[mt] = products of entries 16 mt + 4 hq + k with the lane's column
-template <typename TE, typename TC, bool HELD>
-__device__ __forceinline__ void scores(Entries& e, const TE* base, int which, int D, bool vec, const Column<TC, HELD>& col,
+template <typename TE, typename TC>
+__device__ __forceinline__ void scores(Entries& e, const TE* base, int which, int D, bool vec, const Column<TC>& col,
                                        f32x4 (&s)[2], int lt, int hq) {
   s[0] = s[1] = f32x4{};
-  auto part = [&](int c0, auto first) {
+  for (int c0 = 0; c0 < D; c0 += kC) {
     stage<false>(e, base, which, c0, D, vec);
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const f32x4 b = col.at(HELD ? decltype(first)::value / 16 + c : c0 / 16 + c, hq);
+      const f32x4 b = col.at(c0 / 16 + c, hq);
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const f32x4 a = *reinterpret_cast<const f32x4*>(&e.t[16 * mt + lt][16 * c + 4 * hq]);
@@ -148,12 +90,6 @@ __device__ __forceinline__ void scores(Entries& e, const TE* base, int which, in
       }
     }
     __syncthreads();
-  };
-  if constexpr (HELD) {
-    part(0, std::integral_constant<int, 0>{});
-    if (D > kC) part(kC, std::integral_constant<int, kC>{});
-  } else {
-    for (int c0 = 0; c0 < D; c0 += kC) part(c0, std::integral_constant<int, 0>{});
   }
 }
 
@@ -199,20 +135,6 @@ __device__ __forceinline__ void sums(Entries& e, const TE* base, int which, int 
   }
 }
 
-// Query row r of (b, g) as a column.
-struct QRow {
-  int t, h, pos;  // pos: -1: no such row, or a token past the sequence's
-  bool in;        // a row of the tensor
-};
-__device__ __forceinline__ QRow q_row(const DenseParams& p, const DenseSeq& s, int g, int r) {
-  QRow x;
-  x.t = r / p.G;
-  x.h = g * p.G + r % p.G;
-  x.in = r < p.S * p.G;
-  x.pos = x.in && x.t < s.n ? s.ctx + x.t : -1;
-  return x;
-}
-
 // The keys of a tile as entries.
 template <typename TK>
 __device__ __forceinline__ void key_entries(const DenseParams& p, Entries& e, int b, int g, int j0) {
@@ -228,13 +150,7 @@ __device__ __forceinline__ void key_entries(const DenseParams& p, Entries& e, in
   }
 }
 
-// A tile that all rows of the block see whole (rows that are not there aside).
-__device__ __forceinline__ bool whole_tile(const DenseParams& p, const DenseItem& it, int j0) {
-  const int p0 = it.s.ctx + it.row0 / p.G, p1 = it.s.ctx + min((it.row0 + p.rows - 1) / p.G, it.s.n - 1);
-  return j0 + kE - 1 <= p0 && (j0 + kE <= p.first || p1 - j0 < p.window);
-}
-
-template <typename T, typename TK, bool HELD>
+template <typename T, typename TK>
 __global__ __launch_bounds__(256) void dense_any_fwd_kernel(DenseParams p) {
   __shared__ Entries e;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lt = lane & 15, hq = lane >> 4;
@@ -246,8 +162,7 @@ __global__ __launch_bounds__(256) void dense_any_fwd_kernel(DenseParams p) {
   if (!dense_item(p, wi / p.Hkv, wi % p.Hkv, it)) return;
   const int b = it.b, g = it.g, row = 16 * wave + lt;
   const QRow qr = q_row(p, it.s, g, it.row0 + row);
-  Column<T, HELD> q;
-  q.init(qr.pos >= 0 ? reinterpret_cast<const T*>(p.q) + b * p.q_sb + qr.t * p.q_ss + qr.h * p.q_sh : nullptr, p.Dqk, p.vec, hq);
+  const Column<T> q(qr.pos >= 0 ? reinterpret_cast<const T*>(p.q) + b * p.q_sb + qr.t * p.q_ss + qr.h * p.q_sh : nullptr, p.Dqk, p.vec);
   const TK* kp = reinterpret_cast<const TK*>(p.k);
   const TK* vp = reinterpret_cast<const TK*>(p.v);
   f32x4 acc[8];
@@ -310,7 +225,7 @@ __global__ __launch_bounds__(256) void dense_any_fwd_kernel(DenseParams p) {
   }
 }
 
-template <typename T, bool HELD>
+template <typename T>
 __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   __shared__ Entries e;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lt = lane & 15, hq = lane >> 4;
@@ -323,9 +238,8 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   const int b = it.b, g = it.g, r = it.row0 + 16 * wave + lt;
   const QRow qr = q_row(p, it.s, g, r);
   const bool live = qr.pos >= 0;
-  Column<T, HELD> q, go;
-  q.init(live ? reinterpret_cast<const T*>(p.q) + b * p.q_sb + qr.t * p.q_ss + qr.h * p.q_sh : nullptr, p.Dqk, p.vec, hq);
-  go.init(live ? reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qr.t * p.do_ss + qr.h * p.do_sh : nullptr, p.Dv, p.vec, hq);
+  const Column<T> q(live ? reinterpret_cast<const T*>(p.q) + b * p.q_sb + qr.t * p.q_ss + qr.h * p.q_sh : nullptr, p.Dqk, p.vec);
+  const Column<T> go(live ? reinterpret_cast<const T*>(p.dout) + b * p.do_sb + qr.t * p.do_ss + qr.h * p.do_sh : nullptr, p.Dv, p.vec);
   const int64_t rr = ((int64_t)b * p.Hkv + g) * p.S * p.G + r;
   const float lse = live ? p.row_lse[rr] : 0.f, delta = live ? p.row_delta[rr] : 0.f;
   const T* kp = reinterpret_cast<const T*>(p.k);
@@ -357,35 +271,29 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   for (int i = 0; i < 8; ++i) store4(o, dc * kAnyDims + 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);
 }
 
-// 64 keys a workgroup, 16 a wave; the rows of all heads that see them in order.
-template <typename T, bool HELD>
+// 64 keys a workgroup, 16 a wave; a chunk of the rows of all heads that see them, in order.
+template <typename T>
 __global__ __launch_bounds__(256) void dense_any_dkv_kernel(DenseParams p) {
   __shared__ Entries e;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lt = lane & 15, hq = lane >> 4;
   const int dmax = p.Dqk > p.Dv ? p.Dqk : p.Dv, ndc = (dmax + kAnyDims - 1) / kAnyDims;
-  int wi = blockIdx.x;  // (the first keys, which the most rows see, first)
-  const int dc = wi % ndc;
-  wi /= ndc;
-  const int g = wi % p.Hkv;
-  wi /= p.Hkv;
-  const int b = wi % p.B, j0 = wi / p.B * 64;
-  const DenseSeq s = dense_seq(p, b);
-  const int j = j0 + 16 * wave + lt;
+  const int dc = blockIdx.x % ndc;
+  KeyBlock kb;
+  if (!key_block(p, blockIdx.x / ndc, kb)) return;
+  const DenseSeq s = kb.s;
+  const int b = kb.b, g = kb.g, in = 16 * wave + lt, j = kb.kb * kAnyRows + in;
   const bool live = j < s.n;
-  Column<T, HELD> kc, vc;
-  kc.init(live ? reinterpret_cast<const T*>(p.k) + b * p.k_sb + j * p.k_ss + g * p.k_sh : nullptr, p.Dqk, p.vec, hq);
-  vc.init(live ? reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_ss + g * p.v_sh : nullptr, p.Dv, p.vec, hq);
+  const Column<T> kc(live ? reinterpret_cast<const T*>(p.k) + b * p.k_sb + j * p.k_ss + g * p.k_sh : nullptr, p.Dqk, p.vec);
+  const Column<T> vc(live ? reinterpret_cast<const T*>(p.v) + b * p.v_sb + j * p.v_ss + g * p.v_sh : nullptr, p.Dv, p.vec);
   const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_sb;
   const T* dop = reinterpret_cast<const T*>(p.dout) + b * p.do_sb;
   f32x4 dk[8], dv[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) dk[i] = dv[i] = f32x4{};
-  // the tokens that see one of the keys
-  const int t1 = j0 < p.first ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + 63 + p.window);
-  for (int r0 = j0 * p.G; r0 < t1 * p.G; r0 += kE) {
+  for (int r0 = kb.r0; r0 < kb.r1; r0 += kE) {
     if (tid < kE) {
       const int r = r0 + tid;
-      const QRow x = q_row(p, s, g, r);
+      const QRow x = q_row(p, s, g, r < kb.r1 ? r : p.S * p.G);
       const bool in = x.pos >= 0;
       const int64_t rr = ((int64_t)b * p.Hkv + g) * p.S * p.G + r;
       e.off[0][tid] = in ? x.t * p.q_ss + x.h * p.q_sh : -1;
@@ -410,40 +318,52 @@ __global__ __launch_bounds__(256) void dense_any_dkv_kernel(DenseParams p) {
     sums<true>(e, dop, 1, dc * kAnyDims, p.Dv, p.vec, w, dv, lt, hq);
     sums<true>(e, qp, 0, dc * kAnyDims, p.Dqk, p.vec, ds, dk, lt, hq);
   }
-  if (j >= p.S) return;
-  T* ok = reinterpret_cast<T*>(p.dk) + b * p.dk_sb + j * p.dk_ss + g * p.dk_sh;
-  T* ov = reinterpret_cast<T*>(p.dv) + b * p.dv_sb + j * p.dv_ss + g * p.dv_sh;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = dc * kAnyDims + 16 * i + 4 * hq;
-    store4(ok, d, p.Dqk, p.vec, dk[i] * p.scale);
-    store4(ov, d, p.Dv, p.vec, dv[i]);
+  store_dkv<T>(p, kb, in, dc * kAnyDims, dk, dv, hq);
+}
+
+// Blocks of several chunks: their sums in order, 4 dims of a key a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_any_join_kernel(DenseParams p) {
+  KeyBlock kb;
+  key_block(p, blockIdx.x * p.dkv_parts, kb);
+  if (kb.nc <= 1) return;
+  const int D = p.Dqk + p.Dv, per = (p.Dqk + 3) / 4 + (p.Dv + 3) / 4;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < kAnyRows * per; i += gridDim.y * 256) {
+    const int in = i / per, x = i % per, j = kb.kb * kAnyRows + in;
+    const bool isv = x >= (p.Dqk + 3) / 4;
+    const int d = 4 * (isv ? x - (p.Dqk + 3) / 4 : x), n = isv ? p.Dv : p.Dqk;
+    f32x4 s = {};
+#pragma unroll 4
+    for (int c = 0; c < kb.nc; ++c)
+      s += load4(kb.part + ((int64_t)c * kAnyRows + in) * D + (isv ? p.Dqk : 0), d, n, p.vec);
+    if (j >= p.S) continue;
+    T* o = isv ? reinterpret_cast<T*>(p.dv) + kb.b * p.dv_sb + j * p.dv_ss + kb.g * p.dv_sh
+               : reinterpret_cast<T*>(p.dk) + kb.b * p.dk_sb + j * p.dk_ss + kb.g * p.dk_sh;
+    store4(o, d, n, p.vec, isv ? s : s * p.scale);
   }
 }
 
 template <typename T, typename TK>
 void fwd(const DenseParams& p, hipStream_t s) {
   const unsigned grid = (unsigned)((int64_t)p.slots * p.Hkv * ((p.Dv + kAnyDims - 1) / kAnyDims));
-  if (p.Dqk <= 128) dense_any_fwd_kernel<T, TK, true><<<grid, 256, 0, s>>>(p);
-  else dense_any_fwd_kernel<T, TK, false><<<grid, 256, 0, s>>>(p);
+  dense_any_fwd_kernel<T, TK><<<grid, 256, 0, s>>>(p);
 }
 template <typename T>
 void bwd(const DenseParams& p, hipStream_t s) {
-  const int dmax = p.Dqk > p.Dv ? p.Dqk : p.Dv;
-  const unsigned gq = (unsigned)((int64_t)p.B * p.nrb * p.Hkv * ((p.Dqk + kAnyDims - 1) / kAnyDims));
-  const unsigned gk = (unsigned)((int64_t)((p.S + 63) / 64) * p.B * p.Hkv * ((dmax + kAnyDims - 1) / kAnyDims));
-  if (dmax <= 128) {
-    dense_any_dq_kernel<T, true><<<gq, 256, 0, s>>>(p);
-    dense_any_dkv_kernel<T, true><<<gk, 256, 0, s>>>(p);
+  const int64_t dmax = p.Dqk > p.Dv ? p.Dqk : p.Dv, blocks = (int64_t)((p.S + kAnyRows - 1) / kAnyRows) * p.B * p.Hkv;
+  if (dmax <= kAnyDims) {
+    launch_dense_held_bwd(p, sizeof(T) == 4, s);
   } else {
-    dense_any_dq_kernel<T, false><<<gq, 256, 0, s>>>(p);
-    dense_any_dkv_kernel<T, false><<<gk, 256, 0, s>>>(p);
+    dense_any_dq_kernel<T><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv * ((p.Dqk + kAnyDims - 1) / kAnyDims)), 256, 0, s>>>(p);
+    dense_any_dkv_kernel<T><<<(unsigned)(blocks * p.dkv_parts * ((dmax + kAnyDims - 1) / kAnyDims)), 256, 0, s>>>(p);
   }
+  if (p.dkv_parts > 1) dense_any_join_kernel<T><<<dim3((unsigned)blocks, 4), 256, 0, s>>>(p);
 }
 
 }  // namespace
 
 void launch_dense_any(const DenseParams& p, int dtype, int kv_dtype, hipStream_t s) {
+  if (p.Dqk <= kAnyDims && p.Dv <= kAnyDims) return launch_dense_held(p, dtype, kv_dtype, s);
   if (kv_dtype == SFA_DTYPE_FP8_E4M3) {
     if (dtype == SFA_DTYPE_F32) fwd<float, fp8_t>(p, s);
     else fwd<bf16, fp8_t>(p, s);

@@ -157,9 +157,10 @@ struct DenseParams {
   float* row_lse;
   float* row_delta;
   bool row_neg;
-  float* dkv_part;           // [B Hkv][dkv_parts][kDkvKeys][2 D] partial dK | dV of key blocks cut in chunks
+  float* dkv_part;           // partial dK | dV of key blocks cut in chunks: bf16 matrix kernels [B Hkv][dkv_parts]
+                             // [kDkvKeys][2 D], others [B Hkv][blocks][dkv_parts][kAnyRows][Dqk + Dv]
   int chunk, cut0, cut1, cut_chunk;  // query rows a chunk; of the key blocks [cut0, cut1)
-  int dkv_parts;             // partials a kv head
+  int dkv_parts;             // partials a kv head; others: chunks of a block, at most
 };
 constexpr int kDenseUnits = 256;  // row blocks of a launch that is cut into ranges, at most
 struct DensePlan {
@@ -186,6 +187,9 @@ hipError_t launch_dense_bwd(const DenseParams& p, const DenseBwdPlan& pl, int dt
 constexpr int kAnyRows = 64, kAnyShift = 5, kAnyDims = 128;
 void launch_dense_any(const DenseParams& p, int dtype, int kv_dtype, hipStream_t s);
 void launch_dense_bwd_any(const DenseParams& p, int dtype, hipStream_t s);
+// ... up to 128 dims (sfa_dense_held.hip)
+void launch_dense_held(const DenseParams& p, int dtype, int kv_dtype, hipStream_t s);
+void launch_dense_held_bwd(const DenseParams& p, bool f32, hipStream_t s);
 
 // bf16 queries, head dims 64 and 128, many rows (sfa_dense_wide.hip)
 constexpr int kWideRows = 256;
