@@ -227,6 +227,7 @@ __global__ __launch_bounds__(256, NG == 4 ? 1 : 2) void dense_few_kernel(DensePa
     return bad;
   };
   auto add_bad = [&](uint32_t bad, int j0, const bf16x8 (&pb)[NG], const bf16x8 (&pr)[NG]) {
+    const DenseParams& p = late_params();
     for (; bad != 0; bad &= bad - 1) {
       const int key = __builtin_ctz(bad), at = 4 * (key >> 4) + (key & 3);
       const int64_t vo = dense_row(p, b, j0 + key, p.v_sb, p.v_ss);
@@ -399,26 +400,27 @@ __global__ __launch_bounds__(256, NG == 4 ? 1 : 2) void dense_few_kernel(DensePa
     }
   }
   if (wk != 0) return;
+  const DenseParams& pe = late_params();
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const int row = 16 * i + lt, r = it.row0 + row, t = r / p.G, h = g * p.G + r % p.G;
-    if (r >= p.S * p.G) continue;
+    const int row = 16 * i + lt, r = it.row0 + row, t = r / pe.G, h = g * pe.G + r % pe.G;
+    if (r >= pe.S * pe.G) continue;
     float lse, f;
     if (it.partial) {
       f = dense_part(m_used[i], l_part[i], lse);
-      if (hq == 0) p.part_lse[it.part + row] = lse;
+      if (hq == 0) pe.part_lse[it.part + row] = lse;
     } else {
-      f = dense_finish(p, h, pos[i] >= 0, m_used[i], l_part[i], lse);
-      if (hq == 0) p.lse[b * p.l_sb + t * p.l_ss + h * p.l_sh] = lse;
+      f = dense_finish(pe, h, pos[i] >= 0, m_used[i], l_part[i], lse);
+      if (hq == 0) pe.lse[b * pe.l_sb + t * pe.l_ss + h * pe.l_sh] = lse;
     }
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
       const f32x4 y = oacc[i][o] * f, x = f == 0.f ? f32x4{} : y;
       const int d = 16 * o + 4 * hq;
       if (it.partial) {
-        *reinterpret_cast<f32x4*>(p.part_o + (it.part + row) * D + d) = x;
+        *reinterpret_cast<f32x4*>(pe.part_o + (it.part + row) * D + d) = x;
       } else {
-        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + d) =
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(pe.out) + b * pe.o_sb + t * pe.o_ss + h * pe.o_sh + d) =
             bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
       }
     }

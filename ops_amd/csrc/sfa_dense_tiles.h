@@ -151,9 +151,9 @@ struct TileSource {
           const int q = wave * NI + k, left = ok ? rows - q * RPI : 0;
           // (rows past the last one read some row's chunks: no row of the result sees them)
           const bool there = sub < left;
-          const uint64_t step = left > 0 ? (uint64_t)(q * RPI) : 0;
-          dense_dma16(kt + q * Tile<D>::GROUP, kb + step * (uint64_t)krow, there ? ko : c);
-          dense_dma16(vt + q * Tile<D>::GROUP, vb + step * (uint64_t)vrow, there ? vo : c);
+          const uint32_t step = left > 0 ? (uint32_t)(q * RPI) : 0;  // (times a stride: below 2^31)
+          dense_dma16(kt + q * Tile<D>::GROUP, kb + step * (uint32_t)krow, there ? ko : c);
+          dense_dma16(vt + q * Tile<D>::GROUP, vb + step * (uint32_t)vrow, there ? vo : c);
         }
       }
       mask = !ok ? 0 : rows >= KT ? ~0ull : (1ull << rows) - 1;
@@ -315,6 +315,16 @@ struct RowsOut {
     }
   }
 };
+
+// The kernel's arguments, loaded where they are used from here on: those that only the results
+// need would be held across the loop (scalar registers spill to lanes of vector ones).  1 to 3% in
+// the kernels that use it; the one over latent rows is 3% faster without.
+__device__ __forceinline__ const DenseParams& late_params() {
+  typedef const __attribute__((address_space(4))) DenseParams* args_t;
+  uint64_t a = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const DenseParams*)(args_t)a;
+}
 
 // Where the workgroup's share of a launch is: the row blocks of a (sequence, kv head)
 // on one XCD (workgroup i is on XCD i % 8), whose L2 their keys then stay in; the

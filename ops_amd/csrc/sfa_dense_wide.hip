@@ -246,6 +246,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   // ---- results: lane holds row lr, dims 32 o + 8 i + 4 hq + 0 .. 3 --------------------
   dense_barrier();  // the tiles are read
   {  // (what follows is formed now: held across the loop it spills)
+    const DenseParams& p = late_params();
     int ln = lane;
     asm volatile("" : "+v"(ln));
     const int lr = ln & 31, hq = ln >> 5, row = 32 * wave + lr, r = it.row0 + row, t = r / p.G, h = g * p.G + r % p.G;
