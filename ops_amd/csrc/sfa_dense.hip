@@ -98,7 +98,8 @@ void combine(const DenseParams& p, hipStream_t s) {
   else dense_combine_kernel<T, 64><<<grid, 256, 0, s>>>(p, jr, jd);
 }
 
-// ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse ------------
+// ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse (the bf16 matrix
+// kernels' dq makes its own) ------------
 // 16 lanes a row.  Rows that see nothing get +inf, which makes every weight 0.
 template <typename T>
 __global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
@@ -112,15 +113,7 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
   if (live) {
     const T* o = reinterpret_cast<const T*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh;
     const T* go = reinterpret_cast<const T*>(p.dout) + b * p.do_sb + t * p.do_ss + h * p.do_sh;
-    if (p.vec && sizeof(T) == 2) {
-      for (int d = 8 * lane; d < p.Dv; d += 128) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(o + d), c = *reinterpret_cast<const bf16x8*>(go + d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf((float)a[e], (float)c[e], sum);
-      }
-    } else {
-      for (int d = lane; d < p.Dv; d += 16) sum = fmaf(to_f32(o[d]), to_f32(go[d]), sum);
-    }
+    for (int d = lane; d < p.Dv; d += 16) sum = fmaf(to_f32(o[d]), to_f32(go[d]), sum);
   }
 #pragma unroll
   for (int s = 1; s < 16; s <<= 1) sum += __shfl_xor(sum, s, 64);
@@ -128,13 +121,8 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
   const int64_t li = b * p.l_sb + t * p.l_ss + h * p.l_sh;
   const float lse = live ? p.lse[li] : kNegInf;
   const float delta = live ? sum - (p.dlse != nullptr ? p.dlse[li] : 0.f) : 0.f;
-  if (p.row_neg) {
-    p.row_lse[rr] = lse == kNegInf ? kNegInf : -lse / p.scale;
-    p.row_delta[rr] = -delta;
-  } else {
-    p.row_lse[rr] = lse == kNegInf ? -kNegInf : lse * kLog2e;
-    p.row_delta[rr] = delta;
-  }
+  p.row_lse[rr] = lse == kNegInf ? -kNegInf : lse * kLog2e;
+  p.row_delta[rr] = delta;
 }
 
 // dsink[h] = -sum over the rows of exp(sink - lse) delta, a workgroup a head, in a fixed order.
@@ -317,11 +305,6 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
 hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int dtype, hipStream_t s) {
   DenseParams p = p0;
   p.row_neg = pl.mfma;
-  const int64_t rows = (int64_t)p.B * p.Hkv * p.S * p.G;
-  const unsigned grid = (unsigned)((rows + 15) / 16);
-  if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p);
-  else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
-  if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
   DensePlan q{};
   q.rows = pl.mfma ? kWideRows : kAnyRows;
   q.tile_shift = pl.mfma ? 6 : kAnyShift;
@@ -332,8 +315,15 @@ hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int d
   p.cut1 = pl.cut1;
   p.cut_chunk = pl.cut_chunk;
   p.dkv_parts = pl.parts;
-  if (pl.mfma) launch_dense_bwd_mfma(p, pl.units, s);
-  else launch_dense_bwd_any(p, dtype, s);
+  if (pl.mfma) {  // (whose dq kernel leaves the rows' statistics)
+    launch_dense_bwd_mfma(p, pl.units, s);
+  } else {
+    const unsigned grid = (unsigned)(((int64_t)p.B * p.Hkv * p.S * p.G + 15) / 16);
+    if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p);
+    else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
+    launch_dense_bwd_any(p, dtype, s);
+  }
+  if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
   return hipGetLastError();
 }
 

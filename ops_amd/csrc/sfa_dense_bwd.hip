@@ -54,7 +54,31 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
       ob[s] = live ? y : bf16x8{};
     }
   }
-  const float moff = live ? p.row_lse[rr] * p.scale_log2 : kNegInf, ndelta = live ? p.row_delta[rr] : 0.f;
+  // The row's statistics, which the dk / dv kernel's accumulators start from: -lse / scale
+  // (nothing seen: -inf, which makes every weight 0) and -delta.
+  float moff = kNegInf, ndelta = 0.f;
+  {
+    const bf16* o = reinterpret_cast<const bf16*>(p.out) + b * p.o_sb + (live ? t * p.o_ss + h * p.o_sh : 0) + 8 * hq;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(o + 16 * s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e & 1] = fmaf((float)x[e], (float)ob[s][e], sum[e & 1]);
+    }
+    const float all = xor32_sum(sum[0] + sum[1]);
+    if (live) {
+      const int64_t li = b * p.l_sb + t * p.l_ss + h * p.l_sh;
+      const float lse = p.lse[li];
+      moff = lse == kNegInf ? kNegInf : -lse / p.scale;
+      ndelta = (p.dlse != nullptr ? p.dlse[li] : 0.f) - all;
+    }
+    if (in && hq == 0) {
+      p.row_lse[rr] = moff;
+      p.row_delta[rr] = ndelta;
+    }
+    moff *= p.scale_log2;
+  }
 
   TileSource<D, NW, false, true> src(p, it, wave, lane);
   const int n = it.v1 - it.v0;
