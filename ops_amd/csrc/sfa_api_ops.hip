@@ -467,6 +467,7 @@ int sfa_dense_bwd(const sfa_dense_bwd_args* a, void* workspace, size_t workspace
   p.row_lse = (float*)workspace;
   p.row_delta = (float*)((char*)workspace + pl.row_bytes / 2);
   p.dkv_part = (float*)((char*)workspace + pl.row_bytes);
+  p.dkv_units = (int*)((char*)workspace + pl.row_bytes + pl.dkv_bytes);
   return done(sfa::launch_dense_bwd(p, pl, a->fwd.dtype, (hipStream_t)stream), "sfa_dense_bwd");
 }
 

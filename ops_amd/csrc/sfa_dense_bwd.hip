@@ -22,6 +22,109 @@ namespace {
 typedef Mfma<32> M;
 typedef f32x16 acc_t;
 
+// ---- units of the dk / dv kernel -----------------------------------------------------------
+// A key block's rows are one range of r = t G + h; blocks that many rows see are cut in
+// chunks of p.chunk rows, which leave partial sums that dense_dkv_join_kernel adds in order.
+struct DkvUnit {
+  int kb;          // key block, or -1: none
+  int r0, r1;      // its rows (of the longest sequence)
+  int part, nc;    // first partial of the block (if nc > 1), chunks
+  int c;
+};
+__device__ __forceinline__ int dkv_tokens(const DenseParams& p, int j0) {  // tokens that see a key of the block at j0
+  return j0 < p.first ? p.S : (int)min((int64_t)p.S, (int64_t)j0 + kDkvKeys - 1 + p.window);
+}
+__device__ __forceinline__ int dkv_chunk(const DenseParams& p, int kb) {
+  return kb >= p.cut0 && kb < p.cut1 ? p.cut_chunk : p.chunk;
+}
+__device__ __forceinline__ int dkv_chunks(const DenseParams& p, int kb) {
+  const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
+  const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
+  return (int)((rows + chunk - 1) / chunk);
+}
+// Chunk c of key block kb.  Chunks are counted from the last row that sees the block, so
+// that without a window those of all blocks begin and end at the same rows.
+__device__ __forceinline__ void dkv_rows(const DenseParams& p, DkvUnit& x) {
+  const int j0 = x.kb * kDkvKeys, chunk = dkv_chunk(p, x.kb);
+  const int64_t first = (int64_t)j0 * p.G, last = (int64_t)dkv_tokens(p, j0) * p.G, end = last - (int64_t)x.c * chunk;
+  x.r1 = (int)end;
+  x.r0 = (int)max(first, end - chunk);
+}
+// The units of a (sequence, kv head), in the order of their launch: the longest first, so that the
+// card's last ones are short; those of a full chunk in order of the chunk, then of the block, so
+// that what runs at once reads the same rows (a block's chunks after one another: 0.26 of the
+// reads in L2).  One workgroup beside those of dq counts for each unit how many come before it
+// (in each workgroup of the dk / dv kernel the search took 54 of its 530 us).  More blocks than
+// kSorted: in order of the blocks.
+constexpr int kSorted = 4096;
+__device__ __forceinline__ void dkv_units(const DenseParams& p, int* lds) {
+  const int nkb = (p.S + kDkvKeys - 1) / kDkvKeys, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int* const s_whole = lds;            // chunks of the block's full size
+  int* const s_rest = lds + kSorted;   // rows of its shorter one
+  int* const s_sum = lds + 2 * kSorted;  // [8 waves][2]
+  int* const s_at = s_sum + 16;          // of 512 blocks: the first unit, the first partial, chunks
+  const bool sorted = nkb <= kSorted;
+  auto cut = [&](int kb) { return kb >= p.cut0 && kb < p.cut1; };
+  if (sorted) {
+    for (int kb = tid; kb < nkb; kb += 512) {
+      const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
+      const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
+      s_whole[kb] = (int)(rows / chunk);
+      s_rest[kb] = (int)(rows - rows / chunk * chunk);
+    }
+    dense_barrier();
+  }
+  auto place = [&](int kb, int c0, int step, const int* at0) {
+    const int nc = at0[2];
+    for (int c = c0; c < nc; c += step) {
+      int at = at0[0] + c;
+      if (sorted) {
+        const bool full = c < s_whole[kb], mine = cut(kb);
+        const int size = full ? dkv_chunk(p, kb) : s_rest[kb];
+        at = full && mine ? c : 0;
+#pragma unroll 4
+        for (int k = 0; k < nkb; ++k) {
+          const int whole = s_whole[k], rest = s_rest[k];
+          if (!cut(k)) at += full && !mine ? min(whole, c) + (k < kb && whole > c ? 1 : 0) : whole;
+          else if (!full || mine) at += full ? (k < kb ? whole : 0) : p.cut_chunk >= size ? whole : 0;
+          if (!full || mine) at += rest > size || (!full && rest == size && k < kb) ? 1 : 0;
+        }
+      }
+      *reinterpret_cast<int4*>(p.dkv_units + 4 * (int64_t)at) = int4{kb, c, at0[1], nc};
+    }
+  };
+  int before = 0, parts = 0;  // of the blocks so far
+  for (int k0 = 0; k0 < nkb; k0 += 512) {
+    const int kb = k0 + tid, nc = kb < nkb ? dkv_chunks(p, kb) : 0, np = nc > 1 ? nc : 0;
+    int x = nc, y = np;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int xx = __shfl_up(x, o, 64), yy = __shfl_up(y, o, 64);
+      x += lane >= o ? xx : 0;
+      y += lane >= o ? yy : 0;
+    }
+    if (lane == 63) {
+      s_sum[2 * wave] = x;
+      s_sum[2 * wave + 1] = y;
+    }
+    dense_barrier();
+    int first = before + x - nc, part = parts + y - np;
+    for (int w = 0; w < 8; ++w) {
+      first += w < wave ? s_sum[2 * w] : 0;
+      part += w < wave ? s_sum[2 * w + 1] : 0;
+      before += s_sum[2 * w];
+      parts += s_sum[2 * w + 1];
+    }
+    s_at[3 * tid] = first;
+    s_at[3 * tid + 1] = part;
+    s_at[3 * tid + 2] = nc;
+    dense_barrier();
+    // (as many threads a block as there are)
+    const int blocks = min(512, nkb - k0), sub = 512 / blocks, in = tid / sub;
+    if (in < blocks) place(k0 + in, tid % sub, sub, s_at + 3 * in);  // (s_at: written again behind the next scan's barrier)
+  }
+}
+
 // ---- dq: eight waves of 32 query rows, tiles of 64 keys -------------------------------
 template <int D>
 __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
@@ -32,6 +135,8 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, hq = lane >> 5;
+  static_assert(sizeof(s_kv) >= (2 * kSorted + 16 + 3 * 512) * sizeof(int), "the units' counts");
+  if (blockIdx.x == gridDim.x - 1) return dkv_units(p, reinterpret_cast<int*>(s_kv));
   int slot, g;
   if (!dense_place(p, slot, g)) return;
   DenseItem it;
@@ -214,127 +319,6 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
 }
 
 // ---- dk and dv: 128 keys, tiles of 32 query rows of all heads ----------------------------
-// A key block's rows are one range of r = t G + h; blocks that many rows see are cut in
-// chunks of p.chunk rows, which leave partial sums that dense_dkv_join_kernel adds in order.
-struct DkvUnit {
-  int kb;          // key block, or -1: none
-  int r0, r1;      // its rows (of the longest sequence)
-  int part, nc;    // first partial of the block (if nc > 1), chunks
-  int c;
-};
-__device__ __forceinline__ int dkv_tokens(const DenseParams& p, int j0) {  // tokens that see a key of the block at j0
-  return j0 < p.first ? p.S : (int)min((int64_t)p.S, (int64_t)j0 + kDkvKeys - 1 + p.window);
-}
-__device__ __forceinline__ int dkv_chunk(const DenseParams& p, int kb) {
-  return kb >= p.cut0 && kb < p.cut1 ? p.cut_chunk : p.chunk;
-}
-__device__ __forceinline__ int dkv_chunks(const DenseParams& p, int kb) {
-  const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
-  const int64_t rows = (int64_t)(dkv_tokens(p, j0) - j0) * p.G;
-  return (int)((rows + chunk - 1) / chunk);
-}
-// Chunk c of key block kb.  Chunks are counted from the last row that sees the block, so
-// that without a window those of all blocks begin and end at the same rows.
-__device__ __forceinline__ void dkv_rows(const DenseParams& p, DkvUnit& x) {
-  const int j0 = x.kb * kDkvKeys, chunk = dkv_chunk(p, x.kb);
-  const int64_t first = (int64_t)j0 * p.G, last = (int64_t)dkv_tokens(p, j0) * p.G, end = last - (int64_t)x.c * chunk;
-  x.r1 = (int)end;
-  x.r0 = (int)max(first, end - chunk);
-}
-// Unit u of a (sequence, kv head): the longest first, so that the card's last ones are
-// short; those of a full chunk in order of the chunk, then of the block, so that what runs
-// at once reads the same rows (a block's chunks after one another: 0.26 of the reads in L2).
-// Up to 256 key blocks: a thread for each one's full chunks and one for its rest.
-struct DkvSort {
-  int size[512], num[512], nc[256];
-  int unit[4];  // block, chunk, first partial, chunks of the block
-};
-__device__ __forceinline__ DkvUnit dkv_unit_sorted(const DenseParams& p, int u, DkvSort& sort) {
-  const int nkb = (p.S + kDkvKeys - 1) / kDkvKeys, tid = threadIdx.x, kb = tid >> 1;
-  int size = 0, num = 0, nc = 0;
-  if (kb < nkb) {
-    const int j0 = kb * kDkvKeys, chunk = dkv_chunk(p, kb);
-    const int rows = (dkv_tokens(p, j0) - j0) * p.G, whole = rows / chunk, rest = rows - whole * chunk;
-    nc = whole + (rest > 0 ? 1 : 0);
-    size = tid & 1 ? rest : chunk;
-    num = tid & 1 ? (rest > 0 ? 1 : 0) : whole;
-    if ((tid & 1) == 0) sort.nc[kb] = nc;
-  }
-  sort.size[tid] = size;
-  sort.num[tid] = num;
-  if (tid < 4) sort.unit[tid] = -1;
-  dense_barrier();
-  // the full ones: thread c counts those of chunks 0 .. c - 1
-  int before = 0, here = 0, all = 0;
-  for (int i = 0; i < 2 * nkb; i += 2) {
-    const int m = sort.size[i] == p.chunk ? sort.num[i] : 0;
-    before += min(m, tid);
-    here += m > tid ? 1 : 0;
-    all += m;
-  }
-  if (u < all) {
-    if (u >= before && u < before + here) {
-      int k = u - before, i = 0;
-      for (; i < 2 * nkb; i += 2)
-        if (sort.size[i] == p.chunk && sort.num[i] > tid && k-- == 0) break;
-      sort.unit[0] = i >> 1;
-      sort.unit[1] = tid;
-      sort.unit[3] = sort.nc[i >> 1];
-    }
-  } else if (num > 0 && size < p.chunk) {
-    int first = all;
-    for (int i = 0; i < 2 * nkb; ++i) {
-      const int s = sort.size[i];
-      first += s < p.chunk && (s > size || (s == size && i < tid)) ? sort.num[i] : 0;
-    }
-    if (u >= first && u < first + num) {
-      sort.unit[0] = kb;
-      sort.unit[1] = tid & 1 ? nc - 1 : u - first;
-      sort.unit[3] = nc;
-    }
-  }
-  dense_barrier();
-  DkvUnit x{sort.unit[0], 0, 0, 0, sort.unit[3], sort.unit[1]};
-  if (x.kb >= 0) {
-    for (int k = 0; k < x.kb; ++k) x.part += sort.nc[k] > 1 ? sort.nc[k] : 0;
-    dkv_rows(p, x);
-  }
-  dense_barrier();  // (its place in LDS is loaded over)
-  return x;
-}
-// ... in order of the keys
-__device__ __forceinline__ DkvUnit dkv_unit(const DenseParams& p, int u) {
-  const int lane = threadIdx.x & 63, nkb = (p.S + kDkvKeys - 1) / kDkvKeys;
-  int before = 0, parts = 0;
-  for (int k0 = 0; k0 < nkb; k0 += 64) {
-    const int kb = k0 + lane, nc = kb < nkb ? dkv_chunks(p, kb) : 0, np = nc > 1 ? nc : 0;
-    int incl = nc, pin = np;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(incl, o, 64), z = __shfl_up(pin, o, 64);
-      if (lane >= o) {
-        incl += y;
-        pin += z;
-      }
-    }
-    const int first = before + incl - nc;
-    const uint64_t hit = __ballot(u >= first && u < first + nc);
-    if (hit != 0) {
-      const int w = __builtin_ctzll(hit);
-      DkvUnit x;
-      x.kb = k0 + w;
-      x.nc = __builtin_amdgcn_readlane(nc, w);
-      x.c = u - __builtin_amdgcn_readlane(first, w);
-      x.part = __builtin_amdgcn_readlane(parts + pin - np, w);
-      dkv_rows(p, x);
-      return x;
-    }
-    before += __builtin_amdgcn_readlane(incl, 63);
-    parts += __builtin_amdgcn_readlane(pin, 63);
-  }
-  return DkvUnit{-1, 0, 0, 0, 0, 0};
-}
-
 // Waves 0 .. 3 make p and ds of 32 rows x 128 keys (each 16 rows x 64 keys, 16x16x32: an
 // operand of Q or dO read from LDS serves 64 keys) and leave them in LDS as bf16, in operand
 // order; waves 4 .. 7, one on each SIMD beside one of those, take the last step's for the
@@ -359,11 +343,10 @@ __global__ __launch_bounds__(512, 2) void dense_dkv_kernel(DenseParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = p.B * p.Hkv, gi = blockIdx.x % groups;
   const int b = gi / p.Hkv, g = gi % p.Hkv;
-  static_assert(sizeof(DkvSort) <= sizeof(s_row), "the units are sorted where the rows come later");
-  const bool sorted = p.S <= 256 * kDkvKeys && (int64_t)p.S * p.G <= 512 * (int64_t)p.chunk;
-  const DkvUnit un = sorted ? dkv_unit_sorted(p, blockIdx.x / groups, *reinterpret_cast<DkvSort*>(s_row)) : dkv_unit(p, blockIdx.x / groups);
+  const int4 unit = *reinterpret_cast<const int4*>(p.dkv_units + 4 * (int64_t)(blockIdx.x / groups));
+  DkvUnit un{unit.x, 0, 0, unit.z, unit.w, unit.y};
+  dkv_rows(p, un);
   const int kb = __builtin_amdgcn_readfirstlane(un.kb);
-  if (kb < 0) return;
   const DenseSeq sq = dense_seq(p, b);
   const int end = min(__builtin_amdgcn_readfirstlane(un.r1), sq.n * p.G), begin = __builtin_amdgcn_readfirstlane(un.r0);
   const int nc = __builtin_amdgcn_readfirstlane(un.nc), part = __builtin_amdgcn_readfirstlane(un.part + un.c);
@@ -699,7 +682,7 @@ __global__ __launch_bounds__(256) void dense_dkv_join_kernel(DenseParams p) {
 
 template <int D>
 void launch(const DenseParams& p, int units, hipStream_t s) {
-  dense_dq_kernel<D><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv), 512, 0, s>>>(p);
+  dense_dq_kernel<D><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv + 1), 512, 0, s>>>(p);
   dense_dkv_kernel<D><<<(unsigned)((int64_t)units * p.B * p.Hkv), 512, 0, s>>>(p);
   if (p.dkv_parts > 0)
     dense_dkv_join_kernel<D><<<dim3((unsigned)((p.S + kDkvKeys - 1) / kDkvKeys * p.B * p.Hkv), 4), 256, 0, s>>>(p);

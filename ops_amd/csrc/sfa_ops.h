@@ -159,6 +159,7 @@ struct DenseParams {
   bool row_neg;
   float* dkv_part;           // partial dK | dV of key blocks cut in chunks: bf16 matrix kernels [B Hkv][dkv_parts]
                              // [kDkvKeys][2 D], others [B Hkv][blocks][dkv_parts][kAnyRows][Dqk + Dv]
+  int* dkv_units;            // [units][4] block, chunk, first partial, chunks of the block, in order of the launch
   int chunk, cut0, cut1, cut_chunk;  // query rows a chunk; of the key blocks [cut0, cut1)
   int dkv_parts;             // partials a kv head; others: chunks of a block, at most
 };
@@ -176,10 +177,10 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype);
 hipError_t launch_dense(const DenseParams& p, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s);
 constexpr int kDkvKeys = 128;  // keys a block of the dk / dv kernel
 struct DenseBwdPlan {
-  size_t row_bytes, dkv_bytes;  // row_lse + row_delta; partial dK | dV
+  size_t row_bytes, dkv_bytes, unit_bytes;  // row_lse + row_delta; partial dK | dV; the units
   int chunk, cut0, cut1, cut_chunk, units, parts;  // of the dk / dv kernel: as above; units and partials a kv head
   bool mfma, fits;
-  size_t workspace() const { return row_bytes + dkv_bytes; }
+  size_t workspace() const { return row_bytes + dkv_bytes + unit_bytes; }
 };
 DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype);
 hipError_t launch_dense_bwd(const DenseParams& p, const DenseBwdPlan& pl, int dtype, hipStream_t s);

@@ -156,6 +156,23 @@ def test_key_blocks_cut_in_chunks(dtype, S, heads, D, window):
     _check(_leaves(dtype, B=1, S=S, Hq=heads[0], Hkv=heads[1], D=D), window=window, first=5 if window else 0)
 
 
+def test_more_key_blocks_than_are_sorted():
+    """A window of one: a token's result is its own v, its gradients are do for v and zero for q and
+    k (the only weight is 1), exactly; blocks of 128 keys, some rows padded."""
+    S, n = 4096 * 128 + 300, 4096 * 128 + 171
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q, k, v, do = (torch.randn(1, S, 1, 64, generator=g, device=DEV).to(BF) for _ in range(4))
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    xs = [t.requires_grad_(True) for t in (q, k, v)]
+    out, _ = ops_amd.window_attention(*xs, window=1, lens=lens)
+    dq, dk, dv = torch.autograd.grad(out, xs, do)
+    assert torch.equal(out[:, :n], v[:, :n]) and torch.equal(dv[:, :n], do[:, :n])
+    assert not out[:, n:].any() and not dv[:, n:].any() and not dq[:, n:].any() and not dk[:, n:].any()
+    # (ds = do.v - do.o: 64 products of float32 in two orders, times a row of up to 6)
+    mag = (do.float() * v.detach().float()).abs().sum(-1).max()
+    assert float(torch.stack((dq, dk)).abs().max()) <= 128 * 2.0 ** -24 * float(mag) * 6
+
+
 def test_padded_rows_in_chunks():
     x = _leaves(F32, B=2, S=600, Hq=8, Hkv=1, D=64)
     lens = torch.tensor([600, 33], dtype=torch.int32, device=DEV)
