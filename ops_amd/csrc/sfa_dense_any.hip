@@ -11,7 +11,9 @@
 // leaves a lane with 4 entries of one column, which are the second operand of the
 // sums' product as they are, its first being the staged rows read down a dim.  A workgroup
 // makes 128 dims of its result: wider heads take several, which make the scores again.
-// Bound: the float32 matrix rate (154 TFLOP/s), with all rows staged twice or more.
+// Bound: the float32 matrix rate (153 TFLOP/s), with all rows staged twice or more, each time
+// between two barriers that wait for its loads: 16 TFLOP/s over latent rows (512 tokens behind
+// 14336, 16 heads: 15.7 ms).
 
 #include "sfa_dense_f32.h"
 
@@ -247,6 +249,7 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   f32x4 acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = f32x4{};
+  float dsum = 0.f;  // sum_j p_ij do_i.v_j: delta again, of o before its rounding
   for (int v = it.v0; v < it.v1; ++v) {
     const int j0 = it.tiles.tile(v) << kAnyShift;
     key_entries<T>(p, e, b, g, j0);
@@ -260,12 +263,17 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
       for (int k = 0; k < 4; ++k) {
         const int en = 16 * mt + 4 * hq + k;
         const bool ok = e.off[0][en] >= 0 && live && dense_seen(p, j0 + en, qr.pos);
-        s[mt][k] = ok ? exp2f(fmaf(s[mt][k], p.scale_log2, -lse)) * (dp[mt][k] - delta) : 0.f;
+        const float w = ok ? exp2f(fmaf(s[mt][k], p.scale_log2, -lse)) : 0.f;
+        dsum += ok ? w * dp[mt][k] : 0.f;
+        s[mt][k] = ok ? w * (dp[mt][k] - delta) : 0.f;
       }
     if (whole_tile(p, it, j0)) sums<false>(e, kp, 0, dc * kAnyDims, p.Dqk, p.vec, s, acc, lt, hq);
     else sums<true>(e, kp, 0, dc * kAnyDims, p.Dqk, p.vec, s, acc, lt, hq);
   }
+  dsum += __shfl_xor(dsum, 16, 64);
+  dsum = xor32_sum(dsum);
   if (!qr.in) return;
+  if (live && hq == 0 && dc == 0) p.row_delta[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
   T* o = reinterpret_cast<T*>(p.dq) + b * p.dq_sb + qr.t * p.dq_ss + qr.h * p.dq_sh;
 #pragma unroll
   for (int i = 0; i < 8; ++i) store4(o, dc * kAnyDims + 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);

@@ -5,14 +5,19 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
 //
 // Two kernels, each of which makes the scores again, so that every sum has a fixed
-// order without atomics: seven products for the five that are needed.  Products of 32 x
-// 32 (32x32x16): a lane holds 16 scores of one column (dq: a query row; dk, dv: a key),
-// which rounded to bf16 are the second operand of the sums' products as they are;
-// the first is read from LDS transposed.  A step makes the scores of the next 32 entries
-// beside the weights of this one's, then its sums.  Each wave reads every entry's rows
-// as rows and again transposed: a kilobyte of LDS a product, as much as four SIMDs can
-// take at once, which bounds both kernels together with the products.  p and ds are
-// rounded to bf16 once for their products (2^-8 of each); sums are float32.
+// order without atomics: seven products for the five that are needed.
+//
+// dq: products of 32 x 32 (32x32x16) leave a lane with 16 scores of its query row, which
+// rounded to bf16 are the second operand of the sums' product as they are; the first is read
+// from LDS transposed.  A step makes the scores of the next 32 keys beside the weights of this
+// one's, then its sums.  Each wave reads every key's rows as rows and K's again transposed: a
+// kilobyte of LDS a product, as much as four SIMDs can take at once, which bounds it together
+// with the products.  dk, dv: see there.  p and ds are rounded to bf16 once for their products
+// (2^-8 of each; results 0.0026 rms from float64 where their own rounding is 0.0017: two parts
+// would be half of the products again); sums are float32.
+//
+// 8192 tokens, window 1024, 32 / 8 heads of 128: dq 275 us (0.75 PF/s of its three products), dk
+// and dv 505 (0.54 PF/s of their four); 2 x 4096 tokens without a window, 32 / 2 heads: 405, 765.
 
 #include "sfa_dense_tiles.h"
 
@@ -233,6 +238,9 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
   int st = 0;
   // half 0: sums of keys 0 .. 31 of tile j, scores of its keys 32 .. 63; half 1: sums of
   // those, scores of tile j + 1's first 32
+  // sum_j p_ij do_i.v_j: delta again, but of o before its rounding to bf16 (of dsink, a float32
+  // sum, that rounding is most of the error: 0.003 of it)
+  float dsum = 0.f;
   auto half = [&](int j, auto hc, acc_t& cs, acc_t& cd, acc_t& ns, acc_t& nd) {
     constexpr int H = decltype(hc)::value;
     const int st1 = (st + 1) & (NS - 1);
@@ -283,6 +291,8 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
         if constexpr (e * (NM - OT) / 16 == i) {
           const float w = __builtin_amdgcn_exp2f(fmaf(cs[e], p.scale_log2, moff));
           const float x = w * (cd[e] + ndelta);
+          dsum = fmaf(w, cd[e], dsum);
+          asm volatile("" : "+v"(dsum));  // (added here: all weights held for one sum at the end spill)
           if constexpr (e & 1) {
             pb[e >> 3][(e & 7) - 1] = (bf16)ex;
             pb[e >> 3][e & 7] = (bf16)x;
@@ -305,6 +315,8 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
   }
   src.template wait<0>();
   dense_barrier();  // the tiles are read
+  dsum = xor32_sum(dsum);
+  if (live && hq == 0) p.row_delta[rr] = (p.dlse != nullptr ? p.dlse[b * p.l_sb + t * p.l_ss + h * p.l_sh] : 0.f) - dsum;
   const RowsOut<D / 8> out{&s_kv[0][0][0] + wave * 32 * (D / 8)};
 #pragma unroll
   for (int o = 0; o < OT; ++o)

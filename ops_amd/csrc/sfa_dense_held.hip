@@ -10,7 +10,10 @@
 // in LDS as float32.  A score product (16 entries x 16 columns, 16x16x4) leaves a lane with 4
 // entries of one column, which are the second operand of the sums' product as they are, its
 // first being the same rows read down a dim.  The next tile's rows are loaded to registers
-// beside a tile's products.  Bound: the float32 matrix rate (154 TFLOP/s).
+// beside a tile's products.  Bound: the float32 matrix rate (153 TFLOP/s), of which a step of 1948
+// tokens, 2 x 16 heads of 64 on one, reaches 37: the LDS reads of one operand a product, and one
+// tile's barriers.  (Rows staged anew for each product, 64 dims at a time, as more than 128
+// dims need it: 5.1 times as long.)
 
 #include "sfa_dense_f32.h"
 
@@ -330,6 +333,7 @@ __global__ __launch_bounds__(256, 2) void dense_held_dq_kernel(DenseParams p) {
   f32x4 acc[H / 16];
 #pragma unroll
   for (int i = 0; i < H / 16; ++i) acc[i] = f32x4{};
+  float dsum = 0.f;  // sum_j p_ij do_i.v_j: delta again, of o before its rounding
   KeyEntry<T> ent;
   auto at = [&](int i) { return it.tiles.tile(it.v0 + i) << kAnyShift; };
   walk<H>(p, e, it.v1 - it.v0, ent, kp, p.Dqk, reinterpret_cast<const T*>(p.v), p.Dv, [&](int i) { ent.load(p, b, g, at(i)); },
@@ -344,7 +348,9 @@ __global__ __launch_bounds__(256, 2) void dense_held_dq_kernel(DenseParams p) {
       for (int k = 0; k < 4; ++k) {
         const int en = 16 * mt + 4 * hq + k;
         const bool ok = e.off[buf][0][en] >= 0 && live && dense_seen(p, j0 + en, qr.pos);
-        s[mt][k] = ok ? exp2f(fmaf(s[mt][k], p.scale_log2, -lse)) * (dp[mt][k] - delta) : 0.f;
+        const float w = ok ? exp2f(fmaf(s[mt][k], p.scale_log2, -lse)) : 0.f;
+        dsum += ok ? w * dp[mt][k] : 0.f;
+        s[mt][k] = ok ? w * (dp[mt][k] - delta) : 0.f;
       }
     if (bad) {
       __syncthreads();
@@ -354,7 +360,10 @@ __global__ __launch_bounds__(256, 2) void dense_held_dq_kernel(DenseParams p) {
     sums<H>(e.t[0], s, acc, lt, hq);
     if (bad) add_bad<H>(e, buf, 0, kp, p.Dqk, p.vec, s, acc, lt, hq);
   });
+  dsum += __shfl_xor(dsum, 16, 64);
+  dsum = xor32_sum(dsum);
   if (!qr.in) return;
+  if (live && hq == 0) p.row_delta[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
   T* o = reinterpret_cast<T*>(p.dq) + b * p.dq_sb + qr.t * p.dq_ss + qr.h * p.dq_sh;
 #pragma unroll
   for (int i = 0; i < H / 16; ++i) store4(o, 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);

@@ -9,6 +9,7 @@ import ops_amd
 from tests import dense_ref as ref
 from tests.test_gpu_dense import BF, DEV, F32, _case, _run, _want
 from tests.test_gpu_window import _check, _leaves
+from tests.test_gpu_window import _run as _run_window
 
 pytestmark = pytest.mark.gpu
 
@@ -171,6 +172,17 @@ def test_more_key_blocks_than_are_sorted():
     # (ds = do.v - do.o: 64 products of float32 in two orders, times a row of up to 6)
     mag = (do.float() * v.detach().float()).abs().sum(-1).max()
     assert float(torch.stack((dq, dk)).abs().max()) <= 128 * 2.0 ** -24 * float(mag) * 6
+
+
+@pytest.mark.parametrize("D,Dv,S", [(64, 64, 300), (128, 128, 200), (96, 96, 150), (192, 160, 90)])
+def test_the_sinks_gradient_knows_no_bf16(D, Dv, S):
+    """A float32 sum over all rows: as if o had not been rounded to bf16 (and with float32's bounds)."""
+    x = _leaves(BF, B=2, S=S, Hq=8, Hkv=2, D=D, Dv=Dv)
+    dlse = torch.randn(2, S, 8, device=DEV)
+    for grad in (None, dlse):
+        got = _run_window(*x, dlse=grad, window=70, first=3)
+        want, bound = ref.window(*x[:4], None, 70, 3, x[4], grad, None, F32, 0.0)[5]
+        assert float(((got[5].double() - want).abs() - bound).max()) <= 0.0
 
 
 def test_padded_rows_in_chunks():
