@@ -175,8 +175,11 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype) {
   const int64_t R = (int64_t)p.S * p.G;
   if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128))
     pl.kernel = R <= 16 ? kFew16 : R <= 32 ? kFew32 : R <= 64 ? kFew64 : kWide;
-  if (dtype == SFA_DTYPE_BF16 && kv_dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == kLatentQK && p.Dv == kLatentV && p.v == p.k &&
-      p.v_sb == p.k_sb && p.v_ss == p.k_ss && p.v_sh == p.k_sh)
+  // (e4m3 rows: of whole 16-byte units, as the other rows are, with one scale for both)
+  const bool one_scale = kv_dtype == SFA_DTYPE_BF16 ||
+                         (p.ks == p.vs && p.ks_sb == p.vs_sb && p.ks_ss == p.vs_ss && p.ks_sh == p.vs_sh && (p.k_sb | p.k_ss | p.k_sh) % 16 == 0);
+  if (dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == kLatentQK && p.Dv == kLatentV && p.v == p.k && p.v_sb == p.k_sb &&
+      p.v_ss == p.k_ss && p.v_sh == p.k_sh && one_scale)
     pl.kernel = kLatent;
   const KernelShape& k = kShapes[pl.kernel];
   pl.rows = k.rows;
@@ -214,7 +217,7 @@ hipError_t launch_dense(const DenseParams& p0, const DensePlan& pl, int dtype, i
   DenseParams p = p0;
   set_launch(p, pl);
   if (pl.kernel == kWide) launch_dense_wide(p, kv_dtype, s);
-  else if (pl.kernel == kLatent) launch_dense_mla(p, s);
+  else if (pl.kernel == kLatent) launch_dense_mla(p, kv_dtype == SFA_DTYPE_FP8_E4M3, s);
   else if (pl.kernel >= kFew16) launch_dense_few(p, kv_dtype, s);
   else launch_dense_any(p, dtype, kv_dtype, s);
   if (pl.want > 0) {

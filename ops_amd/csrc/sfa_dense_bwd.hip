@@ -327,7 +327,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
       for (int e = 0; e < 4; ++e) x[e] = (bf16)(dq[o][4 * i + e] * p.scale);
       out.put(lr, 32 * o + 8 * i + 4 * hq, x);
     }
-  out.store(0, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.dq) + b * p.dq_sb + t * p.dq_ss + h * p.dq_sh) : 0, lane);
+  out.store(in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.dq) + b * p.dq_sb + t * p.dq_ss + h * p.dq_sh) : 0, lane);
 }
 
 // ---- dk and dv: 128 keys, tiles of 32 query rows of all heads ----------------------------

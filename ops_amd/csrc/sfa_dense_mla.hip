@@ -1,5 +1,5 @@
 // gfx950 dense attention through a window (sfa_dense.h) over latent rows: head dims 576 and
-// 512, V the first 512 dims of K, bf16.
+// 512, V the first 512 dims of K, bf16 queries, bf16 or e4m3 rows.
 //
 // Eight waves take 64 query rows and tiles of 64 keys (72 KB of LDS, two stages), and divide
 // the two products differently:
@@ -17,6 +17,10 @@
 // maximum by 8 (base 2; 2^8 more at most in a float32 sum) raises a flag, and all of them move
 // it after the barrier that publishes P.  P is rounded to bf16 once for its product (2^-8 of a
 // weight); sums and statistics are float32.
+//
+// e4m3 rows (FP8) come to LDS as they are, two stages of 36 KB, and each wave makes bf16 ones
+// (times their power of two: exact) of its eight at the start of a step, in one stage of 72 KB:
+// a third barrier and 111 KB through LDS a tile (the above: 479 and 3290 us).
 
 #include "sfa_dense_tiles.h"
 
@@ -24,6 +28,7 @@ namespace sfa {
 namespace {
 
 constexpr int kLatentCh = 64, kLatentCr = 8;  // 16-byte chunks of a row's V part, of its rest
+constexpr int kLatentRaw = kLatentQK / 16;    // of an e4m3 row
 
 // Chunk c of row r goes to place c ^ at(r) of its row: one chunk of 16 consecutive rows (K)
 // meets all 16 bank groups, as do aligned groups of four chunks of four consecutive rows (V,
@@ -34,7 +39,7 @@ __device__ __forceinline__ int latent_rest_at(int r) { return (r >> 1) & 7; }
 // The rows of tiles of 64 keys for 8 waves, 8 rows each: an instruction for a row's first 1024
 // bytes, one for the last 128 of all eight.  ONE: a tile's rows have one base and stride
 // (contiguous rows, pages of 64 rows or more); else each its own, found a tile ahead.
-template <bool ONE>
+template <bool ONE, bool FP8>
 struct LatentSource {
   uint64_t kbase;
   int64_t kpage, krow;
@@ -45,13 +50,22 @@ struct LatentSource {
   uint64_t base, mask;   // the tile begin() was called for: its (ONE) or the lane's row's address, rows that are there
   int64_t step;
   int left;
+  const uint8_t* ks;     // FP8: exponents, and that of row wave * 8 + lane / 8 of begin()'s tile
+  int64_t ks_sb, ks_ss;
+  int exponent;
 
   __device__ __forceinline__ LatentSource(const DenseParams& p, const DenseItem& it, int wave_, int lane_)
       : tiles(it.tiles), v0(it.v0), n(it.v1 - it.v0), cap(p.cap), page_shift(p.page_shift), num_pages(p.num_pages), wave(wave_),
         lane(lane_) {
-    kbase = (uint64_t)(uintptr_t)p.k + (uint64_t)(2 * it.g * p.k_sh);
-    kpage = 2 * p.k_sb;
-    krow = 2 * p.k_ss;
+    constexpr int64_t E = FP8 ? 1 : 2;
+    kbase = (uint64_t)(uintptr_t)p.k + (uint64_t)(E * it.g * p.k_sh);
+    kpage = E * p.k_sb;
+    krow = E * p.k_ss;
+    if constexpr (FP8) {
+      ks = p.ks + it.g * p.ks_sh;
+      ks_sb = p.ks_sb;
+      ks_ss = p.ks_ss;
+    }
     trow = nullptr;
     if (p.block_table != nullptr) {
       trow = p.block_table + it.b * p.bt_sb;
@@ -78,12 +92,57 @@ struct LatentSource {
       step = ok ? krow : 0;
       left = ok ? rows : kWideKeys;
       mask = !ok ? 0 : rows >= kWideKeys ? ~0ull : (1ull << rows) - 1;
+      if constexpr (FP8) {
+        const int r = wave * 8 + (lane >> 3);
+        exponent = ok && r < rows ? ks[id * ks_sb + ((j0 & in_page) + r) * ks_ss] : 127;
+      }
       if (((i + 1) & 63) == 0) ids(i + 1);
     } else {
       const int j = j0 + lane;
       const bool ok = on && j < cap && pg >= 0 && pg < num_pages;
       base = ok ? kbase + (uint64_t)(pg * kpage + (j & in_page) * krow) : zero;
       mask = __ballot(ok);
+      if constexpr (FP8) {
+        const int r = wave * 8 + (lane >> 3), id = __shfl(pg, r, 64);
+        exponent = (mask >> r) & 1 ? ks[id * ks_sb + ((j0 + r) & in_page) * ks_ss] : 127;
+      }
+    }
+  }
+  // FP8: the wave's rows as they are
+  __device__ __forceinline__ void raw(u32x4* dst, int ln) const {
+    u32x4* const mine = dst + wave * 8 * kLatentRaw;
+#pragma unroll
+    for (int k = 0; k < (8 * kLatentRaw + 63) / 64; ++k) {
+      const int i = 64 * k + ln, r = min(wave * 8 + i / kLatentRaw, kWideKeys - 1);
+      uint64_t a;
+      if constexpr (ONE) {
+        a = row_at(r);
+      } else {
+        a = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(base >> 32), r, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)base, r, 64);
+      }
+      if (i < 8 * kLatentRaw) dense_dma16(mine + 64 * k, a + (uint64_t)(16 * (i % kLatentRaw)));
+    }
+  }
+  // ... and as bf16 in their places of a tile
+  __device__ __forceinline__ void widen(const u32x4* src, u32x4* kt, u32x4* rt, float scale, int ln) const {
+    const int r = wave * 8 + (ln >> 3);
+    const u32x4* const row = src + r * kLatentRaw;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      const int c = (ln & 7) + 8 * i;
+      if (c >= kLatentRaw) break;
+      const u32x4 x = row[c];
+      u32x4 y[2];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        y[w >> 1][2 * (w & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[w], scale, false));
+        y[w >> 1][2 * (w & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[w], scale, true));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (i < 4) kt[r * kLatentCh + ((2 * c + h) ^ latent_at(r))] = y[h];
+        else rt[r * kLatentCr + ((2 * c + h - kLatentCh) ^ latent_rest_at(r))] = y[h];
+      }
     }
   }
   __device__ __forceinline__ uint64_t row_at(int row) const {  // (ONE; rows past the last: row 0, which no row of theirs sees)
@@ -112,13 +171,15 @@ struct LatentSource {
   }
 };
 
-template <bool ONE>
+template <bool ONE, bool FP8>
 __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   typedef Mfma<16> M16;
   typedef Mfma<32> M;
   constexpr int CH = kLatentCh, CR = kLatentCr, KT = kWideKeys, STEPS = kLatentQK / 32, QR = 16;  // steps of Q in registers
-  __shared__ u32x4 s_k[2][KT * CH];       // dims 0 .. 511 (K and V)
-  __shared__ u32x4 s_r[2][KT * CR];       // dims 512 .. 575, Swz<64>
+  constexpr int LAST = FP8 ? 0 : 1;       // the last stage
+  __shared__ u32x4 s_k[LAST + 1][KT * CH];  // dims 0 .. 511 (K and V)
+  __shared__ u32x4 s_r[LAST + 1][KT * CR];  // dims 512 .. 575
+  __shared__ u32x4 s_raw[2][FP8 ? KT * kLatentRaw : 1];
   __shared__ u32x4 s_p[4][2][kLatentRows];  // P of 16 keys: [lane half][row] keys 4 half + 0 .. 3, 8 + 4 half + 0 .. 3
   __shared__ u32x4 s_q[4][kLatentRows];   // Q's last 32 dims: [8 of them][row]
   __shared__ u32x4 s_q1[4][32];           // the 32 before them, of rows 16 .. 31 and 48 .. 63
@@ -139,7 +200,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   // what all rows of the block see of a tile without a look at each
   const int p0 = it.s.ctx + it.row0 / p.G, p1 = it.s.ctx + min((it.row0 + p.rows - 1) / p.G, it.s.n - 1);
 
-  // The rows of Q come through LDS, where tile 1 goes later (straight from global memory each
+  // The rows of Q come through LDS, where a tile goes later (straight from global memory each
   // load touches 16 rows and four waves load the same: 6 us a workgroup).
   {
     const int r0 = it.row0 + 8 * wave;
@@ -149,7 +210,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     for (int k = 0; k < 8; ++k) {
       const int row = 8 * wave + k;
       const uint64_t a = r0 + k < R && t < it.s.n ? qbase + (uint64_t)(2 * (t * p.q_ss + h * p.q_sh)) : zero;
-      dense_dma16(&s_k[1][row * CH], a, 16u * (uint32_t)(lane ^ latent_at(row)));
+      dense_dma16(&s_k[LAST][row * CH], a, 16u * (uint32_t)(lane ^ latent_at(row)));
       if (++h == p.G) {
         h = 0;
         ++t;
@@ -159,7 +220,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     t = r / p.G;
     h = r - t * p.G;
     const uint64_t a = r < R && t < it.s.n ? qbase + (uint64_t)(2 * (t * p.q_ss + h * p.q_sh)) : zero;
-    dense_dma16(&s_r[1][8 * wave * CR], a + (uint64_t)(16 * (CH + ((lane & 7) ^ latent_rest_at(row)))));
+    dense_dma16(&s_r[LAST][8 * wave * CR], a + (uint64_t)(16 * (CH + ((lane & 7) ^ latent_rest_at(row)))));
   }
   if (tid < kLatentRows) {
     s_m[tid] = kNegInf;
@@ -169,13 +230,17 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     }
   }
 
-  LatentSource<ONE> src(p, it, wave, lane);
+  LatentSource<ONE, FP8> src(p, it, wave, lane);
   const int ntiles = it.v1 - it.v0;
   src.begin(0);
   uint64_t mask = src.mask;
+  if constexpr (FP8) {
+    src.raw(s_raw[0], lane);
+  } else {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) src.row(k, s_k[0], lane);
-  src.rest(s_r[0], lane);
+    for (int k = 0; k < 8; ++k) src.row(k, s_k[0], lane);
+    src.rest(s_r[0], lane);
+  }
   if constexpr (!ONE) src.ids(1);
 
   bf16x8 q[2][QR], q16;  // (Q's last one and a half steps in LDS: there is no register to spare)
@@ -188,8 +253,8 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
       const int row = 32 * rh + 16 * n + lt;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const bf16x8 y = s < 16 ? __builtin_bit_cast(bf16x8, s_k[1][row * CH + ((4 * s + hq) ^ latent_at(lt))])
-                                : __builtin_bit_cast(bf16x8, s_r[1][row * CR + ((4 * (s - 16) + hq) ^ latent_rest_at(lt))]);
+        const bf16x8 y = s < 16 ? __builtin_bit_cast(bf16x8, s_k[LAST][row * CH + ((4 * s + hq) ^ latent_at(lt))])
+                                : __builtin_bit_cast(bf16x8, s_r[LAST][row * CR + ((4 * (s - 16) + hq) ^ latent_rest_at(lt))]);
         if (s < QR) q[n][s < QR ? s : 0] = y;
         else if (s == QR && n == 0) q16 = y;
         else if (kq == 0 && s == QR) s_q1[hq][16 * rh + lt] = __builtin_bit_cast(u32x4, y);
@@ -207,8 +272,8 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   int nbad = 0;
 
   for (int j = 0; j < ntiles; ++j) {
-    const u32x4 *kt = s_k[j & 1], *rt = s_r[j & 1];
-    u32x4 *kn = s_k[(j + 1) & 1], *rn = s_r[(j + 1) & 1];
+    u32x4 *kt = s_k[j & LAST], *rt = s_r[j & LAST];
+    u32x4 *kn = s_k[(j + 1) & LAST], *rn = s_r[(j + 1) & LAST];
     // (lane constants are formed per tile: held across the loop they spill)
     int ln = lane;
     asm volatile("" : "+v"(ln));
@@ -217,6 +282,13 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     const uint32_t kr = lds_addr(rt) + (uint32_t)((16 * kq + lt) * CR) * 16u, rx = 16u * (uint32_t)(hq ^ latent_rest_at(lt));
     // tile j has landed for all waves; tile j - 1 and its P are read
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if constexpr (FP8) {
+      const float scale = scale_of((uint8_t)src.exponent);
+      src.begin(j + 1);
+      src.raw(s_raw[(j + 1) & 1], ln);
+      src.widen(s_raw[j & 1], kt, rt, scale, ln);
+      dense_barrier();
+    }
     // contraction steps in order, the one with Q in LDS first
     auto order = [](int i) { return i == 0 ? STEPS - 1 : i - 1; };
     auto read_k = [&](int s) {
@@ -227,7 +299,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
     for (int n = 0; n < 2; ++n) ql[n] = __builtin_bit_cast(bf16x8, s_q[hq][32 * rh + 16 * n + lt]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) kf[i] = read_k(order(i));
-    src.begin(j + 1);
+    if constexpr (!FP8) src.begin(j + 1);
     if (tid == 0) s_over[(j + 1) & 1] = 0;
     f32x4 sc[2];
     each<STEPS>([&](auto ic) {
@@ -242,8 +314,8 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
       }
       if constexpr (i == 14) ql[0] = __builtin_bit_cast(bf16x8, s_q1[hq][16 * rh + lt]);
       // the next tile's rows
-      if constexpr (i % 2 == 1 && i / 2 < 8) src.row(i / 2, kn, ln);
-      else if constexpr (i == 17) src.rest(rn, ln);
+      if constexpr (!FP8 && i % 2 == 1 && i / 2 < 8) src.row(i / 2, kn, ln);
+      else if constexpr (!FP8 && i == 17) src.rest(rn, ln);
     });
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!ONE) src.ids(j + 2);
@@ -343,7 +415,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
       const int w = nbad & 1;
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
-        u32x4& x = s_k[j & 1][(wave * 8 + i) * CH + ln];
+        u32x4& x = s_k[j & LAST][(wave * 8 + i) * CH + ln];
         u32x4 m;
 #pragma unroll
         for (int e = 0; e < 4; ++e) m[e] = bad16(x[e]);
@@ -379,7 +451,9 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
       const int key = __builtin_ctzll(bad);
       const int64_t at = dense_row(p, b, j0 + key, p.k_sb, p.k_ss);
       if (at < 0) continue;
-      const bf16* v = reinterpret_cast<const bf16*>(p.k) + at + g * p.k_sh + 64 * wave + 4 * half;
+      const int64_t v = at + g * p.k_sh + 64 * wave + 4 * half;
+      float vs = 1.f;
+      if constexpr (FP8) vs = scale_of(p.ks[dense_row(p, b, j0 + key, p.ks_sb, p.ks_ss) + g * p.ks_sh]);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float e = (float)reinterpret_cast<const bf16*>(&s_p[key >> 4][(key >> 2) & 1][32 * n + lr])[4 * ((key >> 3) & 1) + (key & 3)];
@@ -387,10 +461,18 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
         for (int o = 0; o < 2; ++o)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bf16x4 x = *reinterpret_cast<const bf16x4*>(v + 32 * o + 8 * i);
+            f32x4 xf;
+            bf16x4 xb;
+            if constexpr (FP8) {
+              const int w = *reinterpret_cast<const int*>(reinterpret_cast<const uint8_t*>(p.k) + v + 32 * o + 8 * i);
+              xf = f32x4{__builtin_amdgcn_cvt_f32_fp8(w, 0), __builtin_amdgcn_cvt_f32_fp8(w, 1), __builtin_amdgcn_cvt_f32_fp8(w, 2),
+                         __builtin_amdgcn_cvt_f32_fp8(w, 3)} * vs;
+            } else {
+              xb = *reinterpret_cast<const bf16x4*>(reinterpret_cast<const bf16*>(p.k) + v + 32 * o + 8 * i);
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float y = (float)x[c];
+              const float y = FP8 ? xf[c] : (float)xb[c];
               if (e != 0.f && !(fabsf(y) <= 3.402823466e38f)) oacc[o][n][4 * i + c] += e * y;
             }
           }
@@ -414,6 +496,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   }
   dense_barrier();
   const int lr = lane & 31, half = lane >> 5;
+  static_assert(sizeof(s_k) >= 8 * 32 * 16 * 16, "32 float32 rows of 64 dims a wave");
   u32x4* const rows = &s_k[0][0];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -440,13 +523,13 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
         }
     };
     if (it.partial) {
-      const RowsOut<16> out{rows + wave * kLatentRows * 16};
-      results([&](int d, f32x4 x) { out.put(row, d, x); });
-      out.store(32 * n, in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * p.Dv + 64 * wave) : 0, lane);
+      const RowsOut<16> out{rows + wave * 32 * 16};
+      results([&](int d, f32x4 x) { out.put(lr, d, x); });
+      out.store(in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * p.Dv + 64 * wave) : 0, lane);
     } else {
-      const RowsOut<8> out{rows + wave * kLatentRows * 8};
-      results([&](int d, f32x4 x) { out.put(row, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
-      out.store(32 * n, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + 64 * wave) : 0,
+      const RowsOut<8> out{rows + wave * 32 * 8};
+      results([&](int d, f32x4 x) { out.put(lr, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
+      out.store(in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + 64 * wave) : 0,
                 lane);
     }
   }
@@ -454,10 +537,13 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
 
 }  // namespace
 
-void launch_dense_mla(const DenseParams& p, hipStream_t s) {
+void launch_dense_mla(const DenseParams& p, bool fp8, hipStream_t s) {
   const unsigned grid = (unsigned)((int64_t)p.slots * p.Hkv);
-  if (dense_one_base(p, 2, 6)) dense_mla_kernel<true><<<grid, 512, 0, s>>>(p);
-  else dense_mla_kernel<false><<<grid, 512, 0, s>>>(p);
+  const bool one = dense_one_base(p, fp8 ? 1 : 2, 6);
+  if (fp8 && one) dense_mla_kernel<true, true><<<grid, 512, 0, s>>>(p);
+  else if (fp8) dense_mla_kernel<false, true><<<grid, 512, 0, s>>>(p);
+  else if (one) dense_mla_kernel<true, false><<<grid, 512, 0, s>>>(p);
+  else dense_mla_kernel<false, false><<<grid, 512, 0, s>>>(p);
 }
 
 }  // namespace sfa

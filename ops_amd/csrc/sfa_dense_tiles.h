@@ -303,14 +303,14 @@ struct RowsOut {
     *reinterpret_cast<bf16x4*>(reinterpret_cast<char*>(slot(row, d >> 3)) + 8 * ((d >> 2) & 1)) = x;
   }
   __device__ __forceinline__ void put(int row, int d, f32x4 x) const { *reinterpret_cast<f32x4*>(slot(row, d >> 2)) = x; }
-  // rows first .. first + 31 to where lane r % 32 says (0: nowhere)
-  __device__ __forceinline__ void store(int first, uint64_t at, int lane) const {
+  // its 32 rows to where lane r % 32 says (0: nowhere)
+  __device__ __forceinline__ void store(uint64_t at, int lane) const {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int k = 0; k < 32 * CH / 64; ++k) {
       const int i = k * 64 + lane, row = i / CH;
       const uint64_t a = ((uint64_t)(uint32_t)__shfl((int)(at >> 32), row, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)at, row, 64);
-      const u32x4 x = *slot(first + row, i % CH);
+      const u32x4 x = *slot(row, i % CH);
       if (a != 0) *reinterpret_cast<u32x4*>(a + (uint64_t)(16 * (i % CH))) = x;
     }
   }

@@ -280,11 +280,11 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
     if (it.partial) {
       const RowsOut<D / 4> out{rows + wave * 32 * (D / 4)};
       results([&](int d, f32x4 x) { out.put(lr, d, x); });
-      out.store(0, in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * D) : 0, ln);
+      out.store(in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * D) : 0, ln);
     } else {
       const RowsOut<D / 8> out{rows + wave * 32 * (D / 8)};
       results([&](int d, f32x4 x) { out.put(lr, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
-      out.store(0, in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh) : 0, ln);
+      out.store(in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh) : 0, ln);
     }
   }
 }

@@ -201,7 +201,7 @@ void launch_dense_few(const DenseParams& p, int kv_dtype, hipStream_t s);
 
 // ... and over latent rows (sfa_dense_mla.hip): head dims 576 / 512, V the first dims of K
 constexpr int kLatentRows = 64, kLatentQK = 576, kLatentV = 512;
-void launch_dense_mla(const DenseParams& p, hipStream_t s);
+void launch_dense_mla(const DenseParams& p, bool fp8, hipStream_t s);
 
 void launch_dense_bwd_mfma(const DenseParams& p, int units, hipStream_t s);  // (sfa_dense_bwd.hip)
 

@@ -45,6 +45,38 @@ def test_ranges_of_keys(B, S, ctx, heads):
     _both(_latent(S=S, ctx=(ctx,) * B, Hq=heads, page=64))
 
 
+@pytest.mark.parametrize("page", [1, 16, 64, 256])
+@pytest.mark.parametrize("S,ctx,window,first", [(1, (0, 63, 900), None, 0), (70, (1, 130), None, 0), (9, (300, 127, 64), 100, 3),
+                                                (5, (5000,), None, 0), (3, (200, 61), 65, 64)])
+def test_rows_of_8_bits(page, S, ctx, window, first):
+    _both(_latent(fp8=True, S=S, ctx=ctx, Hq=16, page=page, seed=S), window=window, first=first)
+
+
+def test_8_bit_rows_of_no_scale_and_padding():
+    c = _latent(fp8=True, S=70, ctx=(100, 30), n=[70, 20], Hq=16, page=64)
+    want = _run(c)
+    j = 130  # token 30's own row
+    c["ks"][int(c["bt"][0, j // 64]), j % 64, 0] = 255
+    out, lse = _run(c)
+    assert torch.equal(out[:, :30], want[0][:, :30]) and torch.equal(out[1], want[0][1]) and torch.equal(lse[1], want[1][1])
+    assert torch.isnan(out[0, 30:]).all() and torch.isnan(lse[0, 30:]).all()
+    assert not out[1, 20:].any() and torch.isinf(lse[1, 20:]).all()
+
+
+def test_8_bit_rows_of_another_stride():
+    """Rows of 8-byte units only take another way, to the same results."""
+    c = _latent(fp8=True, S=4, ctx=(200, 70), Hq=16, page=16)
+    want = _run(c)
+    num, page = c["k"].shape[:2]
+    wide = torch.zeros(num, page, 1, 584, device=DEV, dtype=torch.uint8)
+    wide[..., 8:] = c["k"].view(torch.uint8)
+    k = wide.view(torch.float8_e4m3fn)[..., 8:]
+    c.update(k=k, v=k[..., :512])
+    got = _run(c)
+    assert float((got[1] - want[1]).abs().max()) < 1e-4
+    ref.check(got, _want(c), 576, BF, 2.0 ** -8)
+
+
 def test_rows_of_another_stride():
     """Latent rows inside wider ones, a pool in another order, q and out of other strides."""
     c = _latent(S=7, ctx=(100, 20), Hq=16, page=16)

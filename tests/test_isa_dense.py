@@ -36,7 +36,7 @@ def _needed(tmp_path):
 @pytest.fixture(scope="module")
 def asm(tmp_path_factory):
     out = {}
-    for stem in ("sfa_dense_wide", "sfa_dense_few", "sfa_dense_mla", "sfa_dense_bwd"):
+    for stem in ("sfa_dense_wide", "sfa_dense_few", "sfa_dense_bwd"):
         src = [s for s in sfa_build.sources() if Path(s).stem == stem]
         assert len(src) == 1
         out[stem] = _device_asm(Path(src[0]), tmp_path_factory.mktemp(stem))
