@@ -496,7 +496,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   }
   dense_barrier();
   const int lr = lane & 31, half = lane >> 5;
-  static_assert(sizeof(s_k) >= 8 * 32 * 16 * 16, "32 float32 rows of 64 dims a wave");
+  static_assert(sizeof(s_k) >= (FP8 ? 1 : 2) * 8 * 32 * 16 * 16, "32 float32 rows of 64 dims a wave, or all 64");
   u32x4* const rows = &s_k[0][0];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -523,11 +523,11 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
         }
     };
     if (it.partial) {
-      const RowsOut<16> out{rows + wave * 32 * 16};
+      const RowsOut<16> out{rows + (FP8 ? wave : 2 * wave + n) * 32 * 16};
       results([&](int d, f32x4 x) { out.put(lr, d, x); });
       out.store(in ? (uint64_t)(uintptr_t)(p.part_o + (it.part + row) * p.Dv + 64 * wave) : 0, lane);
     } else {
-      const RowsOut<8> out{rows + wave * 32 * 8};
+      const RowsOut<8> out{rows + (FP8 ? wave : 2 * wave + n) * 32 * 8};
       results([&](int d, f32x4 x) { out.put(lr, d, bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}); });
       out.store(in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.out) + b * p.o_sb + t * p.o_ss + h * p.o_sh + 64 * wave) : 0,
                 lane);
