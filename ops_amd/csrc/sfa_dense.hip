@@ -302,7 +302,7 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   pl.dkv_bytes = (size_t)(groups * parts) * kDkvKeys * 2 * p.Dqk * sizeof(float);
   pl.unit_bytes = (size_t)units * 4 * sizeof(int);
   const int64_t nrb = ((int64_t)p.S * p.G + kWideRows - 1) / kWideRows;
-  pl.fits = groups * nrb * 512 < most && groups * units * 512 < most && groups * nkb * 256 < most;
+  pl.fits = (groups * nrb + 1) * 512 < most && groups * units * 512 < most && groups * nkb * 256 < most;
   return pl;
 }
 
