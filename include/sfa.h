@@ -447,8 +447,8 @@ SFA_API size_t sfa_dense_fwd_workspace_size(const sfa_dense_args* a, const sfa_k
 SFA_API int sfa_dense_fwd(const sfa_dense_args* a, const sfa_kv_pages* pages, void* workspace, size_t workspace_bytes,
                           void* stream);
 
-/* Its gradients (every sum in a fixed order).  Workspace: two floats a query row, and
- * float32 partials of key blocks that many rows see. */
+/* Its gradients (every sum in a fixed order).  Workspace: two floats a query row (three
+ * with more than 128 dims), and float32 partials of key blocks that many rows see. */
 SFA_API size_t sfa_dense_bwd_workspace_size(const sfa_dense_bwd_args* a);
 SFA_API int sfa_dense_bwd(const sfa_dense_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream);
 

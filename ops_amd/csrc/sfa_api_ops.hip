@@ -465,9 +465,10 @@ int sfa_dense_bwd(const sfa_dense_bwd_args* a, void* workspace, size_t workspace
   if (workspace == nullptr || workspace_bytes < need)
     return fail(SFA_E_WORKSPACE, "sfa_dense_bwd needs %zu workspace bytes (got %zu)", need, workspace_bytes);
   p.row_lse = (float*)workspace;
-  p.row_delta = (float*)((char*)workspace + pl.row_bytes / 2);
-  p.dkv_part = (float*)((char*)workspace + pl.row_bytes);
-  p.dkv_units = (int*)((char*)workspace + pl.row_bytes + pl.dkv_bytes);
+  p.row_delta = (float*)((char*)workspace + pl.row_bytes);
+  p.row_exact = (float*)((char*)workspace + (pl.row_arrays - 1) * pl.row_bytes);
+  p.dkv_part = (float*)((char*)workspace + pl.row_arrays * pl.row_bytes);
+  p.dkv_units = (int*)((char*)workspace + pl.row_arrays * pl.row_bytes + pl.dkv_bytes);
   return done(sfa::launch_dense_bwd(p, pl, a->fwd.dtype, (hipStream_t)stream), "sfa_dense_bwd");
 }
 

@@ -231,12 +231,14 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   DenseBwdPlan pl{};
   const size_t rows = (size_t)p.B * p.Hkv * p.S * p.G;
   // (each a row tile longer: the matrix kernels read whole tiles of them)
-  pl.row_bytes = 2 * ((rows * sizeof(float) + 128 + 255) / 256 * 256);
+  pl.row_bytes = (rows * sizeof(float) + 128 + 255) / 256 * 256;
+  pl.row_arrays = 2;
   const int64_t groups = (int64_t)p.B * p.Hkv, most = (int64_t)1 << 32;
   pl.mfma = dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) &&
             p.k_ss >= 0 && p.v_ss >= 0 && p.k_ss < (int64_t)1 << 24 && p.v_ss < (int64_t)1 << 24;
   if (!pl.mfma) {
     const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
+    pl.row_arrays = dims > 1 ? 3 : 2;
     const int64_t nrb = ((int64_t)p.S * p.G + kAnyRows - 1) / kAnyRows, nkb = ((int64_t)p.S + kAnyRows - 1) / kAnyRows;
     // Few key blocks (two workgroups a CU): their rows in chunks, of four times as many
     // workgroups in all (256 tokens, 32 heads on 2: 8 blocks of up to 4096 rows).
@@ -327,6 +329,7 @@ hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int d
     else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
     launch_dense_bwd_any(p, dtype, s);
   }
+  p.row_delta = p.row_exact;
   if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
   return hipGetLastError();
 }

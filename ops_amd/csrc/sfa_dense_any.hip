@@ -273,7 +273,8 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   dsum += __shfl_xor(dsum, 16, 64);
   dsum = xor32_sum(dsum);
   if (!qr.in) return;
-  if (live && hq == 0 && dc == 0) p.row_delta[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
+  // (an array of its own: the workgroups of the row's other dims may not have read row_delta yet)
+  if (live && hq == 0 && dc == 0) p.row_exact[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
   T* o = reinterpret_cast<T*>(p.dq) + b * p.dq_sb + qr.t * p.dq_ss + qr.h * p.dq_sh;
 #pragma unroll
   for (int i = 0; i < 8; ++i) store4(o, dc * kAnyDims + 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);
@@ -363,7 +364,9 @@ void bwd(const DenseParams& p, hipStream_t s) {
     launch_dense_held_bwd(p, sizeof(T) == 4, s);
   } else {
     dense_any_dq_kernel<T><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv * ((p.Dqk + kAnyDims - 1) / kAnyDims)), 256, 0, s>>>(p);
-    dense_any_dkv_kernel<T><<<(unsigned)(blocks * p.dkv_parts * ((dmax + kAnyDims - 1) / kAnyDims)), 256, 0, s>>>(p);
+    DenseParams q = p;
+    q.row_delta = p.row_exact;
+    dense_any_dkv_kernel<T><<<(unsigned)(blocks * p.dkv_parts * ((dmax + kAnyDims - 1) / kAnyDims)), 256, 0, s>>>(q);
   }
   if (p.dkv_parts > 1) dense_any_join_kernel<T><<<dim3((unsigned)blocks, 4), 256, 0, s>>>(p);
 }

@@ -317,7 +317,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
   src.template wait<0>();
   dense_barrier();  // the tiles are read
   dsum = xor32_sum(dsum);
-  if (live && hq == 0) p.row_delta[rr] = (p.dlse != nullptr ? p.dlse[b * p.l_sb + t * p.l_ss + h * p.l_sh] : 0.f) - dsum;
+  if (live && hq == 0) p.row_exact[rr] = (p.dlse != nullptr ? p.dlse[b * p.l_sb + t * p.l_ss + h * p.l_sh] : 0.f) - dsum;
   const RowsOut<D / 8> out{&s_kv[0][0][0] + wave * 32 * (D / 8)};
 #pragma unroll
   for (int o = 0; o < OT; ++o)

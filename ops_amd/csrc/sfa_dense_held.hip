@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void dense_held_dq_kernel(DenseParams p) {
   dsum += __shfl_xor(dsum, 16, 64);
   dsum = xor32_sum(dsum);
   if (!qr.in) return;
-  if (live && hq == 0) p.row_delta[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
+  if (live && hq == 0) p.row_exact[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
   T* o = reinterpret_cast<T*>(p.dq) + b * p.dq_sb + qr.t * p.dq_ss + qr.h * p.dq_sh;
 #pragma unroll
   for (int i = 0; i < H / 16; ++i) store4(o, 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);
@@ -424,6 +424,7 @@ void fwd(const DenseParams& p, hipStream_t s) {
 template <typename T, int H>
 void bwd(const DenseParams& p, hipStream_t s) {
   dense_held_dq_kernel<T, H><<<(unsigned)((int64_t)p.B * p.nrb * p.Hkv), 256, 0, s>>>(p);
+  // (row_exact is row_delta: one workgroup a row block reads and writes it)
   dense_held_dkv_kernel<T, H><<<(unsigned)((int64_t)((p.S + kAnyRows - 1) / kAnyRows) * p.B * p.Hkv * p.dkv_parts), 256, 0, s>>>(p);
 }
 

@@ -156,6 +156,9 @@ struct DenseParams {
   // matrix kernels (row_neg) -lse / scale and -delta, which their accumulators start from
   float* row_lse;
   float* row_delta;
+  // delta of o before its rounding, which dq leaves for dk, dv and the sink: row_delta again where
+  // one workgroup makes a row's dq, else (heads of more than 128 dims) an array that no dq reads
+  float* row_exact;
   bool row_neg;
   float* dkv_part;           // partial dK | dV of key blocks cut in chunks: bf16 matrix kernels [B Hkv][dkv_parts]
                              // [kDkvKeys][2 D], others [B Hkv][blocks][dkv_parts][kAnyRows][Dqk + Dv]
@@ -177,10 +180,11 @@ DensePlan dense_plan(const DenseParams& p, int dtype, int kv_dtype);
 hipError_t launch_dense(const DenseParams& p, const DensePlan& pl, int dtype, int kv_dtype, hipStream_t s);
 constexpr int kDkvKeys = 128;  // keys a block of the dk / dv kernel
 struct DenseBwdPlan {
-  size_t row_bytes, dkv_bytes, unit_bytes;  // row_lse + row_delta; partial dK | dV; the units
+  size_t row_bytes, dkv_bytes, unit_bytes;  // row_lse (row_delta, row_exact: as much each); partial dK | dV; the units
+  int row_arrays;
   int chunk, cut0, cut1, cut_chunk, units, parts;  // of the dk / dv kernel: as above; units and partials a kv head
   bool mfma, fits;
-  size_t workspace() const { return row_bytes + dkv_bytes + unit_bytes; }
+  size_t workspace() const { return row_arrays * row_bytes + dkv_bytes + unit_bytes; }
 };
 DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype);
 hipError_t launch_dense_bwd(const DenseParams& p, const DenseBwdPlan& pl, int dtype, hipStream_t s);
