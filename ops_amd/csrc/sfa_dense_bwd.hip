@@ -254,7 +254,10 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
     const bool whole = mask[0] == ~0ull && j0 + KT - 1 <= p0 && (j0 + KT <= p.first || p1 - j0 < p.window);
     if (!whole) {
       // infinities and NaN of keys that not every row sees: 0 times them would reach those
-      // that do not (those that do have weights that are no numbers)
+      // that do not (those that do have weights that are no numbers).  Another wave may still be
+      // reading these rows for its scores: half 0 ends without a barrier, as do the first scores;
+      // the first 32 rows of later tiles are read before half 1's.
+      if (H == 1 || j == 0) dense_barrier();
       clear_rows<D, NW>(s_kv[st][0], 32 * H, wave, lane);
       const uint32_t seen = (uint32_t)((seen_of(p, pos, j0) & mask[0]) >> (32 * H)) >> (4 * hq);
 #pragma unroll

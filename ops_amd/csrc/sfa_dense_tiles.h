@@ -272,8 +272,8 @@ __device__ __forceinline__ uint64_t clear_bad(u32x4* vt, unsigned long long* s_b
   return *s_bad;
 }
 
-// Elements of 32 rows from `row` on that are no numbers, cleared; a barrier on both sides
-// of what all waves do with them.
+// Elements of 32 rows from `row` on that are no numbers, cleared, and a barrier.  The caller sees
+// to it that all waves have read what they need of them as they were.
 template <int D, int NW>
 __device__ __forceinline__ void clear_rows(u32x4* t, int row, int wave, int lane) {
   constexpr int N = 32 / Tile<D>::RPI;  // groups of 64 chunks
