@@ -277,7 +277,10 @@ __global__ __launch_bounds__(256) void dense_any_dq_kernel(DenseParams p) {
   if (live && hq == 0 && dc == 0) p.row_exact[rr] = dsum - (p.dlse != nullptr ? p.dlse[b * p.l_sb + qr.t * p.l_ss + qr.h * p.l_sh] : 0.f);
   T* o = reinterpret_cast<T*>(p.dq) + b * p.dq_sb + qr.t * p.dq_ss + qr.h * p.dq_sh;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) store4(o, dc * kAnyDims + 16 * i + 4 * hq, p.Dqk, p.vec, acc[i] * p.scale);
+  for (int i = 0; i < 8; ++i) {  // (padding: 0 times what the others see)
+    const f32x4 y = acc[i] * p.scale, x = live ? y : f32x4{};
+    store4(o, dc * kAnyDims + 16 * i + 4 * hq, p.Dqk, p.vec, x);
+  }
 }
 
 // 64 keys a workgroup, 16 a wave; a chunk of the rows of all heads that see them, in order.

@@ -328,7 +328,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
     for (int i = 0; i < 4; ++i) {
       bf16x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (bf16)(dq[o][4 * i + e] * p.scale);
+      for (int e = 0; e < 4; ++e) x[e] = (bf16)(live ? dq[o][4 * i + e] * p.scale : 0.f);  // (padding: 0 times what the others see)
       out.put(lr, 32 * o + 8 * i + 4 * hq, x);
     }
   out.store(in ? (uint64_t)(uintptr_t)(reinterpret_cast<bf16*>(p.dq) + b * p.dq_sb + t * p.dq_ss + h * p.dq_sh) : 0, lane);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import dense_ref as ref
-from tests.test_gpu_window import BF, _leaves, _run
+from tests.test_gpu_window import BF, F32, _leaves, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,20 @@ def test_a_key_that_some_rows_see(D, value, key):
     gone = score == -math.inf  # (a weight of 0: the token's other rows make its result)
     assert torch.isfinite(dq[0, key:, :4, 4:])[gone].all() and torch.isfinite(out[0, key:, :4])[gone].all()
     assert torch.isnan(dq[0, key:, :4])[~gone].all() and torch.isnan(lse[0, key:, :4])[~gone].all()
+
+
+@pytest.mark.parametrize("dtype,D,Dv", [(BF, 64, 64), (BF, 128, 128), (BF, 40, 40), (F32, 64, 64), (BF, 192, 160), (F32, 300, 300)])
+@pytest.mark.parametrize("which", [1, 2])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_padding_beside_rows_of_infinities(dtype, D, Dv, which, value):
+    """A row of k or v that is no number, of a key that every live token of a later row block
+    sees: padded tokens of that block keep their zeros."""
+    S, lens = 700, torch.tensor([600, 700, 3], dtype=torch.int32, device="cuda")
+    x = list(_leaves(dtype, B=3, S=S, Hq=4, Hkv=2, D=D, Dv=Dv))
+    x[which] = x[which].clone()
+    x[which][:, 1, :, ::3] = value
+    out, lse, dq, dk, dv = _run(*x, lens=lens)[:5]
+    for t in (out, dq, dk, dv):
+        assert not t[0, 600:].any() and not t[2, 3:].any()
+    assert bool((lse[0, 600:] == -math.inf).all())
+    assert torch.isnan(dq[1, 1:]).any()
