@@ -215,7 +215,7 @@ int check_dense(const sfa_dense_args* a, const sfa_kv_pages* pg) {
 }
 
 sfa::DenseParams dense_params(const sfa_dense_args* a, const sfa_kv_pages* pg) {
-  constexpr int kNone = 1 << 30;  // a window past every row
+  constexpr int kMost = 1 << 30;  // a window past every row
   sfa::DenseParams p;
   memset(&p, 0, sizeof(p));
   p.q = a->q; p.k = a->k; p.v = a->v; p.ks = a->k_scale; p.vs = a->v_scale;
@@ -230,7 +230,8 @@ sfa::DenseParams dense_params(const sfa_dense_args* a, const sfa_kv_pages* pg) {
   p.l_sb = a->l_sb; p.l_ss = a->l_ss; p.l_sh = a->l_sh;
   p.B = a->B; p.S = a->S; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv;
   p.Dqk = a->Dqk; p.Dv = a->Dv;
-  p.window = a->window == 0 || a->window > kNone ? kNone : a->window;
+  p.window = a->window == 0 || a->window > kMost ? kMost : a->window;
+  p.over = a->window == 0 ? INT_MAX : a->window - p.window;
   p.first = a->first;
   p.cap = a->S;
   if (pg != nullptr) {

@@ -29,9 +29,18 @@ __device__ __forceinline__ float dense_lse(float m2, float l) {
 struct DenseSeq {
   int ctx, n;  // rows before the first token, tokens
 };
+// A token past the table sees what its window leaves of it, so there only ctx - window counts:
+// what a window of more than 2^30 has over that (p.over; without a window: more than any
+// context) is taken off the context, down to the table's end, and from cap + 2^30 on no window
+// reaches a row (p.cap <= 2^29).  Positions so stay below 2^31 - 1 (S <= 2^29).
+constexpr int kFarCtx = (1 << 30) + (1 << 29) - 1;
 __device__ __forceinline__ DenseSeq dense_seq(const DenseParams& p, int b) {
   DenseSeq s;
-  s.ctx = p.ctx_lens != nullptr ? min(max(p.ctx_lens[b], 0), p.cap) : 0;
+  s.ctx = 0;
+  if (p.ctx_lens != nullptr) {
+    const int c = max(p.ctx_lens[b], 0);
+    s.ctx = max(min(c, p.cap), min(c - p.over, kFarCtx));
+  }
   s.n = p.lens != nullptr ? min(max(p.lens[b], 0), p.S) : p.S;
   return s;
 }
@@ -53,7 +62,7 @@ __device__ __forceinline__ KeyTiles key_tiles(const DenseParams& p, const DenseS
   const int hi = min(s.ctx + t1 + 1, p.cap), lo = max(0, s.ctx + t0 - p.window + 1), one = (1 << shift) - 1;
   const int end = (hi + one) >> shift;
   k.head = lo > 0 ? min((min(p.first, hi) + one) >> shift, end) : 0;
-  k.from = max(lo >> shift, k.head);
+  k.from = max(min(lo >> shift, end), k.head);  // (lo: past all rows, where a context is past the table)
   k.n = k.head + max(end - k.from, 0);
   return k;
 }

@@ -135,7 +135,8 @@ struct DenseParams {
   int64_t o_sb, o_ss, o_sh, l_sb, l_ss, l_sh;
   int64_t bt_sb;
   int B, S, Hq, Hkv, G, Dqk, Dv;
-  int window, first;         // window: 2^30 stands for none
+  int window, first;         // window: up to 2^30, which is more than any distance in a table
+  int over;                  // what the caller's has over that (none: 2^31 - 1)
   int page_shift, num_pages, cap;  // cap: rows a sequence can have
   float scale, scale_log2;
   bool vec;                  // rows are whole 16-byte units (8-bit: 8)

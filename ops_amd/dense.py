@@ -71,8 +71,8 @@ def chunk_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     ``k_cache`` / ``v_cache`` / ``block_table`` as in :func:`ops_amd.sfa_forward_paged`.
     Token ``s`` of sequence ``b`` stands at row ``ctx_lens[b] + s`` and sees the rows up
     to it (``window``: the last ``window`` of them, itself among them, and the
-    ``first`` rows of the sequence); rows on unmapped pages are not seen.  Tokens at
-    or past ``chunk_lens[b]`` (None: S) are padding: zeros and ``lse = -inf``.  A
+    ``first`` rows of the sequence); rows on unmapped pages and past the table are not
+    seen (a context may end behind it).  Tokens at or past ``chunk_lens[b]`` (None: S) are padding: zeros and ``lse = -inf``.  A
     token that sees nothing gives the same (with ``attn_sink`` ``[Hq]``, which adds
     ``exp(sink)`` to each denominator, the sink as its ``lse``).
 
