@@ -234,6 +234,10 @@ sfa::DenseParams dense_params(const sfa_dense_args* a, const sfa_kv_pages* pg) {
   p.over = a->window == 0 ? INT_MAX : a->window - p.window;
   p.first = a->first;
   p.cap = a->S;
+  if (pg == nullptr && (p.window >= a->S || p.first >= a->S)) {  // all earlier rows are seen
+    p.window = kMost;
+    p.first = 0;
+  }
   if (pg != nullptr) {
     p.block_table = pg->block_table; p.bt_sb = pg->bt_sb;
     p.num_pages = pg->num_pages;

@@ -259,7 +259,9 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   // left over from whole rounds of 256 (8192 tokens, window 1024: 0.97 of the CUs' time
   // used for 0.84); else every block is cut in chunks of half a CU's share (with the longest
   // first 0.97).  A partial sum costs 128 keys of float32, written and read; a chunk of fewer
-  // than 512 rows is mostly its start.
+  // than 512 rows is mostly its start.  The first tokens' blocks are cut in about four chunks a
+  // CU at most, however narrow the window (8192 tokens, window 64, 32 / 8 heads of 128, the first
+  // 4096: 1.14 GB of workspace with chunks of the window's blocks, 0.15 so).
   const int64_t nkb = ((int64_t)p.S + kDkvKeys - 1) / kDkvKeys;
   auto block_rows = [&](int64_t kb) {
     const int64_t j0 = kb * kDkvKeys, t1 = j0 < p.first ? p.S : j0 + kDkvKeys - 1 + p.window;
@@ -267,15 +269,16 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   };
   constexpr int64_t kCus = 256, kLeast = 512;
   auto up = [&](int64_t x) { return (x < kLeast ? kLeast : x + 31) / 32 * 32; };
-  int64_t total = 0, widest = 0;  // (of the blocks behind the first tokens)
+  int64_t total = 0, head = 0, widest = 0;  // all rows; of the first tokens' blocks; of a block behind those
   for (int64_t kb = 0; kb < nkb; ++kb) {
     const int64_t r = block_rows(kb);
     total += r;
-    if (kb * kDkvKeys >= p.first && r > widest) widest = r;
+    if (kb * kDkvKeys < p.first) head += r;
+    else if (r > widest) widest = r;
   }
   const int64_t share = total * groups / kCus;
   const bool cut = 3 * widest > 2 * share;
-  const int64_t chunk = up(cut ? share / 2 : widest);
+  const int64_t part = head * groups / kCus / 4, chunk = up(cut ? share / 2 : widest > part ? widest : part);
   int64_t units = 0, parts = 0;
   pl.cut0 = pl.cut1 = 0;
   pl.cut_chunk = (int)up(chunk / 5);
