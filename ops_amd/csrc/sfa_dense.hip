@@ -100,10 +100,11 @@ void combine(const DenseParams& p, hipStream_t s) {
 
 // ---- backward: per query row its LSE (base 2) and delta = sum o do - dlse (the bf16 matrix
 // kernels' dq makes its own) ------------
-// 16 lanes a row.  Rows that see nothing get +inf, which makes every weight 0.
+// 16 lanes a row, from row `first` on.  Rows that see nothing get +inf, which makes every weight 0.
+constexpr int64_t kDeltaRows = (int64_t)1 << 27;  // of a launch: fewer than 2^32 threads
 template <typename T>
-__global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
-  const int64_t rr = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+__global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p, int64_t first) {
+  const int64_t rr = first + (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int lane = threadIdx.x & 15, R = p.S * p.G;
   if (rr >= (int64_t)p.B * p.Hkv * R) return;
   const int b = (int)(rr / ((int64_t)p.Hkv * R)), x = (int)(rr - (int64_t)b * p.Hkv * R), g = x / R, r = x - g * R;
@@ -125,10 +126,12 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(DenseParams p) {
   p.row_delta[rr] = delta;
 }
 
-// dsink[h] = -sum over the rows of exp(sink - lse) delta, a workgroup a head, in a fixed order.
-__global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p) {
+// dsink[h] = -sum over the rows of exp(sink - lse) delta, a workgroup a head (from head `first`
+// on), in a fixed order.
+constexpr int kSinkHeads = 1 << 21;  // of a launch: fewer than 2^32 threads
+__global__ __launch_bounds__(1024) void dense_dsink_kernel(DenseParams p, int first) {
   __shared__ float s_x[1024];
-  const int h = blockIdx.x, g = h / p.G, hl = h % p.G;
+  const int h = first + blockIdx.x, g = h / p.G, hl = h % p.G;
   const float sink = p.sink[h] * kLog2e;
   float sum = 0.f;
   for (int b = 0; b < p.B; ++b) {
@@ -327,13 +330,17 @@ hipError_t launch_dense_bwd(const DenseParams& p0, const DenseBwdPlan& pl, int d
   if (pl.mfma) {  // (whose dq kernel leaves the rows' statistics)
     launch_dense_bwd_mfma(p, pl.units, s);
   } else {
-    const unsigned grid = (unsigned)(((int64_t)p.B * p.Hkv * p.S * p.G + 15) / 16);
-    if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p);
-    else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p);
+    const int64_t rows = (int64_t)p.B * p.Hkv * p.S * p.G;
+    for (int64_t first = 0; first < rows; first += kDeltaRows) {
+      const unsigned grid = (unsigned)(((rows - first < kDeltaRows ? rows - first : kDeltaRows) + 15) / 16);
+      if (dtype == SFA_DTYPE_F32) dense_delta_kernel<float><<<grid, 256, 0, s>>>(p, first);
+      else dense_delta_kernel<bf16><<<grid, 256, 0, s>>>(p, first);
+    }
     launch_dense_bwd_any(p, dtype, s);
   }
   p.row_delta = p.row_exact;
-  if (p.dsink != nullptr) dense_dsink_kernel<<<p.Hq, 1024, 0, s>>>(p);
+  for (int first = 0; p.dsink != nullptr && first < p.Hq; first += kSinkHeads)
+    dense_dsink_kernel<<<p.Hq - first < kSinkHeads ? p.Hq - first : kSinkHeads, 1024, 0, s>>>(p, first);
   return hipGetLastError();
 }
 
