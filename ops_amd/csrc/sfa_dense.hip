@@ -237,7 +237,8 @@ DenseBwdPlan dense_bwd_plan(const DenseParams& p, int dtype) {
   pl.row_bytes = (rows * sizeof(float) + 128 + 255) / 256 * 256;
   pl.row_arrays = 2;
   const int64_t groups = (int64_t)p.B * p.Hkv, most = (int64_t)1 << 32;
-  pl.mfma = dtype == SFA_DTYPE_BF16 && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) &&
+  // (its accumulators start from -lse / scale: no infinity while scale is 2^-100 or more)
+  pl.mfma = dtype == SFA_DTYPE_BF16 && p.scale >= 0x1p-100f && p.vec && p.Dqk == p.Dv && (p.Dqk == 64 || p.Dqk == 128) &&
             p.k_ss >= 0 && p.v_ss >= 0 && p.k_ss < (int64_t)1 << 24 && p.v_ss < (int64_t)1 << 24;
   if (!pl.mfma) {
     const int64_t dims = ((p.Dqk > p.Dv ? p.Dqk : p.Dv) + kAnyDims - 1) / kAnyDims;
