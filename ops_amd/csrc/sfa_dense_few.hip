@@ -41,6 +41,16 @@ __device__ __forceinline__ uint32_t bad8(uint32_t w) {  // bytes of w that are N
   for (int i = 0; i < 4; ++i) m |= (w & (0x7fu << (8 * i))) == (0x7fu << (8 * i)) ? 0xffu << (8 * i) : 0u;
   return m;
 }
+// Infinities and NaN of bf16 elements as the largest finite values: for the weights' second
+// parts, which are 0 or of either sign and would make no number of the first ones' infinities
+// (1% of a step: 438 -> 443 us, 32 contexts of 1K to 32K).
+__device__ __forceinline__ bf16x8 no_infinities(bf16x8 x) {
+  typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  // (positive ones are the upper end of signed 16 bits, negative ones of unsigned)
+  const i16x8 p = __builtin_elementwise_min(__builtin_bit_cast(i16x8, x), i16x8(0x7f7f));
+  return __builtin_bit_cast(bf16x8, __builtin_elementwise_min(__builtin_bit_cast(u16x8, p), u16x8(0xff7f)));
+}
 // at most N of the wave's loads in flight, its LDS reads done
 template <int N>
 __device__ __forceinline__ void few_wait() {
@@ -353,9 +363,9 @@ __global__ __launch_bounds__(256, NG == 4 ? 1 : 2) void dense_few_kernel(DensePa
     if (!whole) bad = clear_bad(part_at(j, true));
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
-      const bf16x8 a = read_v(vt, o);
+      const bf16x8 a = read_v(vt, o), af = FP8 ? a : no_infinities(a);  // (e4m3 has none)
 #pragma unroll
-      for (int i = 0; i < NG; ++i) oacc[i][o] = M::mma(a, pr[i], M::mma(a, pb[i], oacc[i][o]));
+      for (int i = 0; i < NG; ++i) oacc[i][o] = M::mma(af, pr[i], M::mma(a, pb[i], oacc[i][o]));
     }
     if (bad != 0) add_bad(bad, j0, pb, pr);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V's place is read
