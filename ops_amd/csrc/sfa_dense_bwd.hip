@@ -144,7 +144,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
   static_assert(sizeof(s_kv) >= (2 * kSorted + 16 + 3 * 512) * sizeof(int), "the units' counts");
   if (blockIdx.x == gridDim.x - 1) return dkv_units(p, reinterpret_cast<int*>(s_kv));
   int slot, g;
-  if (!dense_place(p, slot, g)) return;
+  dense_place(p, slot, g);
   DenseItem it;
   if (!dense_item(p, slot, g, it)) return;
   const int b = it.b, r = it.row0 + 32 * wave + lr;

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(512, 2) void dense_mla_kernel(DenseParams p) {
   const int rh = wave & 1, kq = wave >> 1;
 
   int slot, g;
-  if (!dense_place(p, slot, g)) return;
+  dense_place(p, slot, g);
   DenseItem it;
   if (!dense_item(p, slot, g, it)) return;
   const int b = it.b, R = p.S * p.G;

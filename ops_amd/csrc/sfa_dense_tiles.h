@@ -329,12 +329,12 @@ __device__ __forceinline__ const DenseParams& late_params() {
 // Where the workgroup's share of a launch is: the row blocks of a (sequence, kv head)
 // on one XCD (workgroup i is on XCD i % 8), whose L2 their keys then stay in; the
 // longest ones, which are a sequence's last, first.
-__device__ __forceinline__ bool dense_place(const DenseParams& p, int& slot, int& g) {
+__device__ __forceinline__ void dense_place(const DenseParams& p, int& slot, int& g) {
   int w = blockIdx.x;
   if (p.want > 0) {
     g = w % p.Hkv;
     slot = w / p.Hkv;
-    return true;
+    return;
   }
   const int groups = p.B * p.Hkv, x = w & 7;
   int group, rb;
@@ -351,7 +351,6 @@ __device__ __forceinline__ bool dense_place(const DenseParams& p, int& slot, int
   }
   g = group % p.Hkv;
   slot = group / p.Hkv * p.nrb + (p.nrb - 1 - rb);
-  return true;
 }
 
 }  // namespace sfa

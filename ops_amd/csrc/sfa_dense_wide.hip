@@ -34,7 +34,7 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
   const int lr = lane & 31, hq = lane >> 5;
 
   int slot, g;
-  if (!dense_place(p, slot, g)) return;
+  dense_place(p, slot, g);
   DenseItem it;
   if (!dense_item(p, slot, g, it)) return;
   const int b = it.b, row = 32 * wave + lr, r = it.row0 + row;
@@ -60,7 +60,6 @@ __global__ __launch_bounds__(512, 2) void dense_wide_kernel(DenseParams p) {
 #pragma unroll
   for (int o = 0; o < OT; ++o) oacc[o] = acc_t{};
   float m_used = kNegInf, l_part = 0.f;
-  const float inv_scale = 1.f / p.scale_log2;
 
   // Operand addresses.  K: row lr, chunk 2 s + hq; V: rows 4 hq + (lane % 16) / 4, 16 dims
   // by lane / 16 % 2.  The places of a row's chunks differ by rows in bits 2 and 3 (D = 64: 1
