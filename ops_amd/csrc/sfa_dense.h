@@ -77,12 +77,6 @@ __device__ __forceinline__ int64_t dense_row(const DenseParams& p, int b, int j,
   return (int64_t)pg * sb + (int64_t)(j & ((1 << p.page_shift) - 1)) * ss;
 }
 
-// The value of a scale's exponent byte.
-__device__ __forceinline__ float scale_of(uint8_t e) {
-  // (2^-127 is no normal number, 255 stands for NaN)
-  return __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : (uint32_t)e << 23);
-}
-
 // ---- key ranges of a launch ("slots") ---------------------------------------------
 // A unit is a (sequence, row block).  p.fit workgroups of a kv head run at once.  With
 // want > 0 (few units) the units' tiles are cut into ranges of up to one length, found

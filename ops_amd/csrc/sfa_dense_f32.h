@@ -9,14 +9,6 @@ namespace sfa {
 constexpr int kE = 1 << kAnyShift;  // entries a tile
 static_assert(kE == 32 && kAnyRows == 64, "four waves of 16 columns, two 16-entry products");
 
-struct fp8_t {
-  uint8_t x;
-};
-template <typename T>
-__device__ __forceinline__ float value_of(T x) {
-  if constexpr (std::is_same<T, fp8_t>::value) return __builtin_amdgcn_cvt_f32_fp8((int)x.x, 0);
-  else return to_f32(x);
-}
 // dims d .. d + 3 of a row of D, zeros past its end
 template <typename T>
 __device__ __forceinline__ f32x4 load4(const T* p, int d, int D, bool vec) {

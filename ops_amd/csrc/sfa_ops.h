@@ -75,6 +75,20 @@ size_t rope_bwd_workspace(const RopeParams& p);
 hipError_t launch_rope_fwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);  // p.ks: to 8-bit pools
 hipError_t launch_rope_bwd(const RopeParams& p, int dtype, bool vec, hipStream_t s);
 
+// ---- 8-bit rows: e4m3 values times the value of the row's exponent byte ----
+struct fp8_t {
+  uint8_t x;
+};
+template <typename T>
+__device__ __forceinline__ float value_of(T x) {
+  if constexpr (std::is_same<T, fp8_t>::value) return __builtin_amdgcn_cvt_f32_fp8((int)x.x, 0);
+  else return to_f32(x);
+}
+__device__ __forceinline__ float scale_of(uint8_t e) {
+  // (2^-127 is no normal number, 255 stands for NaN)
+  return __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : (uint32_t)e << 23);
+}
+
 // ---- attention of a tree of drafted tokens over a paged cache ----
 struct TreeParams {
   const void* q;

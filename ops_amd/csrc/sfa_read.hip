@@ -43,12 +43,6 @@ __device__ __forceinline__ void write8(T* p, const float (&f)[8]) {
     *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
   }
 }
-template <typename T>
-__device__ __forceinline__ float read1(const T* p, float scale) {
-  if constexpr (sizeof(T) == 1) return __builtin_amdgcn_cvt_f32_fp8((int)*reinterpret_cast<const uint8_t*>(p), 0) * scale;
-  else return to_f32(*p);
-}
-
 // VEC: 8 elements of a head at a time, else one.
 template <typename TI, typename TO, bool VEC>
 __global__ __launch_bounds__(256) void cache_read_kernel(ReadParams p, int L) {
@@ -68,23 +62,16 @@ __global__ __launch_bounds__(256) void cache_read_kernel(ReadParams p, int L) {
   for (int c = lane % L; c < n; c += L) {
     const int h = c / per, d = (c - h * per) * E;
     float scale = 1.f;
-    if (sizeof(TI) == 1 && there) {
-      const uint8_t e = sc[h * p.s_sh];
-      scale = __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : (uint32_t)e << 23);
-    }
+    if (sizeof(TI) == 1 && there) scale = scale_of(sc[h * p.s_sh]);
     if constexpr (VEC) {
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (there) read8(src + h * p.c_sh + d, scale, f);
       write8(dst + h * p.o_sh + d, f);
     } else {
-      dst[h * p.o_sh + d] = from_f32<TO>(there ? read1(src + h * p.c_sh + d, scale) : 0.f);
+      dst[h * p.o_sh + d] = from_f32<TO>(there ? value_of(src[h * p.c_sh + d]) * scale : 0.f);
     }
   }
 }
-
-struct byte_t {
-  uint8_t x;
-};
 
 template <typename TI, typename TO>
 void launch(const ReadParams& p, bool vec, hipStream_t s) {
@@ -98,7 +85,7 @@ void launch(const ReadParams& p, bool vec, hipStream_t s) {
 }
 template <typename TO>
 void launch_to(const ReadParams& p, int cache_dtype, bool vec, hipStream_t s) {
-  if (cache_dtype == SFA_DTYPE_FP8_E4M3) launch<byte_t, TO>(p, vec, s);
+  if (cache_dtype == SFA_DTYPE_FP8_E4M3) launch<fp8_t, TO>(p, vec, s);
   else if (cache_dtype == SFA_DTYPE_BF16) launch<bf16, TO>(p, vec, s);
   else launch<float, TO>(p, vec, s);
 }
