@@ -17,8 +17,9 @@
 // parts would be half of the products again); dq's delta takes o as it was rounded to bf16 (dq
 // 0.0026 to 0.0028: another would need o's other half kept).  Sums are float32.
 //
-// 8192 tokens, window 1024, 32 / 8 heads of 128: dq 275 us (0.75 PF/s of its three products), dk
-// and dv 505 (0.54 PF/s of their four); 2 x 4096 tokens without a window, 32 / 2 heads: 405, 765.
+// 8192 tokens, window 1024, 32 / 8 heads of 128: dq 272 us (0.71 PF/s of its three products), dk
+// and dv 422 (0.61 PF/s of their four); 2 x 4096 tokens without a window, 32 / 2 heads: 406, 700.
+// (In long runs; 292 and 491, 432 and 768 in the first passes.)
 
 #include "sfa_dense_tiles.h"
 
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(512, 2) void dense_dq_kernel(DenseParams p) {
 // order; waves 4 .. 7, one on each SIMD beside one of those, take the last step's for the
 // sums of 64 keys x half of the dims.  So no wave holds both the keys' rows and the
 // sums (all in one wave are 320 registers: 929 us at 8192 tokens, window 1024, 32 / 8
-// heads of 128, where this takes 505), the products of one cover the weights of the other, and
+// heads of 128, where this took 505 in as short a run), the products of one cover the weights of the other, and
 // LDS moves 112 KB a step of 1024 clocks' products.  The waves of sums load the rows, five
 // tiles ahead: they have the registers for the addresses (by all waves it was 626, with
 // spills).

