@@ -1,7 +1,7 @@
 // Launch parameters and launchers of the operators around the sparse
 // attention: rotation and norms (sfa_rope.hip), attention of a tree of drafted
-// tokens (sfa_tree.hip), pages of the cache (sfa_pages.hip).  Their C entry
-// points are in sfa_api_ops.hip.
+// tokens (sfa_tree.hip), dense attention (sfa_dense*.hip), rows (sfa_read.hip) and
+// pages of the cache (sfa_pages.hip).  Their C entry points are in sfa_api_ops.hip.
 #pragma once
 
 #include <utility>

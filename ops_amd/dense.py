@@ -72,9 +72,10 @@ def chunk_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     Token ``s`` of sequence ``b`` stands at row ``ctx_lens[b] + s`` and sees the rows up
     to it (``window``: the last ``window`` of them, itself among them, and the
     ``first`` rows of the sequence); rows on unmapped pages and past the table are not
-    seen (a context may end behind it).  Tokens at or past ``chunk_lens[b]`` (None: S) are padding: zeros and ``lse = -inf``.  A
-    token that sees nothing gives the same (with ``attn_sink`` ``[Hq]``, which adds
-    ``exp(sink)`` to each denominator, the sink as its ``lse``).
+    seen (a context may end behind it).  Tokens at or past ``chunk_lens[b]`` (None: S)
+    are padding: zeros and ``lse = -inf``.  A token that sees nothing gives the same
+    (with ``attn_sink`` ``[Hq]``, which adds ``exp(sink)`` to each denominator, the sink as
+    its ``lse``).
 
     ``float8_e4m3fn`` caches with exponent bytes ``k_scales`` / ``v_scales``
     (:func:`ops_amd.qk_norm_rope_append`) are attended to as the values that they
